@@ -55,6 +55,9 @@ extern "C" {
 #define SAGE_DTYPE_F16 1
 #define SAGE_DTYPE_BOOL 2 /* attention masks only */
 
+#define SAGE_CACHE_INT8 0 /* codes of the key / value cache */
+#define SAGE_CACHE_E4M3 1
+
 #define SAGE_KV_BLOCK 32  /* keys per K scale (kernel_build/build_kernels.py:30) */
 #define SAGE_KV_PAD 128   /* K8 / V8T rows are padded to a multiple of this */
 
@@ -241,6 +244,60 @@ int sage_forward_noalloc(const void* q, int64_t qsb, int64_t qss, int64_t qsh, c
                          int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss, int64_t vsh, void* out,
                          int64_t osb, int64_t oss, int64_t osh, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype,
                          int causal, float qs_mul, void* stream);
+
+/*
+ * Rotary positions of Q and, where Hk > 0, of K in the same launch (no counterpart in the reference).  The first rot_dim
+ * channels of every head are pairs (i, i + rot_dim / 2), or (2i, 2i + 1) where interleaved is set; pair i of a token at
+ * position p turns by p * freqs[i] radians: (a, b) -> factor * (a cos - b sin, b cos + a sin).  inverse turns back (the
+ * transpose, for gradients).  The other channels are copied.  rot_dim: a positive multiple of 8, at most D.
+ * q / k and their outputs are addressed like sage_quant_q's q, outputs may not overlap the inputs.  positions: int32 or
+ * (positions64) int64, token s of batch entry b at positions[b * psb + s * pss]; NULL: s.  freqs: float64
+ * [rot_dim / 2], on the device.
+ */
+int sage_rope(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* q_out, int64_t qob, int64_t qos, int64_t qoh,
+              int H, const void* k, int64_t ksb, int64_t kss, int64_t ksh, void* k_out, int64_t kob, int64_t kos,
+              int64_t koh, int Hk, int B, int S, int D, int dtype, const void* positions, int positions64, int64_t psb,
+              int64_t pss, const double* freqs, int rot_dim, int interleaved, float factor, int inverse, void* stream);
+
+/*
+ * The quantized key / value cache (no counterpart in the reference): codes [pages, Hkv, page_size, D] of cache_dtype
+ * SAGE_CACHE_INT8 or SAGE_CACHE_E4M3 and fp32 scales [pages, Hkv, page_size], for K and for V, contiguous and 16-byte
+ * aligned.  Row x of a token and kv head has scale max |x| / Q (Q = 127 or 448) and codes round(Q x / max |x|), ties to
+ * even; a row with an infinity or a NaN gets scale NaN and codes 0.  page_size: a power of two from 16 to 1024.
+ * slots: int32 or (slots64) int64 [B * S]; slot = page * page_size + row.  Slots outside the cache belong to tokens
+ * without one: the write skips them, the read gives zeros.  Two tokens of one write with the same slot leave unspecified
+ * contents in that slot's row.  k / v: (b, s, h) strides as everywhere.
+ */
+int sage_cache_write(const void* k, int64_t ksb, int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss,
+                     int64_t vsh, int B, int S, int dtype, const void* slots, int slots64, void* k8, float* k_scale,
+                     void* v8, float* v_scale, int pages, int page_size, int Hkv, int D, int cache_dtype, void* stream);
+
+/* Rows of the cache as code * scale, rounded to dtype: k, v [B, S, Hkv, D] by their strides. */
+int sage_cache_read(void* k, int64_t ksb, int64_t kss, int64_t ksh, void* v, int64_t vsb, int64_t vss, int64_t vsh,
+                    int B, int S, int dtype, const void* slots, int slots64, const void* k8, const float* k_scale,
+                    const void* v8, const float* v_scale, int pages, int page_size, int Hkv, int D, int cache_dtype,
+                    void* stream);
+
+/*
+ * Attention of T new tokens per sequence over the cache.  lengths[b] (int32, device; clamped to 0 and max_pages *
+ * page_size): the cached keys of sequence b, the T new tokens' own (its last T) among them; block_table: int32 rows of
+ * max_pages entries, table_stride apart: key j is row j % page_size of page block_table[b][j / page_size].  An entry
+ * outside [0, pages) hides its keys.  Query i sees every key before the new ones and, of those, its own and the earlier
+ * ones (causal), all (causal = 0) or, with a tree mask (one byte per element, nonzero = visible, (b, i, j) at tree_mask
+ * + b * msb + i * msq + j * msk), those its row shows; where lengths[b] < T the first new tokens have no key.  A query
+ * without a visible key is written as 0, its logsumexp as -inf.  q / out: [B, T, H, D] by (b, t, h) strides, dtype
+ * bf16 or fp16; lse: fp32 [B, H, T] natural log, or NULL.  sm_scale 0: 1 / sqrt(D).  Codes and scales of keys that no
+ * query of a step sees may hold anything; E4M3 codes of the new tokens must not be NaN.
+ * workspace: sage_cache_attn_workspace bytes, 256-byte aligned (NULL where that is 0).
+ */
+int sage_cache_attn_workspace(int B, int H, int Hkv, int T, int D, int page_size, int max_pages,
+                              int64_t* workspace_bytes);
+int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* out, int64_t osb, int64_t oss,
+                    int64_t osh, float* lse, const void* k8, const float* k_scale, const void* v8,
+                    const float* v_scale, const int* block_table, int64_t table_stride, const int* lengths,
+                    const void* tree_mask, int64_t msb, int64_t msq, int64_t msk, int B, int H, int Hkv, int T, int D,
+                    int dtype, int cache_dtype, int pages, int page_size, int max_pages, int causal, float sm_scale,
+                    void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

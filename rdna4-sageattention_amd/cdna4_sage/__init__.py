@@ -12,6 +12,9 @@ kernels, including two cases the reference sends to SDPA: causal calls with q_le
 attn_masks (bool, or additive of q's dtype; set CDNA4_SAGE_NATIVE_MASK=0 to send masks to SDPA as the reference
 does).
 attention_varlen runs packed variable-length batches in one pass.
+
+For decoding: rope (rotary positions), cache_write / cache_read (an 8-bit key / value cache in pages), cache_attention
+(new tokens, or a tree of drafted ones, over that cache) and cache_step, which is the three of them in a row.
 """
 import os
 
@@ -19,11 +22,15 @@ import torch
 from torch.nn.attention.bias import causal_lower_right
 
 from . import ops
-from ._attention import (ARCHS, HEAD_DIMS, Unsupported, attention_varlen, check_supported, device_arch, lse,
-                         mask_view)
+from ._attention import (ARCHS, HEAD_DIMS, Unsupported, _plain_eager, attention_varlen, check_supported, device_arch,
+                         lse, mask_view)
 from ._attention import attention as _attention_impl
+from ._cache import (KVCache, cache_attention, cache_read, cache_slots, cache_step, cache_write, new_cache)
+from ._rope import rope, rope_frequencies
 
-__all__ = ["sageattn", "attention", "attention_varlen", "lse", "is_available", "Unsupported", "ARCHS", "HEAD_DIMS"]
+__all__ = ["sageattn", "attention", "attention_varlen", "lse", "is_available", "Unsupported", "ARCHS", "HEAD_DIMS",
+           "rope", "rope_frequencies", "KVCache", "new_cache", "cache_slots", "cache_write", "cache_read",
+           "cache_attention", "cache_step"]
 __version__ = "0.1.0"
 
 # Fallbacks call torch's C entry point of SDPA directly: a caller may have monkey-patched
@@ -57,18 +64,6 @@ def is_available(device=None) -> bool:
         return False
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
     return device_arch(dev) in ARCHS
-
-
-def _plain_eager(*ts) -> bool:
-    """True for an eager call on plain tensors: no torch.compile / export tracing, no tensor subclass (fake or
-    functional tensors), no active dispatch mode (make_fx and the like) and no autograd recording on the inputs.  Such
-    calls may run the op's implementation directly; anything else goes through the registered op, so that tracers see
-    its fake implementation and autograd sees an op without a derivative (backward raises, as in the reference)."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
-        return False
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        return False
-    return all(type(t) is torch.Tensor for t in ts)
 
 
 def attention(q, k, v, tensor_layout="HND", sm_scale=None, is_causal=False, attn_mask=None):

@@ -12,6 +12,7 @@ import math
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -30,6 +31,23 @@ _arch_cache = {}
 
 class Unsupported(Exception):
     """The inputs fall outside what the gfx950 kernels handle; use another attention backend."""
+
+
+def _plain_eager(*ts, grad=False) -> bool:
+    """True for an eager call on plain tensors: no torch.compile / export tracing, no tensor subclass (fake or
+    functional tensors), no active dispatch mode (make_fx and the like) and no autograd recording on the inputs.  Such
+    calls may run the op's implementation directly; anything else goes through the registered op, so that tracers see
+    its fake implementation and autograd sees an op without a derivative (backward raises, as in the reference).
+    grad=True: for a call that deals with reverse-mode autograd itself (forward-mode duals and functorch's wrappers then go
+    to the op)."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        return False
+    if grad:
+        return all(type(t) in (torch.Tensor, torch.nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(t)
+                   and forward_ad.unpack_dual(t).tangent is None for t in ts)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        return False
+    return all(type(t) is torch.Tensor for t in ts)
 
 
 def device_arch(device: torch.device) -> str:

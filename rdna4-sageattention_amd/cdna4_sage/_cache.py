@@ -1,0 +1,277 @@
+"""The quantized, paged key / value cache and the attention of new tokens over it, on the gfx950 kernels (no counterpart in
+the reference, which quantizes all keys and values anew in every call, src/rdna4_sage/_attention.py:115-133).
+
+    cache = cdna4_sage.new_cache(pages, 16, kv_heads, head_dim)               # int8, or dtype=torch.float8_e4m3fn
+    slots = cdna4_sage.cache_slots(block_table, lengths, T, 16)               # lengths with the T new tokens counted
+    cdna4_sage.cache_write(cache, k, v, slots)
+    out = cdna4_sage.cache_attention(q, cache, block_table, lengths)          # q [B, H, T, D]
+
+Nothing here reads device memory back, allocates outside torch's caching allocator or keeps state between calls, so
+every call can be captured into a graph.
+"""
+from __future__ import annotations
+
+import functools
+from typing import NamedTuple
+
+import torch
+
+from . import _capi, ops
+from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, device_arch
+from ._rope import _sizes, rope
+
+CACHE_DTYPES = {torch.int8: _capi.CACHE_INT8, torch.float8_e4m3fn: _capi.CACHE_E4M3}
+
+
+class KVCache(NamedTuple):
+    """Codes [pages, kv_heads, page_size, head_dim] (int8 or float8_e4m3fn) and scales [pages, kv_heads, page_size]
+    (float32) of the keys and the values, contiguous: a key is code * scale.  Slot s is row s % page_size of page
+    s // page_size.  page_size is a power of two from 16 to 1024."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def new_cache(pages, page_size, kv_heads, head_dim, dtype=torch.int8, device=None):
+    """An empty KVCache (all zeros)."""
+    shape = (int(pages), int(kv_heads), int(page_size))
+    _check_page(shape[2])
+    if dtype not in CACHE_DTYPES:
+        raise Unsupported(f"cache dtype {dtype} (int8 or float8_e4m3fn)")
+    if head_dim not in HEAD_DIMS:
+        raise Unsupported(f"head_dim {head_dim} (supported {HEAD_DIMS})")
+    if shape[0] <= 0 or shape[1] <= 0:
+        raise Unsupported("a cache needs pages and kv heads")
+    device = torch.device("cuda" if device is None else device)
+    codes = [torch.zeros(shape + (int(head_dim),), dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
+    return KVCache(*codes, *(torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _check_page(page_size):
+    if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+        raise Unsupported(f"page_size {page_size} (a power of two from 16 to 1024)")
+
+
+def check_cache(cache, device=None):
+    """(pages, kv_heads, page_size, head_dim) of a usable cache; raises Unsupported with the reason."""
+    k, v, ks, vs = cache
+    if k.dim() != 4 or v.shape != k.shape or ks.shape != k.shape[:3] or vs.shape != k.shape[:3]:
+        raise Unsupported("cache codes [pages, kv_heads, page_size, head_dim] and scales [pages, kv_heads, page_size] required")
+    if k.dtype not in CACHE_DTYPES or v.dtype != k.dtype:
+        raise Unsupported(f"cache dtype {k.dtype}/{v.dtype} (int8 or float8_e4m3fn)")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise Unsupported("cache scales must be float32")
+    pages, heads, page_size, D = k.shape
+    _check_page(page_size)
+    if D not in HEAD_DIMS:
+        raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
+    if pages == 0 or heads == 0 or pages > _I32_MAX:
+        raise Unsupported("a cache needs pages and kv heads")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise Unsupported("cache tensors must be contiguous")
+    dev = k.device if device is None else device
+    if not (k.is_cuda and k.device == dev and v.device == dev and ks.device == dev and vs.device == dev):
+        raise Unsupported("tensors must be on one ROCm GPU")
+    if device_arch(dev) not in ARCHS:
+        raise Unsupported("not a CDNA4 GPU")
+    return pages, heads, page_size, D
+
+
+def cache_slots(block_table, lengths, count, page_size):
+    """Slots of the last `count` of lengths[b] tokens of every sequence, int64 [B, count], for cache_write and cache_read;
+    -1 where there is no such token or its page is missing (an entry below 0 or a column past the table)."""
+    _check_page(page_size)
+    pos = lengths.to(torch.int64)[:, None] - count + torch.arange(count, device=lengths.device)[None, :]
+    column = torch.div(pos, page_size, rounding_mode="floor")
+    if block_table.shape[1] == 0:
+        return torch.full_like(pos, -1)
+    page = block_table.to(torch.int64).gather(1, column.clamp(0, block_table.shape[1] - 1))
+    there = (pos >= 0) & (column < block_table.shape[1]) & (page >= 0)
+    return torch.where(there, page * page_size + pos % page_size, -1)
+
+
+def _check_slots(slots, device, shape):
+    if slots.dtype not in (torch.int32, torch.int64):
+        raise Unsupported(f"slots {slots.dtype} (int32 or int64)")
+    if slots.device != device:
+        raise Unsupported("tensors must be on one ROCm GPU")
+    if tuple(slots.shape) != shape:
+        raise Unsupported(f"slots of shape {tuple(slots.shape)} for tokens {shape}")
+    return slots.contiguous()
+
+
+def _rows_args(t, layout):
+    """A packed [tokens, heads, D] or a 4D tensor as the kernels address it: tensor, (b, s, h) strides."""
+    return _bsh(t.unsqueeze(0), "NHD") if t.dim() == 3 else _bsh(t, layout)
+
+
+def write_launch(cache, k, v, slots, layout):
+    if layout not in ("HND", "NHD"):
+        raise Unsupported(f"layout {layout!r}")
+    if k.dim() not in (3, 4) or k.shape != v.shape:
+        raise Unsupported("k and v of one shape, 4D or packed [tokens, kv_heads, head_dim], required")
+    if k.dtype not in DTYPES or v.dtype != k.dtype:
+        raise Unsupported(f"dtype {k.dtype}/{v.dtype} (fp16 or bf16 required)")
+    if v.device != k.device:
+        raise Unsupported("tensors must be on one ROCm GPU")
+    pages, Hkv, page_size, D = check_cache(cache, k.device)
+    if k.dim() == 3:
+        (S, h, d), B = k.shape, 1
+        tokens = (S,)
+    else:
+        B, S, h, d = _sizes(k, layout)
+        tokens = (B, S)
+    if (h, d) != (Hkv, D):
+        raise Unsupported(f"{h} heads of {d} channels for a cache of {Hkv} heads of {D}")
+    slots = _check_slots(slots, k.device, tokens)
+    if k.numel() == 0:
+        return
+    if k.numel() > _I32_MAX:
+        raise Unsupported("tensor too large for 32-bit indexing")
+    k, sk = _rows_args(k, layout)
+    v, sv = _rows_args(v, layout)
+    _capi.call_on(k.device, "sage_cache_write", k.data_ptr(), *sk, v.data_ptr(), *sv, B, S, DTYPES[k.dtype],
+                  slots.data_ptr(), int(slots.dtype == torch.int64), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+                  cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D, CACHE_DTYPES[cache.k.dtype])
+
+
+def read_launch(cache, slots, dtype, layout):
+    if layout not in ("HND", "NHD"):
+        raise Unsupported(f"layout {layout!r}")
+    if dtype not in DTYPES:
+        raise Unsupported(f"dtype {dtype} (fp16 or bf16 required)")
+    pages, Hkv, page_size, D = check_cache(cache)
+    if slots.dim() not in (1, 2):
+        raise Unsupported("slots [tokens] or [B, tokens] required")
+    slots = _check_slots(slots, cache.k.device, tuple(slots.shape))
+    out = [torch.empty((*slots.shape, Hkv, D), dtype=dtype, device=slots.device) for _ in range(2)]
+    if slots.numel():
+        if out[0].numel() > _I32_MAX:
+            raise Unsupported("tensor too large for 32-bit indexing")
+        B, S = (1, slots.numel()) if slots.dim() == 1 else slots.shape
+        st = (S * Hkv * D, Hkv * D, D)
+        _capi.call_on(slots.device, "sage_cache_read", out[0].data_ptr(), *st, out[1].data_ptr(), *st, B, S, DTYPES[dtype],
+                      slots.data_ptr(), int(slots.dtype == torch.int64), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+                      cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D,
+                      CACHE_DTYPES[cache.k.dtype])
+    if slots.dim() == 2 and layout == "HND":
+        out = [t.transpose(1, 2) for t in out]
+    return tuple(out)
+
+
+def cache_write(cache, k, v, slots, tensor_layout="HND"):
+    """Quantizes rows of k and v into the cache: per token and kv head one scale, max |x| / 127 (int8) or / 448 (E4M3), and
+    the nearest codes of x / scale, ties to even; a row with an infinity or a NaN is kept as NaN (by its scale).
+    k / v: [B, kv_heads, tokens, head_dim] ("HND") or [B, tokens, kv_heads, head_dim] ("NHD") with slots [B, tokens], or packed
+    [tokens, kv_heads, head_dim] with slots [tokens]; slots int32 or int64.  Tokens whose slot is outside the cache (-1) are
+    left out; two tokens of a call may not share a slot (that slot's row then holds parts of both)."""
+    if _plain_eager(k, v, slots, *cache, grad=True):
+        with torch.no_grad():
+            write_launch(cache, k, v, slots, tensor_layout)
+    else:
+        ops.cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, slots, tensor_layout)
+
+
+def cache_read(cache, slots, dtype=torch.bfloat16, tensor_layout="HND"):
+    """(k, v) of the slots as code * scale, rounded to dtype: packed [tokens, kv_heads, head_dim] for slots [tokens] (as
+    sageattn_varlen takes them), 4D in tensor_layout for slots [B, tokens].  Slots outside the cache (-1) give zeros."""
+    if _plain_eager(slots, *cache):
+        return read_launch(cache, slots, dtype, tensor_layout)
+    return ops.cache_read(*cache, slots, dtype, tensor_layout)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B, H, Hkv, T, D, page_size, max_pages):
+    return _capi.cache_attn_workspace(B, H, Hkv, T, D, page_size, max_pages)
+
+
+def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal, tree_mask, return_lse):
+    """Output (B, T, H, D) contiguous in q's dtype, and the logsumexp [B, H, T] or None."""
+    if layout not in ("HND", "NHD"):
+        raise Unsupported(f"layout {layout!r}")
+    if q.dim() != 4:
+        raise Unsupported("4D q required")
+    if q.dtype not in DTYPES:
+        raise Unsupported(f"dtype {q.dtype} (fp16 or bf16 required)")
+    dev = q.device
+    pages, Hkv, page_size, D = check_cache(cache, dev)
+    B, T, H, d = _sizes(q, layout)
+    if d != D or H % Hkv:
+        raise Unsupported(f"{H} heads of {d} channels for a cache of {Hkv} heads of {D}")
+    if block_table.dim() != 2 or block_table.shape[0] != B or lengths.dim() != 1 or lengths.shape[0] != B:
+        raise Unsupported("block_table [B, max_pages] and lengths [B] required")
+    if block_table.dtype not in (torch.int32, torch.int64) or lengths.dtype not in (torch.int32, torch.int64):
+        raise Unsupported("block_table and lengths must be int32 or int64")
+    if block_table.device != dev or lengths.device != dev:
+        raise Unsupported("tensors must be on one ROCm GPU")
+    mask, ms = None, (0, 0, 0)
+    if tree_mask is not None:
+        if not is_causal:
+            raise Unsupported("tree_mask stands in the place of the causal rule: is_causal=False has none")
+        if tree_mask.dtype != torch.bool or tree_mask.device != dev:
+            raise Unsupported("tree_mask must be a bool tensor on q's device")
+        if tuple(tree_mask.shape) not in ((T, T), (1, T, T), (B, T, T)):
+            raise Unsupported(f"tree_mask of shape {tuple(tree_mask.shape)} for batch {B} and {T} new tokens")
+        mask = tree_mask.expand(B, T, T)
+        ms = mask.stride()
+    out = torch.empty((B, T, H, D), device=dev, dtype=q.dtype)
+    lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
+    max_pages = block_table.shape[1]
+    if q.numel() == 0 or max_pages == 0:   # no query rows, or no keys
+        return out.zero_(), None if lse is None else lse.fill_(float("-inf"))
+    if q.numel() > _I32_MAX:
+        raise Unsupported("tensor too large for 32-bit indexing")
+    q, sq = _bsh(q, layout)
+    table = block_table.to(torch.int32)
+    if table.stride(1) != 1 and max_pages > 1:
+        table = table.contiguous()
+    lengths = lengths.to(torch.int32).contiguous()
+    ws_bytes = _workspace(B, H, Hkv, T, D, page_size, max_pages)
+    ws = torch.empty((ws_bytes,), device=dev, dtype=torch.uint8) if ws_bytes else None
+    _capi.call_on(dev, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), *out.stride()[:3],
+                  None if lse is None else lse.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+                  cache.v.data_ptr(), cache.v_scale.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                  None if mask is None else mask.data_ptr(), *ms, B, H, Hkv, T, D, DTYPES[q.dtype],
+                  CACHE_DTYPES[cache.k.dtype], pages, page_size, max_pages, int(bool(is_causal)), float(sm_scale),
+                  None if ws is None else ws.data_ptr(), ws_bytes)
+    return out, lse
+
+
+def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scale=None, is_causal=True, tree_mask=None,
+                    return_lse=False):
+    """Attention of the T new tokens of every sequence over the cache: q [B, H, T, D] ("HND") or [B, T, H, D] ("NHD"), H a
+    multiple of the cache's kv heads.  lengths [B]: the cached keys of each sequence, the T new tokens' (already
+    written, the last T of them) counted; block_table [B, max_pages]: key j is row j % page_size of page
+    block_table[b, j // page_size], and a page outside the cache (-1) hides its keys.  A query sees every key before the new
+    ones and, of those, its own and the earlier ones (is_causal), all (is_causal=False), or those its row of tree_mask
+    shows: bool [T, T] or [B, T, T], True at (i, j) where new token i sees new token j (a tree of drafted tokens: its
+    ancestors and itself).  A query that sees no key gives 0 (lengths[b] = 0, say).  Returns the output in q's layout and
+    dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  sm_scale: None or a
+    non-positive one stands for 1 / sqrt(D).  Raises Unsupported for what the kernel does not take."""
+    sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
+    ts = [t for t in (q, *cache, block_table, lengths, tree_mask) if t is not None]
+    lse = None
+    if _plain_eager(*ts):
+        out, lse = attention_launch(q, cache, block_table, lengths, tensor_layout, sm, is_causal, tree_mask, return_lse)
+    elif return_lse:
+        out, lse = ops.cache_attention_lse(q, *cache, block_table, lengths, tree_mask, tensor_layout, sm, bool(is_causal))
+    else:
+        out = ops.cache_attention(q, *cache, block_table, lengths, tree_mask, tensor_layout, sm, bool(is_causal))
+    out = out.transpose(1, 2) if tensor_layout == "HND" else out
+    return (out, lse) if return_lse else out
+
+
+def cache_step(q, k, v, cache, slots, block_table, lengths, positions=None, freqs=None, tensor_layout="HND",
+               interleaved=False, factor=1.0, sm_scale=None, tree_mask=None):
+    """One decoding step of an attention layer: turns q and k by their positions (rope; where freqs is None they are
+    taken as they are), writes k and v into the cache (cache_write) and attends over it (cache_attention).  lengths
+    count the new tokens; positions: int [T] or [B, T], by default the tokens' places in their sequence (those of drafted
+    tokens follow from their depth in the tree)."""
+    if freqs is not None:
+        if positions is None:
+            T = q.shape[2] if tensor_layout == "HND" else q.shape[1]
+            positions = lengths[:, None] - T + torch.arange(T, device=lengths.device, dtype=lengths.dtype)
+        q, k = rope(q, k, positions, freqs, tensor_layout, interleaved, factor)
+    cache_write(cache, k, v, slots, tensor_layout)
+    return cache_attention(q, cache, block_table, lengths, tensor_layout, sm_scale, True, tree_mask)

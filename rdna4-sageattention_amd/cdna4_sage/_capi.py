@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libsage_capi.so"
 
 SAGE_OK, SAGE_ERR_INVALID, SAGE_ERR_UNSUPPORTED, SAGE_ERR_HIP = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F16, DTYPE_BOOL = 0, 1, 2
+CACHE_INT8, CACHE_E4M3 = 0, 1
 ABI_VERSION = 6
 
 _lib = None
@@ -56,6 +57,13 @@ SIGNATURES = {
                              _P, _P, _P, _P, _P, _P, _P, _L, _P], _I),
     "sage_forward_noalloc": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L,
                               _I, _I, _I, _I, _I, _I, _I, _I, _F, _P], _I),
+    "sage_rope": ([_P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, _I, _P, _I, _L, _L,
+                   _P, _I, _I, _F, _I, _P], _I),
+    "sage_cache_write": ([_P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "sage_cache_read": ([_P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "sage_cache_attn_workspace": ([_I, _I, _I, _I, _I, _I, _I, _P], _I),
+    "sage_cache_attn": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _L, _P, _P, _L, _L, _L,
+                         _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P], _I),
 }
 
 
@@ -91,6 +99,17 @@ def call(name: str, *args) -> None:
     rc = getattr(lib(), name)(*args)
     if rc != SAGE_OK:
         raise SageError(name, rc, lib().sage_last_error().decode(errors="replace"))
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call with the current stream of `device` as the last argument, that device current."""
+    cur = torch.cuda.current_device()
+    di = cur if device.index is None else device.index
+    if di == cur:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(di))
+    else:
+        with torch.cuda.device(di):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(di))
 
 
 def kv_pad(skv: int) -> int:
@@ -138,3 +157,10 @@ def varlen_layout(batch: int, H: int, Hkv: int, total_q: int, total_k: int):
     rows, ws = ctypes.c_int(), ctypes.c_int64()
     call("sage_varlen_layout", batch, H, Hkv, total_q, total_k, ctypes.byref(rows), ctypes.byref(ws))
     return rows.value, ws.value
+
+
+def cache_attn_workspace(B: int, H: int, Hkv: int, T: int, D: int, page_size: int, max_pages: int) -> int:
+    """Workspace bytes of sage_cache_attn (host arithmetic only)."""
+    ws = ctypes.c_int64()
+    call("sage_cache_attn_workspace", B, H, Hkv, T, D, page_size, max_pages, ctypes.byref(ws))
+    return ws.value

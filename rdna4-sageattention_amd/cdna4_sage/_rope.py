@@ -1,0 +1,180 @@
+"""Rotary positions on the gfx950 kernel (no counterpart in the reference, whose callers rotate q and k with torch).
+
+One launch turns q and k; gradients turn back by the same kernel.  Frequencies are float64 tensors made once per model by
+rope_frequencies, so that positions of 10^6 and more keep their angle.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _capi, ops
+from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, device_arch
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, device=None):
+    """(freqs, factor) for rope: radians per position of the rot_dim / 2 channel pairs, float64 on `device`, and the
+    factor of the rotated channels.  freqs[i] = base^(-2 i / rot_dim).  scaling, for contexts longer than the one a model
+    was trained on, is None or a dict:
+
+    {"type": "linear", "factor": s}: positions interpolated, every frequency divided by s.
+    {"type": "ntk", "factor": s}: the base raised to base * s^(rot_dim / (rot_dim - 2)), which divides the slowest
+        frequency by s and leaves the fastest.
+    {"type": "yarn", "factor": s, "original_length": n, "slow": 1, "fast": 32, "attention_factor": None}: pairs that turn
+        less than `slow` times over n positions divided by s, those of more than `fast` turns kept, linear in the pair's
+        index in between; the rotated channels times attention_factor (0.1 ln s + 1 where None)."""
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim} (positive and even)")
+    if not base > 0:
+        raise ValueError(f"base {base}")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    factor = 1.0
+    if scaling is None:
+        f = base ** (-2.0 * i / rot_dim)
+    else:
+        kind, s = scaling.get("type"), float(scaling.get("factor", 0.0))
+        if not s >= 1.0:
+            raise ValueError(f"scaling factor {s} (at least 1)")
+        if kind == "linear":
+            f = base ** (-2.0 * i / rot_dim) / s
+        elif kind == "ntk":
+            if rot_dim == 2:
+                raise ValueError("ntk scaling needs rot_dim > 2")
+            f = (base * s ** (rot_dim / (rot_dim - 2))) ** (-2.0 * i / rot_dim)
+        elif kind == "yarn":
+            n, slow, fast = (float(scaling[x]) if x in scaling else d for x, d in
+                             (("original_length", 0.0), ("slow", 1.0), ("fast", 32.0)))
+            if not n > 0 or not fast > slow > 0:
+                raise ValueError("yarn scaling needs original_length > 0 and fast > slow > 0")
+            # the (fractional) index of the pair that turns t times over n positions
+            at = [rot_dim * math.log(n / (2.0 * math.pi * t)) / (2.0 * math.log(base)) for t in (fast, slow)]
+            lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rot_dim - 1)
+            ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+            f = base ** (-2.0 * i / rot_dim)
+            f = f * (1.0 - ramp) + f / s * ramp
+            factor = scaling.get("attention_factor")
+            factor = 0.1 * math.log(s) + 1.0 if factor is None else float(factor)
+        else:
+            raise ValueError(f"scaling type {kind!r} ('linear', 'ntk' or 'yarn')")
+    return f.to(device=device), factor
+
+
+def _sizes(x, layout):
+    """(batch, tokens, heads, head_dim)"""
+    return (x.shape[0], x.shape[2], x.shape[1], x.shape[3]) if layout == "HND" else tuple(x.shape)
+
+
+def check_rope(q, k, positions, freqs, layout):
+    if layout not in ("HND", "NHD"):
+        raise Unsupported(f"layout {layout!r}")
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise Unsupported("4D tensors required")
+    if q.dtype not in DTYPES or (k is not None and k.dtype != q.dtype):
+        raise Unsupported(f"dtype {q.dtype} (fp16 or bf16 required, the same for q and k)")
+    B, S, _, D = _sizes(q, layout)
+    if D not in HEAD_DIMS:
+        raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
+    if k is not None and _sizes(k, layout)[::3] + _sizes(k, layout)[1:2] != (B, D, S):
+        raise Unsupported("q and k must have the same batch, length and head_dim")
+    if freqs.dim() != 1 or freqs.dtype != torch.float64:
+        raise Unsupported("freqs must be a 1D float64 tensor (rope_frequencies)")
+    rot = 2 * freqs.numel()
+    if rot == 0 or rot > D or rot % 8:
+        raise Unsupported(f"{rot} rotated channels (a positive multiple of 8 up to head_dim {D})")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise Unsupported(f"positions {positions.dtype} (int32 or int64)")
+        if tuple(positions.shape) not in ((S,), (1, S), (B, S)):
+            raise Unsupported(f"positions of shape {tuple(positions.shape)} for batch {B} and length {S}")
+    for t in (q, k, positions, freqs):
+        if t is not None and not (t.is_cuda and t.device == q.device):
+            raise Unsupported("tensors must be on one ROCm GPU")
+    if device_arch(q.device) not in ARCHS:
+        raise Unsupported("not a CDNA4 GPU")
+    if max(q.numel(), 0 if k is None else k.numel()) > _I32_MAX:
+        raise Unsupported("tensor too large for 32-bit indexing")
+
+
+def rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse):
+    """The rotated q (and k), in new tensors of the inputs' memory order."""
+    check_rope(q, k, positions, freqs, layout)
+    B, S, H, D = _sizes(q, layout)
+    oq = torch.empty_like(q)
+    ok = None if k is None else torch.empty_like(k)
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return oq, ok
+    if q.numel() == 0:   # no query heads: k alone
+        return oq, rope_launch(k, None, positions, freqs, layout, interleaved, factor, inverse)[0]
+    Hk = 0 if k is None else _sizes(k, layout)[2]
+    q, sq = _bsh(q, layout)
+    oq, so = _out_bsh(oq, layout)
+    args = [q.data_ptr(), *sq, oq.data_ptr(), *so, H]
+    if Hk:
+        k, sk = _bsh(k, layout)
+        ok, so = _out_bsh(ok, layout)
+        args += [k.data_ptr(), *sk, ok.data_ptr(), *so, Hk]
+    else:
+        args += [None, 0, 0, 0, None, 0, 0, 0, 0]
+    pos, p64, pb, ps = None, 0, 0, 0
+    if positions is not None:
+        p64, ps = int(positions.dtype == torch.int64), positions.stride(-1)
+        pb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+        pos = positions.data_ptr()
+    freqs = freqs.contiguous()
+    args += [B, S, D, DTYPES[q.dtype], pos, p64, pb, ps, freqs.data_ptr(), 2 * freqs.numel(), int(bool(interleaved)),
+             float(factor), int(bool(inverse))]
+    _capi.call_on(q.device, "sage_rope", *args)
+    return oq, ok
+
+
+def _out_bsh(t, layout):
+    """(b, s, h) strides of an output; one that the kernel cannot store 16-byte vectors into is made contiguous."""
+    s = t.stride()
+    if s[3] != 1 or t.data_ptr() % 16 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        s = t.stride()
+    return t, ((s[0], s[2], s[1]) if layout == "HND" else s[:3])
+
+
+class _Rope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, layout, interleaved, factor, inverse):
+        ctx.save_for_backward(positions, freqs)
+        ctx.how = layout, interleaved, factor, inverse
+        return rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, freqs = ctx.saved_tensors
+        layout, interleaved, factor, inverse = ctx.how
+        need_q, need_k = ctx.needs_input_grad[:2]
+        back = (positions, freqs, layout, interleaved, factor, not inverse)
+        if need_q and need_k:
+            dq, dk = _Rope.apply(dq, dk, *back)
+        elif need_q:
+            dq, dk = _Rope.apply(dq, None, *back)[0], None
+        else:
+            dq, dk = None, _Rope.apply(dk, None, *back)[0] if need_k else None
+        return dq, dk, None, None, None, None, None, None
+
+
+def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved=False, factor=1.0):
+    """Rotary positions: the first 2 * freqs.numel() channels of every head are pairs, (i, i + rot_dim / 2) or, interleaved,
+    (2 i, 2 i + 1), and pair i of a token at position p turns by p * freqs[i] radians, times `factor`; the other
+    channels are copied.  q: [B, heads, tokens, head_dim] for "HND", [B, tokens, heads, head_dim] for "NHD", k alike with
+    heads of its own, bf16 or fp16.  positions: int32 / int64 [tokens] or [B, tokens] (None: 0, 1, ..).  freqs, factor:
+    rope_frequencies.  Returns q, or (q, k), in new tensors.  Differentiable in q and k (to any order); float32
+    arithmetic, rounded once.  Raises Unsupported for what the kernel does not take."""
+    if freqs is None:
+        raise Unsupported("freqs are required (rope_frequencies)")
+    ts = (q,) if k is None else (q, k)
+    if _plain_eager(*ts):
+        out = rope_launch(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
+    elif _plain_eager(*ts, grad=True):
+        out = _Rope.apply(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
+    elif k is None:
+        return ops.rope(q, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
+    else:
+        return ops.rope_qk(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
+    return out[0] if k is None else tuple(out)

@@ -1,0 +1,576 @@
+// Attention of new queries over the quantized, paged key / value cache (layouts: sage_cache.hip).
+//
+// Per sequence b with n_b cached keys, the T queries of one step are the last T of them: query i of head h attends the
+// keys below n_b - T, and of the T new ones those up to its own (causal), those its row of the tree mask shows, or all.
+// o_i = sum_j p_ij s^v_j V_j, p_ij = 2^(x_ij - m_i) / l_i, x_ij = (q_i . K_j) s^k_j c log2 e, over codes K_j, V_j with
+// scales s^k_j, s^v_j.
+//
+// Mapping.  The T * G queries that share a kv head (G = H / Hkv) are the rows of a matrix; a workgroup takes 16 RT of
+// them against a range of the keys, and its 4 waves take turns over tiles of 32 keys.  Codes go straight from memory to
+// registers (every byte is used once, by one wave), and become float16 there: int8 and E4M3 codes are exact in float16,
+// so both products run on v_mfma_f32_16x16x32_f16 with float32 accumulation.
+//  * S^T = K Q^T: A = 16 keys x 32 channels.  Lane (m = l % 16, g = l / 16) loads the D/4 channels from g D/4 on of key
+//    m, and MFMA i takes 8 of them from each g: any order of the channels will do that Q's operand has too.
+//  * The accumulator gives lane (n, g) query n and keys 4g .. 4g + 3 of each 16: with the two 16-key blocks of a tile
+//    that is, packed to float16, the B operand of O^T = V^T P^T for the key order k = 8g + 4t + i <-> key 16t + 4g + i.
+//    V's operand takes that order too: lane (m, g) loads D/16 channels of each of those 8 keys, pairs of keys are
+//    brought together by byte permutes.  Nothing crosses lanes but the row maxima, and nothing passes through LDS.
+//  * Q rows in bfloat16 are brought into float16's range by a power of two per row, which keeps all their bits.
+//  * P in float16 holds 11 bits of p_ij s^v_j: two running references per row, m (of x) for the sum l and m2 (of
+//    x + log2 s^v) for P, each raised only when a tile passes it by 2^8.  The largest product so far lies between 2^6 and
+//    2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an error of 2^-31 of it below.
+// Bound: HBM.  A key costs 2 D + 8 bytes per kv head whatever T and G are.
+#include "sage_cache.h"
+
+namespace sage {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int CA_WAVES = 4;
+constexpr int CA_THREADS = 64 * CA_WAVES;
+constexpr int CA_TILE = 32;                      // keys per wave and step
+constexpr int CA_STEP = CA_TILE * CA_WAVES;      // keys per workgroup and step
+constexpr float CA_SLACK = 8.0f;                 // log2 by which scores may pass their reference
+
+struct CacheAttnArgs {
+  const uint16_t* q;
+  int64_t qsb, qss, qsh;
+  uint16_t* out;
+  int64_t osb, oss, osh;
+  float* lse;                       // [B, H, T] or NULL
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  const int* table;                 // [B] rows of max_pages entries, `tsb` apart
+  const int* lengths;
+  const uint8_t* tree;              // (b, i, j) at b * msb + i * msq + j * msk, or NULL
+  int64_t tsb, msb, msq, msk;
+  int B, H, Hkv, G, T, dtype, causal;
+  int pages, page_size, page_shift, max_pages;
+  int row_blocks, splits;
+  float scale;                      // softmax scale * log2 e
+  float* part_o;                    // [unit][splits][16 RT][D], units = (b, kv head, row block)
+  float* part_lse;                  // [unit][splits][16 RT], log2
+};
+
+template <int BYTES> struct RawBytes { uint32_t w[(BYTES + 3) / 4]; };
+
+__device__ __forceinline__ v4i ld16(const uint8_t* p) { return *reinterpret_cast<const v4i*>(p); }
+__device__ __forceinline__ v2i ld8(const uint8_t* p) { return *reinterpret_cast<const v2i*>(p); }
+
+// bytes 0, 1 (half 0) or 2, 3 (half 1) of a word of codes as two float16; int8 codes come with their sign bit flipped
+template <int CT> __device__ __forceinline__ f16x2 codes_f16(uint32_t w, bool half) {
+  if constexpr (CT == CACHE_INT8) {
+    // 0x64uu is 1024 + uu in float16
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, half ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(f16x2, u) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+  } else {
+    return half ? __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true))
+                : __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false));
+  }
+}
+
+__device__ __forceinline__ f16x8 join4(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// maximum / sum over the 4 lanes (n, 0..3) of a row, in all of them
+__device__ __forceinline__ float row4_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max_xor32_f32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float row4_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return add_xor32_f32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// channel of accumulator (m, tile ct): the lane's D/16 loaded channels in order (96: a word, then two bytes)
+template <int D> __device__ __forceinline__ constexpr int v_channel(int m, int ct) {
+  return D == 96 ? (ct < 4 ? 4 * m + ct : 64 + 2 * m + ct - 4) : m * (D / 16) + ct;
+}
+
+template <int D> struct CacheTile {
+  static constexpr int KW = D / 16, VW = D == 96 ? 2 : D / 64;  // words per lane: of K per 16 keys, of V per key
+  uint32_t k[2][KW];
+  uint32_t v[8][VW];
+  v4f ks[2], vs[2];
+};
+
+template <int D, int CT, int RT>
+__global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnArgs a) {
+  constexpr int NK = D / 32, NC = D / 16;
+  constexpr int ROWS = 16 * RT;
+  constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
+  __shared__ __attribute__((aligned(16))) float so[CA_WAVES][16][LD];
+  __shared__ float sm[CA_WAVES][ROWS], sm2[CA_WAVES][ROWS], sl[CA_WAVES][ROWS];
+
+  // the row blocks of one range of keys on one XCD, next to each other
+  const int id = blockIdx.x;
+  const int grp = id / (8 * a.row_blocks) * 8 + id % 8, rb = id / 8 % a.row_blocks;
+  const int pairs = a.B * a.Hkv;
+  if (grp >= pairs * a.splits) return;
+  const int pair = grp / a.splits, split = grp % a.splits;
+  const int b = pair / a.Hkv, h = pair % a.Hkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int rows = a.T * a.G;
+  const int64_t unit = ((int64_t)pair * a.row_blocks + rb) * a.splits + split;
+
+  const int len = min(max(a.lengths[b], 0), (int)min((int64_t)a.max_pages * a.page_size, (int64_t)0x7FFFFFFF));
+  const int base = len - a.T;  // key of the first new token
+  // keys below `open` are seen by every row
+  const int open = a.tree ? base : a.causal ? base + 1 : len;
+  const int per = ((len + a.splits - 1) / a.splits + CA_STEP - 1) / CA_STEP * CA_STEP;
+  const int k_begin = min((int64_t)split * per, (int64_t)len), k_end = min((int64_t)k_begin + per, (int64_t)len);
+
+  // Q operand and the rows' factors
+  f16x8 qf[RT][NK];
+  float qs[RT];
+  int row_t[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rb * ROWS + rt * 16 + n;
+    const int rr = min(r, rows - 1);
+    const int t = rr / a.G, hq = h * a.G + rr % a.G;
+    row_t[rt] = t;
+    const uint16_t* qp = a.q + b * a.qsb + t * a.qss + hq * a.qsh + g * (D / 4);
+    uint32_t w[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const v4i x = *reinterpret_cast<const v4i*>(qp + 8 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = (uint32_t)x[j];
+    }
+    qs[rt] = a.scale;
+    if (a.dtype == DT_BF16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
+      const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
+      // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
+      const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
+      const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
+      qs[rt] *= down;
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qf[rt][i][2 * j] = (_Float16)(bf16_lo(w[4 * i + j]) * up);
+          qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
+    }
+  }
+
+  float m[RT], m2[RT], f[RT], l[RT];
+  v4f acc[RT][NC];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = m2[rt] = -__builtin_inff();
+    f[rt] = 0.0f;
+    l[rt] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[rt][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const int* table = a.table + b * a.tsb;
+  // a page outside the cache hides its keys: page 0 is read in its place
+  auto page_of = [&](int key) { return table[min(key >> a.page_shift, a.max_pages - 1)]; };
+  auto usable = [&](int page) { return page >= 0 && page < a.pages; };
+  auto load = [&](CacheTile<D>& x, int k0, int p0, int p1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int p = t ? p1 : p0;
+      const int64_t row = ((int64_t)(usable(p) ? p : 0) * a.Hkv + h) * a.page_size + ((k0 + 16 * t) & (a.page_size - 1));
+      const uint8_t* kp = a.k8 + row * D + n * D + g * (D / 4);
+      if constexpr (D == 96) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const v2i w = ld8(kp + 8 * i);
+          x.k[t][2 * i] = w[0], x.k[t][2 * i + 1] = w[1];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const v4i w = ld16(kp + 16 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = (uint32_t)w[j];
+        }
+      }
+      x.ks[t] = *reinterpret_cast<const v4f*>(a.ks + row + 4 * g);
+      x.vs[t] = *reinterpret_cast<const v4f*>(a.vs + row + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* vp = a.v8 + (row + 4 * g + i) * D;
+        uint32_t* w = x.v[4 * t + i];
+        if constexpr (D == 64) {
+          w[0] = *reinterpret_cast<const uint32_t*>(vp + 4 * n);
+        } else if constexpr (D == 96) {
+          w[0] = *reinterpret_cast<const uint32_t*>(vp + 4 * n);
+          w[1] = *reinterpret_cast<const uint16_t*>(vp + 64 + 2 * n);
+        } else if constexpr (D == 128) {
+          const v2i y = ld8(vp + 8 * n);
+          w[0] = y[0], w[1] = y[1];
+        } else {
+          const v4i y = ld16(vp + 16 * n);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = (uint32_t)y[j];
+        }
+      }
+    }
+  };
+
+  auto compute = [&](CacheTile<D>& x, int k0, int p0, int p1) {
+    const bool masked = k0 + CA_TILE > open || !usable(p0) || !usable(p1);
+    v4f s[RT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        uint32_t w0 = x.k[t][2 * i], w1 = x.k[t][2 * i + 1];
+        if (CT == CACHE_INT8) w0 ^= 0x80808080u, w1 ^= 0x80808080u;
+        const f16x8 ka = join4(codes_f16<CT>(w0, false), codes_f16<CT>(w0, true), codes_f16<CT>(w1, false),
+                               codes_f16<CT>(w1, true));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
+      }
+    }
+    uint32_t hidden[RT];  // bit 4 t + i
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) hidden[rt] = 0;
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = j / 4, key = k0 + 16 * t + 4 * g + j % 4, node = key - base;
+        const bool none = key >= len || !usable(t ? p1 : p0);
+        if (none) {  // whatever the memory past a sequence holds: no NaN enters the products
+#pragma unroll
+          for (int i = 0; i < CacheTile<D>::VW; ++i) x.v[j][i] = CT == CACHE_INT8 ? 0x80808080u : 0u;
+          x.vs[t][j % 4] = 0.0f;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          bool hide = none;
+          if (!none && node >= 0) {
+            if (a.tree) hide = a.tree[b * a.msb + row_t[rt] * a.msq + node * a.msk] == 0;
+            else if (a.causal) hide = node > row_t[rt];
+          }
+          hidden[rt] |= (uint32_t)hide << j;
+        }
+      }
+    }
+    f16x8 pf[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float y[8], p[8], pv[8];
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y[j] = s[rt][j / 4][j % 4] * (x.ks[j / 4][j % 4] * qs[rt]);
+        if (masked && (hidden[rt] >> j & 1)) y[j] = -__builtin_inff();
+        top = fmaxf(top, y[j]);
+      }
+      if (__any(top > m[rt] + CA_SLACK)) {
+        const float now = fmaxf(m[rt], row4_max(top));
+        if (now > m[rt]) {
+          l[rt] *= __builtin_amdgcn_exp2f(m[rt] - now);
+          m[rt] = now;
+          f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(m[rt] - m2[rt], 100.0f));
+        }
+      }
+      const float ref = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
+      float pvmax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(y[j] - ref);
+        l[rt] += p[j];
+        pv[j] = p[j] * x.vs[j / 4][j % 4];
+        if (masked && (hidden[rt] >> j & 1)) pv[j] = 0.0f;
+        pvmax = fmaxf(pvmax, pv[j]);
+      }
+      if (__any(pvmax * f[rt] > 0x1p15f || (f[rt] == 0.0f && pvmax > 0.0f))) {
+        const float row = row4_max(pvmax);
+        if (row > 0.0f && row < __builtin_inff()) {
+          const float now = fmaxf(m2[rt], m[rt] + (float)(__builtin_amdgcn_frexp_expf(row) - 7));
+          const float down = __builtin_amdgcn_exp2f(m2[rt] - now);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) acc[rt][c] *= down;
+          m2[rt] = now;
+          f[rt] = __builtin_amdgcn_exp2f(fminf(m[rt] - now, 100.0f));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
+    }
+    // V operand: keys (0, 1), (2, 3) of each block side by side
+#pragma unroll
+    for (int i = 0; i < CacheTile<D>::VW; ++i) {
+      if (CT == CACHE_INT8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.v[j][i] ^= 0x80808080u;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {  // channels 4 i + 2 u, + 1 of the lane
+        if (D == 96 && i == 1 && u == 1) continue;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // bytes (A_2u, B_2u, A_2u+1, B_2u+1)
+          w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i], x.v[2 * j][i], u ? 0x07030602u : 0x05010400u);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int c = 4 * i + 2 * u + o;
+          const f16x8 va = join4(codes_f16<CT>(w[0], o), codes_f16<CT>(w[1], o), codes_f16<CT>(w[2], o), codes_f16<CT>(w[3], o));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], acc[rt][c], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  // two tiles in registers: one is loaded while the other is used
+  int k0 = k_begin + wave * CA_TILE;
+  if (k0 < k_end) {
+    CacheTile<D> x[2];
+    int p[2][2];
+    p[0][0] = page_of(k0), p[0][1] = page_of(k0 + 16);
+    load(x[0], k0, p[0][0], p[0][1]);
+    for (;;) {
+      const int k1 = k0 + CA_STEP;
+      if (k1 < k_end) {
+        p[1][0] = page_of(k1), p[1][1] = page_of(k1 + 16);
+        load(x[1], k1, p[1][0], p[1][1]);
+      }
+      compute(x[0], k0, p[0][0], p[0][1]);
+      if (k1 >= k_end) break;
+      k0 = k1 + CA_STEP;
+      if (k0 < k_end) {
+        p[0][0] = page_of(k0), p[0][1] = page_of(k0 + 16);
+        load(x[0], k0, p[0][0], p[0][1]);
+      }
+      compute(x[1], k1, p[1][0], p[1][1]);
+      if (k0 >= k_end) break;
+    }
+  }
+
+  // join the waves, 16 rows at a time
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = row4_sum(l[rt]);
+    if (g == 0) {
+      sm[wave][rt * 16 + n] = m[rt];
+      sm2[wave][rt * 16 + n] = m2[rt];
+      sl[wave][rt * 16 + n] = l[rt];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rt * 16 + n;
+    float top2 = sm2[0][r];
+#pragma unroll
+    for (int w = 1; w < CA_WAVES; ++w) top2 = fmaxf(top2, sm2[w][r]);
+    const float down = m2[rt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m2[rt] - top2);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) so[wave][n][v_channel<D>(4 * g + i, c)] = acc[rt][c][i] * down;
+    __syncthreads();
+    // 16 threads per row
+    const int row = threadIdx.x / 16, part = threadIdx.x % 16, rr = rt * 16 + row, R = rb * ROWS + rr;
+    float M = sm[0][rr], M2 = sm2[0][rr];
+#pragma unroll
+    for (int w = 1; w < CA_WAVES; ++w) M = fmaxf(M, sm[w][rr]), M2 = fmaxf(M2, sm2[w][rr]);
+    float L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < CA_WAVES; ++w)  // (a NaN sum stays one)
+      L += sm[w][rr] == -__builtin_inff() ? sl[w][rr] : sl[w][rr] * __builtin_amdgcn_exp2f(sm[w][rr] - M);
+    // a row that sees no key: 0, logsumexp -inf
+    const float fin = L == 0.0f ? 0.0f : (M2 == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(M2 - M)) / L;
+    const float lse2 = L == 0.0f ? -__builtin_inff() : M + __builtin_log2f(L);
+    constexpr int PER = D / 16;
+    float o[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      float v = so[0][row][part * PER + i];
+#pragma unroll
+      for (int w = 1; w < CA_WAVES; ++w) v += so[w][row][part * PER + i];
+      o[i] = L == 0.0f ? 0.0f : v * fin;
+    }
+    if (R < rows) {
+      if (a.splits == 1) {
+        const int t = R / a.G, hq = h * a.G + R % a.G;
+        uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + part * PER;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) {
+          const uint32_t w = a.dtype == DT_BF16 ? f32_to_bf16_bits(o[i]) | (f32_to_bf16_bits(o[i + 1]) << 16)
+                                                : f32_to_f16_bits(o[i]) | (f32_to_f16_bits(o[i + 1]) << 16);
+          *reinterpret_cast<uint32_t*>(op + i) = w;
+        }
+        if (a.lse && part == 0) a.lse[((int64_t)b * a.H + hq) * a.T + t] = lse2 * 0.69314718055994530942f;
+      } else {
+        float* op = a.part_o + (unit * ROWS + rr) * D + part * PER;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(op + i) = make_float2(o[i], o[i + 1]);
+        if (part == 0) a.part_lse[unit * ROWS + rr] = lse2;
+      }
+    }
+    if (rt + 1 < RT) __syncthreads();
+  }
+}
+
+// Joins the ranges of keys of a row: o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M), in their order.
+template <int D> __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnArgs a, int block_rows) {
+  constexpr int LPR = D / 4;  // threads per row, 4 channels each
+  const int64_t rows = (int64_t)a.T * a.G;
+  const int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (threadIdx.x >= 256 / LPR * LPR || at >= rows * a.B * a.Hkv) return;
+  const int c = threadIdx.x % LPR * 4;
+  const int pair = (int)(at / rows), R = (int)(at - pair * rows);
+  const int b = pair / a.Hkv, h = pair % a.Hkv;
+  const int64_t unit = ((int64_t)pair * a.row_blocks + R / block_rows) * a.splits;
+  const int rr = R % block_rows;
+  float M = -__builtin_inff();
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_lse[(unit + s) * block_rows + rr]);
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float L = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float x = a.part_lse[(unit + s) * block_rows + rr];
+    if (x == -__builtin_inff()) continue;  // a range without a visible key
+    const float w = __builtin_amdgcn_exp2f(x - M);
+    L += w;
+    o += *reinterpret_cast<const v4f*>(a.part_o + ((unit + s) * block_rows + rr) * D + c) * w;
+  }
+  if (L != 0.0f) o *= 1.0f / L;
+  const int t = R / a.G, hq = h * a.G + R % a.G;
+  uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + c;
+  v2i w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = (int)(a.dtype == DT_BF16 ? f32_to_bf16_bits(o[2 * i]) | (f32_to_bf16_bits(o[2 * i + 1]) << 16)
+                                    : f32_to_f16_bits(o[2 * i]) | (f32_to_f16_bits(o[2 * i + 1]) << 16));
+  *reinterpret_cast<v2i*>(op) = w;
+  if (a.lse && c == 0)
+    a.lse[((int64_t)b * a.H + hq) * a.T + t] = L == 0.0f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.69314718055994530942f;
+}
+
+// Rows per workgroup (16 RT) and ranges of keys for a call.
+struct CachePlan {
+  int rt, row_blocks, splits;
+  int64_t o_bytes, bytes;
+};
+
+static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys) {
+  CachePlan p;
+  const int64_t rows = (int64_t)T * (H / Hkv);
+  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
+  p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
+  const int64_t units = (int64_t)B * Hkv * p.row_blocks;
+  const int64_t most = (max_keys + CA_STEP - 1) / CA_STEP;
+  const int64_t want = (512 + units - 1) / units;
+  p.splits = (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+  if (p.splits > 128) p.splits = 128;
+  const int64_t n = p.splits == 1 ? 0 : units * p.splits * 16 * p.rt;
+  p.o_bytes = (n * D * 4 + 255) / 256 * 256;
+  p.bytes = p.o_bytes + n * 4;
+  return p;
+}
+
+template <int D, int CT> static void cache_attn_launch(const CacheAttnArgs& a, int rt, unsigned blocks, hipStream_t st) {
+  if (rt == 1) cache_attn_kernel<D, CT, 1><<<blocks, CA_THREADS, 0, st>>>(a);
+  else if (rt == 2) cache_attn_kernel<D, CT, 2><<<blocks, CA_THREADS, 0, st>>>(a);
+  else if constexpr (D < 256) cache_attn_kernel<D, CT, 4><<<blocks, CA_THREADS, 0, st>>>(a);
+}
+
+template <int D> static void cache_attn_dims(const CacheAttnArgs& a, int ct, int rt, unsigned blocks, hipStream_t st) {
+  if (ct == CACHE_INT8) cache_attn_launch<D, CACHE_INT8>(a, rt, blocks, st);
+  else cache_attn_launch<D, CACHE_E4M3>(a, rt, blocks, st);
+  if (a.splits > 1) {
+    constexpr int per = 256 / (D / 4);
+    const int64_t rows = (int64_t)a.T * a.G * a.B * a.Hkv;
+    cache_merge_kernel<D><<<(unsigned)((rows + per - 1) / per), 256, 0, st>>>(a, 16 * rt);
+  }
+}
+
+static int cache_attn_sizes(int B, int H, int Hkv, int T, int D, int page_size, int max_pages, const char* who) {
+  SAGE_REQUIRE(B > 0 && H > 0 && Hkv > 0 && T > 0 && max_pages > 0, "%s: sizes must be positive", who);
+  SAGE_REQUIRE(H % Hkv == 0, "%s: heads %d not a multiple of kv heads %d", who, H, Hkv);
+  if (!head_dim_ok(D)) return fail(SAGE_ERR_UNSUPPORTED, "%s: head_dim %d (supported 64, 96, 128, 256)", who, D);
+  if (!cache_page_ok(page_size))
+    return fail(SAGE_ERR_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 1024)", who, page_size);
+  // keys of a sequence and rows of all heads are counted in 32 bits, with room for a step past the end
+  SAGE_REQUIRE((int64_t)max_pages * page_size <= 0x40000000, "%s: more than 2^30 keys per sequence", who);
+  SAGE_REQUIRE((int64_t)B * H * T <= 0x01000000ll * 16, "%s: more than 2^28 query rows", who);
+  return SAGE_OK;
+}
+
+}  // namespace sage
+
+extern "C" {
+
+int sage_cache_attn_workspace(int B, int H, int Hkv, int T, int D, int page_size, int max_pages,
+                              int64_t* workspace_bytes) {
+  using namespace sage;
+  clear_error();
+  SAGE_REQUIRE(workspace_bytes != nullptr, "sage_cache_attn_workspace: workspace_bytes is NULL");
+  const int rc = cache_attn_sizes(B, H, Hkv, T, D, page_size, max_pages, "sage_cache_attn_workspace");
+  if (rc) return rc;
+  *workspace_bytes = cache_plan(B, H, Hkv, T, D, max_pages * page_size).bytes;
+  return SAGE_OK;
+}
+
+int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* out, int64_t osb, int64_t oss,
+                    int64_t osh, float* lse, const void* k8, const float* k_scale, const void* v8,
+                    const float* v_scale, const int* block_table, int64_t table_stride, const int* lengths,
+                    const void* tree_mask, int64_t msb, int64_t msq, int64_t msk, int B, int H, int Hkv, int T, int D,
+                    int dtype, int cache_dtype, int pages, int page_size, int max_pages, int causal, float sm_scale,
+                    void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace sage;
+  clear_error();
+  const char* who = "sage_cache_attn";
+  int rc = cache_check(k8, k_scale, v8, v_scale, pages, page_size, Hkv, D, cache_dtype, who);
+  if (rc) return rc;
+  if ((rc = cache_attn_sizes(B, H, Hkv, T, D, page_size, max_pages, who))) return rc;
+  SAGE_REQUIRE(q && out && block_table && lengths, "%s: q, out, block_table or lengths is NULL", who);
+  SAGE_REQUIRE(aligned16(q) && aligned16(out), "%s: q and out must be 16-byte aligned", who);
+  SAGE_REQUIRE(qsb % 8 == 0 && qss % 8 == 0 && qsh % 8 == 0 && osb % 8 == 0 && oss % 8 == 0 && osh % 8 == 0,
+               "%s: strides must be multiples of 8 elements", who);
+  SAGE_REQUIRE((((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)lse) & 3u) == 0,
+               "%s: block_table, lengths or lse misaligned", who);
+  if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale must be finite and not negative (got %g)",
+               who, (double)sm_scale);
+  const CachePlan p = cache_plan(B, H, Hkv, T, D, max_pages * page_size);
+  SAGE_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace & 255u) == 0 && workspace_bytes >= p.bytes),
+               "%s: workspace of %lld bytes (256-byte aligned), the plan needs %lld", who, (long long)workspace_bytes,
+               (long long)p.bytes);
+  CacheAttnArgs a = {};
+  a.q = (const uint16_t*)q, a.qsb = qsb, a.qss = qss, a.qsh = qsh;
+  a.out = (uint16_t*)out, a.osb = osb, a.oss = oss, a.osh = osh, a.lse = lse;
+  a.k8 = (const uint8_t*)k8, a.v8 = (const uint8_t*)v8, a.ks = k_scale, a.vs = v_scale;
+  a.table = block_table, a.tsb = table_stride, a.lengths = lengths;
+  a.tree = (const uint8_t*)tree_mask, a.msb = msb, a.msq = msq, a.msk = msk;
+  a.B = B, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.T = T, a.dtype = dtype, a.causal = causal;
+  a.pages = pages, a.page_size = page_size, a.max_pages = max_pages;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  a.row_blocks = p.row_blocks, a.splits = p.splits;
+  const double scale = sm_scale > 0.0f ? (double)sm_scale : 1.0 / __builtin_sqrt((double)D);
+  a.scale = (float)(scale * 1.44269504088896340736);
+  a.part_o = (float*)workspace;
+  a.part_lse = (float*)((char*)workspace + p.o_bytes);
+  const int64_t groups = ((int64_t)B * Hkv * p.splits + 7) / 8 * 8;
+  const int64_t blocks = groups * p.row_blocks;
+  SAGE_REQUIRE(blocks <= 0x7FFFFFFF, "%s: too many workgroups", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 64) cache_attn_dims<64>(a, cache_dtype, p.rt, (unsigned)blocks, st);
+  else if (D == 96) cache_attn_dims<96>(a, cache_dtype, p.rt, (unsigned)blocks, st);
+  else if (D == 128) cache_attn_dims<128>(a, cache_dtype, p.rt, (unsigned)blocks, st);
+  else cache_attn_dims<256>(a, cache_dtype, p.rt, (unsigned)blocks, st);
+  return check_launch(who);
+}
+
+}  // extern "C"
