@@ -43,15 +43,24 @@ def _plain_eager(*ts, grad=False) -> bool:
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
         return False
     if grad:
-        return all(type(t) in (torch.Tensor, torch.nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(t)
-                   and forward_ad.unpack_dual(t).tangent is None for t in ts)
+        if torch._C._functorch.peek_interpreter_stack() is not None:
+            return False
+        for t in ts:
+            if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+                return False
+            if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+                return False
+        return True
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
         return False
     return all(type(t) is torch.Tensor for t in ts)
 
 
 def device_arch(device: torch.device) -> str:
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+    return gpu_arch(device.index if device.index is not None else torch.cuda.current_device())
+
+
+def gpu_arch(idx: int) -> str:
     if idx not in _arch_cache:
         _arch_cache[idx] = torch.cuda.get_device_properties(idx).gcnArchName.split(":")[0]
     return _arch_cache[idx]

@@ -17,8 +17,8 @@ from typing import NamedTuple
 import torch
 
 from . import _capi, ops
-from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, device_arch
-from ._rope import _sizes, rope
+from ._attention import (_I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _packed, _plain_eager, gpu_arch)
+from ._rope import rope
 
 CACHE_DTYPES = {torch.int8: _capi.CACHE_INT8, torch.float8_e4m3fn: _capi.CACHE_E4M3}
 
@@ -53,16 +53,18 @@ def _check_page(page_size):
         raise Unsupported(f"page_size {page_size} (a power of two from 16 to 1024)")
 
 
-def check_cache(cache, device=None):
-    """(pages, kv_heads, page_size, head_dim) of a usable cache; raises Unsupported with the reason."""
+def check_cache(cache, gpu=None):
+    """(pages, kv_heads, page_size, head_dim) of a usable cache (on GPU `gpu`); raises Unsupported with the reason."""
     k, v, ks, vs = cache
-    if k.dim() != 4 or v.shape != k.shape or ks.shape != k.shape[:3] or vs.shape != k.shape[:3]:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise Unsupported("cache codes [pages, kv_heads, page_size, head_dim] and scales [pages, kv_heads, page_size] required")
-    if k.dtype not in CACHE_DTYPES or v.dtype != k.dtype:
-        raise Unsupported(f"cache dtype {k.dtype}/{v.dtype} (int8 or float8_e4m3fn)")
+    dtype = k.dtype
+    if dtype not in CACHE_DTYPES or v.dtype != dtype:
+        raise Unsupported(f"cache dtype {dtype}/{v.dtype} (int8 or float8_e4m3fn)")
     if ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise Unsupported("cache scales must be float32")
-    pages, heads, page_size, D = k.shape
+    pages, heads, page_size, D = shape
     _check_page(page_size)
     if D not in HEAD_DIMS:
         raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
@@ -70,10 +72,10 @@ def check_cache(cache, device=None):
         raise Unsupported("a cache needs pages and kv heads")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise Unsupported("cache tensors must be contiguous")
-    dev = k.device if device is None else device
-    if not (k.is_cuda and k.device == dev and v.device == dev and ks.device == dev and vs.device == dev):
+    at = k.get_device()
+    if at < 0 or not at == v.get_device() == ks.get_device() == vs.get_device() or (gpu is not None and gpu != at):
         raise Unsupported("tensors must be on one ROCm GPU")
-    if device_arch(dev) not in ARCHS:
+    if gpu_arch(at) not in ARCHS:
         raise Unsupported("not a CDNA4 GPU")
     return pages, heads, page_size, D
 
@@ -91,73 +93,83 @@ def cache_slots(block_table, lengths, count, page_size):
     return torch.where(there, page * page_size + pos % page_size, -1)
 
 
-def _check_slots(slots, device, shape):
-    if slots.dtype not in (torch.int32, torch.int64):
+def _check_slots(slots, gpu, shape):
+    if slots.dtype != torch.int64 and slots.dtype != torch.int32:
         raise Unsupported(f"slots {slots.dtype} (int32 or int64)")
-    if slots.device != device:
+    if slots.get_device() != gpu:
         raise Unsupported("tensors must be on one ROCm GPU")
-    if tuple(slots.shape) != shape:
-        raise Unsupported(f"slots of shape {tuple(slots.shape)} for tokens {shape}")
+    if slots.shape != shape:
+        raise Unsupported(f"slots of shape {tuple(slots.shape)} for tokens {tuple(shape)}")
     return slots.contiguous()
 
 
 def _rows_args(t, layout):
     """A packed [tokens, heads, D] or a 4D tensor as the kernels address it: tensor, (b, s, h) strides."""
-    return _bsh(t.unsqueeze(0), "NHD") if t.dim() == 3 else _bsh(t, layout)
+    if t.dim() == 4:
+        return _bsh(t, layout)
+    t, s = _packed(t)
+    return t, (0, *s)
 
 
 def write_launch(cache, k, v, slots, layout):
-    if layout not in ("HND", "NHD"):
+    if layout != "HND" and layout != "NHD":
         raise Unsupported(f"layout {layout!r}")
-    if k.dim() not in (3, 4) or k.shape != v.shape:
+    shape = k.shape
+    if len(shape) not in (3, 4) or v.shape != shape:
         raise Unsupported("k and v of one shape, 4D or packed [tokens, kv_heads, head_dim], required")
     if k.dtype not in DTYPES or v.dtype != k.dtype:
         raise Unsupported(f"dtype {k.dtype}/{v.dtype} (fp16 or bf16 required)")
-    if v.device != k.device:
+    gpu = k.get_device()
+    if v.get_device() != gpu:
         raise Unsupported("tensors must be on one ROCm GPU")
-    pages, Hkv, page_size, D = check_cache(cache, k.device)
-    if k.dim() == 3:
-        (S, h, d), B = k.shape, 1
-        tokens = (S,)
+    pages, Hkv, page_size, D = check_cache(cache, gpu)
+    if len(shape) == 3:
+        (S, h, d), B = shape, 1
+        tokens = shape[:1]
     else:
-        B, S, h, d = _sizes(k, layout)
+        (B, h, S, d) = shape if layout == "HND" else (shape[0], shape[2], shape[1], shape[3])
         tokens = (B, S)
-    if (h, d) != (Hkv, D):
+    if h != Hkv or d != D:
         raise Unsupported(f"{h} heads of {d} channels for a cache of {Hkv} heads of {D}")
-    slots = _check_slots(slots, k.device, tokens)
-    if k.numel() == 0:
+    slots = _check_slots(slots, gpu, tokens)
+    n = k.numel()
+    if n == 0:
         return
-    if k.numel() > _I32_MAX:
+    if n > _I32_MAX:
         raise Unsupported("tensor too large for 32-bit indexing")
     k, sk = _rows_args(k, layout)
     v, sv = _rows_args(v, layout)
-    _capi.call_on(k.device, "sage_cache_write", k.data_ptr(), *sk, v.data_ptr(), *sv, B, S, DTYPES[k.dtype],
-                  slots.data_ptr(), int(slots.dtype == torch.int64), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+    _capi.call_on(gpu, "sage_cache_write", k.data_ptr(), *sk, v.data_ptr(), *sv, B, S, DTYPES[k.dtype],
+                  slots.data_ptr(), slots.dtype == torch.int64, cache.k.data_ptr(), cache.k_scale.data_ptr(),
                   cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D, CACHE_DTYPES[cache.k.dtype])
 
 
 def read_launch(cache, slots, dtype, layout):
-    if layout not in ("HND", "NHD"):
+    if layout != "HND" and layout != "NHD":
         raise Unsupported(f"layout {layout!r}")
     if dtype not in DTYPES:
         raise Unsupported(f"dtype {dtype} (fp16 or bf16 required)")
     pages, Hkv, page_size, D = check_cache(cache)
-    if slots.dim() not in (1, 2):
+    shape = slots.shape
+    if len(shape) not in (1, 2):
         raise Unsupported("slots [tokens] or [B, tokens] required")
-    slots = _check_slots(slots, cache.k.device, tuple(slots.shape))
-    out = [torch.empty((*slots.shape, Hkv, D), dtype=dtype, device=slots.device) for _ in range(2)]
-    if slots.numel():
-        if out[0].numel() > _I32_MAX:
+    gpu = cache.k.get_device()
+    slots = _check_slots(slots, gpu, shape)
+    k = torch.empty((*shape, Hkv, D), dtype=dtype, device=slots.device)
+    v = torch.empty_like(k)
+    n = k.numel()
+    if n:
+        if n > _I32_MAX:
             raise Unsupported("tensor too large for 32-bit indexing")
-        B, S = (1, slots.numel()) if slots.dim() == 1 else slots.shape
-        st = (S * Hkv * D, Hkv * D, D)
-        _capi.call_on(slots.device, "sage_cache_read", out[0].data_ptr(), *st, out[1].data_ptr(), *st, B, S, DTYPES[dtype],
-                      slots.data_ptr(), int(slots.dtype == torch.int64), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+        # (both outputs are contiguous: the batch needs no stride of its own)
+        st = (0, Hkv * D, D)
+        _capi.call_on(gpu, "sage_cache_read", k.data_ptr(), *st, v.data_ptr(), *st, 1, slots.numel(), DTYPES[dtype],
+                      slots.data_ptr(), slots.dtype == torch.int64, cache.k.data_ptr(), cache.k_scale.data_ptr(),
                       cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D,
                       CACHE_DTYPES[cache.k.dtype])
-    if slots.dim() == 2 and layout == "HND":
-        out = [t.transpose(1, 2) for t in out]
-    return tuple(out)
+    if len(shape) == 2 and layout == "HND":
+        return k.transpose(1, 2), v.transpose(1, 2)
+    return k, v
 
 
 def cache_write(cache, k, v, slots, tensor_layout="HND"):
@@ -166,9 +178,8 @@ def cache_write(cache, k, v, slots, tensor_layout="HND"):
     k / v: [B, kv_heads, tokens, head_dim] ("HND") or [B, tokens, kv_heads, head_dim] ("NHD") with slots [B, tokens], or packed
     [tokens, kv_heads, head_dim] with slots [tokens]; slots int32 or int64.  Tokens whose slot is outside the cache (-1) are
     left out; two tokens of a call may not share a slot (that slot's row then holds parts of both)."""
-    if _plain_eager(k, v, slots, *cache, grad=True):
-        with torch.no_grad():
-            write_launch(cache, k, v, slots, tensor_layout)
+    if _plain_eager(k, v, slots, *cache, grad=True):   # (codes have no derivative: autograd sees nothing of the write)
+        write_launch(cache, k, v, slots, tensor_layout)
     else:
         ops.cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, slots, tensor_layout)
 
@@ -182,60 +193,76 @@ def cache_read(cache, slots, dtype=torch.bfloat16, tensor_layout="HND"):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace(B, H, Hkv, T, D, page_size, max_pages):
-    return _capi.cache_attn_workspace(B, H, Hkv, T, D, page_size, max_pages)
+def _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages):
+    """Workspace bytes of a call of these sizes on GPU `gpu`."""
+    with torch.cuda.device(gpu):
+        return _capi.cache_attn_workspace(B, H, Hkv, T, D, page_size, max_pages)
 
 
 def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal, tree_mask, return_lse):
     """Output (B, T, H, D) contiguous in q's dtype, and the logsumexp [B, H, T] or None."""
-    if layout not in ("HND", "NHD"):
+    if layout != "HND" and layout != "NHD":
         raise Unsupported(f"layout {layout!r}")
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise Unsupported("4D q required")
     if q.dtype not in DTYPES:
         raise Unsupported(f"dtype {q.dtype} (fp16 or bf16 required)")
-    dev = q.device
-    pages, Hkv, page_size, D = check_cache(cache, dev)
-    B, T, H, d = _sizes(q, layout)
+    gpu = q.get_device()
+    pages, Hkv, page_size, D = check_cache(cache, gpu)
+    (B, H, T, d) = shape if layout == "HND" else (shape[0], shape[2], shape[1], shape[3])
     if d != D or H % Hkv:
         raise Unsupported(f"{H} heads of {d} channels for a cache of {Hkv} heads of {D}")
-    if block_table.dim() != 2 or block_table.shape[0] != B or lengths.dim() != 1 or lengths.shape[0] != B:
+    if block_table.dim() != 2 or block_table.shape[0] != B or lengths.shape != (B,):
         raise Unsupported("block_table [B, max_pages] and lengths [B] required")
-    if block_table.dtype not in (torch.int32, torch.int64) or lengths.dtype not in (torch.int32, torch.int64):
-        raise Unsupported("block_table and lengths must be int32 or int64")
-    if block_table.device != dev or lengths.device != dev:
+    if block_table.get_device() != gpu or lengths.get_device() != gpu:
         raise Unsupported("tensors must be on one ROCm GPU")
+    if block_table.dtype != torch.int32:
+        block_table = _as_int32(block_table)
+    if lengths.dtype != torch.int32:
+        lengths = _as_int32(lengths)
     mask, ms = None, (0, 0, 0)
     if tree_mask is not None:
         if not is_causal:
             raise Unsupported("tree_mask stands in the place of the causal rule: is_causal=False has none")
-        if tree_mask.dtype != torch.bool or tree_mask.device != dev:
+        if tree_mask.dtype != torch.bool or tree_mask.get_device() != gpu:
             raise Unsupported("tree_mask must be a bool tensor on q's device")
         if tuple(tree_mask.shape) not in ((T, T), (1, T, T), (B, T, T)):
             raise Unsupported(f"tree_mask of shape {tuple(tree_mask.shape)} for batch {B} and {T} new tokens")
-        mask = tree_mask.expand(B, T, T)
-        ms = mask.stride()
-    out = torch.empty((B, T, H, D), device=dev, dtype=q.dtype)
-    lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
-    max_pages = block_table.shape[1]
-    if q.numel() == 0 or max_pages == 0:   # no query rows, or no keys
+        ms = tree_mask.stride()
+        if len(ms) == 2 or tree_mask.shape[0] == 1:
+            ms = (0, *ms[-2:])
+        mask = tree_mask.data_ptr()
+    device = q.device
+    out = torch.empty((B, T, H, D), device=device, dtype=q.dtype)
+    lse = torch.empty((B, H, T), device=device, dtype=torch.float32) if return_lse else None
+    max_pages, n = block_table.shape[1], q.numel()
+    if n == 0 or max_pages == 0:   # no query rows, or no keys
         return out.zero_(), None if lse is None else lse.fill_(float("-inf"))
-    if q.numel() > _I32_MAX:
+    if n > _I32_MAX:
         raise Unsupported("tensor too large for 32-bit indexing")
     q, sq = _bsh(q, layout)
-    table = block_table.to(torch.int32)
-    if table.stride(1) != 1 and max_pages > 1:
-        table = table.contiguous()
-    lengths = lengths.to(torch.int32).contiguous()
-    ws_bytes = _workspace(B, H, Hkv, T, D, page_size, max_pages)
-    ws = torch.empty((ws_bytes,), device=dev, dtype=torch.uint8) if ws_bytes else None
-    _capi.call_on(dev, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), *out.stride()[:3],
+    ts = block_table.stride()
+    if ts[1] != 1 and max_pages > 1:
+        block_table = block_table.contiguous()
+        ts = block_table.stride()
+    lengths = lengths.contiguous()
+    ws_bytes = _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages)
+    ws = torch.empty((ws_bytes,), device=device, dtype=torch.uint8) if ws_bytes else None
+    _capi.call_on(gpu, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), T * H * D, H * D, D,
                   None if lse is None else lse.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
-                  cache.v.data_ptr(), cache.v_scale.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(),
-                  None if mask is None else mask.data_ptr(), *ms, B, H, Hkv, T, D, DTYPES[q.dtype],
-                  CACHE_DTYPES[cache.k.dtype], pages, page_size, max_pages, int(bool(is_causal)), float(sm_scale),
-                  None if ws is None else ws.data_ptr(), ws_bytes)
+                  cache.v.data_ptr(), cache.v_scale.data_ptr(), block_table.data_ptr(), ts[0], lengths.data_ptr(),
+                  mask, *ms, B, H, Hkv, T, D, DTYPES[q.dtype], CACHE_DTYPES[cache.k.dtype], pages, page_size, max_pages,
+                  bool(is_causal), sm_scale, None if ws is None else ws.data_ptr(), ws_bytes)
     return out, lse
+
+
+def _as_int32(t):
+    """Lengths and page numbers of another integer type as the kernels read them (beyond 32 bits: at its ends, so that
+    a number out of range stays out of range)."""
+    if t.dtype != torch.int64:
+        raise Unsupported("block_table and lengths must be int32 or int64")
+    return t.clamp(-2**31, _I32_MAX).to(torch.int32)
 
 
 def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scale=None, is_causal=True, tree_mask=None,
@@ -250,9 +277,9 @@ def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scal
     dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  sm_scale: None or a
     non-positive one stands for 1 / sqrt(D).  Raises Unsupported for what the kernel does not take."""
     sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
-    ts = [t for t in (q, *cache, block_table, lengths, tree_mask) if t is not None]
+    ts = (q, *cache, block_table, lengths)
     lse = None
-    if _plain_eager(*ts):
+    if _plain_eager(*ts) and (tree_mask is None or type(tree_mask) is torch.Tensor):
         out, lse = attention_launch(q, cache, block_table, lengths, tensor_layout, sm, is_causal, tree_mask, return_lse)
     elif return_lse:
         out, lse = ops.cache_attention_lse(q, *cache, block_table, lengths, tree_mask, tensor_layout, sm, bool(is_causal))

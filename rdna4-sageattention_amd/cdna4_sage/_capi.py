@@ -101,11 +101,9 @@ def call(name: str, *args) -> None:
         raise SageError(name, rc, lib().sage_last_error().decode(errors="replace"))
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """call with the current stream of `device` as the last argument, that device current."""
-    cur = torch.cuda.current_device()
-    di = cur if device.index is None else device.index
-    if di == cur:
+def call_on(di: int, name: str, *args) -> None:
+    """call with the current stream of GPU `di` as the last argument, that GPU current."""
+    if di == torch._C._cuda_getDevice():
         call(name, *args, torch._C._cuda_getCurrentRawStream(di))
     else:
         with torch.cuda.device(di):

@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import _capi, ops
-from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, device_arch
+from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, gpu_arch
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling=None, device=None):
@@ -60,71 +60,76 @@ def rope_frequencies(rot_dim, base=10000.0, scaling=None, device=None):
     return f.to(device=device), factor
 
 
-def _sizes(x, layout):
-    """(batch, tokens, heads, head_dim)"""
-    return (x.shape[0], x.shape[2], x.shape[1], x.shape[3]) if layout == "HND" else tuple(x.shape)
-
-
 def check_rope(q, k, positions, freqs, layout):
-    if layout not in ("HND", "NHD"):
+    """(batch, tokens, heads, head_dim) of q and the GPU's index; raises Unsupported with the reason."""
+    if layout != "HND" and layout != "NHD":
         raise Unsupported(f"layout {layout!r}")
-    if q.dim() != 4 or (k is not None and k.dim() != 4):
+    shape = q.shape
+    if len(shape) != 4 or (k is not None and k.dim() != 4):
         raise Unsupported("4D tensors required")
     if q.dtype not in DTYPES or (k is not None and k.dtype != q.dtype):
         raise Unsupported(f"dtype {q.dtype} (fp16 or bf16 required, the same for q and k)")
-    B, S, _, D = _sizes(q, layout)
+    (B, H, S, D) = shape if layout == "HND" else (shape[0], shape[2], shape[1], shape[3])
     if D not in HEAD_DIMS:
         raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
-    if k is not None and _sizes(k, layout)[::3] + _sizes(k, layout)[1:2] != (B, D, S):
-        raise Unsupported("q and k must have the same batch, length and head_dim")
+    gpu, big = q.get_device(), q.numel()
+    if k is not None:
+        ks = k.shape
+        if ks[0] != B or ks[3] != D or ks[2 if layout == "HND" else 1] != S:
+            raise Unsupported("q and k must have the same batch, length and head_dim")
+        if k.get_device() != gpu:
+            raise Unsupported("tensors must be on one ROCm GPU")
+        big = max(big, k.numel())
     if freqs.dim() != 1 or freqs.dtype != torch.float64:
         raise Unsupported("freqs must be a 1D float64 tensor (rope_frequencies)")
-    rot = 2 * freqs.numel()
+    rot = 2 * freqs.shape[0]
     if rot == 0 or rot > D or rot % 8:
         raise Unsupported(f"{rot} rotated channels (a positive multiple of 8 up to head_dim {D})")
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype != torch.int64 and positions.dtype != torch.int32:
             raise Unsupported(f"positions {positions.dtype} (int32 or int64)")
-        if tuple(positions.shape) not in ((S,), (1, S), (B, S)):
-            raise Unsupported(f"positions of shape {tuple(positions.shape)} for batch {B} and length {S}")
-    for t in (q, k, positions, freqs):
-        if t is not None and not (t.is_cuda and t.device == q.device):
+        ps = positions.shape
+        if ps != (B, S) and ps != (S,) and ps != (1, S):
+            raise Unsupported(f"positions of shape {tuple(ps)} for batch {B} and length {S}")
+        if positions.get_device() != gpu:
             raise Unsupported("tensors must be on one ROCm GPU")
-    if device_arch(q.device) not in ARCHS:
+    if gpu < 0 or freqs.get_device() != gpu:
+        raise Unsupported("tensors must be on one ROCm GPU")
+    if gpu_arch(gpu) not in ARCHS:
         raise Unsupported("not a CDNA4 GPU")
-    if max(q.numel(), 0 if k is None else k.numel()) > _I32_MAX:
+    if big > _I32_MAX:
         raise Unsupported("tensor too large for 32-bit indexing")
+    return B, S, H, D, gpu
 
 
 def rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse):
     """The rotated q (and k), in new tensors of the inputs' memory order."""
-    check_rope(q, k, positions, freqs, layout)
-    B, S, H, D = _sizes(q, layout)
+    B, S, H, D, gpu = check_rope(q, k, positions, freqs, layout)
     oq = torch.empty_like(q)
     ok = None if k is None else torch.empty_like(k)
-    if q.numel() == 0 and (k is None or k.numel() == 0):
-        return oq, ok
-    if q.numel() == 0:   # no query heads: k alone
+    if q.numel() == 0:   # no tokens, or no query heads: k alone
+        if k is None or k.numel() == 0:
+            return oq, ok
         return oq, rope_launch(k, None, positions, freqs, layout, interleaved, factor, inverse)[0]
-    Hk = 0 if k is None else _sizes(k, layout)[2]
     q, sq = _bsh(q, layout)
     oq, so = _out_bsh(oq, layout)
-    args = [q.data_ptr(), *sq, oq.data_ptr(), *so, H]
-    if Hk:
-        k, sk = _bsh(k, layout)
-        ok, so = _out_bsh(ok, layout)
-        args += [k.data_ptr(), *sk, ok.data_ptr(), *so, Hk]
-    else:
-        args += [None, 0, 0, 0, None, 0, 0, 0, 0]
     pos, p64, pb, ps = None, 0, 0, 0
     if positions is not None:
-        p64, ps = int(positions.dtype == torch.int64), positions.stride(-1)
-        pb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-        pos = positions.data_ptr()
+        st = positions.stride()
+        pos, p64, ps = positions.data_ptr(), positions.dtype == torch.int64, st[-1]
+        if len(st) == 2 and positions.shape[0] > 1:
+            pb = st[0]
     freqs = freqs.contiguous()
-    args += [B, S, D, DTYPES[q.dtype], pos, p64, pb, ps, freqs.data_ptr(), 2 * freqs.numel(), int(bool(interleaved)),
-             float(factor), int(bool(inverse))]
-    _capi.call_on(q.device, "sage_rope", *args)
+    rest = (B, S, D, DTYPES[q.dtype], pos, p64, pb, ps, freqs.data_ptr(), 2 * freqs.shape[0], bool(interleaved), factor,
+            bool(inverse))
+    Hk = 0 if k is None else k.shape[1 if layout == "HND" else 2]
+    if Hk:
+        k, sk = _bsh(k, layout)
+        ok, sko = _out_bsh(ok, layout)
+        _capi.call_on(gpu, "sage_rope", q.data_ptr(), *sq, oq.data_ptr(), *so, H, k.data_ptr(), *sk, ok.data_ptr(), *sko,
+                      Hk, *rest)
+    else:
+        _capi.call_on(gpu, "sage_rope", q.data_ptr(), *sq, oq.data_ptr(), *so, H, None, 0, 0, 0, None, 0, 0, 0, 0, *rest)
     return oq, ok
 
 
@@ -150,12 +155,14 @@ class _Rope(torch.autograd.Function):
         layout, interleaved, factor, inverse = ctx.how
         need_q, need_k = ctx.needs_input_grad[:2]
         back = (positions, freqs, layout, interleaved, factor, not inverse)
+        # (create_graph: the gradients have gradients of their own)
+        turn = _Rope.apply if torch.is_grad_enabled() else rope_launch
         if need_q and need_k:
-            dq, dk = _Rope.apply(dq, dk, *back)
+            dq, dk = turn(dq, dk, *back)
         elif need_q:
-            dq, dk = _Rope.apply(dq, None, *back)[0], None
+            dq, dk = turn(dq, None, *back)[0], None
         else:
-            dq, dk = None, _Rope.apply(dk, None, *back)[0] if need_k else None
+            dq, dk = None, turn(dk, None, *back)[0] if need_k else None
         return dq, dk, None, None, None, None, None, None
 
 
@@ -169,12 +176,13 @@ def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved
     if freqs is None:
         raise Unsupported("freqs are required (rope_frequencies)")
     ts = (q,) if k is None else (q, k)
-    if _plain_eager(*ts):
-        out = rope_launch(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
-    elif _plain_eager(*ts, grad=True):
-        out = _Rope.apply(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
+    if _plain_eager(*ts, grad=True):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+            out = _Rope.apply(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
+        else:
+            out = rope_launch(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
     elif k is None:
         return ops.rope(q, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
     else:
         return ops.rope_qk(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
-    return out[0] if k is None else tuple(out)
+    return out[0] if k is None else out
