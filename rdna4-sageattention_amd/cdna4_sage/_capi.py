@@ -158,7 +158,7 @@ def varlen_layout(batch: int, H: int, Hkv: int, total_q: int, total_k: int):
 
 
 def cache_attn_workspace(B: int, H: int, Hkv: int, T: int, D: int, page_size: int, max_pages: int) -> int:
-    """Workspace bytes of sage_cache_attn (host arithmetic only)."""
+    """Workspace bytes of sage_cache_attn on the current device."""
     ws = ctypes.c_int64()
     call("sage_cache_attn_workspace", B, H, Hkv, T, D, page_size, max_pages, ctypes.byref(ws))
     return ws.value

@@ -1086,7 +1086,7 @@ struct AttnPlan {
   int64_t workspace;  // bytes of partial state
 };
 
-static int device_cus(int* cus) {
+int device_cus(int* cus) {
   static int cache[64] = {0};
   int dev = 0;
   SAGE_HIP_CHECK(hipGetDevice(&dev), "hipGetDevice");

@@ -47,16 +47,72 @@ struct CacheAttnArgs {
   int64_t tsb, msb, msq, msk;
   int B, H, Hkv, G, T, dtype, causal;
   int pages, page_size, page_shift, max_pages;
-  int row_blocks, splits;
+  int row_blocks, workers;
+  int part_rows;                    // rows of a partial: 16 RT, or all of them where that is fewer
   float scale;                      // softmax scale * log2 e
-  float* part_o;                    // [unit][splits][16 RT][D], units = (b, kv head, row block)
-  float* part_lse;                  // [unit][splits][16 RT], log2
+  float* part_o;                    // [kv head][row block][worker][2][part_rows][D]
+  float* part_lse;                  // the same without D, log2
 };
+
+// Work of one kv head and row block: the steps (CA_STEP keys) of all sequences in a row, at least one each, cut into
+// `workers` ranges as equal as whole steps allow, whatever the sequences' lengths.  A worker's range holds whole sequences,
+// whose output it writes, and up to two parts: of the one it begins inside of (partial 0) and of the one that it begins
+// but does not end (partial 1); a second kernel joins those.  The lengths stay on the device: every wave adds them up.
+__device__ __forceinline__ int cache_keys(const CacheAttnArgs& a, int b) {
+  return min(max(a.lengths[b], 0), a.max_pages * a.page_size);
+}
+// An entry of an input table at a wave-uniform index, by a scalar load (the compiler takes a vector load where it cannot
+// rule out that the kernel's stores change the table, and waiting for one is waiting for all loads before it).
+__device__ __forceinline__ int scalar_entry(const int* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) int*)p)[i];
+}
+__device__ __forceinline__ int uniform_keys(const CacheAttnArgs& a, int b) {
+  return min(max(scalar_entry(a.lengths, b), 0), a.max_pages * a.page_size);
+}
+__device__ __forceinline__ int cache_steps(int keys) { return max((keys + CA_STEP - 1) / CA_STEP, 1); }
+
+// sums of x over the lanes up to and with each
+template <int CTRL, int ROWS_MASK> __device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS_MASK, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = dpp_add<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8: within 16 lanes
+  x = dpp_add<0x112, 0xF>(x);
+  x = dpp_add<0x114, 0xF>(x);
+  x = dpp_add<0x118, 0xF>(x);
+  x = dpp_add<0x142, 0xA>(x);  // the last lane of a row to the next: rows 1 and 3, then 2 and 3
+  x = dpp_add<0x143, 0xC>(x);
+  return x;
+}
+// steps of sequences [64 c, 64 c + 64), one per lane
+__device__ __forceinline__ int lane_steps(const CacheAttnArgs& a, int c, int lane) {
+  const int b = 64 * c + lane;
+  return b < a.B ? cache_steps(cache_keys(a, b)) : 0;
+}
+// steps of all sequences; `before`: of those in front of sequence b_of
+__device__ __forceinline__ int all_steps(const CacheAttnArgs& a, int lane, int b_of, int& before) {
+  int total = 0;
+  before = 0;
+  for (int c = 0; 64 * c < a.B; ++c) {
+    const int n = lane_steps(a, c, lane), scan = wave_scan(n);
+    if (b_of / 64 == c) before = total + __builtin_amdgcn_readlane(scan, b_of % 64) - __builtin_amdgcn_readlane(n, b_of % 64);
+    total += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return total;
+}
 
 template <int BYTES> struct RawBytes { uint32_t w[(BYTES + 3) / 4]; };
 
-__device__ __forceinline__ v4i ld16(const uint8_t* p) { return *reinterpret_cast<const v4i*>(p); }
-__device__ __forceinline__ v2i ld8(const uint8_t* p) { return *reinterpret_cast<const v2i*>(p); }
+// A load at a wave-uniform base (pinned to scalar registers) and a lane's 32-bit offset: no 64-bit address per lane
+struct Base {
+  const __attribute__((address_space(1))) uint8_t* p;
+  __device__ __forceinline__ explicit Base(const void* q) : p((const __attribute__((address_space(1))) uint8_t*)q) {
+    asm volatile("" : "+s"(p));
+  }
+  template <typename V> __device__ __forceinline__ V at(uint32_t offset) const {
+    return *(const __attribute__((address_space(1))) V*)(p + offset);
+  }
+};
 
 // bytes 0, 1 (half 0) or 2, 3 (half 1) of a word of codes as two float16; int8 codes come with their sign bit flipped
 template <int CT> __device__ __forceinline__ f16x2 codes_f16(uint32_t w, bool half) {
@@ -96,8 +152,14 @@ template <int D> struct CacheTile {
   v4f ks[2], vs[2];
 };
 
+// rows in front of the first of 16 keys from k0 on; a page outside the cache hides its keys: page 0 is read in its place
+struct CacheRow {
+  int64_t row;
+  bool usable;
+};
+
 template <int D, int CT, int RT>
-__global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnArgs a) {
   constexpr int NK = D / 32, NC = D / 16;
   constexpr int ROWS = 16 * RT;
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
@@ -107,21 +169,38 @@ __global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnA
   // the row blocks of one range of keys on one XCD, next to each other
   const int id = blockIdx.x;
   const int grp = id / (8 * a.row_blocks) * 8 + id % 8, rb = id / 8 % a.row_blocks;
-  const int pairs = a.B * a.Hkv;
-  if (grp >= pairs * a.splits) return;
-  const int pair = grp / a.splits, split = grp % a.splits;
-  const int b = pair / a.Hkv, h = pair % a.Hkv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int rows = a.T * a.G;
-  const int64_t unit = ((int64_t)pair * a.row_blocks + rb) * a.splits + split;
+  int unused;
+  const int total = all_steps(a, lane, -1, unused);
+  const int workers = min(a.workers, total);
+  const int h = grp / a.workers, worker = grp % a.workers;
+  if (h >= a.Hkv || worker >= workers) return;
+  int s0 = (int)((int64_t)worker * total / workers);
+  const int s1 = (int)((int64_t)(worker + 1) * total / workers);
+  // the sequence of step s0, and the step's place in it
+  int b = 0, first = 0;
+  for (int c = 0, sum = 0; 64 * c < a.B; ++c) {
+    const int steps = lane_steps(a, c, lane), scan = wave_scan(steps) + sum;
+    sum = __builtin_amdgcn_readlane(scan, 63);
+    if (sum > s0) {
+      const int at = __builtin_ctzll(__ballot(scan > s0));
+      b = 64 * c + at;
+      first = s0 - (__builtin_amdgcn_readlane(scan, at) - __builtin_amdgcn_readlane(steps, at));
+      break;
+    }
+  }
 
-  const int len = min(max(a.lengths[b], 0), (int)min((int64_t)a.max_pages * a.page_size, (int64_t)0x7FFFFFFF));
+  for (;; ++b, first = 0) {
+  const int len = uniform_keys(a, b);
+  const int steps = cache_steps(len), take = min(steps - first, s1 - s0);
+  const bool whole = take == steps;
+  const int64_t unit = ((((int64_t)h * a.row_blocks + rb) * a.workers + worker) * 2 + (first > 0 ? 0 : 1)) * a.part_rows;
   const int base = len - a.T;  // key of the first new token
   // keys below `open` are seen by every row
   const int open = a.tree ? base : a.causal ? base + 1 : len;
-  const int per = ((len + a.splits - 1) / a.splits + CA_STEP - 1) / CA_STEP * CA_STEP;
-  const int k_begin = min((int64_t)split * per, (int64_t)len), k_end = min((int64_t)k_begin + per, (int64_t)len);
+  const int k_begin = first * CA_STEP, k_end = min(len, (first + take) * CA_STEP);
 
   // Q operand and the rows' factors
   f16x8 qf[RT][NK];
@@ -177,45 +256,53 @@ __global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnA
   }
 
   const int* table = a.table + b * a.tsb;
-  // a page outside the cache hides its keys: page 0 is read in its place
-  auto page_of = [&](int key) { return table[min(key >> a.page_shift, a.max_pages - 1)]; };
-  auto usable = [&](int page) { return page >= 0 && page < a.pages; };
-  auto load = [&](CacheTile<D>& x, int k0, int p0, int p1) {
+  auto page_of = [&](int key) { return scalar_entry(table, min(key >> a.page_shift, a.max_pages - 1)); };
+  auto rows_of = [&](int k0) {
+    const int page = page_of(k0);
+    const bool usable = page >= 0 && page < a.pages;
+    return CacheRow{((int64_t)(usable ? page : 0) * a.Hkv + h) * a.page_size + (k0 & (a.page_size - 1)), usable};
+  };
+  const uint32_t k_off = n * D + g * (D / 4), s_off = 16 * g;
+  const uint32_t v_off = 4 * g * D + (D == 96 ? 4 : D / 16) * n;
+  auto load_k = [&](CacheTile<D>& x, const CacheRow (&at)[2]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int p = t ? p1 : p0;
-      const int64_t row = ((int64_t)(usable(p) ? p : 0) * a.Hkv + h) * a.page_size + ((k0 + 16 * t) & (a.page_size - 1));
-      const uint8_t* kp = a.k8 + row * D + n * D + g * (D / 4);
+      const Base kp(a.k8 + at[t].row * D);
       if constexpr (D == 96) {
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          const v2i w = ld8(kp + 8 * i);
+          const v2i w = kp.at<v2i>(k_off + 8 * i);
           x.k[t][2 * i] = w[0], x.k[t][2 * i + 1] = w[1];
         }
       } else {
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          const v4i w = ld16(kp + 16 * i);
+          const v4i w = kp.at<v4i>(k_off + 16 * i);
 #pragma unroll
           for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = (uint32_t)w[j];
         }
       }
-      x.ks[t] = *reinterpret_cast<const v4f*>(a.ks + row + 4 * g);
-      x.vs[t] = *reinterpret_cast<const v4f*>(a.vs + row + 4 * g);
+      x.ks[t] = Base(a.ks + at[t].row).at<v4f>(s_off);
+    }
+  };
+  auto load_v = [&](CacheTile<D>& x, const CacheRow (&at)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x.vs[t] = Base(a.vs + at[t].row).at<v4f>(s_off);
+      const Base vp(a.v8 + at[t].row * D);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* vp = a.v8 + (row + 4 * g + i) * D;
         uint32_t* w = x.v[4 * t + i];
         if constexpr (D == 64) {
-          w[0] = *reinterpret_cast<const uint32_t*>(vp + 4 * n);
+          w[0] = vp.at<uint32_t>(v_off + i * D);
         } else if constexpr (D == 96) {
-          w[0] = *reinterpret_cast<const uint32_t*>(vp + 4 * n);
-          w[1] = *reinterpret_cast<const uint16_t*>(vp + 64 + 2 * n);
+          w[0] = vp.at<uint32_t>(v_off + i * D);
+          w[1] = vp.at<uint16_t>(v_off + i * D + 64 - 2 * n);
         } else if constexpr (D == 128) {
-          const v2i y = ld8(vp + 8 * n);
+          const v2i y = vp.at<v2i>(v_off + i * D);
           w[0] = y[0], w[1] = y[1];
         } else {
-          const v4i y = ld16(vp + 16 * n);
+          const v4i y = vp.at<v4i>(v_off + i * D);
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[j] = (uint32_t)y[j];
         }
@@ -223,137 +310,128 @@ __global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnA
     }
   };
 
-  auto compute = [&](CacheTile<D>& x, int k0, int p0, int p1) {
-    const bool masked = k0 + CA_TILE > open || !usable(p0) || !usable(p1);
-    v4f s[RT][2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        uint32_t w0 = x.k[t][2 * i], w1 = x.k[t][2 * i + 1];
-        if (CT == CACHE_INT8) w0 ^= 0x80808080u, w1 ^= 0x80808080u;
-        const f16x8 ka = join4(codes_f16<CT>(w0, false), codes_f16<CT>(w0, true), codes_f16<CT>(w1, false),
-                               codes_f16<CT>(w1, true));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
-      }
-    }
-    uint32_t hidden[RT];  // bit 4 t + i
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) hidden[rt] = 0;
-    if (masked) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = j / 4, key = k0 + 16 * t + 4 * g + j % 4, node = key - base;
-        const bool none = key >= len || !usable(t ? p1 : p0);
-        if (none) {  // whatever the memory past a sequence holds: no NaN enters the products
-#pragma unroll
-          for (int i = 0; i < CacheTile<D>::VW; ++i) x.v[j][i] = CT == CACHE_INT8 ? 0x80808080u : 0u;
-          x.vs[t][j % 4] = 0.0f;
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          bool hide = none;
-          if (!none && node >= 0) {
-            if (a.tree) hide = a.tree[b * a.msb + row_t[rt] * a.msq + node * a.msk] == 0;
-            else if (a.causal) hide = node > row_t[rt];
-          }
-          hidden[rt] |= (uint32_t)hide << j;
-        }
-      }
-    }
-    f16x8 pf[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float y[8], p[8], pv[8];
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = s[rt][j / 4][j % 4] * (x.ks[j / 4][j % 4] * qs[rt]);
-        if (masked && (hidden[rt] >> j & 1)) y[j] = -__builtin_inff();
-        top = fmaxf(top, y[j]);
-      }
-      if (__any(top > m[rt] + CA_SLACK)) {
-        const float now = fmaxf(m[rt], row4_max(top));
-        if (now > m[rt]) {
-          l[rt] *= __builtin_amdgcn_exp2f(m[rt] - now);
-          m[rt] = now;
-          f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(m[rt] - m2[rt], 100.0f));
-        }
-      }
-      const float ref = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
-      float pvmax = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(y[j] - ref);
-        l[rt] += p[j];
-        pv[j] = p[j] * x.vs[j / 4][j % 4];
-        if (masked && (hidden[rt] >> j & 1)) pv[j] = 0.0f;
-        pvmax = fmaxf(pvmax, pv[j]);
-      }
-      if (__any(pvmax * f[rt] > 0x1p15f || (f[rt] == 0.0f && pvmax > 0.0f))) {
-        const float row = row4_max(pvmax);
-        if (row > 0.0f && row < __builtin_inff()) {
-          const float now = fmaxf(m2[rt], m[rt] + (float)(__builtin_amdgcn_frexp_expf(row) - 7));
-          const float down = __builtin_amdgcn_exp2f(m2[rt] - now);
-#pragma unroll
-          for (int c = 0; c < NC; ++c) acc[rt][c] *= down;
-          m2[rt] = now;
-          f[rt] = __builtin_amdgcn_exp2f(fminf(m[rt] - now, 100.0f));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
-    }
-    // V operand: keys (0, 1), (2, 3) of each block side by side
-#pragma unroll
-    for (int i = 0; i < CacheTile<D>::VW; ++i) {
-      if (CT == CACHE_INT8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.v[j][i] ^= 0x80808080u;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {  // channels 4 i + 2 u, + 1 of the lane
-        if (D == 96 && i == 1 && u == 1) continue;
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)  // bytes (A_2u, B_2u, A_2u+1, B_2u+1)
-          w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i], x.v[2 * j][i], u ? 0x07030602u : 0x05010400u);
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const int c = 4 * i + 2 * u + o;
-          const f16x8 va = join4(codes_f16<CT>(w[0], o), codes_f16<CT>(w[1], o), codes_f16<CT>(w[2], o), codes_f16<CT>(w[3], o));
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], acc[rt][c], 0, 0, 0);
-        }
-      }
-    }
-  };
-
-  // two tiles in registers: one is loaded while the other is used
+  // One tile in registers: the next tile's K is loaded once this one's scores are there, its V after the output's
+  // products, so that loads are in flight through the whole step.
   int k0 = k_begin + wave * CA_TILE;
   if (k0 < k_end) {
-    CacheTile<D> x[2];
-    int p[2][2];
-    p[0][0] = page_of(k0), p[0][1] = page_of(k0 + 16);
-    load(x[0], k0, p[0][0], p[0][1]);
+    CacheTile<D> x;
+    CacheRow now[2] = {rows_of(k0), rows_of(k0 + 16)};
+    load_k(x, now);
+    load_v(x, now);
     for (;;) {
       const int k1 = k0 + CA_STEP;
-      if (k1 < k_end) {
-        p[1][0] = page_of(k1), p[1][1] = page_of(k1 + 16);
-        load(x[1], k1, p[1][0], p[1][1]);
+      const bool more = k1 < k_end;
+      CacheRow next[2] = {now[0], now[1]};
+      if (more) next[0] = rows_of(k1), next[1] = rows_of(k1 + 16);
+      const bool masked = k0 + CA_TILE > open || !now[0].usable || !now[1].usable;
+      v4f s[RT][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          uint32_t w0 = x.k[t][2 * i], w1 = x.k[t][2 * i + 1];
+          if (CT == CACHE_INT8) w0 ^= 0x80808080u, w1 ^= 0x80808080u;
+          const f16x8 ka = join4(codes_f16<CT>(w0, false), codes_f16<CT>(w0, true), codes_f16<CT>(w1, false),
+                                 codes_f16<CT>(w1, true));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][t] *= x.ks[t] * qs[rt];
       }
-      compute(x[0], k0, p[0][0], p[0][1]);
-      if (k1 >= k_end) break;
-      k0 = k1 + CA_STEP;
-      if (k0 < k_end) {
-        p[0][0] = page_of(k0), p[0][1] = page_of(k0 + 16);
-        load(x[0], k0, p[0][0], p[0][1]);
+      if (more) load_k(x, next);
+      uint32_t hidden[RT];  // bit 4 t + i
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) hidden[rt] = 0;
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = j / 4, key = k0 + 16 * t + 4 * g + j % 4, node = key - base;
+          const bool none = key >= len || !now[t].usable;
+          if (none) {  // whatever the memory past a sequence holds: no NaN enters the products
+#pragma unroll
+            for (int i = 0; i < CacheTile<D>::VW; ++i) x.v[j][i] = CT == CACHE_INT8 ? 0x80808080u : 0u;
+            x.vs[t][j % 4] = 0.0f;
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            bool hide = node > row_t[rt] && a.causal;
+            if (a.tree) hide = node >= 0 && a.tree[b * a.msb + row_t[rt] * a.msq + min(max(node, 0), a.T - 1) * a.msk] == 0;
+            hidden[rt] |= (uint32_t)(hide || none) << j;
+          }
+        }
       }
-      compute(x[1], k1, p[1][0], p[1][1]);
-      if (k0 >= k_end) break;
+      f16x8 pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float pv[8];
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (masked && (hidden[rt] >> j & 1)) s[rt][j / 4][j % 4] = -__builtin_inff();
+          top = fmaxf(top, s[rt][j / 4][j % 4]);
+        }
+        if (__any(top > m[rt] + CA_SLACK)) {
+          const float up = fmaxf(m[rt], row4_max(top));
+          if (up > m[rt]) {
+            l[rt] *= __builtin_amdgcn_exp2f(m[rt] - up);
+            m[rt] = up;
+            f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(m[rt] - m2[rt], 100.0f));
+          }
+        }
+        const float ref = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
+        float pvmax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float p = __builtin_amdgcn_exp2f(s[rt][j / 4][j % 4] - ref);
+          l[rt] += p;
+          pv[j] = p * x.vs[j / 4][j % 4];
+          if (masked && (hidden[rt] >> j & 1)) pv[j] = 0.0f;
+          pvmax = fmaxf(pvmax, pv[j]);
+        }
+        if (__any(pvmax * f[rt] > 0x1p15f || (f[rt] == 0.0f && pvmax > 0.0f))) {
+          const float row = row4_max(pvmax);
+          if (row > 0.0f && row < __builtin_inff()) {
+            const float up = fmaxf(m2[rt], m[rt] + (float)(__builtin_amdgcn_frexp_expf(row) - 7));
+            const float down = __builtin_amdgcn_exp2f(m2[rt] - up);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[rt][c] *= down;
+            m2[rt] = up;
+            f[rt] = __builtin_amdgcn_exp2f(fminf(m[rt] - up, 100.0f));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
+      }
+      // V operand: keys (0, 1), (2, 3) of each block side by side
+#pragma unroll
+      for (int i = 0; i < CacheTile<D>::VW; ++i) {
+        if (CT == CACHE_INT8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x.v[j][i] ^= 0x80808080u;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // channels 4 i + 2 u, + 1 of the lane
+          if (D == 96 && i == 1 && u == 1) continue;
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // bytes (A_2u, B_2u, A_2u+1, B_2u+1)
+            w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i], x.v[2 * j][i], u ? 0x07030602u : 0x05010400u);
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const int c = 4 * i + 2 * u + o;
+            const f16x8 va = join4(codes_f16<CT>(w[0], o), codes_f16<CT>(w[1], o), codes_f16<CT>(w[2], o), codes_f16<CT>(w[3], o));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], acc[rt][c], 0, 0, 0);
+          }
+        }
+      }
+      if (!more) break;
+      load_v(x, next);
+      now[0] = next[0], now[1] = next[1];
+      k0 = k1;
     }
   }
 
@@ -402,7 +480,7 @@ __global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnA
       o[i] = L == 0.0f ? 0.0f : v * fin;
     }
     if (R < rows) {
-      if (a.splits == 1) {
+      if (whole) {
         const int t = R / a.G, hq = h * a.G + R % a.G;
         uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + part * PER;
 #pragma unroll
@@ -413,68 +491,127 @@ __global__ __launch_bounds__(CA_THREADS) void cache_attn_kernel(const CacheAttnA
         }
         if (a.lse && part == 0) a.lse[((int64_t)b * a.H + hq) * a.T + t] = lse2 * 0.69314718055994530942f;
       } else {
-        float* op = a.part_o + (unit * ROWS + rr) * D + part * PER;
+        float* op = a.part_o + (unit + rr) * D + part * PER;
 #pragma unroll
         for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(op + i) = make_float2(o[i], o[i + 1]);
-        if (part == 0) a.part_lse[unit * ROWS + rr] = lse2;
+        if (part == 0) a.part_lse[unit + rr] = lse2;
       }
     }
     if (rt + 1 < RT) __syncthreads();
   }
+  s0 += take;
+  if (s0 >= s1) break;
+  __syncthreads();  // the next sequence's rows go where these were read
+  }
 }
 
-// Joins the ranges of keys of a row: o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M), in their order.
-template <int D> __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnArgs a, int block_rows) {
-  constexpr int LPR = D / 4;  // threads per row, 4 channels each
-  const int64_t rows = (int64_t)a.T * a.G;
-  const int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (threadIdx.x >= 256 / LPR * LPR || at >= rows * a.B * a.Hkv) return;
-  const int c = threadIdx.x % LPR * 4;
-  const int pair = (int)(at / rows), R = (int)(at - pair * rows);
-  const int b = pair / a.Hkv, h = pair % a.Hkv;
-  const int64_t unit = ((int64_t)pair * a.row_blocks + R / block_rows) * a.splits;
-  const int rr = R % block_rows;
-  float M = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_lse[(unit + s) * block_rows + rr]);
-  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-  float L = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float x = a.part_lse[(unit + s) * block_rows + rr];
-    if (x == -__builtin_inff()) continue;  // a range without a visible key
-    const float w = __builtin_amdgcn_exp2f(x - M);
-    L += w;
-    o += *reinterpret_cast<const v4f*>(a.part_o + ((unit + s) * block_rows + rr) * D + c) * w;
+// Joins the parts of the rows of sequences that several workers shared: o = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M).
+// One row per group of `slices` waves, each of which adds up every slices-th part, in an order that the lengths alone
+// decide.
+constexpr int MERGE_SLICES = 16;
+template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merge_kernel(const CacheAttnArgs a, int block_rows, int slices) {
+  constexpr int VEC = D <= 64 ? 1 : D <= 128 ? 2 : 4;  // channels per lane
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  __shared__ float so[MERGE_SLICES][D];
+  __shared__ float sml[MERGE_SLICES][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = a.T * a.G;
+  const int64_t at = slices == 1 ? (int64_t)blockIdx.x * (blockDim.x / 64) + wave : blockIdx.x;
+  if (at >= (int64_t)rows * a.B * a.Hkv) return;
+  const int slice = slices == 1 ? 0 : wave;
+  const int R = (int)(at % rows), h = (int)(at / rows % a.Hkv), b = (int)(at / rows / a.Hkv);
+  int before;
+  const int total = all_steps(a, lane, b, before), steps = cache_steps(uniform_keys(a, b));
+  const int workers = min(a.workers, total);
+  // the last worker that begins at a step or before it
+  auto worker_of = [&](int step) { return (int)((((int64_t)step + 1) * workers - 1) / total); };
+  const int w0 = worker_of(before), parts = worker_of(before + steps - 1) - w0 + 1;
+  if (parts == 1) return;  // written whole
+  const int rb = R / block_rows, rr = R % block_rows;
+  const int64_t unit = ((int64_t)h * a.row_blocks + rb) * a.workers + w0;
+  auto part = [&](int i) { return ((unit + i) * 2 + (i == 0)) * a.part_rows + rr; };
+  const bool mine = lane * VEC < D;
+
+  float M = -__builtin_inff(), L = 0.0f;
+  vec o = 0.0f;
+  for (int i0 = 0; i0 < parts; i0 += 64 * slices) {  // part i0 + lane * slices + slice: one per lane
+    const int i = i0 + lane * slices + slice;
+    const float x = i < parts ? a.part_lse[part(i)] : -__builtin_inff();
+    float top = x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float now = fmaxf(M, top);
+    // (-inf: a part without a visible key; a NaN stays one)
+    const float w = x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - now);
+    if (now > M) {
+      const float down = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(M - now);
+      o *= down, L *= down, M = now;
+    }
+    const int count = min(64, (parts - i0 - slice + slices - 1) / slices);
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) {
+      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+      vec v = 0.0f;
+      if (mine) v = *reinterpret_cast<const vec*>(a.part_o + part(i0 + j * slices + slice) * D + lane * VEC);
+      L += wj;
+      o += v * wj;  // (a part without a visible key holds zeros)
+    }
+  }
+  if (slices > 1) {
+    if (mine) *reinterpret_cast<vec*>(&so[wave][lane * VEC]) = o;
+    if (lane == 0) sml[wave][0] = M, sml[wave][1] = L;
+    __syncthreads();
+    if (wave) return;
+    float top = M;
+    for (int i = 1; i < slices; ++i) top = fmaxf(top, sml[i][0]);
+    const float down = M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(M - top);
+    o *= down, L *= down, M = top;
+    for (int i = 1; i < slices; ++i) {
+      const float w = sml[i][0] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(sml[i][0] - top);
+      L += sml[i][1] * w;
+      if (mine) o += *reinterpret_cast<const vec*>(&so[i][lane * VEC]) * w;
+    }
   }
   if (L != 0.0f) o *= 1.0f / L;
   const int t = R / a.G, hq = h * a.G + R % a.G;
-  uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + c;
-  v2i w;
+  if (mine) {
+    uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + lane * VEC;
+    uint32_t w[VEC];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    w[i] = (int)(a.dtype == DT_BF16 ? f32_to_bf16_bits(o[2 * i]) | (f32_to_bf16_bits(o[2 * i + 1]) << 16)
-                                    : f32_to_f16_bits(o[2 * i]) | (f32_to_f16_bits(o[2 * i + 1]) << 16));
-  *reinterpret_cast<v2i*>(op) = w;
-  if (a.lse && c == 0)
+    for (int i = 0; i < VEC; ++i) w[i] = a.dtype == DT_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
+    if constexpr (VEC == 1) *op = (uint16_t)w[0];
+    else if constexpr (VEC == 2) *reinterpret_cast<uint32_t*>(op) = w[0] | (w[1] << 16);
+    else *reinterpret_cast<v2i*>(op) = v2i{(int)(w[0] | (w[1] << 16)), (int)(w[2] | (w[3] << 16))};
+  }
+  if (a.lse && lane == 0)
     a.lse[((int64_t)b * a.H + hq) * a.T + t] = L == 0.0f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.69314718055994530942f;
 }
 
-// Rows per workgroup (16 RT) and ranges of keys for a call.
+// Rows per workgroup (16 RT) and workers per kv head and row block for a call.
 struct CachePlan {
-  int rt, row_blocks, splits;
+  int rt, row_blocks, workers, part_rows;
   int64_t o_bytes, bytes;
 };
 
-static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys) {
+static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
   p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
-  const int64_t units = (int64_t)B * Hkv * p.row_blocks;
-  const int64_t most = (max_keys + CA_STEP - 1) / CA_STEP;
-  const int64_t want = (512 + units - 1) / units;
-  p.splits = (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
-  if (p.splits > 128) p.splits = 128;
-  const int64_t n = p.splits == 1 ? 0 : units * p.splits * 16 * p.rt;
+  p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
+  const int64_t units = (int64_t)Hkv * p.row_blocks;
+  const int64_t slots = (int64_t)cus * (p.rt == 1 ? 2 : 1);  // workgroups that run at once
+  const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
+  int64_t w = slots / units;
+  if (w < 8) {
+    // few workers per unit: the fewest whose rounds are within a tenth of the best of up to 8
+    auto rounds = [&](int64_t n) { return (double)((units * n + slots - 1) / slots) / (double)n; };
+    double best = rounds(1);
+    for (int64_t n = 2; n <= 8; ++n) best = rounds(n) < best ? rounds(n) : best;
+    for (w = 1; rounds(w) > 1.1 * best; ++w) {}
+  }
+  p.workers = (int)(w > most ? most : w);
+  const int64_t n = p.workers == 1 ? 0 : units * p.workers * 2 * p.part_rows;
   p.o_bytes = (n * D * 4 + 255) / 256 * 256;
   p.bytes = p.o_bytes + n * 4;
   return p;
@@ -489,10 +626,11 @@ template <int D, int CT> static void cache_attn_launch(const CacheAttnArgs& a, i
 template <int D> static void cache_attn_dims(const CacheAttnArgs& a, int ct, int rt, unsigned blocks, hipStream_t st) {
   if (ct == CACHE_INT8) cache_attn_launch<D, CACHE_INT8>(a, rt, blocks, st);
   else cache_attn_launch<D, CACHE_E4M3>(a, rt, blocks, st);
-  if (a.splits > 1) {
-    constexpr int per = 256 / (D / 4);
+  if (a.workers > 1) {
     const int64_t rows = (int64_t)a.T * a.G * a.B * a.Hkv;
-    cache_merge_kernel<D><<<(unsigned)((rows + per - 1) / per), 256, 0, st>>>(a, 16 * rt);
+    const int slices = a.workers <= 8 ? 1 : a.workers <= 128 ? 4 : MERGE_SLICES;
+    const int64_t blocks = slices == 1 ? (rows + 3) / 4 : rows;
+    cache_merge_kernel<D><<<(unsigned)blocks, 64 * (slices == 1 ? 4 : slices), 0, st>>>(a, 16 * rt, slices);
   }
 }
 
@@ -502,7 +640,9 @@ static int cache_attn_sizes(int B, int H, int Hkv, int T, int D, int page_size, 
   if (!head_dim_ok(D)) return fail(SAGE_ERR_UNSUPPORTED, "%s: head_dim %d (supported 64, 96, 128, 256)", who, D);
   if (!cache_page_ok(page_size))
     return fail(SAGE_ERR_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 1024)", who, page_size);
-  // keys of a sequence and rows of all heads are counted in 32 bits, with room for a step past the end
+  // keys of a sequence, steps of all of them and rows of all heads are counted in 32 bits, with room for a step past the end
+  SAGE_REQUIRE((int64_t)B * (((int64_t)max_pages * page_size + CA_STEP - 1) / CA_STEP) <= 0x40000000,
+               "%s: more than 2^37 keys", who);
   SAGE_REQUIRE((int64_t)max_pages * page_size <= 0x40000000, "%s: more than 2^30 keys per sequence", who);
   SAGE_REQUIRE((int64_t)B * H * T <= 0x01000000ll * 16, "%s: more than 2^28 query rows", who);
   return SAGE_OK;
@@ -519,7 +659,9 @@ int sage_cache_attn_workspace(int B, int H, int Hkv, int T, int D, int page_size
   SAGE_REQUIRE(workspace_bytes != nullptr, "sage_cache_attn_workspace: workspace_bytes is NULL");
   const int rc = cache_attn_sizes(B, H, Hkv, T, D, page_size, max_pages, "sage_cache_attn_workspace");
   if (rc) return rc;
-  *workspace_bytes = cache_plan(B, H, Hkv, T, D, max_pages * page_size).bytes;
+  int cus = 0;
+  if (const int e = device_cus(&cus)) return e;
+  *workspace_bytes = cache_plan(B, H, Hkv, T, D, max_pages * page_size, cus).bytes;
   return SAGE_OK;
 }
 
@@ -544,7 +686,9 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale must be finite and not negative (got %g)",
                who, (double)sm_scale);
-  const CachePlan p = cache_plan(B, H, Hkv, T, D, max_pages * page_size);
+  int cus = 0;
+  if ((rc = device_cus(&cus))) return rc;
+  const CachePlan p = cache_plan(B, H, Hkv, T, D, max_pages * page_size, cus);
   SAGE_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace & 255u) == 0 && workspace_bytes >= p.bytes),
                "%s: workspace of %lld bytes (256-byte aligned), the plan needs %lld", who, (long long)workspace_bytes,
                (long long)p.bytes);
@@ -557,12 +701,12 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   a.B = B, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.T = T, a.dtype = dtype, a.causal = causal;
   a.pages = pages, a.page_size = page_size, a.max_pages = max_pages;
   a.page_shift = __builtin_ctz((unsigned)page_size);
-  a.row_blocks = p.row_blocks, a.splits = p.splits;
+  a.row_blocks = p.row_blocks, a.workers = p.workers, a.part_rows = p.part_rows;
   const double scale = sm_scale > 0.0f ? (double)sm_scale : 1.0 / __builtin_sqrt((double)D);
   a.scale = (float)(scale * 1.44269504088896340736);
   a.part_o = (float*)workspace;
   a.part_lse = (float*)((char*)workspace + p.o_bytes);
-  const int64_t groups = ((int64_t)B * Hkv * p.splits + 7) / 8 * 8;
+  const int64_t groups = ((int64_t)Hkv * p.workers + 7) / 8 * 8;
   const int64_t blocks = groups * p.row_blocks;
   SAGE_REQUIRE(blocks <= 0x7FFFFFFF, "%s: too many workgroups", who);
   hipStream_t st = (hipStream_t)stream;

@@ -43,6 +43,8 @@ inline int check_qs_mul(float qs_mul, const char* who) {
   return SAGE_OK;
 }
 
+int device_cus(int* cus);  // CUs of the current device
+
 // head dims of the path, and the channel count of their int8 / E4M3 layouts (96 is stored zero-padded to 128)
 __host__ __device__ constexpr bool head_dim_ok(int d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 __host__ __device__ constexpr int layout_dim(int d) { return d == 96 ? 128 : d; }

@@ -163,18 +163,14 @@ ATTN = dict(q=P, qsb=512, qss=512, qsh=64, out=P, osb=512, oss=512, osh=64, lse=
     (dict(H=7), 1, "multiple"), (dict(D=80), 2, "head_dim"), (dict(n=20), 2, "page_size"), (dict(dtype=2), 2, "dtype"),
     (dict(ct=7), 2, "cache dtype"), (dict(sm=-1.0), 1, "sm_scale"), (dict(sm=float("nan")), 1, "sm_scale"),
     (dict(sm=float("inf")), 1, "sm_scale"), (dict(n=1024, max_pages=1 << 21), 1, "2^30"), (dict(T=1 << 28), 1, "2^28"),
-    (dict(n=256, ws=None, max_pages=64), 1, "workspace"), (dict(n=256, wsb=16, max_pages=64), 1, "workspace"),
-    (dict(n=256, ws=P + 64, max_pages=64), 1, "workspace")])
+    (dict(B=1 << 18, n=1024, max_pages=1 << 20), 1, "2^37")])
 def test_attention_entry_refuses(change, code, message):
     assert _capi.lib().sage_cache_attn(*{**ATTN, **change}.values()) == code
     assert message in _err()
 
 
 @built
-def test_attention_workspace():
+def test_attention_workspace_refuses():
     ws = ctypes.c_int64(-1)
     assert _capi.lib().sage_cache_attn_workspace(1, 8, 2, 1, 64, 16, 4, None) == 1
     assert _capi.lib().sage_cache_attn_workspace(1, 7, 2, 1, 64, 16, 4, ctypes.byref(ws)) == 1 and ws.value == -1
-    assert _capi.cache_attn_workspace(1, 8, 2, 1, 64, 16, 1) == 0                # one step of keys: no split
-    for D in (64, 96, 128, 256):
-        assert _capi.cache_attn_workspace(1, 8, 2, 1, D, 256, 64) > 0

@@ -345,6 +345,21 @@ def test_no_queries_and_no_keys(dev):
     assert not bool(out.any()) and bool((lse == -math.inf).all())
 
 
+def test_workspace(dev):
+    from cdna4_sage import _capi
+
+    sizes = lambda D, n: _capi.cache_attn_workspace(1, 8, 2, 1, D, 256, n)  # noqa: E731
+    assert _capi.cache_attn_workspace(1, 8, 2, 1, 64, 16, 1) == 0               # one step of keys: nothing to join
+    assert all(sizes(D, 64) > 0 for D in (64, 96, 128, 256))
+    P, n = 0x10000, sizes(64, 64)
+    ok = dict(q=P, qsb=512, qss=512, qsh=64, out=P, osb=512, oss=512, osh=64, lse=None, k8=P, ks=P, v8=P, vs=P, table=P,
+              ts=4, lengths=P, tree=None, msb=0, msq=0, msk=0, B=1, H=8, Hkv=2, T=1, D=64, dtype=0, ct=0, pages=4, n=256,
+              max_pages=64, causal=1, sm=0.0, ws=P, wsb=n, stream=None)
+    for bad in (dict(ws=None), dict(wsb=n - 1), dict(ws=P + 64)):   # refused before anything is launched
+        with pytest.raises(_capi.SageError, match="workspace"):
+            _capi.call("sage_cache_attn", *{**ok, **bad}.values())
+
+
 def test_cache_beyond_32_bit_offsets(dev):
     """Codes past 4 GiB: the last pages of a cache of 2 x 4.5 GiB hold a copy of the first ones' rows."""
     page, D, Hkv, H = 256, 128, 8, 16
