@@ -31,7 +31,6 @@ constexpr int CA_WAVES = 4;
 constexpr int CA_THREADS = 64 * CA_WAVES;
 constexpr int CA_TILE = 32;                      // keys per wave and step
 constexpr int CA_STEP = CA_TILE * CA_WAVES;      // keys per workgroup and step
-constexpr float CA_SLACK = 8.0f;                 // log2 by which scores may pass their reference
 
 struct CacheAttnArgs {
   const uint16_t* q;
@@ -159,7 +158,7 @@ struct CacheRow {
 };
 
 template <int D, int CT, int RT>
-__global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnArgs a) {
   constexpr int NK = D / 32, NC = D / 16;
   constexpr int ROWS = 16 * RT;
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
@@ -338,9 +337,8 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : 1) void cache_attn_kernel
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][t] *= x.ks[t] * qs[rt];
       }
+      v4f ks[2] = {x.ks[0], x.ks[1]};
       if (more) load_k(x, next);
       uint32_t hidden[RT];  // bit 4 t + i
 #pragma unroll
@@ -363,43 +361,63 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : 1) void cache_attn_kernel
           }
         }
       }
+      float vs_top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, x.vs[j / 4][j % 4]);
       f16x8 pf[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float pv[8];
-        float top = -__builtin_inff();
+        float c[8], p[8], pv[8];
+        float& M = m[rt];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (masked && (hidden[rt] >> j & 1)) s[rt][j / 4][j % 4] = -__builtin_inff();
-          top = fmaxf(top, s[rt][j / 4][j % 4]);
+          c[j] = ks[j / 4][j % 4] * qs[rt];
+          if (masked && (hidden[rt] >> j & 1)) s[rt][j / 4][j % 4] = -__builtin_inff(), c[j] = 1.0f;
         }
-        if (__any(top > m[rt] + CA_SLACK)) {
-          const float up = fmaxf(m[rt], row4_max(top));
-          if (up > m[rt]) {
-            l[rt] *= __builtin_amdgcn_exp2f(m[rt] - up);
-            m[rt] = up;
-            f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(m[rt] - m2[rt], 100.0f));
+        // the terms against the references so far; where one passes them by too much (or a row has none yet) the references
+        // are raised first
+        auto terms = [&] {
+          const float ref = M == -__builtin_inff() ? 0.0f : M;
+          float top = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], c[j], -ref));
+            top = fmaxf(top, p[j]);
           }
+          return top;
+        };
+        float top = terms();
+        if (__any(!(top <= 0x1p8f) || M == -__builtin_inff())) {
+          float y = -__builtin_inff();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * c[j]);
+          const float up = fmaxf(M, row4_max(y));
+          if (up > M) {
+            l[rt] *= __builtin_amdgcn_exp2f(M - up);
+            M = up;
+            f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(M - m2[rt], 100.0f));
+          }
+          top = terms();
         }
-        const float ref = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
-        float pvmax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float p = __builtin_amdgcn_exp2f(s[rt][j / 4][j % 4] - ref);
-          l[rt] += p;
-          pv[j] = p * x.vs[j / 4][j % 4];
+          l[rt] += p[j];
+          pv[j] = p[j] * x.vs[j / 4][j % 4];
           if (masked && (hidden[rt] >> j & 1)) pv[j] = 0.0f;
-          pvmax = fmaxf(pvmax, pv[j]);
         }
-        if (__any(pvmax * f[rt] > 0x1p15f || (f[rt] == 0.0f && pvmax > 0.0f))) {
-          const float row = row4_max(pvmax);
-          if (row > 0.0f && row < __builtin_inff()) {
-            const float up = fmaxf(m2[rt], m[rt] + (float)(__builtin_amdgcn_frexp_expf(row) - 7));
+        // (a bound of the largest product, by two different keys)
+        if (__any(!(top * vs_top * f[rt] <= 0x1p15f) || f[rt] == 0.0f)) {
+          float most = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, pv[j]);
+          most = row4_max(most);
+          if ((f[rt] == 0.0f || most * f[rt] > 0x1p15f) && most > 0.0f && most < __builtin_inff()) {
+            const float up = fmaxf(m2[rt], M + (float)(__builtin_amdgcn_frexp_expf(most) - 7));
             const float down = __builtin_amdgcn_exp2f(m2[rt] - up);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) acc[rt][c] *= down;
+            for (int ct = 0; ct < NC; ++ct) acc[rt][ct] *= down;
             m2[rt] = up;
-            f[rt] = __builtin_amdgcn_exp2f(fminf(m[rt] - up, 100.0f));
+            f[rt] = __builtin_amdgcn_exp2f(fminf(M - up, 100.0f));
           }
         }
 #pragma unroll
@@ -596,11 +614,11 @@ struct CachePlan {
 static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
-  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
+  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 3;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
-  const int64_t slots = (int64_t)cus * (p.rt == 1 ? 2 : 1);  // workgroups that run at once
+  const int64_t slots = (int64_t)cus * (p.rt == 1 || (p.rt == 2 && D <= 128) ? 2 : 1);  // workgroups that run at once
   const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
   int64_t w = slots / units;
   if (w < 8) {
@@ -620,7 +638,7 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
 template <int D, int CT> static void cache_attn_launch(const CacheAttnArgs& a, int rt, unsigned blocks, hipStream_t st) {
   if (rt == 1) cache_attn_kernel<D, CT, 1><<<blocks, CA_THREADS, 0, st>>>(a);
   else if (rt == 2) cache_attn_kernel<D, CT, 2><<<blocks, CA_THREADS, 0, st>>>(a);
-  else if constexpr (D < 256) cache_attn_kernel<D, CT, 4><<<blocks, CA_THREADS, 0, st>>>(a);
+  else if constexpr (D < 256) cache_attn_kernel<D, CT, 3><<<blocks, CA_THREADS, 0, st>>>(a);
 }
 
 template <int D> static void cache_attn_dims(const CacheAttnArgs& a, int ct, int rt, unsigned blocks, hipStream_t st) {
@@ -628,7 +646,7 @@ template <int D> static void cache_attn_dims(const CacheAttnArgs& a, int ct, int
   else cache_attn_launch<D, CACHE_E4M3>(a, rt, blocks, st);
   if (a.workers > 1) {
     const int64_t rows = (int64_t)a.T * a.G * a.B * a.Hkv;
-    const int slices = a.workers <= 8 ? 1 : a.workers <= 128 ? 4 : MERGE_SLICES;
+    const int slices = a.workers <= 8 || a.workers <= 4 * a.B ? 1 : a.workers <= 128 ? 4 : MERGE_SLICES;
     const int64_t blocks = slices == 1 ? (rows + 3) / 4 : rows;
     cache_merge_kernel<D><<<(unsigned)blocks, 64 * (slices == 1 ? 4 : slices), 0, st>>>(a, 16 * rt, slices);
   }
