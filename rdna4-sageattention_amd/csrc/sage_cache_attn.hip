@@ -6,15 +6,15 @@
 // scales s^k_j, s^v_j.
 //
 // Mapping.  The T * G queries that share a kv head (G = H / Hkv) are the rows of a matrix; a workgroup takes 16 RT of
-// them against a range of the keys, and its 4 waves take turns over tiles of 32 keys.  Codes go straight from memory to
-// registers (every byte is used once, by one wave), and become float16 there: int8 and E4M3 codes are exact in float16,
-// so both products run on v_mfma_f32_16x16x32_f16 with float32 accumulation.
-//  * S^T = K Q^T: A = 16 keys x 32 channels.  Lane (m = l % 16, g = l / 16) loads the D/4 channels from g D/4 on of key
+// them against a range of the keys, and its 4 waves take turns over tiles of 32 keys.  Each wave copies its own tiles
+// to LDS ahead of their use (no barrier: a wave waits for its own loads only) and turns codes to float16 as it reads them:
+// int8 and E4M3 codes are exact there, so both products run on v_mfma_f32_16x16x32_f16 with float32 accumulation.
+//  * S^T = K Q^T: A = 16 keys x 32 channels.  Lane (m = l % 16, g = l / 16) reads the D/4 channels from g D/4 on of key
 //    m, and MFMA i takes 8 of them from each g: any order of the channels will do that Q's operand has too.
 //  * The accumulator gives lane (n, g) query n and keys 4g .. 4g + 3 of each 16: with the two 16-key blocks of a tile
 //    that is, packed to float16, the B operand of O^T = V^T P^T for the key order k = 8g + 4t + i <-> key 16t + 4g + i.
-//    V's operand takes that order too: lane (m, g) loads D/16 channels of each of those 8 keys, pairs of keys are
-//    brought together by byte permutes.  Nothing crosses lanes but the row maxima, and nothing passes through LDS.
+//    V's operand takes that order too: lane (m, g) reads D/16 channels of each of those 8 keys, pairs of keys are
+//    brought together by byte permutes.  Nothing crosses lanes but the row maxima.
 //  * Q rows in bfloat16 are brought into float16's range by a power of two per row, which keeps all their bits.
 //  * P in float16 holds 11 bits of p_ij s^v_j: two running references per row, m (of x) for the sum l and m2 (of
 //    x + log2 s^v) for P, each raised only when a tile passes it by 2^8.  The largest product so far lies between 2^6 and
@@ -100,18 +100,30 @@ __device__ __forceinline__ int all_steps(const CacheAttnArgs& a, int lane, int b
   return total;
 }
 
-template <int BYTES> struct RawBytes { uint32_t w[(BYTES + 3) / 4]; };
-
-// A load at a wave-uniform base (pinned to scalar registers) and a lane's 32-bit offset: no 64-bit address per lane
-struct Base {
-  const __attribute__((address_space(1))) uint8_t* p;
-  __device__ __forceinline__ explicit Base(const void* q) : p((const __attribute__((address_space(1))) uint8_t*)q) {
-    asm volatile("" : "+s"(p));
-  }
-  template <typename V> __device__ __forceinline__ V at(uint32_t offset) const {
-    return *(const __attribute__((address_space(1))) V*)(p + offset);
-  }
-};
+// Copies 16 (or 4) bytes per lane, from a wave-uniform base plus the lane's offset, straight to LDS, where the wave's lanes lie
+// one after the other from `lds` on.  In assembly because the compiler would wait for every copy under way before each
+// read of LDS; the kernel counts its copies itself (wait_loads).  No register is written but m0, and the addresses
+// are read when the copy is issued.
+template <int BYTES> __device__ __forceinline__ void copy_lds(const void* base, uint32_t offset, uint32_t lds) {
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+// the same from an address of each lane's own
+__device__ __forceinline__ void copy_lds_from(const void* p, uint32_t lds, int bytes) {
+  if (bytes == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+template <int N> __device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N <= 63, "vmcnt immediate");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // bytes 0, 1 (half 0) or 2, 3 (half 1) of a word of codes as two float16; int8 codes come with their sign bit flipped
 template <int CT> __device__ __forceinline__ f16x2 codes_f16(uint32_t w, bool half) {
@@ -123,6 +135,13 @@ template <int CT> __device__ __forceinline__ f16x2 codes_f16(uint32_t w, bool ha
     return half ? __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true))
                 : __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false));
   }
+}
+
+// a * b where 0 times anything, an infinity or a NaN among it, is 0
+__device__ __forceinline__ float mul_zero(float a, float b) {
+  float r;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 
 __device__ __forceinline__ f16x8 join4(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
@@ -144,12 +163,24 @@ template <int D> __device__ __forceinline__ constexpr int v_channel(int m, int c
   return D == 96 ? (ct < 4 ? 4 * m + ct : 64 + 2 * m + ct - 4) : m * (D / 16) + ct;
 }
 
+// One tile in LDS, private to its wave: 32 rows of K, 32 of V, then the 32 scales of each.  The 16-byte chunks of a row are
+// swapped by the row's number so that the lanes that read one chunk of 8 rows together reach all banks (96 channels: in
+// order).
 template <int D> struct CacheTile {
-  static constexpr int KW = D / 16, VW = D == 96 ? 2 : D / 64;  // words per lane: of K per 16 keys, of V per key
-  uint32_t k[2][KW];
-  uint32_t v[8][VW];
-  v4f ks[2], vs[2];
+  static constexpr int KV = 32 * D;              // bytes of K, of V
+  static constexpr int BYTES = 2 * KV + 256;
+  static constexpr int COPIES = KV / 1024;       // copies of 1 KiB for K, for V
+  static constexpr int LOADS = 2 * COPIES + 1;   // vector loads per tile
+  static constexpr int VW = D == 96 ? 2 : D / 64;  // words of V per lane and key
+  __device__ static __forceinline__ int swap(int row) { return D == 96 ? 0 : D == 64 ? (row >> 1) & 3 : row & (D / 16 - 1); }
+  // copy j: the lane's byte offset in its block of 16 rows
+  __device__ static __forceinline__ uint32_t offset(int j, int lane) {
+    const int chunk = 64 * j + lane, row = chunk / (D / 16), c = chunk % (D / 16);
+    return (row & 15) * D + 16 * (c ^ swap(row));
+  }
 };
+// tiles of a wave in LDS: as many as let the workgroups that the registers allow share a CU's 160 KiB
+template <int D, int RT> constexpr int ring_tiles() { return D == 64 ? 4 : RT == 3 ? (D == 96 ? 5 : 4) : 2; }
 
 // rows in front of the first of 16 keys from k0 on; a page outside the cache hides its keys: page 0 is read in its place
 struct CacheRow {
@@ -162,7 +193,11 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
   constexpr int NK = D / 32, NC = D / 16;
   constexpr int ROWS = 16 * RT;
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
-  __shared__ __attribute__((aligned(16))) float so[CA_WAVES][16][LD];
+  using Tile = CacheTile<D>;
+  constexpr int NS = ring_tiles<D, RT>();
+  constexpr int JOIN = CA_WAVES * 16 * LD * 4, RING = CA_WAVES * NS * Tile::BYTES;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[JOIN > RING ? JOIN : RING];
+  float (*so)[16][LD] = reinterpret_cast<float (*)[16][LD]>(smem);  // (the waves are joined after their last tile)
   __shared__ float sm[CA_WAVES][ROWS], sm2[CA_WAVES][ROWS], sl[CA_WAVES][ROWS];
 
   // the row blocks of one range of keys on one XCD, next to each other
@@ -201,48 +236,6 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
   const int open = a.tree ? base : a.causal ? base + 1 : len;
   const int k_begin = first * CA_STEP, k_end = min(len, (first + take) * CA_STEP);
 
-  // Q operand and the rows' factors
-  f16x8 qf[RT][NK];
-  float qs[RT];
-  int row_t[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = rb * ROWS + rt * 16 + n;
-    const int rr = min(r, rows - 1);
-    const int t = rr / a.G, hq = h * a.G + rr % a.G;
-    row_t[rt] = t;
-    const uint16_t* qp = a.q + b * a.qsb + t * a.qss + hq * a.qsh + g * (D / 4);
-    uint32_t w[D / 8];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const v4i x = *reinterpret_cast<const v4i*>(qp + 8 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[4 * i + j] = (uint32_t)x[j];
-    }
-    qs[rt] = a.scale;
-    if (a.dtype == DT_BF16) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
-      const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
-      // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
-      const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
-      const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
-      qs[rt] *= down;
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          qf[rt][i][2 * j] = (_Float16)(bf16_lo(w[4 * i + j]) * up);
-          qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-        qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
-    }
-  }
-
   float m[RT], m2[RT], f[RT], l[RT];
   v4f acc[RT][NC];
 #pragma unroll
@@ -261,76 +254,128 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
     const bool usable = page >= 0 && page < a.pages;
     return CacheRow{((int64_t)(usable ? page : 0) * a.Hkv + h) * a.page_size + (k0 & (a.page_size - 1)), usable};
   };
-  const uint32_t k_off = n * D + g * (D / 4), s_off = 16 * g;
-  const uint32_t v_off = 4 * g * D + (D == 96 ? 4 : D / 16) * n;
-  auto load_k = [&](CacheTile<D>& x, const CacheRow (&at)[2]) {
+  uint8_t* ring = smem + wave * (NS * Tile::BYTES);
+  uint32_t from[Tile::COPIES];  // (for head dims 64 and 128 all copies have one offset, but for a constant)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Base kp(a.k8 + at[t].row * D);
-      if constexpr (D == 96) {
+  for (int j = 0; j < Tile::COPIES; ++j) from[j] = Tile::offset(j, lane);
+  const uint32_t ring_at = lds_address(ring);
+  auto issue = [&](CacheRow at0, CacheRow at1, int stage) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(ring_at + stage * Tile::BYTES);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const v2i w = kp.at<v2i>(k_off + 8 * i);
-          x.k[t][2 * i] = w[0], x.k[t][2 * i + 1] = w[1];
-        }
-      } else {
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint8_t* codes = kv ? a.v8 : a.k8;
+      const uint8_t *p0 = codes + at0.row * D, *p1 = codes + at1.row * D;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const v4i w = kp.at<v4i>(k_off + 16 * i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = (uint32_t)w[j];
-        }
-      }
-      x.ks[t] = Base(a.ks + at[t].row).at<v4f>(s_off);
-    }
-  };
-  auto load_v = [&](CacheTile<D>& x, const CacheRow (&at)[2]) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x.vs[t] = Base(a.vs + at[t].row).at<v4f>(s_off);
-      const Base vp(a.v8 + at[t].row * D);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t* w = x.v[4 * t + i];
-        if constexpr (D == 64) {
-          w[0] = vp.at<uint32_t>(v_off + i * D);
-        } else if constexpr (D == 96) {
-          w[0] = vp.at<uint32_t>(v_off + i * D);
-          w[1] = vp.at<uint16_t>(v_off + i * D + 64 - 2 * n);
-        } else if constexpr (D == 128) {
-          const v2i y = vp.at<v2i>(v_off + i * D);
-          w[0] = y[0], w[1] = y[1];
-        } else {
-          const v4i y = vp.at<v4i>(v_off + i * D);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = (uint32_t)y[j];
-        }
+      for (int j = 0; j < Tile::COPIES; ++j) {
+        const uint32_t dst = to + kv * Tile::KV + 1024 * j;
+        if (D == 96 && j == 1) copy_lds_from((lane < 32 ? p0 : p1) + from[j], dst, 16);  // half of it in each block
+        else copy_lds<16>(2 * j / Tile::COPIES ? p1 : p0, from[j], dst);
       }
     }
+    const int64_t row = (lane & 16 ? at1.row : at0.row) + (lane & 15);
+    copy_lds_from((lane < 32 ? a.ks : a.vs) + row, to + 2 * Tile::KV, 4);
   };
+  // where the lane's operands lie in a tile: K of key n, V of key 4 g (keys and chunks further on differ by constants)
+  const int k_at = n * D + (D == 96 ? 24 * g : 16 * ((D / 64 * g) ^ Tile::swap(n)));
+  const int v_per = D == 96 ? 4 : D / 16;  // bytes of a key that the lane starts from
+  const int v_at = 4 * g * D + (v_per * n & 15) + 16 * ((v_per * n >> 4) ^ (D == 96 ? 0 : Tile::swap(4 * g)));
 
-  // One tile in registers: the next tile's K is loaded once this one's scores are there, its V after the output's
-  // products, so that loads are in flight through the whole step.
+  // NS tiles on their way or in use (the last one again where there are fewer)
   int k0 = k_begin + wave * CA_TILE;
-  if (k0 < k_end) {
-    CacheTile<D> x;
-    CacheRow now[2] = {rows_of(k0), rows_of(k0 + 16)};
-    load_k(x, now);
-    load_v(x, now);
-    for (;;) {
-      const int k1 = k0 + CA_STEP;
-      const bool more = k1 < k_end;
-      CacheRow next[2] = {now[0], now[1]};
-      if (more) next[0] = rows_of(k1), next[1] = rows_of(k1 + 16);
-      const bool masked = k0 + CA_TILE > open || !now[0].usable || !now[1].usable;
+  const int tiles = k0 < k_end ? (k_end - k0 + CA_STEP - 1) / CA_STEP : 0;
+  uint32_t usable = 0;  // bits 2 i, 2 i + 1: the two pages of tile i from the current one on
+  if (tiles) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int k = k0 + min(i, tiles - 1) * CA_STEP;
+      const CacheRow at0 = rows_of(k), at1 = rows_of(k + 16);
+      usable |= ((uint32_t)at0.usable | (uint32_t)at1.usable << 1) << 2 * i;
+      issue(at0, at1, i);
+    }
+  }
+
+  // Q operand and the rows' factors
+  f16x8 qf[RT][NK];
+  float qs[RT];
+  int row_t[RT];
+  uint32_t qw[RT][D / 8];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(rb * ROWS + rt * 16 + n, rows - 1);
+    const int t = r / a.G, hq = h * a.G + r % a.G;
+    row_t[rt] = t;
+    const uint16_t* qp = a.q + b * a.qsb + t * a.qss + hq * a.qsh + g * (D / 4);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const v4i x = *reinterpret_cast<const v4i*>(qp + 8 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qw[rt][4 * i + j] = (uint32_t)x[j];
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const uint32_t(&w)[D / 8] = qw[rt];
+    qs[rt] = a.scale;  // (positive: a hidden score stays -inf)
+    if (a.dtype == DT_BF16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
+      const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
+      // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
+      const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
+      const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
+      qs[rt] = fmaxf(qs[rt] * down, 0x1p-126f);
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qf[rt][i][2 * j] = (_Float16)(bf16_lo(w[4 * i + j]) * up);
+          qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
+    }
+#pragma unroll
+    for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(qf[rt][i]));  // waited for here, not in the loop
+  }
+
+  if (tiles) {
+    int stage = 0;
+    for (int left = tiles;; --left, k0 += CA_STEP) {
+      // the loads of the tiles behind this one may be outstanding
+      if (left >= NS) wait_loads<(NS - 1) * Tile::LOADS>();
+      else if (NS > 2 && left == 2) wait_loads<Tile::LOADS>();
+      else wait_loads<0>();
+      uint8_t* tile = ring + stage * Tile::BYTES;
+      const bool more = left > NS;
+      CacheRow next0 = {0, false}, next1 = {0, false};
+      if (more) next0 = rows_of(k0 + NS * CA_STEP), next1 = rows_of(k0 + NS * CA_STEP + 16);
+      const bool masked = k0 + CA_TILE > open || (usable & 3) != 3;
       v4f s[RT][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t kw[D / 16];
+        if constexpr (D == 96) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const v2i w = *reinterpret_cast<const v2i*>(tile + 16 * t * D + k_at + 8 * i);
+            kw[2 * i] = w[0], kw[2 * i + 1] = w[1];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            const v4i w = *reinterpret_cast<const v4i*>(tile + 16 * t * D + (k_at ^ 16 * i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kw[4 * i + j] = (uint32_t)w[j];
+          }
+        }
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-          uint32_t w0 = x.k[t][2 * i], w1 = x.k[t][2 * i + 1];
+          uint32_t w0 = kw[2 * i], w1 = kw[2 * i + 1];
           if (CT == CACHE_INT8) w0 ^= 0x80808080u, w1 ^= 0x80808080u;
           const f16x8 ka = join4(codes_f16<CT>(w0, false), codes_f16<CT>(w0, true), codes_f16<CT>(w1, false),
                                  codes_f16<CT>(w1, true));
@@ -338,42 +383,67 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
           for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
         }
       }
-      v4f ks[2] = {x.ks[0], x.ks[1]};
-      if (more) load_k(x, next);
-      uint32_t hidden[RT];  // bit 4 t + i
+      v4f ks[2], vs[2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) hidden[rt] = 0;
+      for (int t = 0; t < 2; ++t) {
+        ks[t] = *reinterpret_cast<const v4f*>(tile + 2 * Tile::KV + 64 * t + 16 * g);
+        vs[t] = *reinterpret_cast<const v4f*>(tile + 2 * Tile::KV + 128 + 64 * t + 16 * g);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[rt][t] *= ks[t];
+      }
+      // Tiles with hidden keys: their scores become -inf.  The rest needs no selects: a weight of 0 times whatever scale is 0
+      // (the products below are of that kind), and V codes of keys past the sequence or on no page, which may be NaN, become 0
+      // where the lane reads them.
       if (masked) {
+        const int node = k0 + 4 * g - base;  // of bit 0
+        uint32_t gone = 0;                   // bit 4 t + i
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = j / 4, key = k0 + 16 * t + 4 * g + j % 4, node = key - base;
-          const bool none = key >= len || !now[t].usable;
-          if (none) {  // whatever the memory past a sequence holds: no NaN enters the products
-#pragma unroll
-            for (int i = 0; i < CacheTile<D>::VW; ++i) x.v[j][i] = CT == CACHE_INT8 ? 0x80808080u : 0u;
-            x.vs[t][j % 4] = 0.0f;
-          }
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            bool hide = node > row_t[rt] && a.causal;
-            if (a.tree) hide = node >= 0 && a.tree[b * a.msb + row_t[rt] * a.msq + min(max(node, 0), a.T - 1) * a.msk] == 0;
-            hidden[rt] |= (uint32_t)(hide || none) << j;
+          if (k0 + 4 * g + 16 * (j / 4) + j % 4 >= len || !(usable >> (j / 4) & 1)) {
+            gone |= 1u << j;
+            if (CT == CACHE_E4M3) {
+              uint8_t* vp = tile + Tile::KV + (16 * (j / 4) + j % 4) * D;
+              if constexpr (D == 64) *reinterpret_cast<uint32_t*>(vp + (v_at ^ 16 * (j % 4 / 2))) = 0;
+              else if constexpr (D == 128) *reinterpret_cast<v2i*>(vp + (v_at ^ 16 * (j % 4))) = v2i{0, 0};
+              else if constexpr (D == 256) *reinterpret_cast<v4i*>(vp + (v_at ^ 16 * (j % 4))) = v4i{0, 0, 0, 0};
+              else {
+                *reinterpret_cast<uint32_t*>(vp + v_at) = 0;
+                *reinterpret_cast<uint16_t*>(vp + 4 * g * D + 64 + 2 * n) = 0;
+              }
+            }
           }
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          uint32_t hidden = gone;
+          if (a.tree) {
+            const uint8_t* shown = a.tree + b * a.msb + row_t[rt] * a.msq;
+            uint8_t see[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) see[j] = shown[min(max(node + 16 * (j / 4) + j % 4, 0), a.T - 1) * a.msk];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(see[j] == 0 && node + 16 * (j / 4) + j % 4 >= 0) << j;
+          } else if (a.causal) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(node + 16 * (j / 4) + j % 4 > row_t[rt]) << j;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (hidden >> j & 1) s[rt][j / 4][j % 4] = -__builtin_inff();
+        }
+        asm volatile("" ::: "memory");  // (a block of its own: never turned into selects for every tile)
       }
       float vs_top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, x.vs[j / 4][j % 4]);
+      for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, vs[j / 4][j % 4]);
       f16x8 pf[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float c[8], p[8], pv[8];
+        float p[8], pv[8];
         float& M = m[rt];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          c[j] = ks[j / 4][j % 4] * qs[rt];
-          if (masked && (hidden[rt] >> j & 1)) s[rt][j / 4][j % 4] = -__builtin_inff(), c[j] = 1.0f;
-        }
         // the terms against the references so far; where one passes them by too much (or a row has none yet) the references
         // are raised first
         auto terms = [&] {
@@ -381,7 +451,7 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
           float top = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], c[j], -ref));
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], qs[rt], -ref));
             top = fmaxf(top, p[j]);
           }
           return top;
@@ -390,7 +460,7 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
         if (__any(!(top <= 0x1p8f) || M == -__builtin_inff())) {
           float y = -__builtin_inff();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * c[j]);
+          for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * qs[rt]);
           const float up = fmaxf(M, row4_max(y));
           if (up > M) {
             l[rt] *= __builtin_amdgcn_exp2f(M - up);
@@ -402,8 +472,7 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           l[rt] += p[j];
-          pv[j] = p[j] * x.vs[j / 4][j % 4];
-          if (masked && (hidden[rt] >> j & 1)) pv[j] = 0.0f;
+          pv[j] = mul_zero(p[j], vs[j / 4][j % 4]);
         }
         // (a bound of the largest product, by two different keys)
         if (__any(!(top * vs_top * f[rt] <= 0x1p15f) || f[rt] == 0.0f)) {
@@ -424,11 +493,29 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
         for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
       }
       // V operand: keys (0, 1), (2, 3) of each block side by side
+      uint32_t vw[8][Tile::VW];
 #pragma unroll
-      for (int i = 0; i < CacheTile<D>::VW; ++i) {
+      for (int j = 0; j < 8; ++j) {
+        const uint8_t* vp = tile + Tile::KV + (16 * (j / 4) + j % 4) * D;
+        if constexpr (D == 64) {
+          vw[j][0] = *reinterpret_cast<const uint32_t*>(vp + (v_at ^ 16 * (j % 4 / 2)));
+        } else if constexpr (D == 96) {
+          vw[j][0] = *reinterpret_cast<const uint32_t*>(vp + v_at);
+          vw[j][1] = *reinterpret_cast<const uint16_t*>(vp + 4 * g * D + 64 + 2 * n);
+        } else if constexpr (D == 128) {
+          const v2i y = *reinterpret_cast<const v2i*>(vp + (v_at ^ 16 * (j % 4)));
+          vw[j][0] = y[0], vw[j][1] = y[1];
+        } else {
+          const v4i y = *reinterpret_cast<const v4i*>(vp + (v_at ^ 16 * (j % 4)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vw[j][i] = (uint32_t)y[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < Tile::VW; ++i) {
         if (CT == CACHE_INT8) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x.v[j][i] ^= 0x80808080u;
+          for (int j = 0; j < 8; ++j) vw[j][i] ^= 0x80808080u;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {  // channels 4 i + 2 u, + 1 of the lane
@@ -436,7 +523,7 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // bytes (A_2u, B_2u, A_2u+1, B_2u+1)
-            w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i], x.v[2 * j][i], u ? 0x07030602u : 0x05010400u);
+            w[j] = __builtin_amdgcn_perm(vw[2 * j + 1][i], vw[2 * j][i], u ? 0x07030602u : 0x05010400u);
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
             const int c = 4 * i + 2 * u + o;
@@ -446,10 +533,15 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
           }
         }
       }
-      if (!more) break;
-      load_v(x, next);
-      now[0] = next[0], now[1] = next[1];
-      k0 = k1;
+      if (left == 1) break;
+      usable >>= 2;
+      if (more) {
+        usable |= ((uint32_t)next0.usable | (uint32_t)next1.usable << 1) << 2 * (NS - 1);
+        // the tile's reads are done: its place takes the one NS tiles on
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue(next0, next1, stage);
+      }
+      stage = stage + 1 == NS ? 0 : stage + 1;
     }
   }
 
@@ -618,7 +710,7 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
-  const int64_t slots = (int64_t)cus * (p.rt == 1 || (p.rt == 2 && D <= 128) ? 2 : 1);  // workgroups that run at once
+  const int64_t slots = (int64_t)cus * (p.rt == 3 || D == 256 ? 1 : 2);  // workgroups that run at once
   const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
   int64_t w = slots / units;
   if (w < 8) {
@@ -722,6 +814,7 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   a.row_blocks = p.row_blocks, a.workers = p.workers, a.part_rows = p.part_rows;
   const double scale = sm_scale > 0.0f ? (double)sm_scale : 1.0 / __builtin_sqrt((double)D);
   a.scale = (float)(scale * 1.44269504088896340736);
+  if (a.scale < 0x1p-126f) a.scale = 0x1p-126f;
   a.part_o = (float*)workspace;
   a.part_lse = (float*)((char*)workspace + p.o_bytes);
   const int64_t groups = ((int64_t)Hkv * p.workers + 7) / 8 * 8;
