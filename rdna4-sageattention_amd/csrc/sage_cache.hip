@@ -37,7 +37,7 @@ struct CacheRows {
   float* scale[2];
   const void* slots;             // [B * S]
   int slots64, S, tokens, Hkv;
-  int page_size;
+  int page_shift;
   int64_t capacity;              // pages * page_size
 };
 
@@ -45,88 +45,132 @@ struct CacheRows {
 __device__ __forceinline__ int64_t cache_row(const CacheRows& a, int tok, int h) {
   const int64_t slot = a.slots64 ? static_cast<const int64_t*>(a.slots)[tok] : static_cast<const int32_t*>(a.slots)[tok];
   if (slot < 0 || slot >= a.capacity) return -1;
-  const int64_t page = slot / a.page_size;
-  return (page * a.Hkv + h) * a.page_size + (slot - page * a.page_size);
+  const int64_t page = slot >> a.page_shift;
+  return ((page * a.Hkv + h) << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
 }
 
 // One row per row_lanes lanes, neighbouring rows = neighbouring tokens of a head (their codes and scales are neighbours
-// in a page); blockIdx.y = head, blockIdx.z = k or v.
-template <int D, int DT, int CT> __global__ __launch_bounds__(CACHE_THREADS) void cache_write_kernel(const CacheRows a) {
-  constexpr int L = row_lanes<D>();
-  const int tok = blockIdx.x * (CACHE_THREADS / L) + threadIdx.x / L, l = threadIdx.x % L;
-  const int h = blockIdx.y, w = blockIdx.z;
-  if (tok >= a.tokens) return;
-  const int64_t row = cache_row(a, tok, h);
-  if (row < 0) return;
-  const int b = tok / a.S, s = tok - b * a.S;
-  const bool mine = D != 96 || l < 12;
-  v4i x = {0, 0, 0, 0};
-  if (mine) x = *reinterpret_cast<const v4i*>(a.x[w] + b * a.sb[w] + s * a.ss[w] + h * a.sh[w] + 8 * l);
-  uint32_t top = 0;
+// in a page); blockIdx.y = head, blockIdx.z = k or v.  A thread takes U rows, a workgroup's rows apart, whose loads are in
+// flight together.
+template <int D, int U> struct RowsOf {
+  static constexpr int L = row_lanes<D>(), PER = CACHE_THREADS / L;
+  int tok[U], l;
+  bool mine;  // (96 channels leave lanes without any)
+  int64_t row[U], at[U];
+  __device__ __forceinline__ RowsOf(const CacheRows& a, int h, int w) {
+    l = threadIdx.x % L;
+    mine = D != 96 || l < 12;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = (uint32_t)x[i] & 0x7FFF7FFFu;
-    top = max(top, max(u & 0xFFFFu, u >> 16));
-  }
-  top = lanes_max<L>(top);
-  const bool bad = top >= (DT == DT_BF16 ? 0x7F80u : 0x7C00u);
-  const float amax = elem_lo<DT>(top);
-  // rows near the ends of float32's range are brought inside it by a power of two, which changes no quotient
-  const float fit = amax < 0x1p-60f ? 0x1p100f : amax > 0x1p60f ? 0x1p-100f : 1.0f;
-  const float div = amax == 0.0f ? 1.0f : amax * fit, rec = 1.0f / div;
-  constexpr float Q = CT == CACHE_INT8 ? 127.0f : 448.0f;
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // (the correction of the quotient loses the sign of a zero)
-    const float lo = elem_lo<DT>(x[i]), hi = elem_hi<DT>(x[i]);
-    y[2 * i] = __builtin_copysignf(div_by_scale(lo * fit * Q, div, rec), lo);
-    y[2 * i + 1] = __builtin_copysignf(div_by_scale(hi * fit * Q, div, rec), hi);
-  }
-  v2i codes;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float* z = y + 4 * i;
-    int c;
-    if (CT == CACHE_INT8) {
-      c = (int)pack4_i8((int)__builtin_rintf(z[0]), (int)__builtin_rintf(z[1]), (int)__builtin_rintf(z[2]),
-                        (int)__builtin_rintf(z[3]));
-    } else {
-      c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-      c = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+    for (int u = 0; u < U; ++u) {
+      tok[u] = (blockIdx.x * U + u) * PER + threadIdx.x / L;
+      row[u] = tok[u] < a.tokens ? cache_row(a, tok[u], h) : -1;
     }
-    codes[i] = bad ? 0 : c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = min(tok[u], a.tokens - 1), b = t / a.S, s = t - b * a.S;
+      at[u] = b * a.sb[w] + s * a.ss[w] + h * a.sh[w] + 8 * l;
+    }
   }
-  if (mine) *reinterpret_cast<v2i*>(a.codes[w] + row * D + 8 * l) = codes;
-  if (l == 0) a.scale[w][row] = bad ? __builtin_nanf("") : amax / Q;
+};
+
+template <int D, int DT, int CT, int U>
+__global__ __launch_bounds__(CACHE_THREADS) void cache_write_kernel(const CacheRows a) {
+  constexpr int L = row_lanes<D>();
+  const int h = blockIdx.y, w = blockIdx.z;
+  const RowsOf<D, U> r(a, h, w);
+  v4i in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    in[u] = v4i{0, 0, 0, 0};
+    if (r.mine && r.row[u] >= 0) in[u] = *reinterpret_cast<const v4i*>(a.x[w] + r.at[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const v4i x = in[u];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = (uint32_t)x[i] & 0x7FFF7FFFu;
+      top = max(top, max(m & 0xFFFFu, m >> 16));
+    }
+    top = lanes_max<L>(top);
+    const bool bad = top >= (DT == DT_BF16 ? 0x7F80u : 0x7C00u);
+    const float amax = elem_lo<DT>(top);
+    // rows near the ends of float32's range are brought inside it by a power of two, which changes no quotient
+    const float fit = amax < 0x1p-60f ? 0x1p100f : amax > 0x1p60f ? 0x1p-100f : 1.0f;
+    const float div = amax == 0.0f ? 1.0f : amax * fit, rec = 1.0f / div;
+    constexpr float Q = CT == CACHE_INT8 ? 127.0f : 448.0f;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (the correction of the quotient loses the sign of a zero)
+      const float lo = elem_lo<DT>(x[i]), hi = elem_hi<DT>(x[i]);
+      y[2 * i] = __builtin_copysignf(div_by_scale(lo * fit * Q, div, rec), lo);
+      y[2 * i + 1] = __builtin_copysignf(div_by_scale(hi * fit * Q, div, rec), hi);
+    }
+    v2i codes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float* z = y + 4 * i;
+      int c;
+      if (CT == CACHE_INT8) {
+        c = (int)pack4_i8((int)__builtin_rintf(z[0]), (int)__builtin_rintf(z[1]), (int)__builtin_rintf(z[2]),
+                          (int)__builtin_rintf(z[3]));
+      } else {
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+      }
+      codes[i] = bad ? 0 : c;
+    }
+    if (r.row[u] >= 0) {
+      if (r.mine) *reinterpret_cast<v2i*>(a.codes[w] + r.row[u] * D + 8 * r.l) = codes;
+      if (r.l == 0) a.scale[w][r.row[u]] = bad ? __builtin_nanf("") : amax / Q;
+    }
+  }
 }
 
-template <int D, int DT, int CT> __global__ __launch_bounds__(CACHE_THREADS) void cache_read_kernel(const CacheRows a) {
-  constexpr int L = row_lanes<D>();
-  const int tok = blockIdx.x * (CACHE_THREADS / L) + threadIdx.x / L, l = threadIdx.x % L;
+template <int D, int DT, int CT, int U>
+__global__ __launch_bounds__(CACHE_THREADS) void cache_read_kernel(const CacheRows a) {
   const int h = blockIdx.y, w = blockIdx.z;
-  if (tok >= a.tokens || (D == 96 && l >= 12)) return;
-  const int64_t row = cache_row(a, tok, h);
-  const int b = tok / a.S, s = tok - b * a.S;
-  v4i out = {0, 0, 0, 0};
-  if (row >= 0) {
-    const v2i c = *reinterpret_cast<const v2i*>(a.codes[w] + row * D + 8 * l);
-    const float scale = a.scale[w][row];
+  const RowsOf<D, U> r(a, h, w);
+  if (!r.mine) return;
+  v2i c[U];
+  float scale[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    c[u] = v2i{0, 0};
+    scale[u] = 0.0f;
+    if (r.row[u] >= 0) {
+      c[u] = *reinterpret_cast<const v2i*>(a.codes[w] + r.row[u] * D + 8 * r.l);
+      scale[u] = a.scale[w][r.row[u]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (r.tok[u] >= a.tokens) break;
+    v4i out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float lo, hi;
-      code_pair<CT>((uint32_t)c[i / 2], i & 1, lo, hi);
-      out[i] = (int)(f32_to_out_bits<DT>(lo * scale) | (f32_to_out_bits<DT>(hi * scale) << 16));
+      code_pair<CT>((uint32_t)c[u][i / 2], i & 1, lo, hi);
+      out[i] = (int)(f32_to_out_bits<DT>(lo * scale[u]) | (f32_to_out_bits<DT>(hi * scale[u]) << 16));
     }
+    *reinterpret_cast<v4i*>(a.y[w] + r.at[u]) = out;
   }
-  *reinterpret_cast<v4i*>(a.y[w] + b * a.sb[w] + s * a.ss[w] + h * a.sh[w] + 8 * l) = out;
 }
 
 template <int D, int DT, int CT> static void cache_rows_launch(const CacheRows& a, bool write, hipStream_t st) {
-  const int rows = CACHE_THREADS / row_lanes<D>();
-  const dim3 grid((a.tokens + rows - 1) / rows, a.Hkv, 2);
-  if (write) cache_write_kernel<D, DT, CT><<<grid, CACHE_THREADS, 0, st>>>(a);
-  else cache_read_kernel<D, DT, CT><<<grid, CACHE_THREADS, 0, st>>>(a);
+  const int per = CACHE_THREADS / row_lanes<D>();
+  // four rows per thread where that leaves every CU some waves
+  const int u = (int64_t)a.tokens * a.Hkv * row_lanes<D>() >= 4 * 256 * 1024 ? 4 : 1;
+  const dim3 grid((a.tokens + per * u - 1) / (per * u), a.Hkv, 2);
+  if (u == 4) {
+    if (write) cache_write_kernel<D, DT, CT, 4><<<grid, CACHE_THREADS, 0, st>>>(a);
+    else cache_read_kernel<D, DT, CT, 4><<<grid, CACHE_THREADS, 0, st>>>(a);
+  } else {
+    if (write) cache_write_kernel<D, DT, CT, 1><<<grid, CACHE_THREADS, 0, st>>>(a);
+    else cache_read_kernel<D, DT, CT, 1><<<grid, CACHE_THREADS, 0, st>>>(a);
+  }
 }
 template <int D, int DT> static void cache_rows_codes(const CacheRows& a, int ct, bool write, hipStream_t st) {
   if (ct == CACHE_INT8) cache_rows_launch<D, DT, CACHE_INT8>(a, write, st);
@@ -174,7 +218,7 @@ static int cache_rows(const void* k, int64_t ksb, int64_t kss, int64_t ksh, cons
   a.sb[0] = ksb, a.ss[0] = kss, a.sh[0] = ksh, a.sb[1] = vsb, a.ss[1] = vss, a.sh[1] = vsh;
   a.codes[0] = (uint8_t*)k8, a.codes[1] = (uint8_t*)v8, a.scale[0] = ks, a.scale[1] = vs;
   a.slots = slots, a.slots64 = slots64, a.S = S, a.tokens = B * S, a.Hkv = Hkv;
-  a.page_size = page_size, a.capacity = (int64_t)pages * page_size;
+  a.page_shift = __builtin_ctz((unsigned)page_size), a.capacity = (int64_t)pages * page_size;
   if (dtype == SAGE_DTYPE_BF16) cache_rows_dims<DT_BF16>(a, D, cache_dtype, write, (hipStream_t)stream);
   else cache_rows_dims<DT_F16>(a, D, cache_dtype, write, (hipStream_t)stream);
   return check_launch(who);

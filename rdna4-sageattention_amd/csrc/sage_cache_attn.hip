@@ -706,7 +706,7 @@ struct CachePlan {
 static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
-  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 3;
+  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 || 1 ? 2 : 3;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
