@@ -50,8 +50,9 @@ __device__ __forceinline__ int64_t cache_row(const CacheRows& a, int tok, int h)
 }
 
 // One row per row_lanes lanes, neighbouring rows = neighbouring tokens of a head (their codes and scales are neighbours
-// in a page); blockIdx.y = head, blockIdx.z = k or v.  A thread takes U rows, a workgroup's rows apart, whose loads are in
-// flight together.
+// in a page); the heads of some tokens in neighbouring workgroups (read: 130000 tokens of 8 heads x 128 in 194 us, 214 with the
+// heads far apart); blockIdx.y = k or v.  A thread takes U rows, a workgroup's rows apart, whose loads are in flight
+// together.
 template <int D, int U> struct RowsOf {
   static constexpr int L = row_lanes<D>(), PER = CACHE_THREADS / L;
   int tok[U], l;
@@ -62,7 +63,7 @@ template <int D, int U> struct RowsOf {
     mine = D != 96 || l < 12;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      tok[u] = (blockIdx.x * U + u) * PER + threadIdx.x / L;
+      tok[u] = (int)((blockIdx.x / a.Hkv * U + u) * PER) + threadIdx.x / L;
       row[u] = tok[u] < a.tokens ? cache_row(a, tok[u], h) : -1;
     }
 #pragma unroll
@@ -76,7 +77,7 @@ template <int D, int U> struct RowsOf {
 template <int D, int DT, int CT, int U>
 __global__ __launch_bounds__(CACHE_THREADS) void cache_write_kernel(const CacheRows a) {
   constexpr int L = row_lanes<D>();
-  const int h = blockIdx.y, w = blockIdx.z;
+  const int h = blockIdx.x % a.Hkv, w = blockIdx.y;
   const RowsOf<D, U> r(a, h, w);
   v4i in[U];
 #pragma unroll
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(CACHE_THREADS) void cache_write_kernel(const CacheR
 
 template <int D, int DT, int CT, int U>
 __global__ __launch_bounds__(CACHE_THREADS) void cache_read_kernel(const CacheRows a) {
-  const int h = blockIdx.y, w = blockIdx.z;
+  const int h = blockIdx.x % a.Hkv, w = blockIdx.y;
   const RowsOf<D, U> r(a, h, w);
   if (!r.mine) return;
   v2i c[U];
@@ -163,7 +164,7 @@ template <int D, int DT, int CT> static void cache_rows_launch(const CacheRows& 
   const int per = CACHE_THREADS / row_lanes<D>();
   // four rows per thread where that leaves every CU some waves
   const int u = (int64_t)a.tokens * a.Hkv * row_lanes<D>() >= 4 * 256 * 1024 ? 4 : 1;
-  const dim3 grid((a.tokens + per * u - 1) / (per * u), a.Hkv, 2);
+  const dim3 grid((unsigned)((a.tokens + per * u - 1) / (per * u)) * a.Hkv, 2);
   if (u == 4) {
     if (write) cache_write_kernel<D, DT, CT, 4><<<grid, CACHE_THREADS, 0, st>>>(a);
     else cache_read_kernel<D, DT, CT, 4><<<grid, CACHE_THREADS, 0, st>>>(a);
@@ -211,7 +212,7 @@ static int cache_rows(const void* k, int64_t ksb, int64_t kss, int64_t ksh, cons
                "%s: strides must be multiples of 8 elements", who);
   SAGE_REQUIRE(((uintptr_t)slots & (slots64 ? 7u : 3u)) == 0, "%s: slots misaligned", who);
   if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
-  SAGE_REQUIRE((int64_t)B * S <= 0x3FFFFFFF && Hkv <= 65535, "%s: too many tokens or heads", who);
+  SAGE_REQUIRE((int64_t)B * S <= 0x3FFFFFFF && (int64_t)B * S * Hkv <= 0x7FFFFFFF, "%s: too many tokens or heads", who);
   CacheRows a = {};
   if (write) a.x[0] = (const uint16_t*)k, a.x[1] = (const uint16_t*)v;
   else a.y[0] = (uint16_t*)const_cast<void*>(k), a.y[1] = (uint16_t*)const_cast<void*>(v);

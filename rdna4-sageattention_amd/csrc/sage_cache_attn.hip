@@ -54,7 +54,7 @@ struct CacheAttnArgs {
 };
 
 // Work of one kv head and row block: the steps (CA_STEP keys) of all sequences in a row, at least one each, cut into
-// `workers` ranges as equal as whole steps allow, whatever the sequences' lengths.  A worker's range holds whole sequences,
+// `workers` ranges that differ by one step at most, the longer ones first, whatever the sequences' lengths.  A worker's range holds whole sequences,
 // whose output it writes, and up to two parts: of the one it begins inside of (partial 0) and of the one that it begins
 // but does not end (partial 1); a second kernel joins those.  The lengths stay on the device: every wave adds them up.
 __device__ __forceinline__ int cache_keys(const CacheAttnArgs& a, int b) {
@@ -83,6 +83,19 @@ __device__ __forceinline__ int wave_scan(int x) {
   x = dpp_add<0x143, 0xC>(x);
   return x;
 }
+struct Shares {
+  int workers, per, longer;  // ranges; steps of each; ranges with one more
+  __device__ __forceinline__ Shares(int most, int total) {
+    workers = min(most, total);
+    per = total / workers;
+    longer = total - per * workers;
+  }
+  __device__ __forceinline__ int begin(int worker) const { return worker * per + min(worker, longer); }
+  __device__ __forceinline__ int worker_of(int step) const {
+    const int edge = longer * (per + 1);
+    return step < edge ? step / (per + 1) : longer + (step - edge) / per;
+  }
+};
 // steps of sequences [64 c, 64 c + 64), one per lane
 __device__ __forceinline__ int lane_steps(const CacheAttnArgs& a, int c, int lane) {
   const int b = 64 * c + lane;
@@ -208,11 +221,11 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
   const int rows = a.T * a.G;
   int unused;
   const int total = all_steps(a, lane, -1, unused);
-  const int workers = min(a.workers, total);
+  const Shares shares(a.workers, total);
   const int h = grp / a.workers, worker = grp % a.workers;
-  if (h >= a.Hkv || worker >= workers) return;
-  int s0 = (int)((int64_t)worker * total / workers);
-  const int s1 = (int)((int64_t)(worker + 1) * total / workers);
+  if (h >= a.Hkv || worker >= shares.workers) return;
+  int s0 = shares.begin(worker);
+  const int s1 = shares.begin(worker + 1);
   // the sequence of step s0, and the step's place in it
   int b = 0, first = 0;
   for (int c = 0, sum = 0; 64 * c < a.B; ++c) {
@@ -626,16 +639,14 @@ template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merg
   __shared__ float sml[MERGE_SLICES][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = a.T * a.G;
-  const int64_t at = slices == 1 ? (int64_t)blockIdx.x * (blockDim.x / 64) + wave : blockIdx.x;
-  if (at >= (int64_t)rows * a.B * a.Hkv) return;
+  const int at = slices == 1 ? blockIdx.x * (blockDim.x / 64) + wave : blockIdx.x;
+  if (at >= rows * a.B * a.Hkv) return;
   const int slice = slices == 1 ? 0 : wave;
-  const int R = (int)(at % rows), h = (int)(at / rows % a.Hkv), b = (int)(at / rows / a.Hkv);
+  const int pair = at / rows, R = at - pair * rows, b = pair / a.Hkv, h = pair - b * a.Hkv;
   int before;
   const int total = all_steps(a, lane, b, before), steps = cache_steps(uniform_keys(a, b));
-  const int workers = min(a.workers, total);
-  // the last worker that begins at a step or before it
-  auto worker_of = [&](int step) { return (int)((((int64_t)step + 1) * workers - 1) / total); };
-  const int w0 = worker_of(before), parts = worker_of(before + steps - 1) - w0 + 1;
+  const Shares shares(a.workers, total);
+  const int w0 = shares.worker_of(before), parts = shares.worker_of(before + steps - 1) - w0 + 1;
   if (parts == 1) return;  // written whole
   const int rb = R / block_rows, rr = R % block_rows;
   const int64_t unit = ((int64_t)h * a.row_blocks + rb) * a.workers + w0;

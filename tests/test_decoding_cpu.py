@@ -143,7 +143,7 @@ WRITE = dict(k=P, ksb=0, kss=128, ksh=64, v=P, vsb=0, vss=128, vsh=64, B=1, S=4,
     (dict(slots=P + 4), 1, "misaligned"), (dict(kss=100), 1, "strides"), (dict(B=0), 1, "positive"),
     (dict(pages=0), 1, "positive"), (dict(Hkv=0), 1, "positive"), (dict(n=24), 2, "page_size"), (dict(n=8), 2, "page_size"),
     (dict(n=2048), 2, "page_size"), (dict(D=80), 2, "head_dim"), (dict(ct=2), 2, "cache dtype"), (dict(dtype=2), 2, "dtype"),
-    (dict(B=1 << 20, S=1 << 20), 1, "too many"), (dict(Hkv=70000), 1, "too many")])
+    (dict(B=1 << 20, S=1 << 20), 1, "too many"), (dict(B=1 << 14, S=1 << 14, Hkv=9), 1, "too many")])
 @pytest.mark.parametrize("entry", ["sage_cache_write", "sage_cache_read"])
 def test_cache_entries_refuse(entry, change, code, message):
     assert getattr(_capi.lib(), entry)(*{**WRITE, **change}.values()) == code
