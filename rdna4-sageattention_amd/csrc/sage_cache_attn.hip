@@ -43,7 +43,8 @@ struct CacheAttnArgs {
   const int* table;                 // [B] rows of max_pages entries, `tsb` apart
   const int* lengths;
   const uint8_t* tree;              // (b, i, j) at b * msb + i * msq + j * msk, or NULL
-  int64_t tsb, msb, msq, msk;
+  int64_t tsb, msb;
+  int msq, msk;
   int B, H, Hkv, G, T, dtype, causal;
   int pages, page_size, page_shift, max_pages;
   int row_blocks, workers;
@@ -186,14 +187,20 @@ template <int D> struct CacheTile {
   static constexpr int LOADS = 2 * COPIES + 1;   // vector loads per tile
   static constexpr int VW = D == 96 ? 2 : D / 64;  // words of V per lane and key
   __device__ static __forceinline__ int swap(int row) { return D == 96 ? 0 : D == 64 ? (row >> 1) & 3 : row & (D / 16 - 1); }
-  // copy j: the lane's byte offset in its block of 16 rows
-  __device__ static __forceinline__ uint32_t offset(int j, int lane) {
-    const int chunk = 64 * j + lane, row = chunk / (D / 16), c = chunk % (D / 16);
-    return (row & 15) * D + 16 * (c ^ swap(row));
+  // copy j: the lane's byte offset in its block of 16 rows, from copy 0's (96 channels: from the lane's number)
+  __device__ static __forceinline__ uint32_t first(int lane) {
+    return D == 96 ? lane : lane / (D / 16) * D + 16 * (lane % (D / 16) ^ swap(lane / (D / 16)));
+  }
+  __device__ static __forceinline__ uint32_t offset(int j, uint32_t from) {
+    if (D == 96) {
+      const int chunk = 64 * j + from, row = chunk / 6;
+      return (row & 15) * 96 + 16 * (chunk - 6 * row);
+    }
+    return D == 256 ? (from ^ 64 * (j % 4)) + 1024 * (j % 4) : from + (D == 128 ? 1024 * (j % 2) : 0);
   }
 };
 // tiles of a wave in LDS: as many as let the workgroups that the registers allow share a CU's 160 KiB
-template <int D, int RT> constexpr int ring_tiles() { return D == 64 ? 4 : RT == 3 ? (D == 96 ? 5 : 4) : 2; }
+template <int D> constexpr int ring_tiles() { return D == 64 ? 4 : 2; }
 
 // rows in front of the first of 16 keys from k0 on; a page outside the cache hides its keys: page 0 is read in its place
 struct CacheRow {
@@ -201,158 +208,324 @@ struct CacheRow {
   bool usable;
 };
 
+// The rows of a wave against the keys it walks: softmax references and sums, output accumulators, Q's operand.
+template <int D, int RT> struct Rows {
+  static constexpr int NK = D / 32, NC = D / 16;
+  f16x8 qf[RT][NK];
+  float qs[RT];   // factor of the scores to log2 units (positive: a hidden score stays -inf)
+  int row_t[RT];  // the row's new token
+  float m[RT], m2[RT], f[RT], l[RT];
+  v4f acc[RT][NC];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = m2[rt] = -__builtin_inff();
+      f[rt] = 0.0f;
+      l[rt] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[rt][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // rows first, first + 1, .. of sequence b and kv head h (past the last: the last again)
+  __device__ __forceinline__ void load_q(const CacheAttnArgs& a, int b, int h, int first, int n, int g) {
+    uint32_t qw[RT][D / 8];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(first + rt * 16 + n, a.T * a.G - 1);
+      const int t = r / a.G, hq = h * a.G + r % a.G;
+      row_t[rt] = t;
+      const uint16_t* qp = a.q + b * a.qsb + t * a.qss + hq * a.qsh + g * (D / 4);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const v4i x = *reinterpret_cast<const v4i*>(qp + 8 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qw[rt][4 * i + j] = (uint32_t)x[j];
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const uint32_t(&w)[D / 8] = qw[rt];
+      qs[rt] = a.scale;
+      if (a.dtype == DT_BF16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
+        const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
+        // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
+        const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
+        const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
+        qs[rt] = fmaxf(qs[rt] * down, 0x1p-126f);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            qf[rt][i][2 * j] = (_Float16)(bf16_lo(w[4 * i + j]) * up);
+            qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+          qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
+      }
+#pragma unroll
+      for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(qf[rt][i]));  // waited for here, not in the loop
+    }
+  }
+
+  // Scores of hidden keys become -inf (tiles that hold one only).  gone: bit 4 t + i, key 16 t + 4 g + i of the tile is past the
+  // sequence or on no page; node: the number of key 4 g among the new tokens.
+  __device__ __forceinline__ void hide(const CacheAttnArgs& a, int b, int node, uint32_t gone, v4f (&s)[RT][2]) const {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      uint32_t hidden = gone;
+      if (a.tree) {
+        const auto* shown = (const __attribute__((address_space(1))) uint8_t*)(a.tree + b * a.msb);
+        const int row = row_t[rt] * a.msq;  // (a mask's offsets fit 32 bits: checked on the host)
+        uint8_t see[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) see[j] = shown[row + min(max(node + 16 * (j / 4) + j % 4, 0), a.T - 1) * a.msk];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(see[j] == 0 && node + 16 * (j / 4) + j % 4 >= 0) << j;
+      } else if (a.causal) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(node + 16 * (j / 4) + j % 4 > row_t[rt]) << j;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (hidden >> j & 1) s[rt][j / 4][j % 4] = -__builtin_inff();
+    }
+    asm volatile("" ::: "memory");  // (a block of its own: never turned into selects for every tile)
+  }
+
+  // Scores (with K's scales) to the weights' operand: sums and references brought up to date.  The terms are taken against the
+  // references so far; where one passes them by too much (or a row has none yet) the references are raised first.
+  __device__ __forceinline__ void weights(const v4f (&s)[RT][2], const v4f (&vs)[2], f16x8 (&pf)[RT]) {
+    float vs_top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, vs[j / 4][j % 4]);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float p[8], pv[8];
+      float& M = m[rt];
+      auto terms = [&] {
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], qs[rt], -ref));
+          top = fmaxf(top, p[j]);
+        }
+        return top;
+      };
+      float top = terms();
+      if (__any(!(top <= 0x1p8f) || M == -__builtin_inff())) {
+        float y = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * qs[rt]);
+        const float up = fmaxf(M, row4_max(y));
+        if (up > M) {
+          l[rt] *= __builtin_amdgcn_exp2f(M - up);
+          M = up;
+          f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(M - m2[rt], 100.0f));
+        }
+        top = terms();
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        l[rt] += p[j];
+        pv[j] = mul_zero(p[j], vs[j / 4][j % 4]);
+      }
+      // (a bound of the largest product, by two different keys)
+      if (__any(!(top * vs_top * f[rt] <= 0x1p15f) || f[rt] == 0.0f)) {
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, pv[j]);
+        most = row4_max(most);
+        if ((f[rt] == 0.0f || most * f[rt] > 0x1p15f) && most > 0.0f && most < __builtin_inff()) {
+          const float up = fmaxf(m2[rt], M + (float)(__builtin_amdgcn_frexp_expf(most) - 7));
+          const float down = __builtin_amdgcn_exp2f(m2[rt] - up);
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) acc[rt][ct] *= down;
+          m2[rt] = up;
+          f[rt] = __builtin_amdgcn_exp2f(fminf(M - up, 100.0f));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
+    }
+  }
+};
+
+// A worker's place: kv head, row block and steps [s0, s1), the sequence of step s0 and the step's place in it.
+struct Work {
+  int h, rb, worker, s0, s1, b, first;
+  int lane_keys;  // keys of sequence `lane`, where there are no more than 64
+  __device__ __forceinline__ bool find(const CacheAttnArgs& a, int lane) {
+    // the row blocks of one range of keys on one XCD, next to each other
+    const int id = blockIdx.x;
+    const int grp = id / (8 * a.row_blocks) * 8 + id % 8;
+    rb = id / 8 % a.row_blocks;
+    h = grp / a.workers, worker = grp % a.workers;
+    if (h >= a.Hkv) return false;
+    const bool few = a.B <= 64;  // the lengths are read once
+    lane_keys = few && lane < a.B ? cache_keys(a, lane) : 0;
+    int n = lane < a.B ? cache_steps(lane_keys) : 0, scan = few ? wave_scan(n) : 0, unused;
+    const Shares shares(a.workers, few ? __builtin_amdgcn_readlane(scan, 63) : all_steps(a, lane, -1, unused));
+    if (worker >= shares.workers) return false;
+    s0 = shares.begin(worker);
+    s1 = shares.begin(worker + 1);
+    b = first = 0;
+    for (int c = 0, sum = 0; 64 * c < a.B; ++c) {
+      if (!few) n = lane_steps(a, c, lane), scan = wave_scan(n) + sum;
+      sum = __builtin_amdgcn_readlane(scan, 63);
+      if (sum > s0) {
+        const int at = __builtin_ctzll(__ballot(scan > s0));
+        b = 64 * c + at;
+        first = s0 - (__builtin_amdgcn_readlane(scan, at) - __builtin_amdgcn_readlane(n, at));
+        break;
+      }
+    }
+    return true;
+  }
+  __device__ __forceinline__ int keys(const CacheAttnArgs& a) const {
+    return a.B <= 64 ? __builtin_amdgcn_readlane(lane_keys, b) : uniform_keys(a, b);
+  }
+};
+
+// A wave's priority by how much of its workgroup's steps lies behind it.  Workgroups of equal work that share a CU would end far
+// apart, the one that came first served first (6 x 115000 keys: 194 and 237 us; three 132-row workgroups: 87, 105 and
+// 126 us), the last ones alone on their CUs; with those behind served first they end together.
+struct Pace {
+  int total, at, level;
+  __device__ __forceinline__ explicit Pace(int steps) : total(steps), at(0), level(3) {
+    __builtin_amdgcn_s_setprio(3);
+    next();
+  }
+  __device__ __forceinline__ void next() { at = level == 3 ? total / 2 : level == 2 ? total - total / 5 : level == 1 ? total - total / 16 : 0x7FFFFFFF; }
+  __device__ __forceinline__ void done(int steps) {
+    if (steps < at) return;
+    --level;
+    if (level == 2) __builtin_amdgcn_s_setprio(2);
+    else if (level == 1) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+    next();
+  }
+};
+
+// A sequence's part of a worker's range: keys [k_begin, k_end) of its `len`.
+struct Segment {
+  int len, take, base, open, k_begin, k_end;
+  bool whole;
+  int64_t unit;      // rows in front of its partial
+  const int* table;
+  __device__ __forceinline__ Segment(const CacheAttnArgs& a, const Work& w) {
+    len = w.keys(a);
+    const int steps = cache_steps(len);
+    take = min(steps - w.first, w.s1 - w.s0);
+    whole = take == steps;
+    unit = ((((int64_t)w.h * a.row_blocks + w.rb) * a.workers + w.worker) * 2 + (w.first > 0 ? 0 : 1)) * a.part_rows;
+    base = len - a.T;  // key of the first new token
+    open = a.tree ? base : a.causal ? base + 1 : len;  // keys below are seen by every row
+    k_begin = w.first * CA_STEP, k_end = min(len, (w.first + take) * CA_STEP);
+    table = a.table + w.b * a.tsb;
+  }
+  __device__ __forceinline__ CacheRow rows_of(const CacheAttnArgs& a, int h, int key) const {
+    const int page = scalar_entry(table, min(key >> a.page_shift, a.max_pages - 1));
+    const bool usable = page >= 0 && page < a.pages;
+    return CacheRow{((int64_t)(usable ? page : 0) * a.Hkv + h) * a.page_size + (key & (a.page_size - 1)), usable};
+  }
+  // bit 4 t + i: key k0 + 16 t + 4 g + i is past the sequence or (bit t of usable) on no page
+  __device__ __forceinline__ uint32_t gone(int k0, int g, uint32_t usable) const {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k0 + 4 * g + 16 * (j / 4) + j % 4 >= len || !(usable >> (j / 4) & 1)) bits |= 1u << j;
+    return bits;
+  }
+};
+
 template <int D, int CT, int RT>
-__global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 : 3) : 1) void cache_attn_kernel(const CacheAttnArgs a) {
   constexpr int NK = D / 32, NC = D / 16;
   constexpr int ROWS = 16 * RT;
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
   using Tile = CacheTile<D>;
-  constexpr int NS = ring_tiles<D, RT>();
-  constexpr int JOIN = CA_WAVES * 16 * LD * 4, RING = CA_WAVES * NS * Tile::BYTES;
+  // LDS of a wave.  16 rows: NS whole tiles, a tile is replaced once it is done with (memory bounds these calls: as many bytes
+  // under way as LDS holds).  32 rows: K of one tile, V and the scales of two, the next tile is started once this one's scores are
+  // there (three workgroups fit a CU, and arithmetic bounds these calls: 16 sequences of about 4750 keys, 8 kv heads x 128, 132
+  // rows each, 131 us with two whole tiles and two workgroups).
+  constexpr bool EARLY = RT >= 2;
+  constexpr int NS = EARLY ? 1 : ring_tiles<D>();
+  constexpr int PER_WAVE = EARLY ? 3 * Tile::KV + 512 : NS * Tile::BYTES;
+  constexpr int JOIN = CA_WAVES * 16 * LD * 4, RING = CA_WAVES * PER_WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t smem[JOIN > RING ? JOIN : RING];
   float (*so)[16][LD] = reinterpret_cast<float (*)[16][LD]>(smem);  // (the waves are joined after their last tile)
   __shared__ float sm[CA_WAVES][ROWS], sm2[CA_WAVES][ROWS], sl[CA_WAVES][ROWS];
 
-  // the row blocks of one range of keys on one XCD, next to each other
-  const int id = blockIdx.x;
-  const int grp = id / (8 * a.row_blocks) * 8 + id % 8, rb = id / 8 % a.row_blocks;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int rows = a.T * a.G;
-  int unused;
-  const int total = all_steps(a, lane, -1, unused);
-  const Shares shares(a.workers, total);
-  const int h = grp / a.workers, worker = grp % a.workers;
-  if (h >= a.Hkv || worker >= shares.workers) return;
-  int s0 = shares.begin(worker);
-  const int s1 = shares.begin(worker + 1);
-  // the sequence of step s0, and the step's place in it
-  int b = 0, first = 0;
-  for (int c = 0, sum = 0; 64 * c < a.B; ++c) {
-    const int steps = lane_steps(a, c, lane), scan = wave_scan(steps) + sum;
-    sum = __builtin_amdgcn_readlane(scan, 63);
-    if (sum > s0) {
-      const int at = __builtin_ctzll(__ballot(scan > s0));
-      b = 64 * c + at;
-      first = s0 - (__builtin_amdgcn_readlane(scan, at) - __builtin_amdgcn_readlane(steps, at));
-      break;
-    }
-  }
+  Work work;
+  if (!work.find(a, lane)) return;
+  Pace pace(work.s1 - work.s0);
+  int done = 0;
 
-  for (;; ++b, first = 0) {
-  const int len = uniform_keys(a, b);
-  const int steps = cache_steps(len), take = min(steps - first, s1 - s0);
-  const bool whole = take == steps;
-  const int64_t unit = ((((int64_t)h * a.row_blocks + rb) * a.workers + worker) * 2 + (first > 0 ? 0 : 1)) * a.part_rows;
-  const int base = len - a.T;  // key of the first new token
-  // keys below `open` are seen by every row
-  const int open = a.tree ? base : a.causal ? base + 1 : len;
-  const int k_begin = first * CA_STEP, k_end = min(len, (first + take) * CA_STEP);
-
-  float m[RT], m2[RT], f[RT], l[RT];
-  v4f acc[RT][NC];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = m2[rt] = -__builtin_inff();
-    f[rt] = 0.0f;
-    l[rt] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[rt][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  const int* table = a.table + b * a.tsb;
-  auto page_of = [&](int key) { return scalar_entry(table, min(key >> a.page_shift, a.max_pages - 1)); };
-  auto rows_of = [&](int k0) {
-    const int page = page_of(k0);
-    const bool usable = page >= 0 && page < a.pages;
-    return CacheRow{((int64_t)(usable ? page : 0) * a.Hkv + h) * a.page_size + (k0 & (a.page_size - 1)), usable};
-  };
-  uint8_t* ring = smem + wave * (NS * Tile::BYTES);
-  uint32_t from[Tile::COPIES];  // (for head dims 64 and 128 all copies have one offset, but for a constant)
-#pragma unroll
-  for (int j = 0; j < Tile::COPIES; ++j) from[j] = Tile::offset(j, lane);
+  for (;; ++work.b, work.first = 0) {
+  const int b = work.b, h = work.h, rb = work.rb;
+  const Segment seg(a, work);
+  Rows<D, RT> r;
+  r.clear();
+  uint8_t* ring = smem + wave * PER_WAVE;
   const uint32_t ring_at = lds_address(ring);
+  // place of tile `stage`'s K (kv 0), V (1), scales (2) in the wave's LDS
+  auto place = [&](int stage, int kv) {
+    return EARLY ? (kv == 0 ? 0 : kv == 1 ? (1 + stage) * Tile::KV : 3 * Tile::KV + 256 * stage) : stage * Tile::BYTES + kv * Tile::KV;
+  };
+  // where the lane's operands lie in a tile: K of key n, V and scales of key 4 g (keys and chunks further on differ by constants),
+  // and what it copies
+  const int k_at0 = n * D + (D == 96 ? 24 * g : 16 * ((D / 64 * g) ^ Tile::swap(n)));
+  const int v_per = D == 96 ? 4 : D / 16;  // bytes of a key that the lane starts from
+  const int v_at0 = 4 * g * D + (v_per * n & 15) + 16 * ((v_per * n >> 4) ^ (D == 96 ? 0 : Tile::swap(4 * g)));
+  const uint32_t from0 = Tile::first(lane);
+  // 32 rows leave no registers to keep what is derived from these through the loop
+  auto afresh = [&](auto x) {
+    if (EARLY) asm volatile("" : "+v"(x));
+    return x;
+  };
   auto issue = [&](CacheRow at0, CacheRow at1, int stage) {
-    const uint32_t to = __builtin_amdgcn_readfirstlane(ring_at + stage * Tile::BYTES);
+    const uint32_t from = afresh(from0);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
+      const uint32_t to = __builtin_amdgcn_readfirstlane(ring_at + place(stage, kv));
       const uint8_t* codes = kv ? a.v8 : a.k8;
       const uint8_t *p0 = codes + at0.row * D, *p1 = codes + at1.row * D;
 #pragma unroll
       for (int j = 0; j < Tile::COPIES; ++j) {
-        const uint32_t dst = to + kv * Tile::KV + 1024 * j;
-        if (D == 96 && j == 1) copy_lds_from((lane < 32 ? p0 : p1) + from[j], dst, 16);  // half of it in each block
-        else copy_lds<16>(2 * j / Tile::COPIES ? p1 : p0, from[j], dst);
+        const uint32_t dst = to + 1024 * j;
+        if (D == 96 && j == 1) copy_lds_from((lane < 32 ? p0 : p1) + Tile::offset(j, from), dst, 16);  // half of it in each block
+        else copy_lds<16>(2 * j / Tile::COPIES ? p1 : p0, Tile::offset(j, from), dst);
       }
     }
     const int64_t row = (lane & 16 ? at1.row : at0.row) + (lane & 15);
-    copy_lds_from((lane < 32 ? a.ks : a.vs) + row, to + 2 * Tile::KV, 4);
+    copy_lds_from((lane < 32 ? a.ks : a.vs) + row, __builtin_amdgcn_readfirstlane(ring_at + place(stage, 2)), 4);
   };
-  // where the lane's operands lie in a tile: K of key n, V of key 4 g (keys and chunks further on differ by constants)
-  const int k_at = n * D + (D == 96 ? 24 * g : 16 * ((D / 64 * g) ^ Tile::swap(n)));
-  const int v_per = D == 96 ? 4 : D / 16;  // bytes of a key that the lane starts from
-  const int v_at = 4 * g * D + (v_per * n & 15) + 16 * ((v_per * n >> 4) ^ (D == 96 ? 0 : Tile::swap(4 * g)));
-
   // NS tiles on their way or in use (the last one again where there are fewer)
-  int k0 = k_begin + wave * CA_TILE;
-  const int tiles = k0 < k_end ? (k_end - k0 + CA_STEP - 1) / CA_STEP : 0;
+  int k0 = seg.k_begin + wave * CA_TILE;
+  const int tiles = k0 < seg.k_end ? (seg.k_end - k0 + CA_STEP - 1) / CA_STEP : 0;
   uint32_t usable = 0;  // bits 2 i, 2 i + 1: the two pages of tile i from the current one on
   if (tiles) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int k = k0 + min(i, tiles - 1) * CA_STEP;
-      const CacheRow at0 = rows_of(k), at1 = rows_of(k + 16);
+      const CacheRow at0 = seg.rows_of(a, h, k), at1 = seg.rows_of(a, h, k + 16);
       usable |= ((uint32_t)at0.usable | (uint32_t)at1.usable << 1) << 2 * i;
       issue(at0, at1, i);
     }
   }
 
-  // Q operand and the rows' factors
-  f16x8 qf[RT][NK];
-  float qs[RT];
-  int row_t[RT];
-  uint32_t qw[RT][D / 8];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(rb * ROWS + rt * 16 + n, rows - 1);
-    const int t = r / a.G, hq = h * a.G + r % a.G;
-    row_t[rt] = t;
-    const uint16_t* qp = a.q + b * a.qsb + t * a.qss + hq * a.qsh + g * (D / 4);
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const v4i x = *reinterpret_cast<const v4i*>(qp + 8 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qw[rt][4 * i + j] = (uint32_t)x[j];
-    }
-  }
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const uint32_t(&w)[D / 8] = qw[rt];
-    qs[rt] = a.scale;  // (positive: a hidden score stays -inf)
-    if (a.dtype == DT_BF16) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
-      const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
-      // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
-      const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
-      const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
-      qs[rt] = fmaxf(qs[rt] * down, 0x1p-126f);
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          qf[rt][i][2 * j] = (_Float16)(bf16_lo(w[4 * i + j]) * up);
-          qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-        qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
-    }
-#pragma unroll
-    for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(qf[rt][i]));  // waited for here, not in the loop
-  }
+  r.load_q(a, b, h, rb * ROWS, n, g);
 
   if (tiles) {
     int stage = 0;
@@ -361,11 +534,14 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
       if (left >= NS) wait_loads<(NS - 1) * Tile::LOADS>();
       else if (NS > 2 && left == 2) wait_loads<Tile::LOADS>();
       else wait_loads<0>();
-      uint8_t* tile = ring + stage * Tile::BYTES;
+      const int k_at = afresh(k_at0), v_at = afresh(v_at0);
+      const uint8_t* const kt = ring + place(stage, 0);
+      uint8_t* const vt = ring + place(stage, 1);
+      const uint8_t* const st = ring + place(stage, 2);
       const bool more = left > NS;
       CacheRow next0 = {0, false}, next1 = {0, false};
-      if (more) next0 = rows_of(k0 + NS * CA_STEP), next1 = rows_of(k0 + NS * CA_STEP + 16);
-      const bool masked = k0 + CA_TILE > open || (usable & 3) != 3;
+      if (more) next0 = seg.rows_of(a, h, k0 + NS * CA_STEP), next1 = seg.rows_of(a, h, k0 + NS * CA_STEP + 16);
+      const bool masked = k0 + CA_TILE > seg.open || (usable & 3) != 3;
       v4f s[RT][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -375,13 +551,13 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
         if constexpr (D == 96) {
 #pragma unroll
           for (int i = 0; i < 3; ++i) {
-            const v2i w = *reinterpret_cast<const v2i*>(tile + 16 * t * D + k_at + 8 * i);
+            const v2i w = *reinterpret_cast<const v2i*>(kt + 16 * t * D + k_at + 8 * i);
             kw[2 * i] = w[0], kw[2 * i + 1] = w[1];
           }
         } else {
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) {
-            const v4i w = *reinterpret_cast<const v4i*>(tile + 16 * t * D + (k_at ^ 16 * i));
+            const v4i w = *reinterpret_cast<const v4i*>(kt + 16 * t * D + (k_at ^ 16 * i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) kw[4 * i + j] = (uint32_t)w[j];
           }
@@ -393,123 +569,50 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
           const f16x8 ka = join4(codes_f16<CT>(w0, false), codes_f16<CT>(w0, true), codes_f16<CT>(w1, false),
                                  codes_f16<CT>(w1, true));
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[rt][i], s[rt][t], 0, 0, 0);
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, r.qf[rt][i], s[rt][t], 0, 0, 0);
         }
       }
       v4f ks[2], vs[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        ks[t] = *reinterpret_cast<const v4f*>(tile + 2 * Tile::KV + 64 * t + 16 * g);
-        vs[t] = *reinterpret_cast<const v4f*>(tile + 2 * Tile::KV + 128 + 64 * t + 16 * g);
+        ks[t] = *reinterpret_cast<const v4f*>(st + 64 * t + 16 * g);
+        vs[t] = *reinterpret_cast<const v4f*>(st + 128 + 64 * t + 16 * g);
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[rt][t] *= ks[t];
       }
+      if (EARLY && more) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's reads are done: its place takes the next tile's
+        issue(next0, next1, stage ^ 1);
+      }
       // Tiles with hidden keys: their scores become -inf.  The rest needs no selects: a weight of 0 times whatever scale is 0
-      // (the products below are of that kind), and V codes of keys past the sequence or on no page, which may be NaN, become 0
-      // where the lane reads them.
+      // (mul_zero), and V codes of keys past the sequence or on no page, which may be NaN, become 0 where the lane reads them.
       if (masked) {
-        const int node = k0 + 4 * g - base;  // of bit 0
-        uint32_t gone = 0;                   // bit 4 t + i
+        const uint32_t gone = seg.gone(k0, g, usable);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (k0 + 4 * g + 16 * (j / 4) + j % 4 >= len || !(usable >> (j / 4) & 1)) {
-            gone |= 1u << j;
-            if (CT == CACHE_E4M3) {
-              uint8_t* vp = tile + Tile::KV + (16 * (j / 4) + j % 4) * D;
-              if constexpr (D == 64) *reinterpret_cast<uint32_t*>(vp + (v_at ^ 16 * (j % 4 / 2))) = 0;
-              else if constexpr (D == 128) *reinterpret_cast<v2i*>(vp + (v_at ^ 16 * (j % 4))) = v2i{0, 0};
-              else if constexpr (D == 256) *reinterpret_cast<v4i*>(vp + (v_at ^ 16 * (j % 4))) = v4i{0, 0, 0, 0};
-              else {
-                *reinterpret_cast<uint32_t*>(vp + v_at) = 0;
-                *reinterpret_cast<uint16_t*>(vp + 4 * g * D + 64 + 2 * n) = 0;
-              }
+          if (CT == CACHE_E4M3 && (gone >> j & 1)) {
+            uint8_t* vp = vt + (16 * (j / 4) + j % 4) * D;
+            if constexpr (D == 64) *reinterpret_cast<uint32_t*>(vp + (v_at ^ 16 * (j % 4 / 2))) = 0;
+            else if constexpr (D == 128) *reinterpret_cast<v2i*>(vp + (v_at ^ 16 * (j % 4))) = v2i{0, 0};
+            else if constexpr (D == 256) *reinterpret_cast<v4i*>(vp + (v_at ^ 16 * (j % 4))) = v4i{0, 0, 0, 0};
+            else {
+              *reinterpret_cast<uint32_t*>(vp + v_at) = 0;
+              *reinterpret_cast<uint16_t*>(vp + 4 * g * D + 64 + 2 * n) = 0;
             }
           }
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          uint32_t hidden = gone;
-          if (a.tree) {
-            const uint8_t* shown = a.tree + b * a.msb + row_t[rt] * a.msq;
-            uint8_t see[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) see[j] = shown[min(max(node + 16 * (j / 4) + j % 4, 0), a.T - 1) * a.msk];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(see[j] == 0 && node + 16 * (j / 4) + j % 4 >= 0) << j;
-          } else if (a.causal) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) hidden |= (uint32_t)(node + 16 * (j / 4) + j % 4 > row_t[rt]) << j;
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (hidden >> j & 1) s[rt][j / 4][j % 4] = -__builtin_inff();
-        }
-        asm volatile("" ::: "memory");  // (a block of its own: never turned into selects for every tile)
+        r.hide(a, b, k0 + 4 * g - seg.base, gone, s);
       }
-      float vs_top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, vs[j / 4][j % 4]);
       f16x8 pf[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float p[8], pv[8];
-        float& M = m[rt];
-        // the terms against the references so far; where one passes them by too much (or a row has none yet) the references
-        // are raised first
-        auto terms = [&] {
-          const float ref = M == -__builtin_inff() ? 0.0f : M;
-          float top = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j / 4][j % 4], qs[rt], -ref));
-            top = fmaxf(top, p[j]);
-          }
-          return top;
-        };
-        float top = terms();
-        if (__any(!(top <= 0x1p8f) || M == -__builtin_inff())) {
-          float y = -__builtin_inff();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * qs[rt]);
-          const float up = fmaxf(M, row4_max(y));
-          if (up > M) {
-            l[rt] *= __builtin_amdgcn_exp2f(M - up);
-            M = up;
-            f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(M - m2[rt], 100.0f));
-          }
-          top = terms();
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          l[rt] += p[j];
-          pv[j] = mul_zero(p[j], vs[j / 4][j % 4]);
-        }
-        // (a bound of the largest product, by two different keys)
-        if (__any(!(top * vs_top * f[rt] <= 0x1p15f) || f[rt] == 0.0f)) {
-          float most = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) most = fmaxf(most, pv[j]);
-          most = row4_max(most);
-          if ((f[rt] == 0.0f || most * f[rt] > 0x1p15f) && most > 0.0f && most < __builtin_inff()) {
-            const float up = fmaxf(m2[rt], M + (float)(__builtin_amdgcn_frexp_expf(most) - 7));
-            const float down = __builtin_amdgcn_exp2f(m2[rt] - up);
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) acc[rt][ct] *= down;
-            m2[rt] = up;
-            f[rt] = __builtin_amdgcn_exp2f(fminf(M - up, 100.0f));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
-      }
+      r.weights(s, vs, pf);
       // V operand: keys (0, 1), (2, 3) of each block side by side
       uint32_t vw[8][Tile::VW];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint8_t* vp = tile + Tile::KV + (16 * (j / 4) + j % 4) * D;
+        const uint8_t* vp = vt + (16 * (j / 4) + j % 4) * D;
         if constexpr (D == 64) {
           vw[j][0] = *reinterpret_cast<const uint32_t*>(vp + (v_at ^ 16 * (j % 4 / 2)));
         } else if constexpr (D == 96) {
@@ -542,44 +645,46 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
             const int c = 4 * i + 2 * u + o;
             const f16x8 va = join4(codes_f16<CT>(w[0], o), codes_f16<CT>(w[1], o), codes_f16<CT>(w[2], o), codes_f16<CT>(w[3], o));
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], acc[rt][c], 0, 0, 0);
+            for (int rt = 0; rt < RT; ++rt) r.acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], r.acc[rt][c], 0, 0, 0);
           }
         }
       }
+      pace.done(++done);
       if (left == 1) break;
       usable >>= 2;
       if (more) {
         usable |= ((uint32_t)next0.usable | (uint32_t)next1.usable << 1) << 2 * (NS - 1);
-        // the tile's reads are done: its place takes the one NS tiles on
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        issue(next0, next1, stage);
+        if (!EARLY) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's reads are done: its place takes the one NS tiles on
+          issue(next0, next1, stage);
+        }
       }
-      stage = stage + 1 == NS ? 0 : stage + 1;
+      stage = EARLY ? stage ^ 1 : stage + 1 == NS ? 0 : stage + 1;
     }
   }
 
   // join the waves, 16 rows at a time
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    l[rt] = row4_sum(l[rt]);
+    const float sum = row4_sum(r.l[rt]);
     if (g == 0) {
-      sm[wave][rt * 16 + n] = m[rt];
-      sm2[wave][rt * 16 + n] = m2[rt];
-      sl[wave][rt * 16 + n] = l[rt];
+      sm[wave][rt * 16 + n] = r.m[rt];
+      sm2[wave][rt * 16 + n] = r.m2[rt];
+      sl[wave][rt * 16 + n] = sum;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rt * 16 + n;
-    float top2 = sm2[0][r];
+    const int own = rt * 16 + n;
+    float top2 = sm2[0][own];
 #pragma unroll
-    for (int w = 1; w < CA_WAVES; ++w) top2 = fmaxf(top2, sm2[w][r]);
-    const float down = m2[rt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m2[rt] - top2);
+    for (int w = 1; w < CA_WAVES; ++w) top2 = fmaxf(top2, sm2[w][own]);
+    const float down = r.m2[rt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(r.m2[rt] - top2);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) so[wave][n][v_channel<D>(4 * g + i, c)] = acc[rt][c][i] * down;
+      for (int i = 0; i < 4; ++i) so[wave][n][v_channel<D>(4 * g + i, c)] = r.acc[rt][c][i] * down;
     __syncthreads();
     // 16 threads per row
     const int row = threadIdx.x / 16, part = threadIdx.x % 16, rr = rt * 16 + row, R = rb * ROWS + rr;
@@ -603,7 +708,7 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
       o[i] = L == 0.0f ? 0.0f : v * fin;
     }
     if (R < rows) {
-      if (whole) {
+      if (seg.whole) {
         const int t = R / a.G, hq = h * a.G + R % a.G;
         uint16_t* op = a.out + b * a.osb + t * a.oss + hq * a.osh + part * PER;
 #pragma unroll
@@ -614,44 +719,49 @@ __global__ __launch_bounds__(CA_THREADS, RT <= 2 && D <= 128 || RT == 1 ? 2 : 1)
         }
         if (a.lse && part == 0) a.lse[((int64_t)b * a.H + hq) * a.T + t] = lse2 * 0.69314718055994530942f;
       } else {
-        float* op = a.part_o + (unit + rr) * D + part * PER;
+        float* op = a.part_o + (seg.unit + rr) * D + part * PER;
 #pragma unroll
         for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(op + i) = make_float2(o[i], o[i + 1]);
-        if (part == 0) a.part_lse[unit + rr] = lse2;
+        if (part == 0) a.part_lse[seg.unit + rr] = lse2;
       }
     }
     if (rt + 1 < RT) __syncthreads();
   }
-  s0 += take;
-  if (s0 >= s1) break;
+  work.s0 += seg.take;
+  if (work.s0 >= work.s1) break;
   __syncthreads();  // the next sequence's rows go where these were read
   }
 }
 
 // Joins the parts of the rows of sequences that several workers shared: o = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M).
 // One row per group of `slices` waves, each of which adds up every slices-th part, in an order that the lengths alone
-// decide.
+// decide; a wave that does it alone takes `per` rows of one sequence and kv head, one after the other.
 constexpr int MERGE_SLICES = 16;
-template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merge_kernel(const CacheAttnArgs a, int block_rows, int slices) {
+template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merge_kernel(const CacheAttnArgs a, int block_rows, int slices,
+                                                                                              int per) {
   constexpr int VEC = D <= 64 ? 1 : D <= 128 ? 2 : 4;  // channels per lane
   typedef float vec __attribute__((ext_vector_type(VEC)));
   __shared__ float so[MERGE_SLICES][D];
   __shared__ float sml[MERGE_SLICES][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = a.T * a.G;
-  const int at = slices == 1 ? blockIdx.x * (blockDim.x / 64) + wave : blockIdx.x;
-  if (at >= rows * a.B * a.Hkv) return;
-  const int slice = slices == 1 ? 0 : wave;
-  const int pair = at / rows, R = at - pair * rows, b = pair / a.Hkv, h = pair - b * a.Hkv;
+  const bool alone = slices == 1;
+  const int groups = (rows + per - 1) / per;
+  const int at = alone ? blockIdx.x * (blockDim.x / 64) + wave : blockIdx.x;
+  if (at >= groups * a.B * a.Hkv) return;
+  const int slice = alone ? 0 : wave;
+  const int pair = at / groups, group = at - pair * groups, b = pair / a.Hkv, h = pair - b * a.Hkv;
   int before;
   const int total = all_steps(a, lane, b, before), steps = cache_steps(uniform_keys(a, b));
   const Shares shares(a.workers, total);
   const int w0 = shares.worker_of(before), parts = shares.worker_of(before + steps - 1) - w0 + 1;
   if (parts == 1) return;  // written whole
+  const bool mine = lane * VEC < D;
+  const int first = group * per, last = min(first + per, rows);
+  for (int R = first; R < last; ++R) {
   const int rb = R / block_rows, rr = R % block_rows;
   const int64_t unit = ((int64_t)h * a.row_blocks + rb) * a.workers + w0;
   auto part = [&](int i) { return ((unit + i) * 2 + (i == 0)) * a.part_rows + rr; };
-  const bool mine = lane * VEC < D;
 
   float M = -__builtin_inff(), L = 0.0f;
   vec o = 0.0f;
@@ -706,9 +816,10 @@ template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merg
   }
   if (a.lse && lane == 0)
     a.lse[((int64_t)b * a.H + hq) * a.T + t] = L == 0.0f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.69314718055994530942f;
+  }
 }
 
-// Rows per workgroup (16 RT) and workers per kv head and row block for a call.
+// Rows per workgroup (16 rt) and workers per kv head and row block for a call.
 struct CachePlan {
   int rt, row_blocks, workers, part_rows;
   int64_t o_bytes, bytes;
@@ -717,11 +828,17 @@ struct CachePlan {
 static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
-  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 || 1 ? 2 : 3;
+  // Turning a tile's codes to float16 costs a wave as much as the softmax and products of 28 rows, so more rows per block pay where
+  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 117 us against 130 in blocks of 32; 64 rows fill two
+  // blocks of 32).  At 64 the turning is half as much and blocks of 32 keep three workgroups per CU (512 rows: 49 us, 77 in
+  // blocks of 48); at 256 more than 32 rows do not fit the registers.
+  auto cost = [&](int rt) { return (rows + 16 * rt - 1) / (16 * rt) * (28 + 16 * rt); };
+  p.rt = rows <= 16 ? 1 : D == 64 || D == 256 || cost(2) <= cost(3) ? 2 : 3;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
-  const int64_t slots = (int64_t)cus * (p.rt == 3 || D == 256 ? 1 : 2);  // workgroups that run at once
+  // workgroups that run at once
+  const int64_t slots = (int64_t)cus * (D == 256 ? 1 : p.rt == 2 ? 3 : 2);
   const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
   int64_t w = slots / units;
   if (w < 8) {
@@ -731,6 +848,9 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
     for (int64_t n = 2; n <= 8; ++n) best = rounds(n) < best ? rounds(n) : best;
     for (w = 1; rounds(w) > 1.1 * best; ++w) {}
   }
+  // one sequence of up to 512 keys: no parts to join (256 keys, 8 kv heads: 8.9 us, 11.3 with two workers and the joining launch;
+  // 1000 keys: 15 and 12.8)
+  if (B == 1 && most <= 4) w = 1;
   p.workers = (int)(w > most ? most : w);
   const int64_t n = p.workers == 1 ? 0 : units * p.workers * 2 * p.part_rows;
   p.o_bytes = (n * D * 4 + 255) / 256 * 256;
@@ -741,17 +861,21 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
 template <int D, int CT> static void cache_attn_launch(const CacheAttnArgs& a, int rt, unsigned blocks, hipStream_t st) {
   if (rt == 1) cache_attn_kernel<D, CT, 1><<<blocks, CA_THREADS, 0, st>>>(a);
   else if (rt == 2) cache_attn_kernel<D, CT, 2><<<blocks, CA_THREADS, 0, st>>>(a);
-  else if constexpr (D < 256) cache_attn_kernel<D, CT, 3><<<blocks, CA_THREADS, 0, st>>>(a);
+  else if constexpr (D == 96 || D == 128) cache_attn_kernel<D, CT, 3><<<blocks, CA_THREADS, 0, st>>>(a);
 }
 
 template <int D> static void cache_attn_dims(const CacheAttnArgs& a, int ct, int rt, unsigned blocks, hipStream_t st) {
   if (ct == CACHE_INT8) cache_attn_launch<D, CACHE_INT8>(a, rt, blocks, st);
   else cache_attn_launch<D, CACHE_E4M3>(a, rt, blocks, st);
   if (a.workers > 1) {
-    const int64_t rows = (int64_t)a.T * a.G * a.B * a.Hkv;
+    // the waves of a workgroup join a row together where sequences come in many parts
     const int slices = a.workers <= 8 || a.workers <= 4 * a.B ? 1 : a.workers <= 128 ? 4 : MERGE_SLICES;
-    const int64_t blocks = slices == 1 ? (rows + 3) / 4 : rows;
-    cache_merge_kernel<D><<<(unsigned)blocks, 64 * (slices == 1 ? 4 : slices), 0, st>>>(a, 16 * rt, slices);
+    // several rows per wave only where their number fills the GPU twice over (16896 rows: 12 us with one each, 8 with four)
+    const int64_t rows = (int64_t)a.T * a.G * a.B * a.Hkv;
+    const int per = slices == 1 && rows > 8192 ? 4 : 1;
+    const int64_t merges = (int64_t)a.B * a.Hkv * ((a.T * a.G + per - 1) / per);
+    const int64_t blocks = slices == 1 ? (merges + 3) / 4 : merges;
+    cache_merge_kernel<D><<<(unsigned)blocks, 64 * (slices == 1 ? 4 : slices), 0, st>>>(a, 16 * rt, slices, per);
   }
 }
 
@@ -807,6 +931,10 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale must be finite and not negative (got %g)",
                who, (double)sm_scale);
+  if (tree_mask) {
+    auto far = [&](int64_t stride) { return (stride < 0 ? -stride : stride) > 0x3FFFFFFF / (T > 1 ? T - 1 : 1); };
+    SAGE_REQUIRE(!far(msq) && !far(msk), "%s: a tree mask's rows and columns must lie within 2^31 bytes", who);
+  }
   int cus = 0;
   if ((rc = device_cus(&cus))) return rc;
   const CachePlan p = cache_plan(B, H, Hkv, T, D, max_pages * page_size, cus);
@@ -818,7 +946,7 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   a.out = (uint16_t*)out, a.osb = osb, a.oss = oss, a.osh = osh, a.lse = lse;
   a.k8 = (const uint8_t*)k8, a.v8 = (const uint8_t*)v8, a.ks = k_scale, a.vs = v_scale;
   a.table = block_table, a.tsb = table_stride, a.lengths = lengths;
-  a.tree = (const uint8_t*)tree_mask, a.msb = msb, a.msq = msq, a.msk = msk;
+  a.tree = (const uint8_t*)tree_mask, a.msb = msb, a.msq = (int)msq, a.msk = (int)msk;
   a.B = B, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.T = T, a.dtype = dtype, a.causal = causal;
   a.pages = pages, a.page_size = page_size, a.max_pages = max_pages;
   a.page_shift = __builtin_ctz((unsigned)page_size);

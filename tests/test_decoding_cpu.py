@@ -163,7 +163,8 @@ ATTN = dict(q=P, qsb=512, qss=512, qsh=64, out=P, osb=512, oss=512, osh=64, lse=
     (dict(H=7), 1, "multiple"), (dict(D=80), 2, "head_dim"), (dict(n=20), 2, "page_size"), (dict(dtype=2), 2, "dtype"),
     (dict(ct=7), 2, "cache dtype"), (dict(sm=-1.0), 1, "sm_scale"), (dict(sm=float("nan")), 1, "sm_scale"),
     (dict(sm=float("inf")), 1, "sm_scale"), (dict(n=1024, max_pages=1 << 21), 1, "2^30"), (dict(T=1 << 28), 1, "2^28"),
-    (dict(B=1 << 18, n=1024, max_pages=1 << 20), 1, "2^37")])
+    (dict(B=1 << 18, n=1024, max_pages=1 << 20), 1, "2^37"), (dict(T=9, tree=P, msq=1 << 28), 1, "tree mask"),
+    (dict(T=9, tree=P, msk=-(1 << 40)), 1, "tree mask")])
 def test_attention_entry_refuses(change, code, message):
     assert _capi.lib().sage_cache_attn(*{**ATTN, **change}.values()) == code
     assert message in _err()

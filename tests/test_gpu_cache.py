@@ -191,6 +191,9 @@ ATTENTION = [
     (16, 8, 4, 64, 16, [40, 16, 17], E4M3, torch.bfloat16, "HND"),
     (33, 4, 2, 128, 32, [33, 90, 20], E4M3, torch.float16, "NHD"),
     (70, 2, 1, 64, 16, [70, 101], torch.int8, torch.bfloat16, "HND"),
+    (35, 4, 2, 96, 16, [36, 200], torch.int8, torch.float16, "HND"),
+    (50, 1, 1, 128, 64, [300, 7], E4M3, torch.bfloat16, "HND"),
+    (40, 2, 2, 256, 16, [140, 41], E4M3, torch.float16, "NHD"),
 ]
 
 
@@ -220,6 +223,25 @@ def test_long_sequences_split_over_workgroups(dev, T, H, Hkv, code):
     table[:, 399] = -2**31
     q = torch.randn(4, H, T, D, generator=g).to(torch.bfloat16)
     _compare(dev, q, cache, table, lengths, tree=_tree(g, 4, T))
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,D,longest", [
+    (70, 1, 8, 4, 64, 500),       # more sequences than lanes, ragged, some empty
+    (130, 2, 2, 2, 96, 200),
+    (70, 16, 8, 8, 64, 60),       # thousands of rows to join
+    (4, 1, 16, 8, 128, 4000),     # sequences in many parts
+    (1, 3, 8, 1, 256, 9000),
+    (1, 1, 1, 1, 64, 40000),
+])
+def test_batches_and_splits_of_every_kind(dev, B, T, H, Hkv, D, longest):
+    g = torch.Generator().manual_seed(B + longest)
+    lengths = torch.randint(0, longest + 1, (B,), generator=g).to(torch.int32)
+    lengths[0] = longest
+    page = 32
+    pages = int(((lengths + page - 1) // page).sum()) + 1
+    cache = random_cache(g, pages, page, Hkv, D, torch.int8)
+    q = torch.randn(B, H, T, D, generator=g).to(torch.bfloat16)
+    _compare(dev, q, cache, _table(g, lengths, page, pages), lengths)
 
 
 @pytest.mark.parametrize("code", [torch.int8, E4M3])
