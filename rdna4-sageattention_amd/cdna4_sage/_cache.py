@@ -26,7 +26,8 @@ CACHE_DTYPES = {torch.int8: _capi.CACHE_INT8, torch.float8_e4m3fn: _capi.CACHE_E
 class KVCache(NamedTuple):
     """Codes [pages, kv_heads, page_size, head_dim] (int8 or float8_e4m3fn) and scales [pages, kv_heads, page_size]
     (float32) of the keys and the values, contiguous: a key is code * scale.  Slot s is row s % page_size of page
-    s // page_size.  page_size is a power of two from 16 to 1024."""
+    s // page_size.  page_size is a power of two from 16 to 1024.  float32 holds what the kernels derive from cached
+    values of magnitude up to 2^100; E4M3 codes are finite (cache_write keeps a NaN in the scale)."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor

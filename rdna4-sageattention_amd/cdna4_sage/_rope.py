@@ -172,7 +172,8 @@ def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved
     channels are copied.  q: [B, heads, tokens, head_dim] for "HND", [B, tokens, heads, head_dim] for "NHD", k alike with
     heads of its own, bf16 or fp16.  positions: int32 / int64 [tokens] or [B, tokens] (None: 0, 1, ..).  freqs, factor:
     rope_frequencies.  Returns q, or (q, k), in new tensors.  Differentiable in q and k (to any order); float32
-    arithmetic, rounded once.  Raises Unsupported for what the kernel does not take."""
+    arithmetic, rounded once.  Before a backward pass is captured into a graph, drop the eager graphs of the same leaves:
+    torch would wait for their streams, which ends the capture.  Raises Unsupported for what the kernel does not take."""
     if freqs is None:
         raise Unsupported("freqs are required (rope_frequencies)")
     ts = (q,) if k is None else (q, k)

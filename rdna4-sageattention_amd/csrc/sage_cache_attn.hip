@@ -19,7 +19,10 @@
 //  * P in float16 holds 11 bits of p_ij s^v_j: two running references per row, m (of x) for the sum l and m2 (of
 //    x + log2 s^v) for P, each raised only when a tile passes it by 2^8.  The largest product so far lies between 2^6 and
 //    2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an error of 2^-31 of it below.
-// Bound: HBM.  A key costs 2 D + 8 bytes per kv head whatever T and G are.
+// Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000 keys, 8
+// kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us, 3.6 TB/s), the turning of codes and the softmax's
+// vector instructions beyond (132 rows over 16 x 4750 keys: 112 us, 0.37 PFLOP/s of products).
+// Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
 #include "sage_cache.h"
 
 namespace sage {
@@ -423,7 +426,7 @@ struct Segment {
   __device__ __forceinline__ Segment(const CacheAttnArgs& a, const Work& w) {
     len = w.keys(a);
     const int steps = cache_steps(len);
-    take = min(steps - w.first, w.s1 - w.s0);
+    take = max(min(steps - w.first, w.s1 - w.s0), 1);  // (1 and more, even if another stream rewrote the lengths by now)
     whole = take == steps;
     unit = ((((int64_t)w.h * a.row_blocks + w.rb) * a.workers + w.worker) * 2 + (w.first > 0 ? 0 : 1)) * a.part_rows;
     base = len - a.T;  // key of the first new token
@@ -453,9 +456,9 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
   using Tile = CacheTile<D>;
   // LDS of a wave.  16 rows: NS whole tiles, a tile is replaced once it is done with (memory bounds these calls: as many bytes
-  // under way as LDS holds).  32 rows: K of one tile, V and the scales of two, the next tile is started once this one's scores are
-  // there (three workgroups fit a CU, and arithmetic bounds these calls: 16 sequences of about 4750 keys, 8 kv heads x 128, 132
-  // rows each, 131 us with two whole tiles and two workgroups).
+  // under way as LDS holds).  32 rows and more: K of one tile, V and the scales of two, the next tile is started once this one's
+  // scores are there (three workgroups of 32 rows fit a CU, and arithmetic bounds these calls: 200 rows' chunks over 2 x 9500 keys,
+  // 140 us, 161 with two whole tiles and two workgroups).
   constexpr bool EARLY = RT >= 2;
   constexpr int NS = EARLY ? 1 : ring_tiles<D>();
   constexpr int PER_WAVE = EARLY ? 3 * Tile::KV + 512 : NS * Tile::BYTES;
@@ -728,7 +731,7 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
     if (rt + 1 < RT) __syncthreads();
   }
   work.s0 += seg.take;
-  if (work.s0 >= work.s1) break;
+  if (work.s0 >= work.s1 || work.b + 1 >= a.B) break;
   __syncthreads();  // the next sequence's rows go where these were read
   }
 }
@@ -829,7 +832,7 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
   // Turning a tile's codes to float16 costs a wave as much as the softmax and products of 28 rows, so more rows per block pay where
-  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 117 us against 130 in blocks of 32; 64 rows fill two
+  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 112 us against 130 in blocks of 32; 64 rows fill two
   // blocks of 32).  At 64 the turning is half as much and blocks of 32 keep three workgroups per CU (512 rows: 49 us, 77 in
   // blocks of 48); at 256 more than 32 rows do not fit the registers.
   auto cost = [&](int rt) { return (rows + 16 * rt - 1) / (16 * rt) * (28 + 16 * rt); };

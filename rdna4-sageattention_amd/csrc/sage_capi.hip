@@ -158,7 +158,7 @@ const char* sage_manifest_json(void) {
          "\"rope\": {\"layouts\": [\"halves\", \"interleaved\"], \"rot_dim\": \"multiple of 8\", \"angles\": \"turns in float64\"}, "
          "\"cache\": {\"codes\": [\"int8\", \"e4m3\"], \"scale\": \"fp32 per (token, kv head)\", "
          "\"layout\": \"[pages, kv_heads, page_size, head_dim]\", \"page_size\": \"power of two, 16 to 1024\", "
-         "\"attn\": {\"threads\": 256, \"keys_per_wave\": 32, \"rows\": [16, 32, 64], \"mfma\": \"v_mfma_f32_16x16x32_f16\"}}}";
+         "\"attn\": {\"threads\": 256, \"keys_per_wave\": 32, \"rows\": [16, 32, 48], \"mfma\": \"v_mfma_f32_16x16x32_f16\"}}}";
 }
 
 int sage_forward_workspace(int B, int H, int Hkv, int Sq, int Skv, int D, int causal, int64_t* workspace_bytes) {

@@ -7,6 +7,10 @@
 // Angles: a float32 product p f_i is wrong in its turns from p ~ 10^5 on (a relative error of 2^-24 of 10^5 radians is
 // 0.006), so the turns p f_i / 2 pi are taken in float64, their whole part is dropped there, and the rest, within half
 // a turn, is exact to 2^-25 in float32, where sine and cosine are evaluated.
+//
+// Bound: HBM where there is much to turn, 4 bytes per element: 2 x 8192 tokens of 32 + 8 heads x 128 in 69 us, 4.9 TB/s, the
+// rate of a large copy.  A thread takes 8 or 16 elements of each of its heads as 16-byte vectors (angles once for all of them, while
+// the loads are under way).
 #include "sage_common.h"
 #include "sage_host.h"
 
@@ -174,7 +178,9 @@ extern "C" int sage_rope(const void* q, int64_t qsb, int64_t qss, int64_t qsh, v
   a.H = H, a.heads = H + Hk, a.S = S, a.tokens = B * S, a.D = D, a.R = rot_dim;
   const int mode = interleaved ? ROPE_PAIRS : rot_dim % 16 == 0 ? ROPE_HALF8 : ROPE_HALF4;
   a.chunks = (mode == ROPE_PAIRS ? rot_dim / 8 : mode == ROPE_HALF8 ? rot_dim / 16 : rot_dim / 8) + (D - rot_dim) / 8;
-  const int hp = (int64_t)a.tokens * a.chunks * a.heads >= 4 * 256 * 1024 ? 4 : 1;
+  // four heads per thread share its angles, one where that leaves too few threads (16384 tokens of 40 heads x 128: 68.5 us with
+  // four, 96 with one; 6141 of 20 x 64: 11.7 and 13.9; 1000 of 40 x 128, 320000 threads with one: 9.4 and 8.9)
+  const int hp = (int64_t)a.tokens * a.chunks * a.heads >= 512 * 1024 ? 4 : 1;
   a.slots = (a.heads + hp - 1) / hp;
   a.token_inner = qss < qsh;
   const int64_t blocks = ((int64_t)a.tokens * a.slots * a.chunks + ROPE_THREADS - 1) / ROPE_THREADS;

@@ -1,4 +1,4 @@
-"""What the decoding operators refuse, their host arithmetic and the addresses their kernels read, without a GPU."""
+"""What the decoding operators refuse and their host arithmetic, without a GPU."""
 import ctypes
 import math
 

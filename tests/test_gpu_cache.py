@@ -97,6 +97,32 @@ def test_write_and_read_four_dimensional(dev, layout):
             assert torch.equal(r.cpu(), want)
 
 
+@pytest.mark.parametrize("D, heads, tokens", [(64, 5, 53001), (96, 3, 44003), (128, 7, 19001), (256, 3, 22007)])
+@pytest.mark.parametrize("code", [torch.int8, E4M3])
+def test_many_rows_as_in_small_calls(dev, D, heads, tokens, code):
+    """Rows of calls that take several per thread, some without a slot at their ends: bit for bit those of small calls."""
+    g = torch.Generator().manual_seed(D + heads)
+    n, dtype = 64, torch.float16 if D == 96 else torch.bfloat16
+    pages = -(-tokens // n) + 1
+    k, v = (torch.randn(tokens, heads, D, generator=g).to(dtype).to(dev) for _ in range(2))
+    slots = torch.randperm(pages * n, generator=g)[:tokens].to(dev)
+    slots[-5:] = torch.tensor([-1, pages * n, int(slots[-3]), -7, 2**40], device=dev)
+    one, small = (cdna4_sage.new_cache(pages, n, heads, D, code, dev) for _ in range(2))
+    cdna4_sage.cache_write(one, k, v, slots)
+    for i in range(0, tokens, 999):
+        cdna4_sage.cache_write(small, k[i:i + 999], v[i:i + 999], slots[i:i + 999])
+    for x, y in zip(one, small):
+        assert torch.equal(as_int8(x) if x.dtype != torch.float32 else x, as_int8(y) if y.dtype != torch.float32 else y)
+    codes, scale = quantize(v[-9:].cpu(), code)
+    at = int(slots[-3])
+    assert _codes_equal(codes[-3], one.v[at // n, :, at % n]) and _scales_equal(scale[-3], one.v_scale[at // n, :, at % n])
+    got = cdna4_sage.cache_read(one, slots, dtype)
+    for i in range(0, tokens, 999):
+        for a, b in zip(got, cdna4_sage.cache_read(small, slots[i:i + 999], dtype)):
+            assert torch.equal(a[i:i + 999], b)
+    assert not bool(got[0][-2:].any()) and bool(got[0][-3].any())
+
+
 def test_read_of_every_e4m3_code_and_nan_rows(dev):
     codes = torch.zeros(1, 1, 16, 128, dtype=torch.int8)
     codes[0, 0, :2] = torch.arange(256).to(torch.uint8).view(torch.int8).view(2, 128)
@@ -351,6 +377,35 @@ def test_scales_masks_and_tables_in_other_forms(dev):
     big = torch.tensor([2**31 - 1, 96, -7], dtype=torch.int32)
     table[:, :] = torch.arange(9).view(3, 3)
     _compare(dev, q, cache, table, big)
+
+
+def test_refusals(dev):
+    cache = cdna4_sage.new_cache(4, 16, 2, 64, device=dev)
+    q = torch.zeros(2, 4, 3, 64, dtype=torch.float16, device=dev)
+    table, lengths = torch.zeros(2, 2, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+    tree = torch.ones(3, 3, dtype=torch.bool, device=dev)
+    ok = dict(q=q, cache=cache, block_table=table, lengths=lengths, tensor_layout="HND", sm_scale=None, is_causal=True,
+              tree_mask=None)
+    cdna4_sage.cache_attention(**ok)
+    wide = cdna4_sage.new_cache(4, 16, 2, 128, device=dev)
+    bad = [dict(q=q.float()), dict(q=q[0]), dict(q=q.cpu()), dict(q=q[:, :3]), dict(cache=wide), dict(tensor_layout="x"),
+           dict(block_table=table[:1]), dict(block_table=table.float()), dict(block_table=table.cpu()), dict(block_table=table[0]),
+           dict(lengths=lengths[:1]), dict(lengths=lengths.float()), dict(lengths=lengths.cpu()),
+           dict(lengths=lengths.view(2, 1)), dict(tree_mask=tree.int()), dict(tree_mask=tree[:2]), dict(tree_mask=tree.cpu()),
+           dict(tree_mask=tree.expand(3, 3, 3)), dict(tree_mask=tree, is_causal=False),
+           dict(cache=cache._replace(v=cache.v.cpu())), dict(cache=cache._replace(k=cache.k.transpose(0, 1)))]
+    for kw in bad:
+        with pytest.raises(cdna4_sage.Unsupported):
+            cdna4_sage.cache_attention(**{**ok, **kw})
+    x, slots = torch.zeros(3, 2, 64, dtype=torch.float16, device=dev), torch.zeros(3, dtype=torch.int64, device=dev)
+    for k, v, s in ((x, x, slots[:2]), (x, x, slots.float()), (x, x, slots.cpu()), (x, x.cpu(), slots), (x[:, :1], x[:, :1], slots),
+                    (x.view(1, 3, 2, 64), x.view(1, 3, 2, 64), slots), (x[..., :32], x[..., :32], slots)):
+        with pytest.raises(cdna4_sage.Unsupported):
+            cdna4_sage.cache_write(cache, k, v, s, "NHD")
+    for s in (slots.float(), slots.cpu(), slots.view(1, 1, 3)):
+        with pytest.raises(cdna4_sage.Unsupported):
+            cdna4_sage.cache_read(cache, s)
+    assert not bool(cache.k_scale.any())
 
 
 def test_no_queries_and_no_keys(dev):

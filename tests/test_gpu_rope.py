@@ -137,6 +137,60 @@ def test_gradients_match_formula_and_differences(dev, interleaved, rot):
     _check(g4, dq, pos, freqs, interleaved, factor)
 
 
+@pytest.mark.parametrize("D, rot, interleaved", [(128, 128, False), (64, 24, False), (96, 40, True)])
+def test_many_tokens_as_in_small_calls(dev, D, rot, interleaved):
+    """Calls that turn several heads per thread: bit for bit what small ones give, for heads that are no multiple of them."""
+    H, Hk, S = 11, 3, 5303
+    q, k = (t.to(dev) for t in _inputs(1, S, H, Hk, D, torch.bfloat16, "NHD"))
+    freqs = cdna4_sage.rope_frequencies(rot)[0].to(dev)
+    pos = torch.arange(S, device=dev) * 37 - 1000
+    got = cdna4_sage.rope(q, k, pos, freqs, "NHD", interleaved)
+    for i in range(0, S, 700):
+        want = cdna4_sage.rope(q[:, i:i + 700], k[:, i:i + 700], pos[i:i + 700], freqs, "NHD", interleaved)
+        for a, b in zip(got, want):
+            assert torch.equal(a[:, i:i + 700], b)
+
+
+def test_refusals(dev):
+    q, k = (t.to(dev) for t in _inputs(2, 8, 4, 2, 64, torch.bfloat16, "NHD"))
+    freqs = cdna4_sage.rope_frequencies(64)[0].to(dev)
+    pos = torch.arange(8, device=dev)
+    ok = dict(q=q, k=k, positions=pos, freqs=freqs, tensor_layout="NHD")
+    cdna4_sage.rope(**ok)
+    for kw in (dict(q=q.float()), dict(k=k.half()), dict(q=q[0]), dict(k=k[0]), dict(k=k[:1]), dict(k=k[:, :7]), dict(k=k.cpu()),
+               dict(q=q[..., :32], k=None), dict(freqs=None), dict(freqs=freqs.float()), dict(freqs=freqs[:3]),
+               dict(freqs=freqs.cpu()), dict(freqs=torch.cat([freqs, freqs])), dict(positions=pos.float()),
+               dict(positions=pos[:7]), dict(positions=pos.cpu()), dict(positions=pos.expand(3, 8)), dict(tensor_layout="x")):
+        with pytest.raises(cdna4_sage.Unsupported):
+            cdna4_sage.rope(**{**ok, **kw})
+
+
+def test_training_step_in_a_graph(dev):
+    q, k = (t.to(dev).requires_grad_(True) for t in _inputs(2, 40, 6, 2, 64, torch.float16, "HND"))
+    freqs = cdna4_sage.rope_frequencies(32)[0].to(dev)
+    pos = torch.arange(40, device=dev)
+    dq, dk = (torch.randn_like(t) for t in (q, k))
+
+    def step():
+        out = cdna4_sage.rope(q, k, pos, freqs, "NHD")
+        return torch.autograd.grad(out, (q, k), (dq, dk.mean(2, keepdim=True).expand_as(k)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        pos.add_(11), dq.mul_(-0.5)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+
+
 def test_stream_and_graph(dev):
     B, S, H, Hk, D = 2, 64, 8, 2, 128
     q, k = (t.to(dev) for t in _inputs(B, S, H, Hk, D, torch.bfloat16, "NHD"))
