@@ -16,12 +16,13 @@
 //    V's operand takes that order too: lane (m, g) reads D/16 channels of each of those 8 keys, pairs of keys are
 //    brought together by byte permutes.  Nothing crosses lanes but the row maxima.
 //  * Q rows in bfloat16 are brought into float16's range by a power of two per row, which keeps all their bits.
-//  * P in float16 holds 11 bits of p_ij s^v_j: two running references per row, m (of x) for the sum l and m2 (of
-//    x + log2 s^v) for P, each raised only when a tile passes it by 2^8.  The largest product so far lies between 2^6 and
-//    2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an error of 2^-31 of it below.
+//  * P in float16 holds 11 bits of p_ij s^v_j, p_ij = 2^(x_ij - m): the running reference m of a row is set by its first product
+//    above 0, which it brings to 2^6, and raised when a tile's products pass 2^15 (32 bits hold the sum l at any m).
+//    The largest product so far lies between 2^6 and 2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an
+//    error of 2^-31 of it below.
 // Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000 keys, 8
 // kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us, 3.6 TB/s), the turning of codes and the softmax's
-// vector instructions beyond (132 rows over 16 x 4750 keys: 112 us, 0.37 PFLOP/s of products).
+// vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
 // Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
 #include "sage_cache.h"
 
@@ -165,6 +166,9 @@ __device__ __forceinline__ f16x8 join4(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// 2^(x / 2), a factor to be taken twice: weights between parts below float32's range still count for values far above 1
+__device__ __forceinline__ float half_weight(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
+
 // maximum / sum over the 4 lanes (n, 0..3) of a row, in all of them
 __device__ __forceinline__ float row4_max(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -217,14 +221,15 @@ template <int D, int RT> struct Rows {
   f16x8 qf[RT][NK];
   float qs[RT];   // factor of the scores to log2 units (positive: a hidden score stays -inf)
   int row_t[RT];  // the row's new token
-  float m[RT], m2[RT], f[RT], l[RT];
+  float m[RT], l[RT];
+  float limit[RT];  // of a product: 2^15, -1 while there was none above 0
   v4f acc[RT][NC];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = m2[rt] = -__builtin_inff();
-      f[rt] = 0.0f;
+      m[rt] = -__builtin_inff();
+      limit[rt] = -1.0f;
       l[rt] = 0.0f;
 #pragma unroll
       for (int c = 0; c < NC; ++c) acc[rt][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -303,17 +308,17 @@ template <int D, int RT> struct Rows {
   }
 
   // Scores (with K's scales) to the weights' operand: sums and references brought up to date.  The terms are taken against the
-  // references so far; where one passes them by too much (or a row has none yet) the references are raised first.
+  // references so far; where a product could pass 2^15, or a row has no reference from a product yet, the references are
+  // looked at first.
   __device__ __forceinline__ void weights(const v4f (&s)[RT][2], const v4f (&vs)[2], f16x8 (&pf)[RT]) {
-    float vs_top = 0.0f;
+    float vs_top = 0x1p-85f;  // (a weight stays within 2^100 whatever its scale is)
 #pragma unroll
     for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, vs[j / 4][j % 4]);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float p[8], pv[8];
       float& M = m[rt];
-      auto terms = [&] {
-        const float ref = M == -__builtin_inff() ? 0.0f : M;
+      auto terms = [&](float ref) {
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -322,41 +327,38 @@ template <int D, int RT> struct Rows {
         }
         return top;
       };
-      float top = terms();
-      if (__any(!(top <= 0x1p8f) || M == -__builtin_inff())) {
+      const float top = terms(M == -__builtin_inff() ? 0.0f : M);
+      if (__any(!(top * vs_top <= limit[rt]))) {  // (a bound of the largest product, by two different keys)
         float y = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * qs[rt]);
-        const float up = fmaxf(M, row4_max(y));
-        if (up > M) {
-          l[rt] *= __builtin_amdgcn_exp2f(M - up);
-          M = up;
-          f[rt] = m2[rt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fminf(M - m2[rt], 100.0f));
+        y = row4_max(y);
+        terms(y == -__builtin_inff() ? 0.0f : y);
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, mul_zero(p[j], vs[j / 4][j % 4]));
+        most = row4_max(most);
+        const bool first = limit[rt] < 0.0f, product = most > 0.0f && most < __builtin_inff();
+        // the reference that brings the largest product to [2^6, 2^7), and no weight beyond 2^92
+        float to = fmaxf(y - 92.0f, product ? y + (float)(__builtin_amdgcn_frexp_expf(most) - 7) : -__builtin_inff());
+        if (first) to = product ? fmaxf(to, M - 92.0f) : fmaxf(M, y);
+        if (first ? to > -__builtin_inff() : to > M + 8.0f) {
+          const float down = __builtin_amdgcn_exp2f(M - to);
+          l[rt] *= down;
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) acc[rt][ct] *= down;  // (zeros still, where down is large)
+          M = to;
+          if (product) limit[rt] = 0x1p15f;
         }
-        top = terms();
+        terms(M == -__builtin_inff() ? 0.0f : M);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         l[rt] += p[j];
         pv[j] = mul_zero(p[j], vs[j / 4][j % 4]);
       }
-      // (a bound of the largest product, by two different keys)
-      if (__any(!(top * vs_top * f[rt] <= 0x1p15f) || f[rt] == 0.0f)) {
-        float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, pv[j]);
-        most = row4_max(most);
-        if ((f[rt] == 0.0f || most * f[rt] > 0x1p15f) && most > 0.0f && most < __builtin_inff()) {
-          const float up = fmaxf(m2[rt], M + (float)(__builtin_amdgcn_frexp_expf(most) - 7));
-          const float down = __builtin_amdgcn_exp2f(m2[rt] - up);
-#pragma unroll
-          for (int ct = 0; ct < NC; ++ct) acc[rt][ct] *= down;
-          m2[rt] = up;
-          f[rt] = __builtin_amdgcn_exp2f(fminf(M - up, 100.0f));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)(pv[j] * f[rt]);
+      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)pv[j];
     }
   }
 };
@@ -458,14 +460,14 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
   // LDS of a wave.  16 rows: NS whole tiles, a tile is replaced once it is done with (memory bounds these calls: as many bytes
   // under way as LDS holds).  32 rows and more: K of one tile, V and the scales of two, the next tile is started once this one's
   // scores are there (three workgroups of 32 rows fit a CU, and arithmetic bounds these calls: 200 rows' chunks over 2 x 9500 keys,
-  // 140 us, 161 with two whole tiles and two workgroups).
+  // 136 us, 161 with two whole tiles and two workgroups).
   constexpr bool EARLY = RT >= 2;
   constexpr int NS = EARLY ? 1 : ring_tiles<D>();
   constexpr int PER_WAVE = EARLY ? 3 * Tile::KV + 512 : NS * Tile::BYTES;
   constexpr int JOIN = CA_WAVES * 16 * LD * 4, RING = CA_WAVES * PER_WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t smem[JOIN > RING ? JOIN : RING];
   float (*so)[16][LD] = reinterpret_cast<float (*)[16][LD]>(smem);  // (the waves are joined after their last tile)
-  __shared__ float sm[CA_WAVES][ROWS], sm2[CA_WAVES][ROWS], sl[CA_WAVES][ROWS];
+  __shared__ float sm[CA_WAVES][ROWS], sl[CA_WAVES][ROWS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -672,7 +674,6 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
     const float sum = row4_sum(r.l[rt]);
     if (g == 0) {
       sm[wave][rt * 16 + n] = r.m[rt];
-      sm2[wave][rt * 16 + n] = r.m2[rt];
       sl[wave][rt * 16 + n] = sum;
     }
   }
@@ -680,26 +681,26 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int own = rt * 16 + n;
-    float top2 = sm2[0][own];
+    float top = sm[0][own];
 #pragma unroll
-    for (int w = 1; w < CA_WAVES; ++w) top2 = fmaxf(top2, sm2[w][own]);
-    const float down = r.m2[rt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(r.m2[rt] - top2);
+    for (int w = 1; w < CA_WAVES; ++w) top = fmaxf(top, sm[w][own]);
+    const float down = r.m[rt] == -__builtin_inff() ? 1.0f : half_weight(r.m[rt] - top);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) so[wave][n][v_channel<D>(4 * g + i, c)] = r.acc[rt][c][i] * down;
+      for (int i = 0; i < 4; ++i) so[wave][n][v_channel<D>(4 * g + i, c)] = r.acc[rt][c][i] * down * down;
     __syncthreads();
     // 16 threads per row
     const int row = threadIdx.x / 16, part = threadIdx.x % 16, rr = rt * 16 + row, R = rb * ROWS + rr;
-    float M = sm[0][rr], M2 = sm2[0][rr];
+    float M = sm[0][rr];
 #pragma unroll
-    for (int w = 1; w < CA_WAVES; ++w) M = fmaxf(M, sm[w][rr]), M2 = fmaxf(M2, sm2[w][rr]);
+    for (int w = 1; w < CA_WAVES; ++w) M = fmaxf(M, sm[w][rr]);
     float L = 0.0f;
 #pragma unroll
     for (int w = 0; w < CA_WAVES; ++w)  // (a NaN sum stays one)
       L += sm[w][rr] == -__builtin_inff() ? sl[w][rr] : sl[w][rr] * __builtin_amdgcn_exp2f(sm[w][rr] - M);
     // a row that sees no key: 0, logsumexp -inf
-    const float fin = L == 0.0f ? 0.0f : (M2 == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(M2 - M)) / L;
+    const float fin = 1.0f / L;
     const float lse2 = L == 0.0f ? -__builtin_inff() : M + __builtin_log2f(L);
     constexpr int PER = D / 16;
     float o[PER];
@@ -776,10 +777,10 @@ template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merg
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float now = fmaxf(M, top);
     // (-inf: a part without a visible key; a NaN stays one)
-    const float w = x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - now);
+    const float w = x == -__builtin_inff() ? 0.0f : half_weight(x - now);
     if (now > M) {
-      const float down = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(M - now);
-      o *= down, L *= down, M = now;
+      const float down = M == -__builtin_inff() ? 0.0f : half_weight(M - now);
+      o = o * down * down, L = L * down * down, M = now;
     }
     const int count = min(64, (parts - i0 - slice + slices - 1) / slices);
 #pragma unroll 8
@@ -787,8 +788,8 @@ template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merg
       const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
       vec v = 0.0f;
       if (mine) v = *reinterpret_cast<const vec*>(a.part_o + part(i0 + j * slices + slice) * D + lane * VEC);
-      L += wj;
-      o += v * wj;  // (a part without a visible key holds zeros)
+      L += wj * wj;
+      o += v * wj * wj;  // (a part without a visible key holds zeros)
     }
   }
   if (slices > 1) {
@@ -798,12 +799,12 @@ template <int D> __global__ __launch_bounds__(64 * MERGE_SLICES) void cache_merg
     if (wave) return;
     float top = M;
     for (int i = 1; i < slices; ++i) top = fmaxf(top, sml[i][0]);
-    const float down = M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(M - top);
-    o *= down, L *= down, M = top;
+    const float down = M == -__builtin_inff() ? 1.0f : half_weight(M - top);
+    o = o * down * down, L = L * down * down, M = top;
     for (int i = 1; i < slices; ++i) {
-      const float w = sml[i][0] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(sml[i][0] - top);
-      L += sml[i][1] * w;
-      if (mine) o += *reinterpret_cast<const vec*>(&so[i][lane * VEC]) * w;
+      const float w = sml[i][0] == -__builtin_inff() ? 1.0f : half_weight(sml[i][0] - top);
+      L += sml[i][1] * w * w;
+      if (mine) o += *reinterpret_cast<const vec*>(&so[i][lane * VEC]) * w * w;
     }
   }
   if (L != 0.0f) o *= 1.0f / L;
@@ -832,7 +833,7 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
   // Turning a tile's codes to float16 costs a wave as much as the softmax and products of 28 rows, so more rows per block pay where
-  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 112 us against 130 in blocks of 32; 64 rows fill two
+  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 110 us against 130 in blocks of 32; 64 rows fill two
   // blocks of 32).  At 64 the turning is half as much and blocks of 32 keep three workgroups per CU (512 rows: 49 us, 77 in
   // blocks of 48); at 256 more than 32 rows do not fit the registers.
   auto cost = [&](int rt) { return (rows + 16 * rt - 1) / (16 * rt) * (28 + 16 * rt); };

@@ -352,6 +352,29 @@ def test_rows_of_very_different_magnitudes(dev, dtype):
     _compare(dev, q.to(dtype), cache, table, lengths)
 
 
+@pytest.mark.parametrize("rows", [3, 20, 44])
+@pytest.mark.parametrize("score, value, zeros", [(1, 1, 0), (1, -1, 0), (-1, 1, 0), (-1, -1, 0), (1, 0, 300), (-1, 0, 300), (0, 1, 520),
+                                                 (0, -1, 40)])
+def test_scores_and_values_that_change_along_the_sequence(dev, rows, score, value, zeros):
+    """Scores that rise or fall by some hundreds and values that grow or shrink by 2^160 along the keys, values of 0 first
+    (rows whose sum is all from them for a while): the running reference follows and loses no weight that counts."""
+    g = torch.Generator().manual_seed(rows)
+    page, D, n = 16, 128, 610
+    cache = list(random_cache(g, 40, page, 1, D, torch.int8))
+    lengths = torch.tensor([n], dtype=torch.int32)
+    table = torch.arange(40, dtype=torch.int32)[None]
+    at = torch.arange(640).view(40, 1, page) / 640
+    q = torch.randn(1, rows, 1, D, generator=g).abs() * 4
+    if score:
+        cache[0] = torch.sign(torch.randn(1, 1, 1, D, generator=g)).expand(40, 1, page, D).to(torch.int8) * 40 + cache[0] // 16
+        cache[2] = cache[2] * 0 + 0.04 * (at if score > 0 else 1 - at)
+    if value:
+        cache[3] = cache[3] * 2.0 ** (160 * value * (at - 0.5))
+    cache[3].view(-1)[:zeros] = 0
+    _compare(dev, q.to(torch.bfloat16), cache, table, lengths)
+    _compare(dev, -q.to(torch.bfloat16), cache, table, lengths, sm_scale=0.7)
+
+
 def test_scales_masks_and_tables_in_other_forms(dev):
     g = torch.Generator().manual_seed(9)
     page, D, Hkv, H, T = 32, 64, 2, 6, 4
