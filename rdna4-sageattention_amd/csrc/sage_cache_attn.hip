@@ -21,7 +21,7 @@
 //    The largest product so far lies between 2^6 and 2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an
 //    error of 2^-31 of it below.
 // Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000 keys, 8
-// kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us, 3.6 TB/s), the turning of codes and the softmax's
+// kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes and the softmax's
 // vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
 // Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
 #include "sage_cache.h"
@@ -899,8 +899,8 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
     for (int64_t n = 2; n <= 8; ++n) best = rounds(n) < best ? rounds(n) : best;
     for (w = 1; rounds(w) > 1.1 * best; ++w) {}
   }
-  // one sequence of up to 512 keys: no parts to join (256 keys, 8 kv heads: 8.9 us, 11.3 with two workers and the joining launch;
-  // 1000 keys: 15 and 12.8)
+  // one sequence of up to 512 keys: no parts to join (8 kv heads, 256 keys: 8.9 us, 10.9 with several workers and the joining
+  // launch; 512: 10.4 and 11.0; 1000: 15 and 11.1)
   if (B == 1 && most <= 4) w = 1;
   p.workers = (int)(w > most ? most : w);
   const int64_t n = p.workers == 1 ? 0 : units * p.workers * 2 * p.part_rows;
