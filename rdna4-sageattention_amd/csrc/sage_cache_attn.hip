@@ -425,7 +425,7 @@ struct Segment {
   bool whole;
   int64_t unit;      // rows in front of its partial
   const int* table;
-  __device__ __forceinline__ Segment(const CacheAttnArgs& a, const Work& w) {
+  __device__ __forceinline__ Segment(const CacheAttnArgs& a, const Work& w, int block_rows) {
     len = w.keys(a);
     const int steps = cache_steps(len);
     take = max(min(steps - w.first, w.s1 - w.s0), 1);  // (1 and more, even if another stream rewrote the lengths by now)
@@ -434,6 +434,7 @@ struct Segment {
     base = len - a.T;  // key of the first new token
     open = a.tree ? base : a.causal ? base + 1 : len;  // keys below are seen by every row
     k_begin = w.first * CA_STEP, k_end = min(len, (w.first + take) * CA_STEP);
+    if (a.causal && !a.tree) k_end = min(k_end, open + (min((w.rb + 1) * block_rows, a.T * a.G) - 1) / a.G);  // the last row's keys
     table = a.table + w.b * a.tsb;
   }
   __device__ __forceinline__ CacheRow rows_of(const CacheAttnArgs& a, int h, int key) const {
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
 
   for (;; ++work.b, work.first = 0) {
   const int b = work.b, h = work.h, rb = work.rb;
-  const Segment seg(a, work);
+  const Segment seg(a, work, ROWS);
   Rows<D, RT> r;
   r.clear();
   uint8_t* ring = smem + wave * PER_WAVE;

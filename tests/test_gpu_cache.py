@@ -352,6 +352,20 @@ def test_rows_of_very_different_magnitudes(dev, dtype):
     _compare(dev, q.to(dtype), cache, table, lengths)
 
 
+@pytest.mark.parametrize("T, H, Hkv, D, code", [(150, 3, 1, 128, torch.int8), (301, 1, 1, 64, E4M3), (97, 4, 2, 256, torch.int8)])
+def test_prompts_of_many_row_blocks(dev, T, H, Hkv, D, code):
+    """Prompts whose earlier rows end before the later ones' keys begin, one behind a prefix, one longer than its keys."""
+    g = torch.Generator().manual_seed(T)
+    lengths = torch.tensor([T, T + 333, T - 40], dtype=torch.int32)
+    page = 16
+    pages = sum(-(-int(x) // page) for x in lengths) + 1
+    cache = random_cache(g, pages, page, Hkv, D, code, spread=0.2)
+    q = torch.randn(3, H, T, D, generator=g).to(torch.bfloat16)
+    table = _table(g, lengths, page, pages)
+    _compare(dev, q, cache, table, lengths)
+    _compare(dev, q, cache, table, lengths, is_causal=False)
+
+
 @pytest.mark.parametrize("rows", [3, 20, 44])
 @pytest.mark.parametrize("score, value, zeros", [(1, 1, 0), (1, -1, 0), (-1, 1, 0), (-1, -1, 0), (1, 0, 300), (-1, 0, 300), (0, 1, 520),
                                                  (0, -1, 40)])
@@ -596,6 +610,50 @@ def test_streams_and_graph(dev):
             assert torch.equal(out, want), i
         assert torch.isfinite(noise)
         lengths += torch.tensor([1, 3, 1], dtype=torch.int32, device=dev)   # the graphs read the lengths on the device
+
+
+def test_threads_on_streams_of_their_own(dev):
+    """Calls of several sizes at once, from threads with a stream each: every one gives what it gives alone."""
+    import threading
+
+    g = torch.Generator().manual_seed(21)
+    page, D, Hkv = 16, 64, 2
+    cache = _to(dev, random_cache(g, 200, page, Hkv, D, E4M3))
+    freqs = cdna4_sage.rope_frequencies(D)[0].to(dev)
+
+    def job(i):
+        gi = torch.Generator().manual_seed(i)
+        lengths = torch.randint(1, 700, (3 + i,), generator=gi, dtype=torch.int32)
+        table = torch.randint(0, 200, (3 + i, 44), generator=gi, dtype=torch.int32).to(dev)
+        q = torch.randn(3 + i, 4, 1 + 3 * i, D, generator=gi).to(torch.bfloat16).to(dev)
+        lengths = lengths.to(dev)
+
+        def run():
+            x = cdna4_sage.rope(q, None, None, freqs)
+            return cdna4_sage.cache_attention(x, cache, table, lengths, return_lse=True)
+
+        return run
+
+    jobs = [job(i) for i in range(4)]
+    want = [run() for run in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(15):
+                got = jobs[i]()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_traced(dev):
