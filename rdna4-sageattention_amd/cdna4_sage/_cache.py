@@ -196,6 +196,9 @@ def cache_read(cache, slots, dtype=torch.bfloat16, tensor_layout="HND"):
 @functools.lru_cache(maxsize=4096)
 def _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages):
     """Workspace bytes of a call of these sizes on GPU `gpu`."""
+    if max_pages * page_size > 2**30 or B * -(-max_pages * page_size // 128) > 2**30:
+        raise Unsupported(f"block_table of {max_pages} pages of {page_size} keys for batch {B} (at most 2^30 keys per sequence, 2^37 "
+                          "in all)")
     with torch.cuda.device(gpu):
         return _capi.cache_attn_workspace(B, H, Hkv, T, D, page_size, max_pages)
 
@@ -242,13 +245,13 @@ def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal
         return out.zero_(), None if lse is None else lse.fill_(float("-inf"))
     if n > _I32_MAX:
         raise Unsupported("tensor too large for 32-bit indexing")
+    ws_bytes = _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages)
     q, sq = _bsh(q, layout)
     ts = block_table.stride()
     if ts[1] != 1 and max_pages > 1:
         block_table = block_table.contiguous()
         ts = block_table.stride()
     lengths = lengths.contiguous()
-    ws_bytes = _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages)
     ws = torch.empty((ws_bytes,), device=device, dtype=torch.uint8) if ws_bytes else None
     _capi.call_on(gpu, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), T * H * D, H * D, D,
                   None if lse is None else lse.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),

@@ -430,6 +430,7 @@ def test_refusals(dev):
            dict(lengths=lengths[:1]), dict(lengths=lengths.float()), dict(lengths=lengths.cpu()),
            dict(lengths=lengths.view(2, 1)), dict(tree_mask=tree.int()), dict(tree_mask=tree[:2]), dict(tree_mask=tree.cpu()),
            dict(tree_mask=tree.expand(3, 3, 3)), dict(tree_mask=tree, is_causal=False),
+           dict(block_table=table[:, :1].expand(2, 2**26 + 1)),    # more keys than the kernel counts
            dict(cache=cache._replace(v=cache.v.cpu())), dict(cache=cache._replace(k=cache.k.transpose(0, 1)))]
     for kw in bad:
         with pytest.raises(cdna4_sage.Unsupported):
