@@ -51,9 +51,11 @@ def _plain_eager(*ts, grad=False) -> bool:
             if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
                 return False
         return True
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        return False
-    return all(type(t) is torch.Tensor for t in ts)
+    recording = torch.is_grad_enabled()
+    for t in ts:
+        if type(t) is not torch.Tensor or (recording and t.requires_grad):
+            return False
+    return True
 
 
 def device_arch(device: torch.device) -> str:

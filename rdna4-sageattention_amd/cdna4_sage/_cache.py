@@ -58,14 +58,15 @@ def check_cache(cache, gpu=None):
     """(pages, kv_heads, page_size, head_dim) of a usable cache (on GPU `gpu`); raises Unsupported with the reason."""
     k, v, ks, vs = cache
     shape = k.shape
-    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
+    pages, heads, page_size, D = shape if len(shape) == 4 else (0, 0, 0, 0)
+    rows = (pages, heads, page_size)
+    if len(shape) != 4 or v.shape != shape or ks.shape != rows or vs.shape != rows:
         raise Unsupported("cache codes [pages, kv_heads, page_size, head_dim] and scales [pages, kv_heads, page_size] required")
     dtype = k.dtype
     if dtype not in CACHE_DTYPES or v.dtype != dtype:
         raise Unsupported(f"cache dtype {dtype}/{v.dtype} (int8 or float8_e4m3fn)")
     if ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise Unsupported("cache scales must be float32")
-    pages, heads, page_size, D = shape
     _check_page(page_size)
     if D not in HEAD_DIMS:
         raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
@@ -156,7 +157,7 @@ def read_launch(cache, slots, dtype, layout):
         raise Unsupported("slots [tokens] or [B, tokens] required")
     gpu = cache.k.get_device()
     slots = _check_slots(slots, gpu, shape)
-    k = torch.empty((*shape, Hkv, D), dtype=dtype, device=slots.device)
+    k = cache.k.new_empty((*shape, Hkv, D), dtype=dtype)
     v = torch.empty_like(k)
     n = k.numel()
     if n:
@@ -204,7 +205,7 @@ def _workspace(gpu, B, H, Hkv, T, D, page_size, max_pages):
 
 
 def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal, tree_mask, return_lse):
-    """Output (B, T, H, D) contiguous in q's dtype, and the logsumexp [B, H, T] or None."""
+    """Output in q's layout and dtype, contiguous as (B, T, H, D), and the logsumexp [B, H, T] or None."""
     if layout != "HND" and layout != "NHD":
         raise Unsupported(f"layout {layout!r}")
     shape = q.shape
@@ -237,9 +238,9 @@ def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal
         if len(ms) == 2 or tree_mask.shape[0] == 1:
             ms = (0, *ms[-2:])
         mask = tree_mask.data_ptr()
-    device = q.device
-    out = torch.empty((B, T, H, D), device=device, dtype=q.dtype)
-    lse = torch.empty((B, H, T), device=device, dtype=torch.float32) if return_lse else None
+    # (one allocation call each: the host's time is most of a small call's)
+    out = q.new_empty_strided(shape, (T * H * D, D, H * D, 1) if layout == "HND" else (T * H * D, H * D, D, 1))
+    lse = q.new_empty((B, H, T), dtype=torch.float32) if return_lse else None
     max_pages, n = block_table.shape[1], q.numel()
     if n == 0 or max_pages == 0:   # no query rows, or no keys
         return out.zero_(), None if lse is None else lse.fill_(float("-inf"))
@@ -252,7 +253,7 @@ def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal
         block_table = block_table.contiguous()
         ts = block_table.stride()
     lengths = lengths.contiguous()
-    ws = torch.empty((ws_bytes,), device=device, dtype=torch.uint8) if ws_bytes else None
+    ws = q.new_empty(ws_bytes // 2) if ws_bytes else None   # (q's elements are of 2 bytes, the workspace's of 4)
     _capi.call_on(gpu, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), T * H * D, H * D, D,
                   None if lse is None else lse.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
                   cache.v.data_ptr(), cache.v_scale.data_ptr(), block_table.data_ptr(), ts[0], lengths.data_ptr(),
@@ -282,14 +283,14 @@ def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scal
     non-positive one stands for 1 / sqrt(D).  Raises Unsupported for what the kernel does not take."""
     sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
     ts = (q, *cache, block_table, lengths)
-    lse = None
     if _plain_eager(*ts) and (tree_mask is None or type(tree_mask) is torch.Tensor):
         out, lse = attention_launch(q, cache, block_table, lengths, tensor_layout, sm, is_causal, tree_mask, return_lse)
     elif return_lse:
         out, lse = ops.cache_attention_lse(q, *cache, block_table, lengths, tree_mask, tensor_layout, sm, bool(is_causal))
+        out = out.transpose(1, 2) if tensor_layout == "HND" else out
     else:
         out = ops.cache_attention(q, *cache, block_table, lengths, tree_mask, tensor_layout, sm, bool(is_causal))
-    out = out.transpose(1, 2) if tensor_layout == "HND" else out
+        out = out.transpose(1, 2) if tensor_layout == "HND" else out
     return (out, lse) if return_lse else out
 
 

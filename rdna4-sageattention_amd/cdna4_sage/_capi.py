@@ -96,7 +96,10 @@ def lib():
 
 
 def call(name: str, *args) -> None:
-    rc = getattr(lib(), name)(*args)
+    _check(name, getattr(lib(), name)(*args))
+
+
+def _check(name: str, rc: int) -> None:
     if rc != SAGE_OK:
         raise SageError(name, rc, lib().sage_last_error().decode(errors="replace"))
 
@@ -104,7 +107,9 @@ def call(name: str, *args) -> None:
 def call_on(di: int, name: str, *args) -> None:
     """call with the current stream of GPU `di` as the last argument, that GPU current."""
     if di == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(di))
+        rc = getattr(_lib or lib(), name)(*args, torch._C._cuda_getCurrentRawStream(di))
+        if rc != SAGE_OK:
+            _check(name, rc)
     else:
         with torch.cuda.device(di):
             call(name, *args, torch._C._cuda_getCurrentRawStream(di))

@@ -131,8 +131,9 @@ def cache_attention(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_scale
     1 / sqrt(head_dim)."""
     from . import _cache
 
-    return _cache.attention_launch(q, _cache.KVCache(k8, v8, k_scale, v_scale), block_table, lengths, layout, sm_scale,
-                                   is_causal, tree_mask, False)[0]
+    out, _ = _cache.attention_launch(q, _cache.KVCache(k8, v8, k_scale, v_scale), block_table, lengths, layout, sm_scale,
+                                     is_causal, tree_mask, False)
+    return out.transpose(1, 2) if layout == "HND" else out
 
 
 @cache_attention.register_fake
@@ -148,8 +149,9 @@ def cache_attention_lse(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_s
     """cache_attention and the logsumexp of its rows, fp32 [batch, heads, tokens]."""
     from . import _cache
 
-    return _cache.attention_launch(q, _cache.KVCache(k8, v8, k_scale, v_scale), block_table, lengths, layout, sm_scale,
-                                   is_causal, tree_mask, True)
+    out, lse = _cache.attention_launch(q, _cache.KVCache(k8, v8, k_scale, v_scale), block_table, lengths, layout, sm_scale,
+                                       is_causal, tree_mask, True)
+    return out.transpose(1, 2) if layout == "HND" else out, lse
 
 
 @cache_attention_lse.register_fake
