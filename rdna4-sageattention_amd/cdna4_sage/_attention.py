@@ -45,10 +45,11 @@ def _plain_eager(*ts, grad=False) -> bool:
     if grad:
         if torch._C._functorch.peek_interpreter_stack() is not None:
             return False
+        duals = forward_ad._current_level >= 0
         for t in ts:
             if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
                 return False
-            if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            if duals and forward_ad.unpack_dual(t).tangent is not None:
                 return False
         return True
     recording = torch.is_grad_enabled()

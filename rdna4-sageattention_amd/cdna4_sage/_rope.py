@@ -178,7 +178,7 @@ def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved
         raise Unsupported("freqs are required (rope_frequencies)")
     ts = (q,) if k is None else (q, k)
     if _plain_eager(*ts, grad=True):
-        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
             out = _Rope.apply(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
         else:
             out = rope_launch(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
