@@ -20,9 +20,9 @@
 //    above 0, which it brings to 2^6, and raised when a tile's products pass 2^15 (32 bits hold the sum l at any m).
 //    The largest product so far lies between 2^6 and 2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an
 //    error of 2^-31 of it below.
-// Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000 keys, 8
-// kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes and the softmax's
-// vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
+// Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000
+// keys, 8 kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes
+// and the softmax's vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
 // Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
 #include "sage_cache.h"
 
@@ -59,8 +59,8 @@ struct CacheAttnArgs {
 };
 
 // Work of one kv head and row block: the steps (CA_STEP keys) of all sequences in a row, at least one each, cut into
-// `workers` ranges that differ by one step at most, the longer ones first, whatever the sequences' lengths.  A worker's range holds whole sequences,
-// whose output it writes, and up to two parts: of the one it begins inside of (partial 0) and of the one that it begins
+// `workers` ranges that differ by one step at most, the longer ones first, whatever the sequences' lengths.  A worker's
+// range holds whole sequences, whose output it writes, and up to two parts: of the one it begins inside of (partial 0) and of the one that it begins
 // but does not end (partial 1); a second kernel joins those.  The lengths stay on the device: every wave adds them up.
 __device__ __forceinline__ int cache_keys(const CacheAttnArgs& a, int b) {
   return min(max(a.lengths[b], 0), a.max_pages * a.page_size);
@@ -408,7 +408,9 @@ struct Pace {
     __builtin_amdgcn_s_setprio(3);
     next();
   }
-  __device__ __forceinline__ void next() { at = level == 3 ? total / 2 : level == 2 ? total - total / 5 : level == 1 ? total - total / 16 : 0x7FFFFFFF; }
+  __device__ __forceinline__ void next() {
+    at = level == 3 ? total / 2 : level == 2 ? total - total / 5 : level == 1 ? total - total / 16 : 0x7FFFFFFF;
+  }
   __device__ __forceinline__ void done(int steps) {
     if (steps < at) return;
     --level;
@@ -453,17 +455,17 @@ struct Segment {
 };
 
 template <int D, int CT, int RT>
-__global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 : 3) : 1) void cache_attn_kernel(const CacheAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, D == 64 && RT == 2 ? 3 : D == 256 && RT == 2 ? 1 : 2) void cache_attn_kernel(const CacheAttnArgs a) {
   constexpr int NK = D / 32, NC = D / 16;
   constexpr int ROWS = 16 * RT;
   constexpr int LD = D + 4;  // LDS row stride of the joining of the waves, in floats
   using Tile = CacheTile<D>;
-  // LDS of a wave.  16 rows: NS whole tiles, a tile is replaced once it is done with (memory bounds these calls: as many bytes
-  // under way as LDS holds).  32 rows and more: K of one tile, V and the scales of two, the next tile is started once this one's
-  // scores are there (three workgroups of 32 rows fit a CU, and arithmetic bounds these calls: 200 rows' chunks over 2 x 9500 keys,
-  // 136 us, 161 with two whole tiles and two workgroups).
-  constexpr bool EARLY = RT >= 2;
-  constexpr int NS = EARLY ? 1 : ring_tiles<D>();
+  // LDS of a wave: NS whole tiles, a tile is replaced once it is done with (as many bytes under way as the LDS of the workgroups
+  // that share a CU holds).  48 rows: K of one tile, V and the scales of two, the next tile is started once this one's scores are
+  // there (132 rows over 16 x 4750 keys: 111 us, 112 with two whole tiles).  Blocks of 32 rows at head dim 128 in a third of a CU's
+  // registers, with spills: 64 rows over 8 x 5000 keys 58 us, in half of them 45.
+  constexpr bool EARLY = RT == 3;
+  constexpr int NS = EARLY ? 1 : RT == 2 ? 2 : ring_tiles<D>();
   constexpr int PER_WAVE = EARLY ? 3 * Tile::KV + 512 : NS * Tile::BYTES;
   constexpr int JOIN = CA_WAVES * 16 * LD * 4, RING = CA_WAVES * PER_WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t smem[JOIN > RING ? JOIN : RING];
@@ -495,9 +497,9 @@ __global__ __launch_bounds__(CA_THREADS, RT == 1 ? 2 : D <= 128 ? (RT == 3 ? 2 :
   const int v_per = D == 96 ? 4 : D / 16;  // bytes of a key that the lane starts from
   const int v_at0 = 4 * g * D + (v_per * n & 15) + 16 * ((v_per * n >> 4) ^ (D == 96 ? 0 : Tile::swap(4 * g)));
   const uint32_t from0 = Tile::first(lane);
-  // 32 rows leave no registers to keep what is derived from these through the loop
+  // 32 rows and more leave no registers to keep what is derived from these through the loop
   auto afresh = [&](auto x) {
-    if (EARLY) asm volatile("" : "+v"(x));
+    if (RT >= 2) asm volatile("" : "+v"(x));
     return x;
   };
   auto issue = [&](CacheRow at0, CacheRow at1, int stage) {
@@ -880,18 +882,21 @@ struct CachePlan {
 static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
-  // Turning a tile's codes to float16 costs a wave as much as the softmax and products of 28 rows, so more rows per block pay where
-  // they are not padding: blocks of 48 at head dims 96 and 128 (132 rows: 110 us against 130 in blocks of 32; 64 rows fill two
-  // blocks of 32).  At 64 the turning is half as much and blocks of 32 keep three workgroups per CU (512 rows: 49 us, 77 in
-  // blocks of 48); at 256 more than 32 rows do not fit the registers.
-  auto cost = [&](int rt) { return (rows + 16 * rt - 1) / (16 * rt) * (28 + 16 * rt); };
-  p.rt = rows <= 16 ? 1 : D == 64 || D == 256 || cost(2) <= cost(3) ? 2 : 3;
+  const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
+  // Blocks of 32 rows, or of 48 at head dims 96 and 128 where they are long walks and not padding: turning a tile's codes to float16
+  // costs as much as the softmax and products of some 28 rows, so a tile of 48 rows takes 1.2 times one of 32, but a call some
+  // 13 us more (its prologue and its joining of the waves).  In us with 32 and 48, 8 kv heads x 128: 132 rows over 16 sequences of
+  // up to 9001 keys 128 and 110, 96 rows over 16 of up to 16000 152 and 139; 96 over 8 of up to 8000 54 and 58, 800 over 2 of
+  // up to 16000 134 and 136, 48 over 4 of up to 6000 33 and 40.  (The lengths are on the device: the table's width stands for
+  // them.)  At 64 the turning is half as much, at 256 more than 32 rows do not fit the registers.
+  const int64_t n2 = (rows + 31) / 32, n3 = (rows + 47) / 48;
+  const bool wide = (D == 96 || D == 128) && (double)most * Hkv * (5 * n2 - 6 * n3) > 90.0 * 2 * cus;
+  p.rt = rows <= 16 ? 1 : wide ? 3 : 2;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
   // workgroups that run at once
-  const int64_t slots = (int64_t)cus * (D == 256 ? 1 : p.rt == 2 ? 3 : 2);
-  const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
+  const int64_t slots = (int64_t)cus * (D == 256 ? 1 : D == 64 && p.rt == 2 ? 3 : 2);
   int64_t w = slots / units;
   if (w < 8) {
     // few workers per unit: the fewest whose rounds are within a tenth of the best of up to 8
