@@ -434,9 +434,10 @@ struct Segment {
     whole = take == steps;
     unit = ((((int64_t)w.h * a.row_blocks + w.rb) * a.workers + w.worker) * 2 + (w.first > 0 ? 0 : 1)) * a.part_rows;
     base = len - a.T;  // key of the first new token
-    open = a.tree ? base : a.causal ? base + 1 : len;  // keys below are seen by every row
+    // keys below `open` are seen by every row of the block; its last row sees none from k_end on
+    open = a.tree ? base : a.causal ? base + 1 + w.rb * block_rows / a.G : len;
     k_begin = w.first * CA_STEP, k_end = min(len, (w.first + take) * CA_STEP);
-    if (a.causal && !a.tree) k_end = min(k_end, open + (min((w.rb + 1) * block_rows, a.T * a.G) - 1) / a.G);  // the last row's keys
+    if (a.causal && !a.tree) k_end = min(k_end, base + 1 + (min((w.rb + 1) * block_rows, a.T * a.G) - 1) / a.G);
     table = a.table + w.b * a.tsb;
   }
   __device__ __forceinline__ CacheRow rows_of(const CacheAttnArgs& a, int h, int key) const {
