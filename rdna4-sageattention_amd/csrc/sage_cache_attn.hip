@@ -883,29 +883,35 @@ struct CachePlan {
 static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, int cus) {
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
-  const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);
-  // Blocks of 32 rows, or of 48 at head dims 96 and 128 where they are long walks and not padding: turning a tile's codes to float16
-  // costs as much as the softmax and products of some 28 rows, so a tile of 48 rows takes 1.2 times one of 32, but a call some
-  // 13 us more (its prologue and its joining of the waves).  In us with 32 and 48, 8 kv heads x 128: 132 rows over 16 sequences of
-  // up to 9001 keys 128 and 110, 96 rows over 16 of up to 16000 152 and 139; 96 over 8 of up to 8000 54 and 58, 800 over 2 of
-  // up to 16000 134 and 136, 48 over 4 of up to 6000 33 and 40.  (The lengths are on the device: the table's width stands for
-  // them.)  At 64 the turning is half as much, at 256 more than 32 rows do not fit the registers.
-  const int64_t n2 = (rows + 31) / 32, n3 = (rows + 47) / 48;
-  const bool wide = (D == 96 || D == 128) && (double)most * Hkv * (5 * n2 - 6 * n3) > 90.0 * 2 * cus;
-  p.rt = rows <= 16 ? 1 : wide ? 3 : 2;
+  const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);  // (the lengths are on the device: the table's width)
+  // Time of a call in blocks of 16 rt rows, in steps of a workgroup of 32 rows, with the number w of workers for it: rounds of
+  // workgroups that run at once, times a walk and what a workgroup costs beside it, which is 4 steps more where parts are
+  // written and joined and 7 more in blocks of 48 rows (13 us).  A step of those takes 1.2 times one of 32 rows: turning codes to
+  // float16 costs as much as the softmax and products of some 28 rows.
+  auto time = [&](int rt, int64_t& w) {
+    const int64_t units = Hkv * ((rows + 16 * rt - 1) / (16 * rt));
+    const int64_t slots = (int64_t)cus * (D == 256 ? 1 : D == 64 && rt == 2 ? 3 : 2);
+    const bool many = slots / units >= 8;  // one round whatever w is
+    double best = 0.0;
+    w = 0;
+    for (int64_t n = many ? slots / units : 1; n <= (many ? slots / units : 8); ++n) {
+      const int64_t rounds = (units * n + slots - 1) / slots;
+      const double t = rounds * ((double)most / n * (rt == 3 ? 1.2 : 1.0) + (n == 1 ? 3.0 : 7.0) + (rt == 3 ? 7.0 : 0.0));
+      if (w == 0 || t < best) best = t, w = n;
+    }
+    return best;
+  };
+  int64_t w = 0, w3 = 0;
+  p.rt = rows <= 16 ? 1 : 2;
+  const double t = time(p.rt, w);
+  // Blocks of 48 rows at head dims 96 and 128 (at 64 the turning is half as much, at 256 they do not fit the registers).  In us with
+  // 32 and 48, 8 kv heads x 128: 132 rows over 16 sequences of up to 9001 keys 128 and 110, 96 rows over 16 of up to 16000 152
+  // and 139, a prompt of 8192 962 and 834; 96 over 8 of up to 8000 54 and 58, 48 over 4 of up to 6000 33 and 40, a prompt of 2048
+  // 103 and 250.
+  if (rows > 16 && (D == 96 || D == 128) && time(3, w3) < t) p.rt = 3, w = w3;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
   const int64_t units = (int64_t)Hkv * p.row_blocks;
-  // workgroups that run at once
-  const int64_t slots = (int64_t)cus * (D == 256 ? 1 : D == 64 && p.rt == 2 ? 3 : 2);
-  int64_t w = slots / units;
-  if (w < 8) {
-    // few workers per unit: the fewest whose rounds are within a tenth of the best of up to 8
-    auto rounds = [&](int64_t n) { return (double)((units * n + slots - 1) / slots) / (double)n; };
-    double best = rounds(1);
-    for (int64_t n = 2; n <= 8; ++n) best = rounds(n) < best ? rounds(n) : best;
-    for (w = 1; rounds(w) > 1.1 * best; ++w) {}
-  }
   // one sequence of up to 512 keys: no parts to join (8 kv heads, 256 keys: 8.9 us, 10.9 with several workers and the joining
   // launch; 512: 10.4 and 11.0; 1000: 15 and 11.1)
   if (B == 1 && most <= 4) w = 1;
