@@ -95,8 +95,10 @@ def attention_slack(mag, big, out, D, dtype):
     subnormals, are off by up to 2^-25, that is 2^-31 of the largest; each is multiplied by its code, so together by at
     most 2^-31 max_j (p_j s_j) sum_j |code_j|.  No multiple of sum_j p_j |v_j| bounds that: in a channel where the keys of
     large products have code 0 the sum can be as small as one likes.  attention's second term of mag times 2^-11 is twice
-    that."""
-    return mag * (2.0 ** -11 + 2.0 ** -20 + 2.0 * score_slack(big, D).unsqueeze(-1)) + out.abs() * step(dtype) + 1e-30
+    that.  A float16 output below 2^-14 lies between multiples of 2^-24 and is rounded by up to 2^-25, more than half a step
+    relative to it (9.5017e-06, the value of a single visible key, has the neighbours 9.4771e-06 and 9.5367e-06)."""
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-30
+    return mag * (2.0 ** -11 + 2.0 ** -20 + 2.0 * score_slack(big, D).unsqueeze(-1)) + out.abs() * step(dtype) + tiny
 
 
 def lse_slack(big, lse, D):

@@ -352,6 +352,26 @@ def test_rows_of_very_different_magnitudes(dev, dtype):
     _compare(dev, q.to(dtype), cache, table, lengths)
 
 
+@pytest.mark.parametrize("kind", ["causal", "full", "tree"])
+@pytest.mark.parametrize("T, H, Hkv, D, code, dtype", [(33, 8, 2, 128, torch.int8, torch.bfloat16), (35, 4, 1, 128, E4M3, torch.float16),
+                                                       (45, 6, 2, 96, torch.int8, torch.float16), (29, 5, 1, 96, E4M3, torch.bfloat16),
+                                                       (27, 5, 1, 96, E4M3, torch.bfloat16)])
+def test_wide_tables(dev, T, H, Hkv, D, code, dtype, kind):
+    """Tables of far more columns than the lengths use, whose width alone makes the largest blocks of rows."""
+    g = torch.Generator().manual_seed(T)
+    lengths = torch.tensor([T + 400, T, 0, T - 7, 1300], dtype=torch.int32)
+    page = 64
+    pages = sum(-(-max(int(x), 0) // page) for x in lengths) + 2
+    cache = random_cache(g, pages, page, Hkv, D, code, spread=0.2)
+    q = torch.randn(5, H, T, D, generator=g).to(dtype)
+    table = _table(g, lengths, page, pages, columns=2500)
+    tree = _tree(g, 5, T) if kind == "tree" else None
+    _compare(dev, q, cache, table, lengths, is_causal=kind != "full", tree=tree)
+    holes = table.clone()
+    holes[0, 2] = -1
+    _compare(dev, q, cache, holes, lengths, is_causal=kind != "full", tree=tree)
+
+
 @pytest.mark.parametrize("T, H, Hkv, D, code", [(150, 3, 1, 128, torch.int8), (301, 1, 1, 64, E4M3), (97, 4, 2, 256, torch.int8)])
 def test_prompts_of_many_row_blocks(dev, T, H, Hkv, D, code):
     """Prompts whose earlier rows end before the later ones' keys begin, one behind a prefix, one longer than its keys."""
