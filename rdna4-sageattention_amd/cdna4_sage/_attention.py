@@ -40,23 +40,37 @@ def _plain_eager(*ts, grad=False) -> bool:
     its fake implementation and autograd sees an op without a derivative (backward raises, as in the reference).
     grad=True: for a call that deals with reverse-mode autograd itself (forward-mode duals and functorch's wrappers then go
     to the op)."""
+    if grad:
+        return (_plain_tensors(*ts) and torch._C._functorch.peek_interpreter_stack() is None
+                and not (forward_ad._current_level >= 0 and _any_tangent(ts)))
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
         return False
-    if grad:
-        if torch._C._functorch.peek_interpreter_stack() is not None:
-            return False
-        duals = forward_ad._current_level >= 0
-        for t in ts:
-            if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
-                return False
-            if duals and forward_ad.unpack_dual(t).tangent is not None:
-                return False
-        return True
     recording = torch.is_grad_enabled()
     for t in ts:
         if type(t) is not torch.Tensor or (recording and t.requires_grad):
             return False
     return True
+
+
+def _plain_tensors(*ts) -> bool:
+    """True outside of tracing and dispatch modes, for tensors of no subclass (functorch's wrappers count as plain)."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        return False
+    for t in ts:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
+
+
+def _any_tangent(ts) -> bool:
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
+def refuse_tangents(what, *ts):
+    """Raises for inputs with forward-mode tangents, which a registered op would drop without a word.  A tracer cannot
+    look at them: while it traces inside a forward-mode level, every call raises."""
+    if forward_ad._current_level >= 0 and (torch.compiler.is_compiling() or _any_tangent(ts)):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def device_arch(device: torch.device) -> str:

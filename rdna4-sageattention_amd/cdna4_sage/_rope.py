@@ -8,9 +8,11 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi, ops
-from ._attention import _I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_eager, gpu_arch
+from ._attention import (_I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _plain_tensors, gpu_arch,
+                         refuse_tangents)
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling=None, device=None):
@@ -142,21 +144,33 @@ def _out_bsh(t, layout):
     return t, ((s[0], s[2], s[1]) if layout == "HND" else s[:3])
 
 
+def _transformed():
+    """Inside a forward-mode level or one of torch.func's transforms."""
+    return forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+
+
 class _Rope(torch.autograd.Function):
+    """rope_launch with its derivatives.  The rotation is linear: tangents turn as the inputs do, gradients turn back, and
+    each is an application of its own, so that derivatives have derivatives and torch.func's transforms compose."""
+
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, layout, interleaved, factor, inverse):
-        ctx.save_for_backward(positions, freqs)
-        ctx.how = layout, interleaved, factor, inverse
+    def forward(q, k, positions, freqs, layout, interleaved, factor, inverse):
         return rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse)
 
     @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, positions, freqs, *how = inputs
+        ctx.save_for_backward(positions, freqs)
+        ctx.save_for_forward(positions, freqs)
+        ctx.how = how
+
+    @staticmethod
     def backward(ctx, dq, dk):
-        positions, freqs = ctx.saved_tensors
-        layout, interleaved, factor, inverse = ctx.how
+        *how, inverse = ctx.how
         need_q, need_k = ctx.needs_input_grad[:2]
-        back = (positions, freqs, layout, interleaved, factor, not inverse)
+        back = (*ctx.saved_tensors, *how, not inverse)
         # (create_graph: the gradients have gradients of their own)
-        turn = _Rope.apply if torch.is_grad_enabled() else rope_launch
+        turn = _Rope.apply if _transformed() or torch.is_grad_enabled() else rope_launch
         if need_q and need_k:
             dq, dk = turn(dq, dk, *back)
         elif need_q:
@@ -165,25 +179,57 @@ class _Rope(torch.autograd.Function):
             dq, dk = None, turn(dk, None, *back)[0] if need_k else None
         return dq, dk, None, None, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # (an input without a tangent comes with one of zeros)
+        return _Rope.apply(tq, tk, *ctx.saved_tensors, *ctx.how)
+
+    @staticmethod
+    def vmap(info, in_dims, q, k, positions, freqs, *how):
+        n = info.batch_size
+        if in_dims[3] is not None:   # frequencies of each entry's own: one launch each
+            outs = [_Rope.apply(*(t if d is None else t.select(d, i) for t, d in zip((q, k, positions, freqs), in_dims)), *how)
+                    for i in range(n)]
+            return (torch.stack([o[0] for o in outs]), None if k is None else torch.stack([o[1] for o in outs])), \
+                (0, None if k is None else 0)
+
+        def first(t, d):
+            return t.expand(n, *t.shape) if d is None else t.movedim(d, 0)
+
+        # the mapped dimension joins the batch
+        q, k = first(q, in_dims[0]), None if k is None else first(k, in_dims[1])
+        B = q.shape[1]
+        if positions is not None and (in_dims[2] is not None or positions.dim() > 1):
+            positions = first(positions, in_dims[2])
+            if positions.dim() == 2:
+                positions = positions[:, None]
+            if positions.dim() != 3 or positions.shape[1] not in (1, B):
+                raise Unsupported(f"positions of shape {tuple(positions.shape[1:])} for batch {B}")
+            positions = positions.expand(n, B, positions.shape[2]).flatten(0, 1)
+        oq, ok = _Rope.apply(q.flatten(0, 1), None if k is None else k.flatten(0, 1), positions, freqs, *how)
+        return (oq.unflatten(0, (n, B)), None if k is None else ok.unflatten(0, (n, B))), (0, None if k is None else 0)
+
 
 def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved=False, factor=1.0):
     """Rotary positions: the first 2 * freqs.numel() channels of every head are pairs, (i, i + rot_dim / 2) or, interleaved,
     (2 i, 2 i + 1), and pair i of a token at position p turns by p * freqs[i] radians, times `factor`; the other
     channels are copied.  q: [B, heads, tokens, head_dim] for "HND", [B, tokens, heads, head_dim] for "NHD", k alike with
     heads of its own, bf16 or fp16.  positions: int32 / int64 [tokens] or [B, tokens] (None: 0, 1, ..).  freqs, factor:
-    rope_frequencies.  Returns q, or (q, k), in new tensors.  Differentiable in q and k (to any order); float32
+    rope_frequencies.  Returns q, or (q, k), in new tensors.  Differentiable in q and k (to any order, in reverse and forward
+    mode, by torch.func's transforms too; under torch.compile in reverse mode, forward mode raises); float32
     arithmetic, rounded once.  Before a backward pass is captured into a graph, drop the eager graphs of the same leaves:
     torch would wait for their streams, which ends the capture.  Raises Unsupported for what the kernel does not take."""
     if freqs is None:
         raise Unsupported("freqs are required (rope_frequencies)")
     ts = (q,) if k is None else (q, k)
-    if _plain_eager(*ts, grad=True):
-        if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
-            out = _Rope.apply(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
+    args = (positions, freqs, tensor_layout, interleaved, factor, False)
+    if _plain_tensors(*ts):
+        if ((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled()) or _transformed():
+            out = _Rope.apply(q, k, *args)
         else:
-            out = rope_launch(q, k, positions, freqs, tensor_layout, interleaved, factor, False)
-    elif k is None:
+            out = rope_launch(q, k, *args)
+        return out[0] if k is None else out
+    refuse_tangents("rope under a tracer", *ts)
+    if k is None:
         return ops.rope(q, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
-    else:
-        return ops.rope_qk(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
-    return out[0] if k is None else out
+    return ops.rope_qk(q, k, positions, freqs, tensor_layout, bool(interleaved), float(factor), False)
