@@ -17,7 +17,8 @@ from typing import NamedTuple
 import torch
 
 from . import _capi, ops
-from ._attention import (_I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _packed, _plain_eager, gpu_arch)
+from ._attention import (_I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, _packed, _plain_eager, gpu_arch,
+                         refuse_tangents)
 from ._rope import rope
 
 CACHE_DTYPES = {torch.int8: _capi.CACHE_INT8, torch.float8_e4m3fn: _capi.CACHE_E4M3}
@@ -179,7 +180,8 @@ def cache_write(cache, k, v, slots, tensor_layout="HND"):
     the nearest codes of x / scale, ties to even; a row with an infinity or a NaN is kept as NaN (by its scale).
     k / v: [B, kv_heads, tokens, head_dim] ("HND") or [B, tokens, kv_heads, head_dim] ("NHD") with slots [B, tokens], or packed
     [tokens, kv_heads, head_dim] with slots [tokens]; slots int32 or int64.  Tokens whose slot is outside the cache (-1) are
-    left out; two tokens of a call may not share a slot (that slot's row then holds parts of both)."""
+    left out; two tokens of a call may not share a slot (that slot's row then holds parts of both).  Codes have no
+    derivative: gradients and tangents of k and v end here."""
     if _plain_eager(k, v, slots, *cache, grad=True):   # (codes have no derivative: autograd sees nothing of the write)
         write_launch(cache, k, v, slots, tensor_layout)
     else:
@@ -188,7 +190,9 @@ def cache_write(cache, k, v, slots, tensor_layout="HND"):
 
 def cache_read(cache, slots, dtype=torch.bfloat16, tensor_layout="HND"):
     """(k, v) of the slots as code * scale, rounded to dtype: packed [tokens, kv_heads, head_dim] for slots [tokens] (as
-    sageattn_varlen takes them), 4D in tensor_layout for slots [B, tokens].  Slots outside the cache (-1) give zeros."""
+    sageattn_varlen takes them), 4D in tensor_layout for slots [B, tokens].  Slots outside the cache (-1) give zeros.  No derivative in the scales: a
+    backward pass and tangents raise."""
+    refuse_tangents("cache_read", *cache)
     if _plain_eager(slots, *cache):
         return read_launch(cache, slots, dtype, tensor_layout)
     return ops.cache_read(*cache, slots, dtype, tensor_layout)
@@ -280,9 +284,11 @@ def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scal
     shows: bool [T, T] or [B, T, T], True at (i, j) where new token i sees new token j (a tree of drafted tokens: its
     ancestors and itself).  A query that sees no key gives 0 (lengths[b] = 0, say).  Returns the output in q's layout and
     dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  sm_scale: None or a
-    non-positive one stands for 1 / sqrt(D).  Raises Unsupported for what the kernel does not take."""
+    non-positive one stands for 1 / sqrt(D).  There is no derivative: a backward pass and inputs with forward-mode tangents
+    raise.  Raises Unsupported for what the kernel does not take."""
     sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
     ts = (q, *cache, block_table, lengths)
+    refuse_tangents("cache_attention", *ts)
     if _plain_eager(*ts) and (tree_mask is None or type(tree_mask) is torch.Tensor):
         out, lse = attention_launch(q, cache, block_table, lengths, tensor_layout, sm, is_causal, tree_mask, return_lse)
     elif return_lse:

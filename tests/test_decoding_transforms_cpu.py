@@ -116,3 +116,44 @@ def test_a_tracer_refuses_tangents():
     torch._dynamo.reset()
     with pytest.raises(Exception):
         torch.compile(lambda x, u: torch.func.jvp(_rope1, (x,), (u,))[1], backend="aot_eager", fullgraph=True)(q, t)
+
+
+# ---- the cache's operators, which have no derivative ------------------------------------------------------------------
+
+def _attend(monkeypatch, read=False):
+    """cache_attention (or cache_read) of q and the scales with its launch replaced by a product."""
+    from cdna4_sage import _cache
+
+    def launch(q, cache, table, lengths, layout, *rest):
+        q.data_ptr()
+        return q * cache.k_scale.sum(), None
+
+    monkeypatch.setattr(_cache, "attention_launch", launch)
+    monkeypatch.setattr(_cache, "read_launch", lambda cache, slots, dtype, layout: (cache.k_scale * 2, cache.v_scale * 2))
+    cache = cdna4_sage.new_cache(2, 16, 2, 64, device="cpu")
+    table, lengths, slots = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(3, dtype=torch.int64)
+    if read:
+        return lambda _, scale: cdna4_sage.cache_read(cache._replace(k_scale=scale), slots)[0], cache
+    return lambda q, scale: cdna4_sage.cache_attention(q, cache._replace(k_scale=scale), table, lengths, "NHD"), cache
+
+
+@pytest.mark.parametrize("read", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+def test_the_cache_refuses_tangents(monkeypatch, read, grad):
+    call, cache = _attend(monkeypatch, read)
+    q, s = torch.randn(1, 1, 4, 64), cache.k_scale + 1
+    call(q, s)
+    with forward_ad.dual_level():
+        call(q, s)                                            # no tangent: as ever
+        with pytest.raises(NotImplementedError):
+            call(q, forward_ad.make_dual(s.clone().requires_grad_(grad), s))
+        if not read:
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(q.clone().requires_grad_(grad), q), s)
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda x: call(q, x), (s,), (s,))
+    with pytest.raises(NotImplementedError):
+        torch.vmap(lambda x, u: torch.func.jvp(lambda y: call(q, y), (x,), (u,))[1])(s[None], s[None])
+    # (one of the transformed function's constants has none)
+    out, tangent = torch.func.jvp(lambda x: x * call(q, s).sum(), (s,), (s,))
+    assert torch.equal(out, tangent)
