@@ -163,6 +163,8 @@ class _Rope(torch.autograd.Function):
         ctx.save_for_backward(positions, freqs)
         ctx.save_for_forward(positions, freqs)
         ctx.how = how
+        if not _transformed():   # the output of an input that needs no gradient needs none either
+            ctx.mark_non_differentiable(*(y for y, need in zip(output, ctx.needs_input_grad) if y is not None and not need))
 
     @staticmethod
     def backward(ctx, dq, dk):

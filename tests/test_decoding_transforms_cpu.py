@@ -157,3 +157,24 @@ def test_the_cache_refuses_tangents(monkeypatch, read, grad):
     # (one of the transformed function's constants has none)
     out, tangent = torch.func.jvp(lambda x: x * call(q, s).sum(), (s,), (s,))
     assert torch.equal(out, tangent)
+
+
+def test_only_outputs_of_inputs_that_need_a_gradient_need_one():
+    for flags in ((True, False), (False, True), (True, True), (False, False)):
+        q, k = (_r(10 + i).requires_grad_(flag) for i, flag in enumerate(flags))
+        out = _rope2(q, k)
+        assert tuple(y.requires_grad for y in out) == flags
+        if not any(flags):
+            continue
+        got = torch.autograd.grad([y for y in out if y.requires_grad], [x for x in (q, k) if x.requires_grad],
+                                  [_r(20 + i) for i in range(sum(flags))], create_graph=True)
+        for i, x in enumerate(got):
+            _same(x, _turn(_r(20 + i), True, back=True))
+    with torch.no_grad():
+        assert not any(y.requires_grad for y in _rope2(_r(1).requires_grad_(True), _r(2)))
+    # (a gradient of a gradient in one of two)
+    q, k = _r(11).requires_grad_(True), _r(12)
+    u = _r(13).requires_grad_(True)
+    (g,) = torch.autograd.grad(_rope2(q, k)[0], q, u, create_graph=True)
+    (gg,) = torch.autograd.grad(g, u, _r(14))
+    _same(gg, _turn(_r(14), True))
