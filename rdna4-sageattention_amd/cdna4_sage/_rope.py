@@ -105,16 +105,16 @@ def check_rope(q, k, positions, freqs, layout):
 
 
 def rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse):
-    """The rotated q (and k), in new tensors of the inputs' memory order."""
+    """The rotated q (and k), in new tensors (out_like)."""
     B, S, H, D, gpu = check_rope(q, k, positions, freqs, layout)
-    oq = torch.empty_like(q)
-    ok = None if k is None else torch.empty_like(k)
+    oq = out_like(q)
+    ok = None if k is None else out_like(k)
     if q.numel() == 0:   # no tokens, or no query heads: k alone
         if k is None or k.numel() == 0:
             return oq, ok
         return oq, rope_launch(k, None, positions, freqs, layout, interleaved, factor, inverse)[0]
     q, sq = _bsh(q, layout)
-    oq, so = _out_bsh(oq, layout)
+    so = _bsh(oq, layout)[1]
     pos, p64, pb, ps = None, 0, 0, 0
     if positions is not None:
         st = positions.stride()
@@ -127,7 +127,7 @@ def rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse):
     Hk = 0 if k is None else k.shape[1 if layout == "HND" else 2]
     if Hk:
         k, sk = _bsh(k, layout)
-        ok, sko = _out_bsh(ok, layout)
+        sko = _bsh(ok, layout)[1]
         _capi.call_on(gpu, "sage_rope", q.data_ptr(), *sq, oq.data_ptr(), *so, H, k.data_ptr(), *sk, ok.data_ptr(), *sko,
                       Hk, *rest)
     else:
@@ -135,13 +135,14 @@ def rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse):
     return oq, ok
 
 
-def _out_bsh(t, layout):
-    """(b, s, h) strides of an output; one that the kernel cannot store 16-byte vectors into is made contiguous."""
-    s = t.stride()
-    if s[3] != 1 or t.data_ptr() % 16 or s[0] % 8 or s[1] % 8 or s[2] % 8:
-        t = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        s = t.stride()
-    return t, ((s[0], s[2], s[1]) if layout == "HND" else s[:3])
+def out_like(t):
+    """An output for t: in t's memory order, or contiguous where the kernel cannot store 16-byte vectors in that order (the
+    ops' fake implementations promise the same)."""
+    out = torch.empty_like(t)
+    s = out.stride()
+    if len(s) == 4 and (s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8):
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return out
 
 
 def _transformed():
@@ -217,10 +218,11 @@ def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved
     (2 i, 2 i + 1), and pair i of a token at position p turns by p * freqs[i] radians, times `factor`; the other
     channels are copied.  q: [B, heads, tokens, head_dim] for "HND", [B, tokens, heads, head_dim] for "NHD", k alike with
     heads of its own, bf16 or fp16.  positions: int32 / int64 [tokens] or [B, tokens] (None: 0, 1, ..).  freqs, factor:
-    rope_frequencies.  Returns q, or (q, k), in new tensors.  Differentiable in q and k (to any order, in reverse and forward
-    mode, by torch.func's transforms too; under torch.compile in reverse mode, forward mode raises); float32
-    arithmetic, rounded once.  Before a backward pass is captured into a graph, drop the eager graphs of the same leaves:
-    torch would wait for their streams, which ends the capture.  Raises Unsupported for what the kernel does not take."""
+    rope_frequencies.  Returns q, or (q, k), in new tensors, of the inputs' memory order where head_dim is innermost there.
+    Differentiable in q and k (to any order, in reverse and forward mode, by torch.func's transforms too; under torch.compile
+    in reverse mode, forward mode raises); float32 arithmetic, rounded once.  Before a backward pass is captured into a graph,
+    drop the eager graphs of the same leaves: torch would wait for their streams, which ends the capture.  Raises
+    Unsupported for what the kernel does not take."""
     if freqs is None:
         raise Unsupported("freqs are required (rope_frequencies)")
     ts = (q,) if k is None else (q, k)

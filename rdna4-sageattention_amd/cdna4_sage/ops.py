@@ -59,7 +59,9 @@ def rope(x: torch.Tensor, positions: Optional[torch.Tensor], freqs: torch.Tensor
 
 @rope.register_fake
 def _fake_rope(x, positions, freqs, layout, interleaved, factor, inverse):
-    return torch.empty_like(x)
+    from . import _rope
+
+    return _rope.out_like(x)
 
 
 @torch.library.custom_op("cdna4_sage::rope_qk", mutates_args=())
@@ -73,7 +75,9 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor],
 
 @rope_qk.register_fake
 def _fake_rope_qk(q, k, positions, freqs, layout, interleaved, factor, inverse):
-    return torch.empty_like(q), torch.empty_like(k)
+    from . import _rope
+
+    return _rope.out_like(q), _rope.out_like(k)
 
 
 def _rope_setup(ctx, inputs, output):

@@ -178,3 +178,34 @@ def test_only_outputs_of_inputs_that_need_a_gradient_need_one():
     (g,) = torch.autograd.grad(_rope2(q, k)[0], q, u, create_graph=True)
     (gg,) = torch.autograd.grad(g, u, _r(14))
     _same(gg, _turn(_r(14), True))
+
+
+# ---- what tracers are told about the outputs --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_rope_outputs_have_the_strides_that_tracers_are_told(monkeypatch, layout):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    monkeypatch.undo()                         # the launch itself, without its kernel
+    monkeypatch.setattr(_rope._capi, "call_on", lambda *a: None)
+
+    def check(q, k, positions, freqs, layout):
+        b, s, h, d = q.shape if layout == "NHD" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+        return b, s, h, d, 0
+
+    monkeypatch.setattr(_rope, "check_rope", check)
+    base = torch.zeros(2, 8, 16, 64, dtype=torch.float16)
+    forms = [base, base.transpose(1, 2), base.permute(0, 1, 3, 2).contiguous().transpose(2, 3),
+             base.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0), torch.zeros(0, 8, 16, 64, dtype=torch.float16), base[:, :, :1].expand(2, 8, 16, 64),
+             torch.zeros(2, 8, 16, 65, dtype=torch.float16)[..., :64], base[:1],
+             torch.zeros(12345 + 8192, dtype=torch.float16).as_strided((1, 8, 16, 64), (12345, 1024, 64, 1))]
+    f = cdna4_sage.rope_frequencies(64)[0]
+    for x in forms:
+        real = torch.ops.cdna4_sage.rope_qk(x, x, None, f, layout, False, 1.0, False)
+        one = torch.ops.cdna4_sage.rope(x, None, f, layout, False, 1.0, False)
+        with FakeTensorMode() as mode:
+            y = mode.from_tensor(x)
+            fake = torch.ops.cdna4_sage.rope_qk(y, y, None, mode.from_tensor(f), layout, False, 1.0, False)
+            only = torch.ops.cdna4_sage.rope(y, None, mode.from_tensor(f), layout, False, 1.0, False)
+        for a, b in zip((*real, one), (*fake, only)):
+            assert a.shape == b.shape and a.stride() == b.stride(), x.stride()

@@ -45,3 +45,22 @@ def test_transforms(dev, layout, interleaved, dtype):
     per = torch.arange(5 * S, device=dev).view(5, S)
     got = torch.vmap(lambda y, p: cdna4_sage.rope(y, None, p, freqs, layout, interleaved))(many, per)
     assert torch.equal(got, torch.stack([cdna4_sage.rope(y, None, p, freqs, layout, interleaved) for y, p in zip(many, per)]))
+
+
+def test_traced_with_head_dim_outside(dev):
+    """Inputs and gradients whose memory order has another dimension innermost, against the eager call."""
+    g = torch.Generator().manual_seed(2)
+    q, k, dq = (torch.randn(2, h, 64, 16, generator=g).half().to(dev).transpose(2, 3) for h in (4, 2, 4))
+    freqs = cdna4_sage.rope_frequencies(64)[0].to(dev)
+    want = cdna4_sage.rope(q.contiguous(), k.contiguous(), None, freqs)
+    fn = torch.compile(lambda a, b: [y * 1.0 for y in cdna4_sage.rope(a, b, None, freqs)], backend="aot_eager", fullgraph=True)
+    for got in (fn(q, k), cdna4_sage.rope(q, k, None, freqs)):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    torch.library.opcheck(torch.ops.cdna4_sage.rope_qk.default, (q, k, None, freqs, "HND", False, 1.0, False),
+                          test_utils=("test_schema", "test_faketensor"))
+    x = q.detach().requires_grad_(True)
+    (a,) = torch.autograd.grad(fn(x, k)[0], x, dq)
+    y = q.contiguous().requires_grad_(True)
+    (b,) = torch.autograd.grad(cdna4_sage.rope(y, None, None, freqs), y, dq.contiguous())
+    assert torch.equal(a, b)
