@@ -701,8 +701,10 @@ __global__ __launch_bounds__(CA_THREADS, D == 64 && RT == 2 ? 3 : D == 256 && RT
     for (int w = 1; w < CA_WAVES; ++w) M = fmaxf(M, sm[w][rr]);
     float L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < CA_WAVES; ++w)  // (a NaN sum stays one)
-      L += sm[w][rr] == -__builtin_inff() ? sl[w][rr] : sl[w][rr] * __builtin_amdgcn_exp2f(sm[w][rr] - M);
+    for (int w = 0; w < CA_WAVES; ++w) {  // (a NaN sum stays one; references of one row lie up to some 190 apart by the sizes of values alone)
+      const float down = sm[w][rr] == -__builtin_inff() ? 1.0f : half_weight(sm[w][rr] - M);
+      L += sl[w][rr] * down * down;
+    }
     // a row that sees no key: 0, logsumexp -inf
     const float fin = 1.0f / L;
     const float lse2 = L == 0.0f ? -__builtin_inff() : M + __builtin_log2f(L);
