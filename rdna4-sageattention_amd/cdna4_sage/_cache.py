@@ -21,6 +21,7 @@ from ._attention import (_I32_MAX, ARCHS, DTYPES, HEAD_DIMS, Unsupported, _bsh, 
                          refuse_tangents)
 from ._rope import rope
 
+_F32_NORMAL, _F32_MAX = torch.finfo(torch.float32).smallest_normal, torch.finfo(torch.float32).max
 CACHE_DTYPES = {torch.int8: _capi.CACHE_INT8, torch.float8_e4m3fn: _capi.CACHE_E4M3}
 
 
@@ -283,10 +284,12 @@ def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scal
     ones and, of those, its own and the earlier ones (is_causal), all (is_causal=False), or those its row of tree_mask
     shows: bool [T, T] or [B, T, T], True at (i, j) where new token i sees new token j (a tree of drafted tokens: its
     ancestors and itself).  A query that sees no key gives 0 (lengths[b] = 0, say).  Returns the output in q's layout and
-    dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  sm_scale: None or a
-    non-positive one stands for 1 / sqrt(D).  There is no derivative: a backward pass and inputs with forward-mode tangents
+    dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  sm_scale: a
+    positive normal number of float32; None or a non-positive one stands for 1 / sqrt(D).  There is no derivative: a backward pass and inputs with forward-mode tangents
     raise.  Raises Unsupported for what the kernel does not take."""
     sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
+    if sm and not _F32_NORMAL <= sm <= _F32_MAX:
+        raise Unsupported(f"sm_scale {sm} (float32's normal numbers)")
     ts = (q, *cache, block_table, lengths)
     refuse_tangents("cache_attention", *ts)
     if _plain_eager(*ts) and (tree_mask is None or type(tree_mask) is torch.Tensor):

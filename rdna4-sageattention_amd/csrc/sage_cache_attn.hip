@@ -24,6 +24,8 @@
 // keys, 8 kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes
 // and the softmax's vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
 // Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
+#include <cmath>
+
 #include "sage_cache.h"
 
 namespace sage {
@@ -53,7 +55,8 @@ struct CacheAttnArgs {
   int pages, page_size, page_shift, max_pages;
   int row_blocks, workers;
   int part_rows;                    // rows of a partial: 16 RT, or all of them where that is fewer
-  float scale;                      // softmax scale * log2 e
+  float scale;                      // softmax scale * log2 e = scale 2^scale_exp, scale in [1/2, 1)
+  int scale_exp;
   float* part_o;                    // [kv head][row block][worker][2][part_rows][D]
   float* part_lse;                  // the same without D, log2
 };
@@ -219,7 +222,10 @@ struct CacheRow {
 template <int D, int RT> struct Rows {
   static constexpr int NK = D / 32, NC = D / 16;
   f16x8 qf[RT][NK];
-  float qs[RT];   // factor of the scores to log2 units (positive: a hidden score stays -inf)
+  // Factor of the scores to log2 units, from one power of two, so that no step of it leaves float32's range.  Positive: a hidden
+  // score stays -inf.  Below 2^-126 it has fewer bits, within 2^-150 of the exact factor: a score, which is below 2^124 before it,
+  // is off by no more than 2^-26.
+  float qs[RT];
   int row_t[RT];  // the row's new token
   float m[RT], l[RT];
   float limit[RT];  // of a product: 2^15, -1 while there was none above 0
@@ -255,7 +261,7 @@ template <int D, int RT> struct Rows {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const uint32_t(&w)[D / 8] = qw[rt];
-      qs[rt] = a.scale;
+      int power = a.scale_exp;
       if (a.dtype == DT_BF16) {
         float top = 0.0f;
 #pragma unroll
@@ -263,8 +269,7 @@ template <int D, int RT> struct Rows {
         const uint32_t e = max(__float_as_uint(row4_max(top)) >> 23, 15u);  // of the row's largest magnitude
         // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
         const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
-        const float down = e == 255u ? 1.0f : __uint_as_float((e - 14u) << 23);
-        qs[rt] = fmaxf(qs[rt] * down, 0x1p-126f);
+        power += e == 255u ? 0 : (int)e - 141;
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
@@ -277,6 +282,7 @@ template <int D, int RT> struct Rows {
         for (int i = 0; i < NK; ++i)
           qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
       }
+      qs[rt] = fminf(fmaxf(__builtin_ldexpf(a.scale, power), 0x1p-149f), 0x1.fffffep127f);
 #pragma unroll
       for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(qf[rt][i]));  // waited for here, not in the loop
     }
@@ -997,8 +1003,8 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   SAGE_REQUIRE((((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)lse) & 3u) == 0,
                "%s: block_table, lengths or lse misaligned", who);
   if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
-  SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale must be finite and not negative (got %g)",
-               who, (double)sm_scale);
+  SAGE_REQUIRE(sm_scale == 0.0f || (sm_scale >= 0x1p-126f && sm_scale <= 0x1.fffffep127f),
+               "%s: sm_scale must be 0 or a positive normal number (got %g)", who, (double)sm_scale);
   if (tree_mask) {
     auto far = [&](int64_t stride) { return (stride < 0 ? -stride : stride) > 0x3FFFFFFF / (T > 1 ? T - 1 : 1); };
     SAGE_REQUIRE(!far(msq) && !far(msk), "%s: a tree mask's rows and columns must lie within 2^31 bytes", who);
@@ -1020,8 +1026,7 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   a.page_shift = __builtin_ctz((unsigned)page_size);
   a.row_blocks = p.row_blocks, a.workers = p.workers, a.part_rows = p.part_rows;
   const double scale = sm_scale > 0.0f ? (double)sm_scale : 1.0 / __builtin_sqrt((double)D);
-  a.scale = (float)(scale * 1.44269504088896340736);
-  if (a.scale < 0x1p-126f) a.scale = 0x1p-126f;
+  a.scale = (float)std::frexp(scale * 1.44269504088896340736, &a.scale_exp);
   a.part_o = (float*)workspace;
   a.part_lse = (float*)((char*)workspace + p.o_bytes);
   const int64_t groups = ((int64_t)Hkv * p.workers + 7) / 8 * 8;

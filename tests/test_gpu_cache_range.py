@@ -9,6 +9,25 @@ from test_gpu_cache import _compare
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("rows", [3, 20, 44])
+@pytest.mark.parametrize("power, sm_scale", [(-112, None), (-120, None), (-131, None), (-100, 2.0**-30), (-112, 2.0**-20),
+                                             (10, 2.0**-126)])
+def test_small_queries_and_scales_beside_large_keys(dev, rows, power, sm_scale):
+    """Scores that are far from both ends of float32's range, of factors that are not: keys of 2^99, queries and scales down
+    to the smallest."""
+    g = torch.Generator().manual_seed(rows)
+    page, D, n = 16, 256, 70
+    cache = list(random_cache(g, 5, page, 1, D, torch.int8))
+    sign = torch.sign(torch.randn(D, generator=g))
+    cache[0] = (sign * torch.randint(60, 128, (5, 1, page, D), generator=g)).to(torch.int8)
+    cache[2] = 2.0 ** (92.0 * torch.rand(5, 1, page, generator=g).sqrt())
+    cache[2][-1] = 2.0**92
+    q = (sign * torch.rand(1, rows, 1, D, generator=g) * 2.0**power).to(torch.bfloat16)
+    assert bool(q.any())
+    lengths = torch.tensor([n], dtype=torch.int32)
+    _compare(dev, q, cache, torch.arange(5, dtype=torch.int32)[None], lengths, sm_scale=sm_scale)
+
+
 @pytest.mark.parametrize("rows, D", [(1, 64), (2, 128), (24, 96), (20, 256), (44, 128)])
 @pytest.mark.parametrize("high", [0, 1, 2, 3])
 def test_neighbouring_tiles_of_very_different_values(dev, rows, D, high):
