@@ -335,6 +335,15 @@ template <int D, int RT> struct Rows {
       };
       const float top = terms(M == -__builtin_inff() ? 0.0f : M);
       if (__any(!(top * vs_top <= limit[rt]))) {  // (a bound of the largest product, by two different keys)
+        // Whether a reference is raised follows from the row's own products alone, or its last bits would depend on the scales of keys
+        // that it does not see and on the other rows of the wave.
+        bool raise = false;
+        if (__any(limit[rt] > 0.0f)) {
+          float now = 0.0f;  // (0 times the infinite scale of a hidden key: NaN, which fmaxf leaves out)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) now = fmaxf(now, p[j] * fmaxf(vs[j / 4][j % 4], 0x1p-85f));
+          raise = row4_max(now) > limit[rt];
+        }
         float y = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 8; ++j) y = fmaxf(y, s[rt][j / 4][j % 4] * qs[rt]);
@@ -348,7 +357,7 @@ template <int D, int RT> struct Rows {
         // the reference that brings the largest product to [2^6, 2^7), and no weight beyond 2^92
         float to = fmaxf(y - 92.0f, product ? y + (float)(__builtin_amdgcn_frexp_expf(most) - 7) : -__builtin_inff());
         if (first) to = product ? fmaxf(to, M - 92.0f) : fmaxf(M, y);
-        if (first ? to > -__builtin_inff() : to > M + 8.0f) {
+        if (first ? to > -__builtin_inff() : raise) {
           const float down = __builtin_amdgcn_exp2f(M - to);
           l[rt] *= down;
 #pragma unroll

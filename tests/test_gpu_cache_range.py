@@ -1,12 +1,17 @@
 """cache_attention at the ends of its range: tiny and infinite queries, values of very different sizes side by side, places
 that a row does not see, and the joining of many rows that come in several parts each."""
+import math
+
 import pytest
 import torch
 
+import cdna4_sage
 from cache_util import random_cache
-from test_gpu_cache import _compare
+from test_gpu_cache import _compare, _to
 
 pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("rows", [3, 20, 44])
@@ -43,3 +48,45 @@ def test_neighbouring_tiles_of_very_different_values(dev, rows, D, high):
     _compare(dev, q, cache, table, lengths)
     cache[3] = torch.where(tile == high, 2.0**-93, 2.0**86) * (1 + torch.rand(8, 1, page, generator=g))
     _compare(dev, q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("rows, D", [(1, 64), (3, 128), (20, 128), (44, 128), (44, 96), (20, 256)])
+@pytest.mark.parametrize("code", [torch.int8, E4M3])
+def test_a_row_never_changes_with_what_it_does_not_see(dev, rows, D, code):
+    """Weights whose largest lies within a factor of two of where the running reference is raised, beside scales of hidden
+    keys, and beside other rows, that are far above: the bits stay."""
+    page, n = 16, 150
+    differ = 0
+    for seed in range(12):
+        g = torch.Generator().manual_seed(100 * seed + rows)
+        cache = list(random_cache(g, 10, page, 1, D, code))
+        codes = cache[0].float()
+        codes.view(160, D)[:] = torch.randint(-2, 3, (160, D), generator=g)
+        codes.view(160, D)[140] = 96
+        cache[0] = codes.to(code)
+        q = (0.5 + torch.rand(1, rows, 1, D, generator=g)).to(torch.float16)
+        # the score of key 140 is 7.6 to 8.3 in units of ln 2, those of the others next to 0
+        cache[2] = cache[2] * 0 + 2.0**-12
+        cache[2].view(-1)[140] = (7.6 + seed / 16) * math.log(2) / (96 * D) * D**0.5
+        table, lengths = torch.arange(10, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+        run = lambda q, c, l=lengths, **kw: cdna4_sage.cache_attention(  # noqa: E731
+            q.to(dev), _to(dev, c), table.to(dev), l.to(dev), return_lse=True, **kw)
+        clean = run(q, cache)
+        for value in (math.inf, 1e30, 1e4):
+            dirty = [t.clone() for t in cache]
+            dirty[3].view(-1)[n:] = value
+            for a, b in zip(clean, run(q, dirty)):
+                differ += not torch.equal(a, b)
+        # the last row alone changes: queries of other rows do not reach the first ones
+        if rows > 1:
+            other = q.clone()
+            other[0, -1] *= 30
+            for a, b in zip(clean, run(other, cache)):
+                differ += not torch.equal(a[:, :-1], b[:, :-1])
+        # what comes behind a new token: the first of two new tokens beside a second of other sizes
+        two = torch.cat([q, q], 2)
+        late = [t.clone() for t in cache]
+        late[3].view(-1)[n - 1] = 1e20
+        for a, b in zip(run(two, cache), run(two, late)):
+            differ += not torch.equal(a[:, :, 0], b[:, :, 0])
+    assert differ == 0
