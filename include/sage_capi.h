@@ -285,9 +285,10 @@ int sage_cache_read(void* k, int64_t ksb, int64_t kss, int64_t ksh, void* v, int
  * outside [0, pages) hides its keys.  Query i sees every key before the new ones and, of those, its own and the earlier
  * ones (causal), all (causal = 0) or, with a tree mask (one byte per element, nonzero = visible, (b, i, j) at tree_mask
  * + b * msb + i * msq + j * msk), those its row shows; where lengths[b] < T the first new tokens have no key.  A query
- * without a visible key is written as 0, its logsumexp as -inf.  q / out: [B, T, H, D] by (b, t, h) strides, dtype
- * bf16 or fp16; lse: fp32 [B, H, T] natural log, or NULL.  sm_scale: 0 (1 / sqrt(D)) or a normal number.  Codes and scales of keys that no
- * query of a step sees may hold anything; E4M3 codes of the new tokens must not be NaN.
+ * without a visible key is written as 0, its logsumexp as -inf; any other one that holds an infinity or a NaN as NaN,
+ * both.  q / out: [B, T, H, D] by (b, t, h) strides, dtype bf16 or fp16; lse: fp32 [B, H, T] natural log, or NULL.
+ * sm_scale: 0 (1 / sqrt(D)) or a normal number.  Codes and scales of keys that no query of a step sees may hold
+ * anything; E4M3 codes of the new tokens must not be NaN.
  * workspace: sage_cache_attn_workspace bytes, 256-byte aligned (NULL where that is 0).
  */
 int sage_cache_attn_workspace(int B, int H, int Hkv, int T, int D, int page_size, int max_pages,

@@ -32,6 +32,7 @@ namespace sage {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int CA_WAVES = 4;
 constexpr int CA_THREADS = 64 * CA_WAVES;
@@ -262,6 +263,7 @@ template <int D, int RT> struct Rows {
     for (int rt = 0; rt < RT; ++rt) {
       const uint32_t(&w)[D / 8] = qw[rt];
       int power = a.scale_exp;
+      bool endless;  // the row holds an infinity: each of its scores is one or NaN, and its weights are NaN whatever the signs
       if (a.dtype == DT_BF16) {
         float top = 0.0f;
 #pragma unroll
@@ -270,6 +272,7 @@ template <int D, int RT> struct Rows {
         // largest magnitude to [2^14, 2^15): a value 2^-28 of it still keeps its 8 bits
         const float up = e == 255u ? 1.0f : __uint_as_float((268u - e) << 23);
         power += e == 255u ? 0 : (int)e - 141;
+        endless = e == 255u;
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
@@ -278,10 +281,16 @@ template <int D, int RT> struct Rows {
             qf[rt][i][2 * j + 1] = (_Float16)(bf16_hi(w[4 * i + j]) * up);
           }
       } else {
+        u16x2 top = {0, 0};
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+        endless = row4_max((float)max(top[0], top[1])) >= (float)0x7C00;
 #pragma unroll
         for (int i = 0; i < NK; ++i)
           qf[rt][i] = __builtin_bit_cast(f16x8, v4i{(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2], (int)w[4 * i + 3]});
       }
+      // (scores of NaN: those of -inf would count as hidden)
+      if (endless) qf[rt][0] = __builtin_bit_cast(f16x8, v4i{0x7E007E00, 0x7E007E00, 0x7E007E00, 0x7E007E00});
       qs[rt] = fminf(fmaxf(__builtin_ldexpf(a.scale, power), 0x1p-149f), 0x1.fffffep127f);
 #pragma unroll
       for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(qf[rt][i]));  // waited for here, not in the loop

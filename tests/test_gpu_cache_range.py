@@ -7,7 +7,7 @@ import torch
 
 import cdna4_sage
 from cache_util import random_cache
-from test_gpu_cache import _compare, _to
+from test_gpu_cache import _compare, _table, _to
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,38 @@ def test_a_row_never_changes_with_what_it_does_not_see(dev, rows, D, code):
         for a, b in zip(run(two, cache), run(two, late)):
             differ += not torch.equal(a[:, :, 0], b[:, :, 0])
     assert differ == 0
+
+
+@pytest.mark.parametrize("T, H, Hkv, D", [(1, 4, 2, 64), (3, 10, 1, 128), (7, 7, 1, 96), (5, 8, 2, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("code", [torch.int8, E4M3])
+def test_an_infinite_query_gives_nan_where_it_sees_a_key(dev, T, H, Hkv, D, dtype, sign, code):
+    """The infinite channel meets codes of one sign only, or none but zeros: scores of -inf, +inf or NaN alone."""
+    g = torch.Generator().manual_seed(T)
+    lengths = torch.tensor([90, T, max(T - 2, 0), 0], dtype=torch.int32)
+    page, pages = 16, 16
+    cache = list(random_cache(g, pages, page, Hkv, D, code))
+    c = int(torch.randint(0, D, (1,), generator=g))
+    k = cache[0].float()
+    k[..., c] = sign * k[..., c].abs().clamp(min=1)
+    k[..., (c + 1) % D] = 0
+    cache[0] = k.to(code)
+    table = _table(g, lengths, page, pages)
+    q = torch.randn(4, H, T, D, generator=g).to(dtype)
+    clean = cdna4_sage.cache_attention(q.to(dev), _to(dev, cache), table.to(dev), lengths.to(dev), return_lse=True)
+    bad = torch.zeros(4, H, T, dtype=torch.bool)
+    bad[:, 0, T - 1], bad[:, H - 1, 0], bad[:, H // 2, T // 2] = True, True, True
+    for at, value in ((c, -math.inf), (c, math.inf), ((c + 1) % D, math.inf), (c, math.nan)):
+        x = q.clone()
+        x[..., at][bad] = value
+        out, lse = cdna4_sage.cache_attention(x.to(dev), _to(dev, cache), table.to(dev), lengths.to(dev), return_lse=True)
+        sees = torch.zeros(4, H, T, dtype=torch.bool)
+        for b, n in enumerate(lengths.tolist()):
+            sees[b, :, max(T - n, 0):] = True
+        want = bad & sees
+        assert torch.equal(torch.isnan(out.cpu()).all(-1), want) and torch.equal(torch.isnan(out.cpu()).any(-1), want)
+        assert torch.equal(torch.isnan(lse.cpu()), want)
+        assert not bool(out.cpu()[~sees].any()) and bool((lse.cpu()[~sees] == -math.inf).all())
+        for a, b in zip((out.cpu(), lse.cpu()), clean):
+            assert torch.equal(a[~want], b.cpu()[~want])
