@@ -7,7 +7,8 @@ import torch
 
 import cdna4_sage
 from cache_util import random_cache
-from test_gpu_cache import _compare, _table, _to
+from cdna4_sage import _capi
+from test_gpu_cache import _compare, _table, _to, _tree
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +126,50 @@ def test_an_infinite_query_gives_nan_where_it_sees_a_key(dev, T, H, Hkv, D, dtyp
         assert not bool(out.cpu()[~sees].any()) and bool((lse.cpu()[~sees] == -math.inf).all())
         for a, b in zip((out.cpu(), lse.cpu()), clean):
             assert torch.equal(a[~want], b.cpu()[~want])
+
+
+def _parts(lengths, workers):
+    """Ranges that each sequence's steps (128 keys, one at least) lie in, cut evenly as the kernel's header says."""
+    steps = [max(-(-int(n) // 128), 1) for n in lengths]
+    total = sum(steps)
+    workers = min(workers, total)
+    per, longer = divmod(total, workers)
+    of = lambda s: s // (per + 1) if s < longer * (per + 1) else longer + (s - longer * (per + 1)) // per  # noqa: E731
+    out, at = [], 0
+    for s in steps:
+        out.append(of(at + s - 1) - of(at) + 1)
+        at += s
+    return out
+
+
+@pytest.mark.parametrize("D, T, H, Hkv, B, long, columns, rt, code, dtype", [
+    (128, 35, 6, 2, 41, 4000, 125, 2, torch.int8, torch.bfloat16),
+    (128, 35, 6, 2, 41, 4000, 940, 3, torch.int8, torch.float16),
+    (96, 21, 5, 1, 83, 3000, 94, 2, E4M3, torch.float16),
+    (96, 21, 10, 2, 43, 3000, 1500, 3, E4M3, torch.bfloat16),
+    (256, 13, 6, 2, 107, 3500, 112, 2, torch.int8, torch.bfloat16),
+    (64, 27, 6, 2, 53, 3500, 120, 2, E4M3, torch.float16),
+    (128, 1, 32, 4, 270, 6000, 200, 1, torch.int8, torch.bfloat16),
+])
+@pytest.mark.parametrize("kind", ["causal", "tree"])
+def test_many_rows_in_several_parts(dev, D, T, H, Hkv, B, long, columns, rt, code, dtype, kind):
+    """More than 8192 rows to join, of sequences in 1, 2 to 4 and more than 4 parts; groups of four rows that cross blocks of
+    rows, and last ones of fewer."""
+    g = torch.Generator().manual_seed(D + T)
+    page = 32
+    lengths = torch.randint(max(T - 3, 0), 700, (B,), generator=g).to(torch.int32)
+    lengths[B // 3] = long
+    lengths[B // 2] = 0
+    rows = T * (H // Hkv)
+    assert rows * B * Hkv > 8192
+    part_rows = min(rows, 16 * rt)
+    unit = Hkv * -(-rows // (16 * rt)) * 2 * part_rows
+    # the plan's ranges from its workspace: [unit][ranges] rows of D + 1 floats
+    workers = _capi.cache_attn_workspace(B, H, Hkv, T, D, page, columns) // (4 * (D + 1) * unit)
+    parts = _parts(lengths, workers)
+    assert 8 < workers <= 4 * B and max(parts) > 4 and any(2 <= p <= 4 for p in parts), (workers, sorted(set(parts)))
+    pages = sum(-(-int(x) // page) for x in lengths) + 1
+    cache = random_cache(g, pages, page, Hkv, D, code, spread=0.2)
+    q = torch.randn(B, H, T, D, generator=g).to(dtype)
+    table = _table(g, lengths, page, pages, columns=columns)
+    _compare(dev, q, cache, table, lengths, "NHD" if kind == "tree" else "HND", tree=_tree(g, B, T) if kind == "tree" else None)
