@@ -1,0 +1,62 @@
+"""cache_attention's sharing of work: every XCD its part for any number of kv heads, and tables wider than the sequences are
+long.  Times are compared within one run, in turn, with wide margins."""
+import pytest
+import torch
+
+import cdna4_sage
+from cache_util import random_cache
+from test_gpu_cache import _compare, _table, _tree
+
+pytestmark = pytest.mark.gpu
+
+
+def _times(calls, n=20):
+    """GPU time of n calls of each, back to back: the medians of 7 rounds in turn, in us a call."""
+    for call in calls:
+        for _ in range(3):
+            call()
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    out = [[] for _ in calls]
+    for _ in range(7):
+        for call, times in zip(calls, out):
+            torch.cuda.synchronize()
+            start.record()
+            for _ in range(n):
+                call()
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end) * 1e3 / n)
+    return [sorted(t)[3] for t in out]
+
+
+def _prompt(dev, T, Hkv, columns=0, B=1, D=128, H=None):
+    page = 16
+    need = -(-T // page)
+    cache = cdna4_sage.new_cache(B * need, page, Hkv, D, device=dev)
+    k = torch.randn(B * T, Hkv, D, device=dev).to(torch.bfloat16)
+    table = torch.full((B, max(need, columns)), -1, dtype=torch.int32)
+    table[:, :need] = torch.arange(B * need).view(B, need)
+    table, lengths = table.to(dev), torch.full((B,), T, dtype=torch.int32, device=dev)
+    cdna4_sage.cache_write(cache, k, k, cdna4_sage.cache_slots(table, lengths, T, page).view(-1))
+    q = torch.randn(B, 4 * Hkv if H is None else H, T, D, device=dev).to(torch.bfloat16)
+    return lambda: cdna4_sage.cache_attention(q, cache, table, lengths)
+
+
+def test_few_heads_use_the_whole_card(dev):
+    """An eighth (a quarter) of the work of eight kv heads takes far less than their time."""
+    one, two, eight = _times([_prompt(dev, 2048, h) for h in (1, 2, 8)])
+    assert one < 0.7 * eight and two < 0.7 * eight, (one, two, eight)
+
+
+@pytest.mark.parametrize("T, H, Hkv, D, columns", [
+    (19, 6, 3, 64, 0), (70, 5, 5, 128, 0), (33, 11, 11, 96, 0), (150, 3, 3, 256, 0), (64, 9, 9, 128, 0), (40, 12, 12, 64, 300),
+    (55, 10, 10, 128, 700), (21, 7, 7, 256, 400), (9, 13, 13, 96, 64), (130, 1, 1, 128, 40)])
+def test_every_number_of_ranges(dev, T, H, Hkv, D, columns):
+    """Numbers of kv heads, ranges and row blocks that eight does not divide: each item is done once."""
+    g = torch.Generator().manual_seed(T)
+    lengths = torch.tensor([T, T + 170, 0], dtype=torch.int32)
+    page = 16
+    pages = sum(-(-int(x) // page) for x in lengths) + 1
+    cache = random_cache(g, pages, page, Hkv, D, torch.int8)
+    q = torch.randn(3, H, T, D, generator=g).to(torch.bfloat16)
+    _compare(dev, q, cache, _table(g, lengths, page, pages, columns=columns or None), lengths, tree=_tree(g, 3, T) if T % 2 else None)
