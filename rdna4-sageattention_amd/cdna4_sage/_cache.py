@@ -283,11 +283,13 @@ def cache_attention(q, cache, block_table, lengths, tensor_layout="HND", sm_scal
     block_table[b, j // page_size], and a page outside the cache (-1) hides its keys.  A query sees every key before the new
     ones and, of those, its own and the earlier ones (is_causal), all (is_causal=False), or those its row of tree_mask
     shows: bool [T, T] or [B, T, T], True at (i, j) where new token i sees new token j (a tree of drafted tokens: its
-    ancestors and itself).  A query that sees no key gives 0 (lengths[b] = 0, say).  Returns the output in q's layout and
-    dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf where no key is seen.  A query
-    that holds an infinity or a NaN gives NaN, in both, where it sees a key.  sm_scale: a
-    positive normal number of float32; None or a non-positive one stands for 1 / sqrt(D).  There is no derivative: a backward pass and inputs with forward-mode tangents
-    raise.  Raises Unsupported for what the kernel does not take."""
+    ancestors and itself).  A query that sees no key gives 0 (lengths[b] = 0, say), one that sees some and holds an infinity
+    or a NaN gives NaN.  Returns the output in q's layout and dtype; return_lse adds the fp32 natural logsumexp [B, H, T], -inf
+    where no key is seen.  sm_scale: a positive normal number of float32; None or a non-positive one stands for 1 / sqrt(D).
+    Launch and workspace are planned for the table's width, the lengths being on the device: where they are known to stay
+    below a bound, block_table[:, :pages] says so and copies nothing (too wide a table costs short prompts up to 1.4 times
+    their time).  There is no derivative: a backward pass and inputs with forward-mode tangents raise.  Raises Unsupported
+    for what the kernel does not take."""
     sm = float(sm_scale) if sm_scale is not None and sm_scale > 0 else 0.0
     if sm and not _F32_NORMAL <= sm <= _F32_MAX:
         raise Unsupported(f"sm_scale {sm} (float32's normal numbers)")

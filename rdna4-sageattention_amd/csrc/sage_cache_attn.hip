@@ -39,6 +39,8 @@ constexpr int CA_THREADS = 64 * CA_WAVES;
 constexpr int CA_TILE = 32;                      // keys per wave and step
 constexpr int CA_STEP = CA_TILE * CA_WAVES;      // keys per workgroup and step
 
+constexpr int MOST_CHOICES = 8;
+
 struct CacheAttnArgs {
   const uint16_t* q;
   int64_t qsb, qss, qsh;
@@ -54,7 +56,9 @@ struct CacheAttnArgs {
   int msq, msk;
   int B, H, Hkv, G, T, dtype, causal;
   int pages, page_size, page_shift, max_pages;
-  int row_blocks, workers;
+  int row_blocks, workers;          // workers: the most ranges of keys
+  int choose;                       // the lengths decide how many of 1 .. workers <= MOST_CHOICES there are:
+  float step_time[MOST_CHOICES], fixed_time[MOST_CHOICES];  // n take steps * step_time[n - 1] + fixed_time[n - 1]
   int part_rows;                    // rows of a partial: 16 RT, or all of them where that is fewer
   float scale;                      // softmax scale * log2 e = scale 2^scale_exp, scale in [1/2, 1)
   int scale_exp;
@@ -63,7 +67,7 @@ struct CacheAttnArgs {
 };
 
 // Work of one kv head and row block: the steps (CA_STEP keys) of all sequences in a row, at least one each, cut into
-// `workers` ranges that differ by one step at most, the longer ones first, whatever the sequences' lengths.  A worker's
+// ranges that differ by one step at most, the longer ones first, whatever the sequences' lengths.  A worker's
 // range holds whole sequences, whose output it writes, and up to two parts: of the one it begins inside of (partial 0) and of the one that it begins
 // but does not end (partial 1); a second kernel joins those.  The lengths stay on the device: every wave adds them up.
 __device__ __forceinline__ int cache_keys(const CacheAttnArgs& a, int b) {
@@ -94,7 +98,17 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 struct Shares {
   int workers, per, longer;  // ranges; steps of each; ranges with one more
-  __device__ __forceinline__ Shares(int most, int total) {
+  __device__ __forceinline__ Shares(const CacheAttnArgs& a, int total) {
+    int most = a.workers;
+    if (a.choose) {
+      float best = __builtin_inff();
+#pragma unroll
+      for (int i = 0; i < MOST_CHOICES; ++i) {
+        const float t = __builtin_fmaf((float)total, a.step_time[i], a.fixed_time[i]);
+        if (i < a.workers && t < best) best = t, most = i + 1;
+      }
+      most = __builtin_amdgcn_readfirstlane(most);
+    }
     workers = min(most, total);
     per = total / workers;
     longer = total - per * workers;
@@ -395,7 +409,7 @@ struct Work {
     const bool few = a.B <= 64;  // the lengths are read once
     lane_keys = few && lane < a.B ? cache_keys(a, lane) : 0;
     int n = lane < a.B ? cache_steps(lane_keys) : 0, scan = few ? wave_scan(n) : 0, unused;
-    const Shares shares(a.workers, few ? __builtin_amdgcn_readlane(scan, 63) : all_steps(a, lane, -1, unused));
+    const Shares shares(a, few ? __builtin_amdgcn_readlane(scan, 63) : all_steps(a, lane, -1, unused));
     // The row blocks of one range of keys on one XCD, next to each other: the ranges dealt to the XCDs one by one where that gives
     // each as many, the row blocks of all ranges in a row cut into eighths elsewhere (32-row blocks of 12 heads x 256, 36 ranges:
     // 547 us dealt, 387 cut; a prompt of 2048 of one head: 89 and 37).
@@ -798,7 +812,7 @@ __global__ __launch_bounds__(PER > 1 ? 256 : 64 * MERGE_SLICES) void cache_merge
   const int pair = at / groups, group = at - pair * groups, b = pair / a.Hkv, h = pair - b * a.Hkv;
   int before;
   const int total = all_steps(a, lane, b, before), steps = cache_steps(uniform_keys(a, b));
-  const Shares shares(a.workers, total);
+  const Shares shares(a, total);
   const int w0 = shares.worker_of(before), parts = shares.worker_of(before + steps - 1) - w0 + 1;
   if (parts == 1) return;  // written whole
   const bool mine = lane * VEC < D;
@@ -909,9 +923,10 @@ __global__ __launch_bounds__(PER > 1 ? 256 : 64 * MERGE_SLICES) void cache_merge
   }
 }
 
-// Rows per workgroup (16 rt) and workers per kv head and row block for a call.
+// Rows per workgroup (16 rt) and the most workers per kv head and row block for a call.
 struct CachePlan {
-  int rt, row_blocks, workers, part_rows;
+  int rt, row_blocks, workers, part_rows, choose;
+  float step_time[MOST_CHOICES], fixed_time[MOST_CHOICES];
   int64_t o_bytes, bytes;
 };
 
@@ -919,38 +934,54 @@ static CachePlan cache_plan(int B, int H, int Hkv, int T, int D, int max_keys, i
   CachePlan p;
   const int64_t rows = (int64_t)T * (H / Hkv);
   const int64_t most = (int64_t)B * ((max_keys + CA_STEP - 1) / CA_STEP);  // (the lengths are on the device: the table's width)
-  // Time of a call in blocks of 16 rt rows, in steps of a workgroup of 32 rows, with the number w of workers for it: rounds of
-  // workgroups that run at once, times a walk and what a workgroup costs beside it, which is 4 steps more where parts are
-  // written and joined and 7 more in blocks of 48 rows (13 us).  A step of those takes 1.2 times one of 32 rows: turning codes to
-  // float16 costs as much as the softmax and products of some 28 rows.
-  auto time = [&](int rt, int64_t& w) {
-    const int64_t units = Hkv * ((rows + 16 * rt - 1) / (16 * rt));
-    const int64_t slots = (int64_t)cus * (D == 256 ? 1 : D == 64 && rt == 2 ? 3 : 2);
-    const bool many = slots / units >= 8;  // one round whatever w is
-    double best = 0.0;
-    w = 0;
-    for (int64_t n = many ? slots / units : 1; n <= (many ? slots / units : 8); ++n) {
-      const int64_t rounds = (units * n + slots - 1) / slots;
-      const double t = rounds * ((double)most / n * (rt == 3 ? 1.2 : 1.0) + (n == 1 ? 3.0 : 7.0) + (rt == 3 ? 7.0 : 0.0));
-      if (w == 0 || t < best) best = t, w = n;
+  auto units_of = [&](int rt) { return Hkv * ((rows + 16 * rt - 1) / (16 * rt)); };
+  auto slots_of = [&](int rt) { return (int64_t)cus * (D == 256 ? 1 : D == 64 && rt == 2 ? 3 : 2); };
+  // Time of a call in blocks of 16 rt rows, in steps of a workgroup of 32 rows, with n ranges: rounds of workgroups that run at
+  // once, times a walk and what a workgroup costs beside it, which is 4 steps more where parts are written and joined
+  // and 7 more in blocks of 48 rows (13 us).  A step of those takes 1.2 times one of 32 rows: turning codes to float16 costs as
+  // much as the softmax and products of some 28 rows.
+  auto time = [&](int rt, int64_t n, float& per_step, float& fixed) {
+    const int64_t rounds = (units_of(rt) * n + slots_of(rt) - 1) / slots_of(rt);
+    per_step = (float)rounds * (rt == 3 ? 1.2f : 1.0f) / (float)n;
+    fixed = (float)rounds * ((n == 1 ? 3.0f : 7.0f) + (rt == 3 ? 7.0f : 0.0f));
+    return __builtin_fmaf((float)most, per_step, fixed);
+  };
+  // the number w of ranges for it, of as many as are worth a look
+  auto best = [&](int rt, int64_t& w) {
+    const int64_t fill = slots_of(rt) / units_of(rt);
+    float per_step, fixed;
+    if (fill >= MOST_CHOICES) return w = fill, time(rt, fill, per_step, fixed);  // one round whatever w is
+    float least = time(rt, w = 1, per_step, fixed);
+    for (int64_t n = 2; n <= MOST_CHOICES; ++n) {
+      const float t = time(rt, n, per_step, fixed);
+      if (t < least) least = t, w = n;
     }
-    return best;
+    return least;
   };
   int64_t w = 0, w3 = 0;
   p.rt = rows <= 16 ? 1 : 2;
-  const double t = time(p.rt, w);
+  const float t = best(p.rt, w);
   // Blocks of 48 rows at head dims 96 and 128 (at 64 the turning is half as much, at 256 they do not fit the registers).  In us with
   // 32 and 48, 8 kv heads x 128: 132 rows over 16 sequences of up to 9001 keys 128 and 110, 96 rows over 16 of up to 16000 152
-  // and 139, a prompt of 8192 962 and 834; 96 over 8 of up to 8000 54 and 58, 48 over 4 of up to 6000 33 and 40, a prompt of 2048
-  // 103 and 250.
-  if (rows > 16 && (D == 96 || D == 128) && time(3, w3) < t) p.rt = 3, w = w3;
+  // and 139, a prompt of 8192 962 and 834; 96 over 8 of up to 8000 54 and 58, 48 over 4 of up to 6000 33 and 40, four prompts of 512
+  // 75 and 96.
+  if (rows > 16 && (D == 96 || D == 128) && best(3, w3) < t) p.rt = 3, w = w3;
   p.row_blocks = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   p.part_rows = (int)(rows < 16 * p.rt ? rows : 16 * p.rt);
-  const int64_t units = (int64_t)Hkv * p.row_blocks;
+  const int64_t units = units_of(p.rt);
+  p.choose = slots_of(p.rt) / units < MOST_CHOICES;
   // one sequence of up to 512 keys: no parts to join (8 kv heads, 256 keys: 8.9 us, 10.9 with several workers and the joining
   // launch; 512: 10.4 and 11.0; 1000: 15 and 11.1)
   if (B == 1 && most <= 4) w = 1;
-  p.workers = (int)(w > most ? most : w);
+  // parts of 256 MiB at most: where they would take more there are rounds enough without
+  const int64_t part_bytes = units * 2 * p.part_rows * (D + 1) * 4, fit = (256 << 20) / part_bytes;
+  w = w > most ? most : w;
+  p.workers = (int)(w > fit ? fit > 1 ? fit : 1 : w);
+  // A table may be far wider than its sequences are long, so where w came from the estimate the device takes the best of up to w
+  // ranges once more, by the lengths (a prompt of 2048, 32 / 8 heads x 128, with a table of 131072 keys: 250 us in 4 ranges, 100
+  // in one).
+  p.choose = p.choose && p.workers > 1;
+  for (int i = 0; i < MOST_CHOICES; ++i) time(p.rt, i + 1, p.step_time[i], p.fixed_time[i]);
   const int64_t n = p.workers == 1 ? 0 : units * p.workers * 2 * p.part_rows;
   p.o_bytes = (n * D * 4 + 255) / 256 * 256;
   p.bytes = p.o_bytes + n * 4;
@@ -1051,7 +1082,8 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
   a.B = B, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.T = T, a.dtype = dtype, a.causal = causal;
   a.pages = pages, a.page_size = page_size, a.max_pages = max_pages;
   a.page_shift = __builtin_ctz((unsigned)page_size);
-  a.row_blocks = p.row_blocks, a.workers = p.workers, a.part_rows = p.part_rows;
+  a.row_blocks = p.row_blocks, a.workers = p.workers, a.part_rows = p.part_rows, a.choose = p.choose;
+  for (int i = 0; i < MOST_CHOICES; ++i) a.step_time[i] = p.step_time[i], a.fixed_time[i] = p.fixed_time[i];
   const double scale = sm_scale > 0.0f ? (double)sm_scale : 1.0 / __builtin_sqrt((double)D);
   a.scale = (float)std::frexp(scale * 1.44269504088896340736, &a.scale_exp);
   a.part_o = (float*)workspace;

@@ -60,3 +60,38 @@ def test_every_number_of_ranges(dev, T, H, Hkv, D, columns):
     cache = random_cache(g, pages, page, Hkv, D, torch.int8)
     q = torch.randn(3, H, T, D, generator=g).to(torch.bfloat16)
     _compare(dev, q, cache, _table(g, lengths, page, pages, columns=columns or None), lengths, tree=_tree(g, 3, T) if T % 2 else None)
+
+
+def test_a_wide_table_costs_little(dev):
+    """Prompts with a table as wide as a captured step keeps it, against one of their own width."""
+    for T in (1024, 2048):
+        narrow, wide = _times([_prompt(dev, T, 8), _prompt(dev, T, 8, 8192)])
+        assert wide < 1.7 * narrow, (T, narrow, wide)
+
+
+def test_workspaces_stay_small(dev):
+    from cdna4_sage import _capi
+
+    for B, H, Hkv, T, D in ((1, 32, 8, 2048, 128), (1, 64, 8, 8192, 128), (16, 32, 8, 8192, 128), (1, 24, 24, 4096, 96),
+                            (2, 16, 4, 8192, 64), (1, 12, 12, 4096, 256), (1, 32, 8, 512, 128), (64, 32, 8, 1, 128)):
+        for columns in (64, 512, 8192, 65536):
+            assert _capi.cache_attn_workspace(B, H, Hkv, T, D, 16, columns) <= 2**28, (B, H, T, columns)
+
+
+@pytest.mark.parametrize("B, T, H, Hkv, D, longest, columns", [
+    (2, 300, 8, 8, 128, 2600, (0, 2000)),      # few sequences' walks: several ranges, or one, by the lengths
+    (1, 350, 6, 6, 96, 350, (0, 4096)),
+    (1, 700, 6, 3, 64, 1900, (0, 2048)),
+    (3, 200, 6, 6, 256, 900, (0, 1024)),
+    (66, 65, 12, 12, 256, 130, (600,)),        # more sequences than lanes
+])
+def test_ranges_follow_the_lengths(dev, B, T, H, Hkv, D, longest, columns):
+    g = torch.Generator().manual_seed(T + D)
+    lengths = torch.randint(T // 2, longest + 1, (B,), generator=g).to(torch.int32)
+    lengths[0] = longest
+    page = 16
+    pages = sum(-(-int(x) // page) for x in lengths) + 1
+    cache = random_cache(g, pages, page, Hkv, D, torch.int8)
+    q = torch.randn(B, H, T, D, generator=g).to(torch.bfloat16)
+    for n in columns:
+        _compare(dev, q, cache, _table(torch.Generator().manual_seed(1), lengths, page, pages, columns=n or None), lengths)
