@@ -84,6 +84,15 @@ def check_cache(cache, gpu=None):
     return pages, heads, page_size, D
 
 
+def _addresses(cache):
+    """Addresses of the codes and scales, k's first, as the C entries take them."""
+    k, v, ks, vs = cache
+    at = k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr()
+    if (at[0] | at[1] | at[2] | at[3]) % 16:
+        raise Unsupported("cache tensors must start on 16-byte boundaries")
+    return at
+
+
 def cache_slots(block_table, lengths, count, page_size):
     """Slots of the last `count` of lengths[b] tokens of every sequence, int64 [B, count], for cache_write and cache_read;
     -1 where there is no such token or its page is missing (an entry below 0 or a column past the table)."""
@@ -144,8 +153,8 @@ def write_launch(cache, k, v, slots, layout):
     k, sk = _rows_args(k, layout)
     v, sv = _rows_args(v, layout)
     _capi.call_on(gpu, "sage_cache_write", k.data_ptr(), *sk, v.data_ptr(), *sv, B, S, DTYPES[k.dtype],
-                  slots.data_ptr(), slots.dtype == torch.int64, cache.k.data_ptr(), cache.k_scale.data_ptr(),
-                  cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D, CACHE_DTYPES[cache.k.dtype])
+                  slots.data_ptr(), slots.dtype == torch.int64, *_addresses(cache), pages, page_size, Hkv, D,
+                  CACHE_DTYPES[cache.k.dtype])
 
 
 def read_launch(cache, slots, dtype, layout):
@@ -168,8 +177,7 @@ def read_launch(cache, slots, dtype, layout):
         # (both outputs are contiguous: the batch needs no stride of its own)
         st = (0, Hkv * D, D)
         _capi.call_on(gpu, "sage_cache_read", k.data_ptr(), *st, v.data_ptr(), *st, 1, slots.numel(), DTYPES[dtype],
-                      slots.data_ptr(), slots.dtype == torch.int64, cache.k.data_ptr(), cache.k_scale.data_ptr(),
-                      cache.v.data_ptr(), cache.v_scale.data_ptr(), pages, page_size, Hkv, D,
+                      slots.data_ptr(), slots.dtype == torch.int64, *_addresses(cache), pages, page_size, Hkv, D,
                       CACHE_DTYPES[cache.k.dtype])
     if len(shape) == 2 and layout == "HND":
         return k.transpose(1, 2), v.transpose(1, 2)
@@ -242,6 +250,10 @@ def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal
         ms = tree_mask.stride()
         if len(ms) == 2 or tree_mask.shape[0] == 1:
             ms = (0, *ms[-2:])
+        if T == 1:   # (strides that are never taken)
+            ms = (ms[0], 0, 0)
+        elif max(ms[1], ms[2]) * (T - 1) >= 2**30:
+            raise Unsupported("a tree mask whose rows or columns reach over 2^30 bytes")
         mask = tree_mask.data_ptr()
     # (one allocation call each: the host's time is most of a small call's)
     out = q.new_empty_strided(shape, (T * H * D, D, H * D, 1) if layout == "HND" else (T * H * D, H * D, D, 1))
@@ -260,8 +272,7 @@ def attention_launch(q, cache, block_table, lengths, layout, sm_scale, is_causal
     lengths = lengths.contiguous()
     ws = q.new_empty(ws_bytes // 2) if ws_bytes else None   # (q's elements are of 2 bytes, the workspace's of 4)
     _capi.call_on(gpu, "sage_cache_attn", q.data_ptr(), *sq, out.data_ptr(), T * H * D, H * D, D,
-                  None if lse is None else lse.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
-                  cache.v.data_ptr(), cache.v_scale.data_ptr(), block_table.data_ptr(), ts[0], lengths.data_ptr(),
+                  None if lse is None else lse.data_ptr(), *_addresses(cache), block_table.data_ptr(), ts[0], lengths.data_ptr(),
                   mask, *ms, B, H, Hkv, T, D, DTYPES[q.dtype], CACHE_DTYPES[cache.k.dtype], pages, page_size, max_pages,
                   bool(is_causal), sm_scale, None if ws is None else ws.data_ptr(), ws_bytes)
     return out, lse
