@@ -145,27 +145,32 @@ def out_like(t):
     return out
 
 
-def _transformed():
-    """Inside a forward-mode level or one of torch.func's transforms."""
-    return forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+_transform = torch._C._functorch.peek_interpreter_stack   # the innermost of torch.func's transforms, or None
+
+
+def _derived(*args):
+    """rope_launch under autograd, in forward-mode levels and torch.func's transforms."""
+    return (_Rope if _transform() is None else _RopeTransformed).apply(*args)
 
 
 class _Rope(torch.autograd.Function):
     """rope_launch with its derivatives.  The rotation is linear: tangents turn as the inputs do, gradients turn back, and
-    each is an application of its own, so that derivatives have derivatives and torch.func's transforms compose."""
+    each is an application of its own, so that derivatives have derivatives."""
 
     @staticmethod
-    def forward(q, k, positions, freqs, layout, interleaved, factor, inverse):
-        return rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        _, _, positions, freqs, *how = inputs
+    def forward(ctx, *args):
+        out = rope_launch(*args)
+        _, k, positions, freqs, *ctx.how = args
         ctx.save_for_backward(positions, freqs)
-        ctx.save_for_forward(positions, freqs)
-        ctx.how = how
-        if not _transformed():   # the output of an input that needs no gradient needs none either
-            ctx.mark_non_differentiable(*(y for y, need in zip(output, ctx.needs_input_grad) if y is not None and not need))
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, freqs)
+        elif k is not None:
+            # the output of an input that needs no gradient needs none either (one of the two does)
+            if not ctx.needs_input_grad[0]:
+                ctx.mark_non_differentiable(out[0])
+            elif not ctx.needs_input_grad[1]:
+                ctx.mark_non_differentiable(out[1])
+        return out
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -173,7 +178,7 @@ class _Rope(torch.autograd.Function):
         need_q, need_k = ctx.needs_input_grad[:2]
         back = (*ctx.saved_tensors, *how, not inverse)
         # (create_graph: the gradients have gradients of their own)
-        turn = _Rope.apply if _transformed() or torch.is_grad_enabled() else rope_launch
+        turn = _derived if torch.is_grad_enabled() or forward_ad._current_level >= 0 or _transform() is not None else rope_launch
         if need_q and need_k:
             dq, dk = turn(dq, dk, *back)
         elif need_q:
@@ -185,13 +190,28 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     def jvp(ctx, tq, tk, *_):
         # (an input without a tangent comes with one of zeros)
-        return _Rope.apply(tq, tk, *ctx.saved_tensors, *ctx.how)
+        return _derived(tq, tk, *ctx.saved_tensors, *ctx.how)
+
+
+class _RopeTransformed(_Rope):
+    """_Rope in the form that torch.func's transforms take, which takes longer a call."""
+
+    @staticmethod
+    def forward(q, k, positions, freqs, layout, interleaved, factor, inverse):
+        return rope_launch(q, k, positions, freqs, layout, interleaved, factor, inverse)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, positions, freqs, *ctx.how = inputs
+        ctx.save_for_backward(positions, freqs)
+        ctx.save_for_forward(positions, freqs)
 
     @staticmethod
     def vmap(info, in_dims, q, k, positions, freqs, *how):
         n = info.batch_size
-        if in_dims[3] is not None:   # frequencies of each entry's own: one launch each
-            outs = [_Rope.apply(*(t if d is None else t.select(d, i) for t, d in zip((q, k, positions, freqs), in_dims)), *how)
+        most = max(t.numel() // (1 if d is None else n) for t, d in zip((q, k), in_dims) if t is not None)
+        if in_dims[3] is not None or n * most > _I32_MAX:   # frequencies of each entry's own, or too large: one launch each
+            outs = [_derived(*(t if d is None else t.select(d, i) for t, d in zip((q, k, positions, freqs), in_dims)), *how)
                     for i in range(n)]
             return (torch.stack([o[0] for o in outs]), None if k is None else torch.stack([o[1] for o in outs])), \
                 (0, None if k is None else 0)
@@ -209,7 +229,7 @@ class _Rope(torch.autograd.Function):
             if positions.dim() != 3 or positions.shape[1] not in (1, B):
                 raise Unsupported(f"positions of shape {tuple(positions.shape[1:])} for batch {B}")
             positions = positions.expand(n, B, positions.shape[2]).flatten(0, 1)
-        oq, ok = _Rope.apply(q.flatten(0, 1), None if k is None else k.flatten(0, 1), positions, freqs, *how)
+        oq, ok = _derived(q.flatten(0, 1), None if k is None else k.flatten(0, 1), positions, freqs, *how)
         return (oq.unflatten(0, (n, B)), None if k is None else ok.unflatten(0, (n, B))), (0, None if k is None else 0)
 
 
@@ -228,7 +248,9 @@ def rope(q, k=None, positions=None, freqs=None, tensor_layout="HND", interleaved
     ts = (q,) if k is None else (q, k)
     args = (positions, freqs, tensor_layout, interleaved, factor, False)
     if _plain_tensors(*ts):
-        if ((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled()) or _transformed():
+        if _transform() is not None:
+            out = _RopeTransformed.apply(q, k, *args)
+        elif ((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
             out = _Rope.apply(q, k, *args)
         else:
             out = rope_launch(q, k, *args)
