@@ -16,10 +16,14 @@
 //    V's operand takes that order too: lane (m, g) reads D/16 channels of each of those 8 keys, pairs of keys are
 //    brought together by byte permutes.  Nothing crosses lanes but the row maxima.
 //  * Q rows in bfloat16 are brought into float16's range by a power of two per row, which keeps all their bits.
-//  * P in float16 holds 11 bits of p_ij s^v_j, p_ij = 2^(x_ij - m): the running reference m of a row is set by its first product
-//    above 0, which it brings to 2^6, and raised when a tile's products pass 2^15 (32 bits hold the sum l at any m).
-//    The largest product so far lies between 2^6 and 2^15, so a product keeps all 11 bits down to 2^-20 of the largest and an
-//    error of 2^-31 of it below.
+//  * P in float16: 11 bits of p_ij s^v_j, p_ij = 2^(x_ij - m); in blocks of 16 rows a second number takes what the first leaves, 22
+//    bits in all, and its product hides behind HBM (one token over 48 x 4100 keys 30.0 us with one number, 30.6 with two; 16 rows
+//    over 8 x 3000, 24 kv heads, 38 and 39).  Blocks of 32 and 48 rows take one: 132 rows over 16 x 4750 keys 107 us with one, 124
+//    with two, a prompt of 4096 289 and 329, and a float16 output is off by 2.9e-4 of its size then where rounding alone gives
+//    2.1e-4, a bfloat16 one by no more than its rounding.
+//  * The running reference m of a row is set by its first product above 0, which it brings to 2^6, and raised when one of its own
+//    products passes 2^15 (32 bits hold the sum l at any m).  The largest product so far lies between 2^6 and 2^15, so a product
+//    keeps all 11 bits down to 2^-20 of the largest and an error of 2^-31 of it below.
 // Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000
 // keys, 8 kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes
 // and the softmax's vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
@@ -236,6 +240,7 @@ struct CacheRow {
 // The rows of a wave against the keys it walks: softmax references and sums, output accumulators, Q's operand.
 template <int D, int RT> struct Rows {
   static constexpr int NK = D / 32, NC = D / 16;
+  static constexpr int PARTS = RT == 1 ? 2 : 1;  // float16 numbers per weight
   f16x8 qf[RT][NK];
   // Factor of the scores to log2 units, from one power of two, so that no step of it leaves float32's range.  Positive: a hidden
   // score stays -inf.  Below 2^-126 it has fewer bits, within 2^-150 of the exact factor: a score, which is below 2^124 before it,
@@ -339,7 +344,7 @@ template <int D, int RT> struct Rows {
   // Scores (with K's scales) to the weights' operand: sums and references brought up to date.  The terms are taken against the
   // references so far; where a product could pass 2^15, or a row has no reference from a product yet, the references are
   // looked at first.
-  __device__ __forceinline__ void weights(const v4f (&s)[RT][2], const v4f (&vs)[2], f16x8 (&pf)[RT]) {
+  __device__ __forceinline__ void weights(const v4f (&s)[RT][2], const v4f (&vs)[2], f16x8 (&pf)[RT][PARTS]) {
     float vs_top = 0x1p-85f;  // (a weight stays within 2^100 whatever its scale is)
 #pragma unroll
     for (int j = 0; j < 8; ++j) vs_top = fmaxf(vs_top, vs[j / 4][j % 4]);
@@ -396,7 +401,11 @@ template <int D, int RT> struct Rows {
         pv[j] = mul_zero(p[j], vs[j / 4][j % 4]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pf[rt][j] = (_Float16)pv[j];
+      for (int j = 0; j < 8; ++j) pf[rt][0][j] = (_Float16)pv[j];
+      if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[rt][1][j] = (_Float16)(pv[j] - (float)pf[rt][0][j]);
+      }
     }
   }
 };
@@ -662,7 +671,7 @@ __global__ __launch_bounds__(CA_THREADS, D == 64 && RT == 2 ? 3 : D == 256 && RT
         }
         r.hide(a, b, k0 + 4 * g - seg.base, gone, s);
       }
-      f16x8 pf[RT];
+      f16x8 pf[RT][r.PARTS];
       r.weights(s, vs, pf);
       // V operand: keys (0, 1), (2, 3) of each block side by side
       uint32_t vw[8][Tile::VW];
@@ -701,7 +710,11 @@ __global__ __launch_bounds__(CA_THREADS, D == 64 && RT == 2 ? 3 : D == 256 && RT
             const int c = 4 * i + 2 * u + o;
             const f16x8 va = join4(codes_f16<CT>(w[0], o), codes_f16<CT>(w[1], o), codes_f16<CT>(w[2], o), codes_f16<CT>(w[3], o));
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) r.acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt], r.acc[rt][c], 0, 0, 0);
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+              for (int part = 0; part < r.PARTS; ++part)
+                r.acc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[rt][part], r.acc[rt][c], 0, 0, 0);
+            }
           }
         }
       }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cdna4_sage
-from cache_util import random_cache
+from cache_util import attention, random_cache, score_slack
 from cdna4_sage import _capi
 from test_gpu_cache import _compare, _table, _to, _tree
 
@@ -173,3 +173,22 @@ def test_many_rows_in_several_parts(dev, D, T, H, Hkv, B, long, columns, rt, cod
     q = torch.randn(B, H, T, D, generator=g).to(dtype)
     table = _table(g, lengths, page, pages, columns=columns)
     _compare(dev, q, cache, table, lengths, "NHD" if kind == "tree" else "HND", tree=_tree(g, B, T) if kind == "tree" else None)
+
+
+@pytest.mark.parametrize("T, H, Hkv, D, n, code", [(1, 8, 1, 64, 100, torch.int8), (1, 16, 2, 128, 300, E4M3), (4, 12, 3, 96, 120, torch.int8),
+                                                   (1, 16, 1, 256, 90, torch.int8), (16, 2, 2, 64, 1500, E4M3)])
+def test_weights_of_few_rows_keep_their_bits(dev, T, H, Hkv, D, n, code):
+    """Up to 16 rows per kv head: two float16 numbers per weight, each rounded to the nearest (2^-11 and 2^-11 of the rest: 2^-22),
+    where one would leave 2^-11.  Scores are small, so products lie within 2^-9 of the largest, which is at 2^6 or more: the second
+    number's own steps, 2^-24, are below 2^-22 of the product too."""
+    g = torch.Generator().manual_seed(n)
+    page = 32
+    pages = -(-n // page)
+    cache = random_cache(g, pages, page, Hkv, D, code)
+    q = (torch.randn(1, H, T, D, generator=g) / 64).to(torch.float16)
+    table, lengths = torch.arange(pages, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+    want, _, mag, big = attention(q.double(), cache, table, lengths)
+    got = cdna4_sage.cache_attention(q.to(dev), _to(dev, cache), table.to(dev), lengths.to(dev)).double().cpu()
+    # (the float32 sums and exponentials: 2^-20, as attention_slack has it)
+    room = mag * (2.0**-22 + 2.0**-20 + 2.0 * score_slack(big, D).unsqueeze(-1)) + want.abs() * 2.0**-11 + 2.0**-25
+    assert bool(((got - want).abs() <= room).all()), float(((got - want).abs() / room).max())
