@@ -25,8 +25,8 @@
 //    products passes 2^15 (32 bits hold the sum l at any m).  The largest product so far lies between 2^6 and 2^15, so a product
 //    keeps all 11 bits down to 2^-20 of the largest and an error of 2^-31 of it below.
 // Bound: HBM for up to 16 rows, where a key costs 2 D + 8 bytes per kv head whatever T and G are (one token over 6 x 115000
-// keys, 8 kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 30 us in all, 3.6 TB/s), the turning of codes
-// and the softmax's vector instructions beyond (132 rows over 16 x 4750 keys: 110 us, 0.37 PFLOP/s of products).
+// keys, 8 kv heads x 128: 254 us, 5.8 TB/s; over 48 x 4100, 4 kv heads x 64: 31 us in all, 3.5 TB/s), the turning of codes
+// and the softmax's vector instructions beyond (132 rows over 16 x 4750 keys: 107 us, 0.38 PFLOP/s of products).
 // Range: float32 holds K's scores and V's products on the way, for values of magnitude up to 2^100.
 #include <cmath>
 
@@ -228,7 +228,7 @@ template <int D> struct CacheTile {
     return D == 256 ? (from ^ 64 * (j % 4)) + 1024 * (j % 4) : from + (D == 128 ? 1024 * (j % 2) : 0);
   }
 };
-// tiles of a wave in LDS: as many as let the workgroups that the registers allow share a CU's 160 KiB
+// tiles of a wave in LDS (blocks of 16 rows): two workgroups then share a CU's 160 KiB, three at head dim 96, one at 256
 template <int D> constexpr int ring_tiles() { return D == 64 ? 4 : 2; }
 
 // rows in front of the first of 16 keys from k0 on; a page outside the cache hides its keys: page 0 is read in its place
