@@ -17,8 +17,8 @@
 //    brought together by byte permutes.  Nothing crosses lanes but the row maxima.
 //  * Q rows in bfloat16 are brought into float16's range by a power of two per row, which keeps all their bits.
 //  * P in float16: 11 bits of p_ij s^v_j, p_ij = 2^(x_ij - m); in blocks of 16 rows a second number takes what the first leaves, 22
-//    bits in all, and its product hides behind HBM (one token over 48 x 4100 keys 30.0 us with one number, 30.6 with two; 16 rows
-//    over 8 x 3000, 24 kv heads, 38 and 39).  Blocks of 32 and 48 rows take one: 132 rows over 16 x 4750 keys 107 us with one, 124
+//    bits in all, and its product all but hides behind HBM (one token over 48 x 4100 keys 30.4 us with one number, 31.2 with two,
+//    over 64 x 600 29.0 and 30.4, over 1000 11.6 and 11.7; 16 rows over 8 x 3000, 24 kv heads, 38 and 39).  Blocks of 32 and 48 rows take one: 132 rows over 16 x 4750 keys 107 us with one, 124
 //    with two, a prompt of 4096 289 and 329, and a float16 output is off by 2.9e-4 of its size then where rounding alone gives
 //    2.1e-4, a bfloat16 one by no more than its rounding.
 //  * The running reference m of a row is set by its first product above 0, which it brings to 2^6, and raised when one of its own

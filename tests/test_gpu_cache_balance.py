@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import cdna4_sage
-from cache_util import random_cache
+from cache_util import attention, attention_slack, random_cache
 from test_gpu_cache import _compare, _table, _tree
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +95,41 @@ def test_ranges_follow_the_lengths(dev, B, T, H, Hkv, D, longest, columns):
     q = torch.randn(B, H, T, D, generator=g).to(torch.bfloat16)
     for n in columns:
         _compare(dev, q, cache, _table(torch.Generator().manual_seed(1), lengths, page, pages, columns=n or None), lengths)
+
+
+def test_replays_whose_lengths_change_the_ranges(dev):
+    """A captured chunk with a wide table, replayed with lengths of one range and of several: every replay as the eager call and
+    as float64 attention."""
+    g = torch.Generator().manual_seed(3)
+    B, T, H, Hkv, D, page, columns = 2, 300, 8, 8, 128, 64, 300
+    pages = 120
+    cache = random_cache(g, pages, page, Hkv, D, torch.int8)
+    q = torch.randn(B, H, T, D, generator=g).to(torch.bfloat16)
+    need = torch.randperm(pages, generator=g).to(torch.int32).view(B, 60)
+    table = torch.cat([need, torch.full((B, columns - 60), -1, dtype=torch.int32)], 1)
+    on = [cdna4_sage.KVCache(*(t.to(dev) for t in cache)), q.to(dev), table.to(dev),
+          torch.tensor([T, T], dtype=torch.int32, device=dev)]
+    call = lambda: cdna4_sage.cache_attention(on[1], on[0], on[2], on[3], return_lse=True)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for lengths in ([T, T], [3800, 300], [0, 0], [3840, 3840], [1, 900], [T, T]):
+        on[3].copy_(torch.tensor(lengths, dtype=torch.int32))
+        want = call()
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), lengths
+    on[3].copy_(torch.tensor([3800, 300], dtype=torch.int32))
+    few = attention(q[:, :2].double(), [t[:, :2] for t in cache], table, torch.tensor([3800, 300]))
+    off = (call()[0][:, :2].double().cpu() - few[0]).abs()
+    assert bool((off <= attention_slack(few[2], few[3], few[0], D, q.dtype)).all())
