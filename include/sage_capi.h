@@ -54,6 +54,7 @@ extern "C" {
 #define SAGE_DTYPE_BF16 0
 #define SAGE_DTYPE_F16 1
 #define SAGE_DTYPE_BOOL 2 /* attention masks only */
+#define SAGE_DTYPE_F32 3  /* relative position biases and their tables only */
 
 #define SAGE_CACHE_INT8 0 /* codes of the key / value cache */
 #define SAGE_CACHE_E4M3 1
@@ -299,6 +300,63 @@ int sage_cache_attn(const void* q, int64_t qsb, int64_t qss, int64_t qsh, void* 
                     const void* tree_mask, int64_t msb, int64_t msq, int64_t msk, int B, int H, int Hkv, int T, int D,
                     int dtype, int cache_dtype, int pages, int page_size, int max_pages, int causal, float sm_scale,
                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A learned relative position bias by buckets (no counterpart in the reference): table entry (bucket, head) at table +
+ * bucket * tb + head * th, of dtype SAGE_DTYPE_BF16, F16 or F32.  The key d tokens ahead of its query: side = buckets / 2
+ * where two_sided, else buckets; n = |d|, or max(-d, 0) one-sided; near = side / 2; bucket n below near, then near +
+ * floor(ln(n / near) / ln(max_distance / near) * (side - near)), side - 1 at most; two-sided, keys ahead add side.
+ * borders: side - near whole numbers in host memory, the smallest n of the buckets near, near + 1, ..;
+ * sage_bias_borders computes them exactly.  buckets: 2 to 256, two-sided even and at least 4; max_distance above near.
+ *
+ * sage_relative_bias: out [H, q_len, kv_len], contiguous, of dtype bf16, fp16 or fp32; key j is at position j, query i at
+ * offset + i, with `offset` read from offset_at (int64, or int32 where offset64 is 0; device memory) where that is not NULL.
+ * sage_relative_bias_grad: dtable = the sums of dbias (element strides sh, sq and 1) over each bucket's pairs, in fp32, one order.
+ */
+int sage_bias_borders(int buckets, int two_sided, int max_distance, int* borders);
+int sage_relative_bias(const void* table, int table_dtype, int64_t tb, int64_t th, int H, int buckets, int two_sided,
+                       const int* borders, int q_len, int kv_len, int64_t offset, const void* offset_at, int offset64, void* out,
+                       int dtype, void* stream);
+int sage_relative_bias_grad_workspace(int H, int buckets, int q_len, int kv_len, int dtype, int64_t* workspace_bytes);
+int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype, int H, int buckets, int two_sided,
+                            const int* borders, int q_len, int kv_len, int64_t offset, const void* offset_at, int offset64,
+                            void* dtable, int table_dtype, int64_t tb, int64_t th, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/*
+ * Attention on 16-bit inputs with its backward pass (no counterpart in the reference, whose attention has no derivative):
+ * softmax(sm_scale q k^T + bias) v, sm_scale 0 for 1 / sqrt(D), scores, statistics and sums in fp32.  q, out, dout, dq
+ * [B, H, Sq, D], k, v, dk, dv [B, Hkv, Skv, D] by (b, s, h) strides, dtype bf16 or fp16; lse fp32 [B, H, Sq], natural log.
+ * causal: query i sees the keys j <= i + Skv - Sq.  mask: one byte per element, nonzero = visible, (b, h, i, j) at mask +
+ * b * msb + h * msh + i * msq + j * msk, or NULL.  buckets: 0, or of a relative position bias (above; query i at position
+ * i + Skv - Sq) whose last bucket begins at a distance of at most 768.  A query that sees no key is written as 0 (lse -inf) and
+ * has no gradient; what hidden keys and such queries hold does not matter; a query that sees an infinity or a NaN is NaN.
+ *
+ * Packed batches (cu_q, cu_k not NULL; int32 [B + 1], device memory): B sequences one behind the other, Sq and Skv the totals of
+ * rows, lse [H, Sq], batch strides unused, no mask; each sequence with its own diagonal and positions.  Rows that no sequence
+ * covers, and all rows where offsets fall or pass the totals, are written as 0 (their lse stays as it is).
+ *
+ * sage_train_workspace: the bytes of the state, which the forward pass writes and the backward pass reads, and of the backward
+ * pass' workspace; both 256-byte aligned.  sage_train_bwd: dq NULL (then dtable too) or dk and dv NULL leave those out; dtable
+ * NULL leaves the table's gradient out.  Equal inputs give equal bits.
+ */
+int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, int Skv, int D, int has_mask, int64_t msb, int64_t msh,
+                         int64_t msq, int buckets, int two_sided, const int* borders, int64_t* state_bytes,
+                         int64_t* workspace_bytes);
+int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* k, int64_t ksb, int64_t kss, int64_t ksh,
+                   const void* v, int64_t vsb, int64_t vss, int64_t vsh, void* out, int64_t osb, int64_t oss, int64_t osh,
+                   float* lse, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype, int causal, float sm_scale,
+                   const int* cu_q, const int* cu_k, const void* mask, int64_t msb, int64_t msh, int64_t msq, int64_t msk,
+                   const void* table, int table_dtype, int64_t tb, int64_t th, int buckets, int two_sided, const int* borders,
+                   void* state, int64_t state_bytes, void* stream);
+int sage_train_bwd(const void* dout, int64_t gsb, int64_t gss, int64_t gsh, const void* q, int64_t qsb, int64_t qss, int64_t qsh,
+                   const void* k, int64_t ksb, int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss, int64_t vsh,
+                   const void* out, int64_t osb, int64_t oss, int64_t osh, const float* lse, void* dq, int64_t dqb, int64_t dqs,
+                   int64_t dqh, void* dk, int64_t dkb, int64_t dks, int64_t dkh, void* dv, int64_t dvb, int64_t dvs, int64_t dvh,
+                   int B, int H, int Hkv, int Sq, int Skv, int D, int dtype, int causal, float sm_scale, const int* cu_q,
+                   const int* cu_k, int has_mask, int64_t msb, int64_t msh, int64_t msq, void* dtable, int table_dtype,
+                   int64_t tb, int64_t th, int buckets, int two_sided, const int* borders, const void* state,
+                   int64_t state_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent       # rdna4-sageattention_amd/
@@ -26,7 +28,8 @@ LIB = PKG / "libsage_capi.so"
 MANIFEST = PKG / "manifest.json"
 ARCH = "gfx950"
 SOURCES = ("sage_capi.hip", "sage_quant.hip", "sage_attn.hip", "sage_lse.hip", "sage_varlen.hip", "sage_mask.hip",
-           "sage_rope.hip", "sage_cache.hip", "sage_cache_attn.hip")
+           "sage_rope.hip", "sage_cache.hip", "sage_cache_attn.hip", "sage_bias.hip", "sage_train.hip", "sage_train_fwd.hip",
+           "sage_train_bwd.hip")
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -52,16 +55,26 @@ def hipcc() -> str:
 def build(verbose: bool = False) -> Path:
     """Compile every kernel variant for gfx950 into libsage_capi.so and refresh manifest.json."""
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), *[str(CSRC / s) for s in SOURCES]]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    # hipcc's host pass does not know the packed-fp32 feature and says so; that line is harmless
-    noise = [ln for ln in (res.stderr or "").splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
-    if res.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
-    if verbose and noise:
-        print("\n".join(noise), file=sys.stderr)
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        # hipcc's host pass does not know the packed-fp32 feature and says so; that line is harmless
+        noise = [ln for ln in (res.stderr or "").splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
+        if res.returncode != 0:
+            raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
+        if verbose and noise:
+            print("\n".join(noise), file=sys.stderr)
+
+    with tempfile.TemporaryDirectory() as objects:
+        # one compiler per source, a few at a time
+        outs = [str(Path(objects) / (s + ".o")) for s in SOURCES]
+        compile_flags = [f for f in HIP_FLAGS if f != "-shared"]
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda so: run([hipcc(), *compile_flags, f"-I{INCLUDE}", "-c", "-o", so[1], str(CSRC / so[0])]),
+                          zip(SOURCES, outs)))
+        run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", str(tmp), *outs])
     os.replace(tmp, LIB)
     # the manifest comes from the library itself, queried in a child process (no GPU or torch needed)
     probe = ("import ctypes,sys; l=ctypes.CDLL(sys.argv[1]); l.sage_manifest_json.restype=ctypes.c_char_p; "

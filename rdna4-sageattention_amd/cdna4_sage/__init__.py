@@ -15,6 +15,9 @@ attention_varlen runs packed variable-length batches in one pass.
 
 For decoding: rope (rotary positions), cache_write / cache_read (an 8-bit key / value cache in pages), cache_attention
 (new tokens, or a tree of drafted ones, over that cache) and cache_step, which is the three of them in a row.
+
+For training: attention_train (attention on 16-bit inputs with its backward pass), attention_train_varlen (packed sequences) and
+relative_bias (a learned bias by relative position, with its gradient).
 """
 import os
 
@@ -27,10 +30,11 @@ from ._attention import (ARCHS, HEAD_DIMS, Unsupported, _plain_eager, attention_
 from ._attention import attention as _attention_impl
 from ._cache import (KVCache, cache_attention, cache_read, cache_slots, cache_step, cache_write, new_cache)
 from ._rope import rope, rope_frequencies
+from ._train import attention_train, attention_train_varlen, relative_bias
 
 __all__ = ["sageattn", "attention", "attention_varlen", "lse", "is_available", "Unsupported", "ARCHS", "HEAD_DIMS",
            "rope", "rope_frequencies", "KVCache", "new_cache", "cache_slots", "cache_write", "cache_read",
-           "cache_attention", "cache_step"]
+           "cache_attention", "cache_step", "attention_train", "attention_train_varlen", "relative_bias"]
 __version__ = "0.1.0"
 
 # Fallbacks call torch's C entry point of SDPA directly: a caller may have monkey-patched

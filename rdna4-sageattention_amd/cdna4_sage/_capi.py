@@ -18,7 +18,7 @@ import torch  # noqa: F401  (load torch's HIP runtime first)
 LIB_PATH = Path(__file__).resolve().parent / "libsage_capi.so"
 
 SAGE_OK, SAGE_ERR_INVALID, SAGE_ERR_UNSUPPORTED, SAGE_ERR_HIP = 0, 1, 2, 3
-DTYPE_BF16, DTYPE_F16, DTYPE_BOOL = 0, 1, 2
+DTYPE_BF16, DTYPE_F16, DTYPE_BOOL, DTYPE_F32 = 0, 1, 2, 3
 CACHE_INT8, CACHE_E4M3 = 0, 1
 ABI_VERSION = 6
 
@@ -64,6 +64,16 @@ SIGNATURES = {
     "sage_cache_attn_workspace": ([_I, _I, _I, _I, _I, _I, _I, _P], _I),
     "sage_cache_attn": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _L, _P, _P, _L, _L, _L,
                          _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P], _I),
+    "sage_bias_borders": ([_I, _I, _I, _P], _I),
+    "sage_relative_bias": ([_P, _I, _L, _L, _I, _I, _I, _P, _I, _I, _L, _P, _I, _P, _I, _P], _I),
+    "sage_relative_bias_grad_workspace": ([_I, _I, _I, _I, _I, _P], _I),
+    "sage_relative_bias_grad": ([_P, _L, _L, _I, _I, _I, _I, _P, _I, _I, _L, _P, _I, _P, _I, _L, _L, _P, _L, _P], _I),
+    "sage_train_workspace": ([_I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _L, _I, _I, _P, _P, _P], _I),
+    "sage_train_fwd": ([_P, _L, _L, _L] * 4 + [_P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _L, _L, _L,
+                                               _P, _I, _L, _L, _I, _I, _P, _P, _L, _P], _I),
+    "sage_train_bwd": ([_P, _L, _L, _L] * 5 + [_P] + [_P, _L, _L, _L] * 3 +
+                       [_I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _L, _L, _L, _P, _I, _L, _L, _I, _I, _P, _P, _L, _P, _L,
+                        _P], _I),
 }
 
 
@@ -166,4 +176,31 @@ def cache_attn_workspace(B: int, H: int, Hkv: int, T: int, D: int, page_size: in
     """Workspace bytes of sage_cache_attn on the current device."""
     ws = ctypes.c_int64()
     call("sage_cache_attn_workspace", B, H, Hkv, T, D, page_size, max_pages, ctypes.byref(ws))
+    return ws.value
+
+
+@functools.lru_cache(maxsize=256)
+def bias_borders(buckets: int, two_sided: bool, max_distance: int):
+    """The borders of a relative position bias' far buckets, as the C array that the calls take."""
+    side = buckets // 2 if two_sided else buckets
+    out = (ctypes.c_int * (side - side // 2))()
+    call("sage_bias_borders", buckets, int(two_sided), max_distance, out)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def train_workspace(packed: bool, B: int, H: int, Hkv: int, Sq: int, Skv: int, D: int, mask, bias):
+    """(state bytes, workspace bytes) of sage_train_fwd / sage_train_bwd; mask: None or whether it has a batch, head and
+    row axis; bias: None or (buckets, two_sided, max_distance).  Host arithmetic only."""
+    state, ws = ctypes.c_int64(), ctypes.c_int64()
+    m = (0, 0, 0, 0) if mask is None else (1, *mask)
+    b = (0, 0, None) if bias is None else (bias[0], int(bias[1]), bias_borders(*bias))
+    call("sage_train_workspace", int(packed), B, H, Hkv, Sq, Skv, D, *m, *b, ctypes.byref(state), ctypes.byref(ws))
+    return state.value, ws.value
+
+
+def bias_grad_workspace(H: int, buckets: int, q_len: int, kv_len: int, dtype: int) -> int:
+    """Workspace bytes of sage_relative_bias_grad."""
+    ws = ctypes.c_int64()
+    call("sage_relative_bias_grad_workspace", H, buckets, q_len, kv_len, dtype, ctypes.byref(ws))
     return ws.value

@@ -1,10 +1,10 @@
 """torch.library registration: torch.ops.cdna4_sage.attention (and attention_masked, rope, cache_write, cache_read,
-cache_attention), traceable by torch.compile.
+cache_attention, attention_train, relative_bias), traceable by torch.compile.
 
 Same schema as the reference's rdna4_sage::attention (src/rdna4_sage/ops.py:7-17); the rdna4_sage package of this
 repo registers that name too, for callers that use it directly.
 """
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -162,3 +162,123 @@ def cache_attention_lse(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_s
 def _fake_cache_attention_lse(q, k8, v8, k_scale, v_scale, block_table, lengths, tree_mask, layout, sm_scale, is_causal):
     out = _fake(q, None, None, layout, sm_scale, is_causal)
     return out, q.new_empty((out.shape[0], out.shape[2], out.shape[1]), dtype=torch.float32)
+
+
+# ---- attention for training and the relative position bias (no counterparts in the reference) --------------------------------
+
+def _mask_axes(attn_mask, q, k, layout):
+    from . import _train
+
+    return [] if attn_mask is None else list(_train._axes_of(attn_mask, q, k, layout))
+
+
+@torch.library.custom_op("cdna4_sage::attention_train", mutates_args=())
+def attention_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn_mask: Optional[torch.Tensor],
+                    table: Optional[torch.Tensor], cu_q: Optional[torch.Tensor], cu_k: Optional[torch.Tensor], layout: str,
+                    sm_scale: float, is_causal: bool, bidirectional: bool,
+                    max_distance: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Attention on 16-bit inputs: (out, lse, the state that the backward pass reads); packed sequences where cu_q is given."""
+    from . import _train
+
+    return _train.forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, is_causal, bidirectional,
+                                 max_distance)[:3]
+
+
+@attention_train.register_fake
+def _fake_attention_train(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, is_causal, bidirectional, max_distance):
+    from . import _capi, _rope
+
+    packed = cu_q is not None
+    if packed:
+        out, (Sq, H, D), (Skv, Hkv, _), B = q.new_empty(q.shape), q.shape, k.shape, cu_q.shape[0] - 1
+        lse = q.new_empty((H, Sq), dtype=torch.float32)
+    else:
+        out, (B, H, Sq, D) = _rope.out_like(q), q.shape if layout == "HND" else [q.shape[i] for i in (0, 2, 1, 3)]
+        Hkv, Skv = (k.shape[1], k.shape[2]) if layout == "HND" else (k.shape[2], k.shape[1])
+        lse = q.new_empty((B, H, Sq), dtype=torch.float32)
+    state = 0
+    if q.numel() != 0 and k.numel() != 0:
+        state = _capi.train_workspace(packed, int(B), int(H), int(Hkv), int(Sq), int(Skv), int(D),
+                                      tuple(_mask_axes(attn_mask, q, k, layout)) or None,
+                                      None if table is None else (int(table.shape[0]), bidirectional, max_distance))[0]
+    return out, lse, q.new_empty((state,), dtype=torch.uint8)
+
+
+@torch.library.custom_op("cdna4_sage::attention_train_backward", mutates_args=())
+def attention_train_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             lse: torch.Tensor, state: torch.Tensor, table: Optional[torch.Tensor],
+                             cu_q: Optional[torch.Tensor], cu_k: Optional[torch.Tensor], layout: str, sm_scale: float,
+                             is_causal: bool, bidirectional: bool, max_distance: int,
+                             mask_axes: List[int]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv, dtable), the last one empty without a table; mask_axes: whether the mask had a batch, head and row axis."""
+    from . import _train
+
+    dq, dk, dv, dt = _train.backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, is_causal,
+                                            bidirectional, max_distance, tuple(mask_axes) or None,
+                                            (True, True, table is not None))
+    return dq, dk, dv, q.new_empty(0) if dt is None else dt
+
+
+@attention_train_backward.register_fake
+def _fake_attention_train_backward(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, is_causal,
+                                   bidirectional, max_distance, mask_axes):
+    from . import _rope
+
+    like = _rope.out_like if cu_q is None else (lambda t: t.new_empty(t.shape))
+    return like(q), like(k), like(v), q.new_empty(0) if table is None else table.new_empty(table.shape)
+
+
+def _train_setup(ctx, inputs, output):
+    q, k, v, attn_mask, table, cu_q, cu_k, *ctx.how = inputs
+    ctx.axes = _mask_axes(attn_mask, q, k, ctx.how[0])
+    ctx.save_for_backward(q, k, v, *output, table, cu_q, cu_k)
+    ctx.mark_non_differentiable(output[1], output[2])
+
+
+def _train_backward(ctx, dout, *_):
+    dq, dk, dv, dt = attention_train_backward(dout, *ctx.saved_tensors, *ctx.how, ctx.axes)
+    return (dq, dk, dv, None, dt if ctx.saved_tensors[6] is not None else None) + (None,) * 7
+
+
+attention_train.register_autograd(_train_backward, setup_context=_train_setup)
+
+
+@torch.library.custom_op("cdna4_sage::relative_bias", mutates_args=())
+def relative_bias(table: torch.Tensor, q_len: int, kv_len: int, bidirectional: bool, max_distance: int, dtype: torch.dtype,
+                  offset: int, offset_at: Optional[torch.Tensor]) -> torch.Tensor:
+    """The bias [heads, q_len, kv_len] of a table [buckets, heads] by relative position."""
+    from . import _train
+
+    return _train.bias_launch(table, q_len, kv_len, bidirectional, max_distance, dtype, offset, offset_at)
+
+
+@relative_bias.register_fake
+def _fake_relative_bias(table, q_len, kv_len, bidirectional, max_distance, dtype, offset, offset_at):
+    return table.new_empty((table.shape[1], q_len, kv_len), dtype=dtype)
+
+
+@torch.library.custom_op("cdna4_sage::relative_bias_backward", mutates_args=())
+def relative_bias_backward(dbias: torch.Tensor, buckets: int, dtype: torch.dtype, bidirectional: bool, max_distance: int,
+                           offset: int, offset_at: Optional[torch.Tensor]) -> torch.Tensor:
+    """The gradient [buckets, heads] of relative_bias' table."""
+    from . import _train
+
+    return _train.bias_grad_launch(dbias, buckets, dtype, bidirectional, max_distance, offset, offset_at)
+
+
+@relative_bias_backward.register_fake
+def _fake_relative_bias_backward(dbias, buckets, dtype, bidirectional, max_distance, offset, offset_at):
+    return dbias.new_empty((buckets, dbias.shape[0]), dtype=dtype)
+
+
+def _bias_setup(ctx, inputs, output):
+    table, _, _, bidirectional, max_distance, _, offset, offset_at = inputs
+    ctx.how = table.shape[0], table.dtype, bidirectional, max_distance, offset
+    ctx.save_for_backward(offset_at)
+
+
+def _bias_backward(ctx, dbias):
+    return (relative_bias_backward(dbias, *ctx.how, *ctx.saved_tensors),) + (None,) * 7
+
+
+relative_bias.register_autograd(_bias_backward, setup_context=_bias_setup)

@@ -1,0 +1,290 @@
+// Attention on 16-bit inputs for training: what its forward and backward kernels share.
+//
+// x_ij = (q_i . k_j) * sm_scale + bias(j - i), hidden pairs at -inf; lse_i = ln sum_j e^x_ij; p_ij = e^(x_ij - lse_i);
+// o_i = sum_j p_ij v_j.  Backward: D_i = do_i . o_i; ds_ij = p_ij (do_i . v_j - D_i); dv_j = sum_i p_ij do_i;
+// dq_i = sm_scale sum_j ds_ij k_j; dk_j = sm_scale sum_i ds_ij q_i.  All sums, statistics and scores in fp32; p and ds are
+// rounded to the inputs' 16 bits where they become an operand of the next product.
+//
+// One form serves the three kernels.  A wave owns 32 columns (queries in the forward and dq kernels, keys in the dk / dv
+// kernel), one per lane of a half wave, their operands in registers, and the workgroup streams 64-row tiles of the other side
+// through LDS.  v_mfma_f32_32x32x16 with A = 32 rows x 16 channels of the tile and B = the columns gives the accumulator in
+// which lane l holds column l % 32 and, in register v, row 8 (v / 4) + 4 (l / 32) + v % 4 of the block: row statistics of a
+// query are per lane there.  The second product of each score tile (p v, ds k, p^T do, ds^T q) sums over the tile's rows, and a
+// sum may take its terms in any order: registers 8 s .. 8 s + 7 of the scores, rounded, are already its B operand for the 16
+// rows 16 s .. 16 s + 15, when the A operand (the tile, transposed) takes the rows in that order too.  The transposed operand
+// comes from the same LDS tile by ds_read_b64_tr_b16: of four rows x 16 channels that a group of 16 lanes addresses, lane i gets
+// channel i's four rows.  No score goes through LDS and nothing is transposed in memory.
+#pragma once
+
+#include "sage_bias.h"
+#include "sage_common.h"
+#include "sage_host.h"
+
+namespace sage {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int TR_COLS = 128;     // columns per workgroup, 4 waves x 32
+constexpr int TR_ROWS = 64;      // rows per streamed tile
+constexpr int TR_THREADS = 256;
+constexpr float TR_LOG2E = 1.4426950408889634f;
+
+// Arguments of the three kernels and the preparation.  Strides in elements: b (batch), s (token), h (head).
+struct TrainArgs {
+  const uint16_t *q, *k, *v, *o, *dout;
+  uint16_t *out, *dq, *dk, *dv;
+  int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, ob, os, oh, gb, gs, gh;   // o and out: o*, dout: g*
+  int64_t dqb, dqs, dqh, dkb, dks, dkh, dvb, dvs, dvh;
+  int B, H, Hkv, Sq, Skv;          // packed: B sequences, Sq / Skv the totals of tokens
+  int q_tiles, k_tiles;            // 128-column tiles of a batch entry (packed: of the whole batch, an upper bound)
+  int causal;                      // bottom-right: query i of a sequence sees keys j <= i + (kv_len - q_len)
+  float scale, c;                  // sm_scale, sm_scale * log2(e)
+  float* lse;                      // fp32 [B, H, Sq] (packed [H, Sq]), natural log
+  // backward: -lse * log2(e) and -D of every row, -inf and 0 in the padding: rows of `pad` entries per (b, h) (packed: per
+  // h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
+  float *nl, *nd;
+  int64_t pad;
+  uint32_t* norms;                 // fp16: the largest squared norms of dout's and v's rows, as bits
+  // packed batches: offsets and the (sequence, tile) of each tile id, sequence -1 for none
+  const int *cu_q, *cu_k;
+  const int2 *q_tab, *k_tab;
+  // boolean masks as bits: word w of row i holds keys 32 w ..; word w of row i at bits + b*mb + h*mh + w*mw + i*mi
+  const uint32_t* bits;
+  int64_t mb, mh, mw, mi;
+  // bias by distance: [H, 2 reach + 1] fp32 times log2(e); entry reach + d for key - query = d, clamped to +-reach
+  const float* bias;
+  int reach;
+  float* bias_part;                // backward: [H][parts][buckets] sums of ds, a part for every tile of queries
+  int64_t parts;
+};
+
+template <int D> struct TrGeo {
+  static constexpr int ROWB = 2 * D;                    // bytes per LDS row
+  static constexpr int KCH = D / 8;                     // 16-byte chunks per row
+  static constexpr int TILE = TR_ROWS * ROWB;           // bytes per tile
+  static constexpr int LOADS = TILE / 1024 / 4;         // 1 KiB direct loads per wave and tile
+  static constexpr int NK = D / 16;                     // products over the channels per 32 x 32 block
+  static constexpr int NDB = D / 32;                    // 32-channel blocks
+};
+
+// Position of 16-byte chunk c in LDS row `row` (an involution).  Two kinds of reads have to spread over the 64 banks: 16 rows'
+// same chunk (row operands) and 4 consecutive rows' 4 neighbouring chunks (transposed operands).
+template <int D> __device__ __forceinline__ int tr_swz(int row, int c) {
+  if (D == 64) return c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));  // (two rows per 256 bytes)
+  if (D == 96) return c ^ ((row >> 2) & 3);                              // (192-byte rows turn by 64 bytes each)
+  return c ^ (((row & 3) << 2) | ((row >> 2) & 3));
+}
+
+template <int DT> __device__ __forceinline__ v16f tr_mfma(v4i a, v4i b, v16f c) {
+  if constexpr (DT == DT_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// two floats to 16 bits each, to nearest even, one instruction
+template <int DT> __device__ __forceinline__ int tr_pack(float a, float b) {
+  if constexpr (DT == DT_BF16) return __builtin_bit_cast(int, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  else return __builtin_bit_cast(int, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+__device__ __forceinline__ void tr_copy16(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void tr_copy4(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+}
+
+// A workgroup's loads of 64-row tiles: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.
+template <int D> struct TrLoader {
+  using G = TrGeo<D>;
+  int row[G::LOADS];      // of the tile
+  int elem[G::LOADS];     // channel
+  __device__ __forceinline__ void init(int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < G::LOADS; ++j) {
+      const int L = (wave * G::LOADS + j) * 64 + lane;
+      row[j] = L / G::KCH;
+      elem[j] = tr_swz<D>(row[j], L % G::KCH) * 8;
+    }
+  }
+  // rows row0 .. row0 + 63 of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave) const {
+#pragma unroll
+    for (int j = 0; j < G::LOADS; ++j) {
+      const int r = min(row0 + row[j], len - 1);
+      tr_copy16(base + r * stride + elem[j], lds + (wave * G::LOADS + j) * 1024);
+    }
+  }
+};
+
+// Byte offsets of a lane's operands in a tile.  Row operands: row l % 32 (a block of 32 rows adds 32 * ROWB), chunk 2 i + half.
+// Transposed operands: rows 16 s + 8 e + 4 half + (l % 16) / 4, channels 32 db + 16 ((l / 16) % 2) + 4 (l % 4) ..; s adds
+// 16 * ROWB.
+template <int D> struct TrAddr {
+  using G = TrGeo<D>;
+  int row[G::NK], col[G::NDB][2];
+  __device__ __forceinline__ void init_rows(int lane) {
+    const int ln = lane & 31, hf = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < G::NK; ++i) row[i] = ln * G::ROWB + tr_swz<D>(ln, 2 * i + hf) * 16;
+  }
+  __device__ __forceinline__ void init_cols(int lane) {
+    const int hf = lane >> 5, r = (lane & 15) >> 2, c = lane & 3, g = (lane >> 4) & 1;
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int rw = 8 * e + 4 * hf + r;
+        col[db][e] = rw * G::ROWB + tr_swz<D>(rw, 4 * db + 2 * g + (c >> 1)) * 16 + (c & 1) * 8;
+      }
+  }
+  __device__ __forceinline__ v4i rows(const uint8_t* lds, int blk, int i) const {
+    return *reinterpret_cast<const v4i*>(lds + row[i] + blk * 32 * G::ROWB);
+  }
+  __device__ __forceinline__ v4i cols(const uint8_t* lds, int s, int db) const {
+    v4i r;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(lds + col[db][e] + s * 16 * G::ROWB));
+      const v2i y = __builtin_bit_cast(v2i, x);
+      r[2 * e] = y[0];
+      r[2 * e + 1] = y[1];
+    }
+    return r;
+  }
+};
+
+// Channels 32 db .. of column l % 32, held as acc registers (row 8 (v / 4) + 4 half + v % 4 = channel), times f, to 16 bits at p:
+// one exchange between the halves makes 16-byte stores.
+template <int DT> __device__ __forceinline__ void tr_store(const v16f& acc, float f, uint16_t* p, int hf, bool on) {
+#pragma unroll
+  for (int gp = 0; gp < 2; ++gp) {
+    v4i w;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int lo = tr_pack<DT>(acc[8 * gp + 2 * e] * f, acc[8 * gp + 2 * e + 1] * f);
+      const int hi = tr_pack<DT>(acc[8 * gp + 4 + 2 * e] * f, acc[8 * gp + 4 + 2 * e + 1] * f);
+      const auto r = __builtin_amdgcn_permlane32_swap((unsigned)lo, (unsigned)hi, false, false);
+      w[e] = (int)r[0];
+      w[2 + e] = (int)r[1];
+    }
+    if (on) *reinterpret_cast<v4i*>(p + 16 * gp + 8 * hf) = w;
+  }
+}
+
+// What a workgroup works on: a 128-column tile of one head of one sequence.
+struct TrSeq {
+  int b, h;                // batch entry (packed: sequence) and head
+  int c0;                  // first column of the tile in the sequence
+  int q_len, k_len;
+  int64_t qr, kr;          // first row of the sequence in q and k (packed), 0 otherwise
+  int64_t lr;              // its row 0 in nl / nd
+  int part;                // the tile's number among all of a head
+};
+
+// The tile of workgroup `id`; false where there is none.  keys: column tiles of keys (heads are kv heads).  Heads of one batch
+// entry that share the streamed side follow each other on one XCD; causal launches take long tiles first.
+template <bool KEYS> __device__ __forceinline__ bool tr_tile(const TrainArgs& a, int id, TrSeq& s) {
+  const int heads = KEYS ? a.Hkv : a.H, tiles = KEYS ? a.k_tiles : a.q_tiles;
+  const int pairs = a.cu_q ? heads : a.B * heads;
+  int bh, t;
+  if (a.causal) {
+    causal_tile(id, pairs, tiles, bh, t);
+    if (KEYS) t = tiles - 1 - t;   // (the first keys are seen by the most queries)
+  } else {
+    const int lg = xcd_remap(id, pairs * tiles);
+    bh = lg / tiles;
+    t = lg % tiles;
+  }
+  s.part = a.cu_q ? t : bh / heads * tiles + t;
+  s.h = a.cu_q ? bh : bh % heads;
+  if (a.cu_q) {
+    const int2 e = (KEYS ? a.k_tab : a.q_tab)[t];
+    if (e.x < 0) return false;
+    s.b = e.x;
+    s.c0 = e.y * TR_COLS;
+    const int q0 = a.cu_q[e.x], k0 = a.cu_k[e.x];
+    s.q_len = a.cu_q[e.x + 1] - q0;
+    s.k_len = a.cu_k[e.x + 1] - k0;
+    s.qr = q0;
+    s.kr = k0;
+    s.lr = q0 / 64 * 64 + (int64_t)64 * e.x;
+  } else {
+    s.b = bh / heads;
+    s.c0 = t * TR_COLS;
+    s.q_len = a.Sq;
+    s.k_len = a.Skv;
+    s.qr = s.kr = 0;
+    s.lr = 0;
+  }
+  return true;
+}
+
+__device__ __forceinline__ int64_t tr_stat_row(const TrainArgs& a, const TrSeq& s, int h) {
+  return a.cu_q ? h * a.pad + s.lr : ((int64_t)s.b * a.H + h) * a.pad;
+}
+
+// Largest distance of a bias inside the kernels: it and four waves' sums by distance have to fit the LDS that tiles of 256
+// channels leave.
+constexpr int TR_REACH = 768;
+
+// Hidden pairs and the bias of one 32 x 32 block of scores whose columns are queries: register v of lane l is key
+// key0 + 8 (v / 4) + 4 (l / 32) + v % 4.  Values at the keys of `bits` (the word of the lane's query and these 32 keys) that are 0,
+// and behind `lim`, become -inf.
+__device__ __forceinline__ void tr_hide_keys(v16f& x, int key0, int lim, uint32_t bits, int hf) {
+  const int room = lim - key0 - 4 * hf;
+  const uint32_t w = bits >> (4 * hf);
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int r = 8 * (v >> 2) + (v & 3);
+    if (r > room || !((w >> r) & 1u)) x[v] = -INFINITY;
+  }
+}
+
+// Whether a wave's 16-bit vector of finite sums is finite: 0 or NaN
+template <int N> __device__ __forceinline__ float tr_nonfinite(const v16f (&a)[N]) {
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) t = __builtin_fmaf(a[i][v], 0.0f, t);
+  return t;
+}
+
+// The infinities and NaN of a tile become 0; poison[r] is set where row r had one.  A hidden pair has weight 0, but 0 times an
+// infinity is NaN: results that come out non-finite are computed a second time from tiles cleaned like this, in which the rows
+// that see a poisoned one get NaN by their scores.  Two barriers are the caller's.
+template <int D, int DT> __device__ __forceinline__ void tr_clean(uint8_t* tile, int* poison, int tid) {
+  using G = TrGeo<D>;
+  constexpr uint32_t E = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
+  for (int i = tid; i < G::TILE / 16; i += TR_THREADS) {
+    v4i* p = reinterpret_cast<v4i*>(tile) + i;
+    v4i w = *p;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t u = (uint32_t)w[e];
+      if ((u & E) == E) u &= 0xFFFF0000u, bad = true;
+      if ((u & (E << 16)) == (E << 16)) u &= 0x0000FFFFu, bad = true;
+      w[e] = (int)u;
+    }
+    if (bad) {
+      *p = w;
+      if (poison) poison[i / G::KCH] = 1;
+    }
+  }
+}
+
+template <int D, int DT> int train_fwd_launch(const TrainArgs& a, hipStream_t st);
+template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap& m, hipStream_t st);
+
+}  // namespace sage

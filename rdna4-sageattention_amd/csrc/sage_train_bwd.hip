@@ -1,0 +1,541 @@
+// Backward pass of the attention for training: see sage_train.h for the form.
+//
+// Two kernels, each of which recomputes the scores and the gradient of the probabilities: one owns queries and streams keys
+// (dq), one owns keys and streams queries (dk, dv).  That is seven products for the five of the formulas, and it needs neither
+// atomics nor partial results in memory: every gradient is one sum in a fixed order, so equal inputs give equal bits.  A single
+// kernel would have to add dq over its workgroups: 4 bytes written and read for every 2 * 128 keys' products of a channel.
+#include "sage_train.h"
+
+namespace sage {
+
+// fp16 holds ds only in a window of 2^30.  |do_i . v_j - D_i| <= 2 max |do| max |v|, so ds times this power of two stays below
+// 2^15, and full precision reaches down to 2^-29 of the bound.  (bf16 has float32's exponents: 0.)
+__device__ __forceinline__ int tr_exponent(const uint32_t* norms) {
+  const float n = __uint_as_float(norms[0]) * __uint_as_float(norms[1]);   // the squared bound / 4
+  if (!(n > 0.0f && n < INFINITY)) return 0;
+  int e;
+  (void)frexpf(n, &e);                       // n < 2^e, so the bound is below 2^(e / 2 + 1)
+  return min(max(13 - ((e + 1) >> 1), -100), 100);
+}
+// P is at most 1 and is taken times 2^15 in fp16 where it is an operand
+template <int DT> constexpr float BWD_SHIFT = DT == DT_F16 ? 15.0f : 0.0f;
+
+// ---- preparation: -lse * log2(e) and -D of every row; the norms of fp16 inputs -----------------------------------------------
+
+template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_prep(TrainArgs a, int row_blocks, int norm_blocks) {
+  constexpr int LPR = D == 96 ? 16 : D / 8;       // lanes per row (12 of the 16 at head dim 96)
+  constexpr int ROWS = TR_THREADS / LPR;
+  const int tid = threadIdx.x, r = tid / LPR, l = tid % LPR;
+  const bool has = l * 8 < D;
+  float top = 0.0f;                               // largest squared norm of this thread's rows
+  auto row_sum = [&](float x) {
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+  };
+  if ((int)blockIdx.x >= row_blocks) {            // fp16: the rows of v
+    const int64_t n = (int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * a.Skv;
+    for (int64_t x = (int64_t)(blockIdx.x - row_blocks) * ROWS + r; x < n; x += (int64_t)norm_blocks * ROWS) {
+      const int64_t h = x % a.Hkv, t = x / a.Hkv, j = t % a.Skv, b = t / a.Skv;
+      float s = 0.0f;
+      if (has) {
+        const v4i w = *reinterpret_cast<const v4i*>(a.v + b * a.vb + j * a.vs + h * a.vh + l * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = elem_lo<DT>(w[e]), x1 = elem_hi<DT>(w[e]);
+          s = __builtin_fmaf(x0, x0, __builtin_fmaf(x1, x1, s));
+        }
+      }
+      s = row_sum(s);
+      if (s < INFINITY) top = fmaxf(top, s);
+    }
+  } else {
+    // 128 rows of one head
+    const int tiles = a.q_tiles, bh = blockIdx.x / tiles, t = blockIdx.x % tiles;
+    TrSeq s;
+    s.b = bh / a.H, s.h = bh % a.H, s.c0 = t * TR_COLS, s.q_len = a.Sq, s.qr = 0, s.lr = 0;
+    if (a.cu_q) {
+      const int2 e = a.q_tab[t];
+      if (e.x < 0) return;
+      const int q0 = a.cu_q[e.x];
+      s.b = e.x, s.c0 = e.y * TR_COLS, s.q_len = a.cu_q[e.x + 1] - q0, s.qr = q0, s.lr = q0 / 64 * 64 + (int64_t)64 * e.x;
+    }
+    const int64_t at = tr_stat_row(a, s, s.h);
+    const int64_t lse_at = a.cu_q ? (int64_t)s.h * a.Sq + s.qr : ((int64_t)s.b * a.H + s.h) * a.Sq;
+    const int end = min(s.c0 + TR_COLS, (s.q_len + 63) / 64 * 64);
+    const uint16_t* op = a.o + (a.cu_q ? 0 : s.b * a.ob) + s.qr * a.os + s.h * a.oh + l * 8;
+    const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * a.gh + l * 8;
+    for (int i = s.c0 + r; i < end; i += ROWS) {
+      float d = 0.0f, g2 = 0.0f;
+      if (i < s.q_len && has) {
+        const v4i x = *reinterpret_cast<const v4i*>(op + i * a.os), g = *reinterpret_cast<const v4i*>(gp + i * a.gs);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float g0 = elem_lo<DT>(g[e]), g1 = elem_hi<DT>(g[e]);
+          d = __builtin_fmaf(elem_lo<DT>(x[e]), g0, __builtin_fmaf(elem_hi<DT>(x[e]), g1, d));
+          if (DT == DT_F16) g2 = __builtin_fmaf(g0, g0, __builtin_fmaf(g1, g1, g2));
+        }
+      }
+      d = row_sum(d);
+      if (DT == DT_F16) {
+        g2 = row_sum(g2);
+        if (g2 < INFINITY) top = fmaxf(top, g2);
+      }
+      if (l == 0) {
+        // a row that sees nothing: p = 0; one with an infinity or a NaN in it: p = NaN wherever it sees a key
+        const float lse = i < s.q_len ? a.lse[lse_at + i] : -INFINITY;
+        float nl = lse * -TR_LOG2E, nd = -d;
+        if (lse == -INFINITY) nl = -INFINITY, nd = 0.0f;
+        else if (!(fabsf(lse) < INFINITY) || !(fabsf(d) < INFINITY)) nl = NAN;
+        a.nl[at + i] = nl;
+        a.nd[at + i] = nd;
+      }
+    }
+  }
+  if (DT == DT_F16) {
+    top = wave_max_pos(top);
+    if ((tid & 63) == 0 && top > 0.0f) atomicMax(a.norms + ((int)blockIdx.x >= row_blocks ? 1 : 0), __float_as_uint(top));
+  }
+}
+
+__global__ void train_norms_zero(uint32_t* norms) {
+  if (threadIdx.x < 2) norms[threadIdx.x] = 0;
+}
+
+// ---- dq (and the bias' gradient by distance) ---------------------------------------------------------------------------------
+
+template <int D, int DT, bool EX>
+__global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainArgs a, BiasMap map) {
+  using G = TrGeo<D>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
+  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  extern __shared__ float by_distance[];   // EX with bias_part: 4 waves x (2 reach + 1)
+
+  TrSeq s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool biased = EX && a.bias, want_part = EX && a.bias_part;
+  const int R = 2 * a.reach + 1;
+  if (!tr_tile<false>(a, blockIdx.x, s)) {
+    if (want_part)   // (only packed batches have unused tiles)
+      for (int x = tid; x < map.buckets; x += TR_THREADS) a.bias_part[(s.h * a.parts + s.part) * map.buckets + x] = 0.0f;
+    return;
+  }
+  const int ln = lane & 31, hf = lane >> 5;
+  const int hk = s.h / (a.H / a.Hkv);
+  const int off = s.k_len - s.q_len;
+  const int w0 = s.c0 + wave * 32, i = w0 + ln;
+  const bool on = i < s.q_len;
+  const int ir = on ? i : s.q_len - 1;
+
+  const uint16_t* kp = a.k + (a.cu_q ? 0 : s.b * a.kb) + s.kr * a.ks + hk * a.kh;
+  const uint16_t* vp = a.v + (a.cu_q ? 0 : s.b * a.vb) + s.kr * a.vs + hk * a.vh;
+  const int64_t at_row = tr_stat_row(a, s, s.h);
+  float nl = on ? a.nl[at_row + i] : -INFINITY;
+  const float nd = on ? a.nd[at_row + i] : 0.0f;
+  const bool empty = nl == -INFINITY;   // sees nothing: its q and dout may hold anything
+
+  v4i qf[G::NK], gf[G::NK];
+  {
+    const uint16_t* p = a.q + (a.cu_q ? 0 : s.b * a.qb) + (s.qr + ir) * a.qs + s.h * a.qh + 8 * hf;
+    const uint16_t* g = a.dout + (a.cu_q ? 0 : s.b * a.gb) + (s.qr + ir) * a.gs + s.h * a.gh + 8 * hf;
+#pragma unroll
+    for (int x = 0; x < G::NK; ++x) {
+      qf[x] = *reinterpret_cast<const v4i*>(p + 16 * x);
+      gf[x] = *reinterpret_cast<const v4i*>(g + 16 * x);
+      if (empty) qf[x] = v4i{0, 0, 0, 0}, gf[x] = v4i{0, 0, 0, 0};
+    }
+  }
+  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
+  nl += (float)ex;
+
+  TrLoader<D> ld;
+  ld.init(wave, lane);
+  TrAddr<D> at;
+  at.init_rows(lane);
+  at.init_cols(lane);
+
+  int kv_end = s.k_len;
+  if (a.causal) kv_end = min(kv_end, min(s.c0 + TR_COLS, s.q_len) + off);
+  const int ntiles = kv_end > 0 ? (kv_end + TR_ROWS - 1) / TR_ROWS : 0;
+  const int lim = a.causal ? min(s.k_len - 1, ir + off) : s.k_len - 1;
+  int t_mask = s.k_len / TR_ROWS, t_end = ntiles;
+  if (a.causal) {
+    t_mask = min(t_mask, max(0, w0 + off + 1) / TR_ROWS);
+    t_end = min(t_end, (max(0, min(w0 + 31, s.q_len - 1) + off + 1) + TR_ROWS - 1) / TR_ROWS);
+  }
+  if (w0 >= s.q_len) t_end = 0;
+  const uint32_t* bits = nullptr;
+  if (EX && a.bits) {
+    bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
+    t_mask = 0;
+  }
+  float* mine = by_distance + wave * R;
+  if (biased)
+    for (int x = tid; x < R; x += TR_THREADS) bl[x] = a.bias[(int64_t)s.h * R + x];
+
+  v16f dq[G::NDB];
+  // the bias' gradient: the lane's sums of ds and p over the keys at distance -reach and farther behind, reach and farther ahead,
+  // and of ds over the others
+  float flo = 0.0f, fhi = 0.0f, plo = 0.0f, phi = 0.0f, fnear = 0.0f;
+
+  auto issue = [&](int t) {
+    ld.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave);
+    ld.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave);
+  };
+  auto tile = [&](int t, bool masked) {
+    const uint8_t* kt = smem[t & 1][0];
+    const uint8_t* vt = smem[t & 1][1];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      v16f x = {}, dp;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dp[v] = nd;
+#pragma unroll
+      for (int kk = 0; kk < G::NK; ++kk) {
+        x = tr_mfma<DT>(at.rows(kt, kb, kk), qf[kk], x);
+        dp = tr_mfma<DT>(at.rows(vt, kb, kk), gf[kk], dp);
+      }
+      const int key0 = t * TR_ROWS + 32 * kb;
+      const int d0 = key0 + 4 * hf - (ir + off);
+      const int wlo = key0 - (min(w0 + 31, s.q_len - 1) + off), whi = key0 + 31 - (w0 + off);
+      const bool near = biased && !(whi <= -a.reach || wlo >= a.reach);
+      if (EX) {
+        if (near) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int d = min(max(d0 + 8 * (v >> 2) + (v & 3), -a.reach), a.reach);
+            x[v] = __builtin_fmaf(x[v], a.c, bl[a.reach + d]);
+          }
+        } else {
+          const float far = biased ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(x[v], a.c, far);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(EX ? x[v] + nl : __builtin_fmaf(x[v], a.c, nl));
+      if (masked) {
+        uint32_t w = ~0u;
+        if (EX && bits && key0 < s.k_len) w = bits[(int64_t)(key0 >> 5) * a.mw];
+        const int room = lim - key0 - 4 * hf;
+        w >>= 4 * hf;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int r = 8 * (v >> 2) + (v & 3);
+          if (r > room || !((w >> r) & 1u)) x[v] = 0.0f, dp[v] = 0.0f;
+        }
+      }
+      if (want_part) {
+        // d[v]: of ds; every lane of a half wave has a distance of its own, so one half at a time adds without conflicts and in
+        // one order
+        float all = 0.0f, ps = 0.0f;
+        if (near) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int d = d0 + 8 * (v >> 2) + (v & 3);
+            const float y = x[v] * dp[v];
+            if (d <= -a.reach) flo += y, plo += x[v];
+            else if (d >= a.reach) fhi += y, phi += x[v];
+            else {
+              fnear += y;
+              __attribute__((address_space(3))) float* slot = (__attribute__((address_space(3))) float*)(mine + a.reach + d);
+              if (hf == 0) {
+                __builtin_amdgcn_ds_faddf(slot, y, 0, 0, false);
+                asm volatile("; the lower half's" ::: "memory");   // (keeps the two from becoming one)
+              } else {
+                __builtin_amdgcn_ds_faddf(slot, y, 0, 0, false);
+                asm volatile("; the upper half's" ::: "memory");
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) all += x[v] * dp[v], ps += x[v];
+          if (whi <= -a.reach) flo += all, plo += ps;
+          else fhi += all, phi += ps;
+        }
+      }
+      v4i ds[2];
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) ds[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v] * dp[v], x[v + 1] * dp[v + 1]);
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int db = 0; db < G::NDB; ++db) dq[db] = tr_mfma<DT>(at.cols(kt, 2 * kb + st, db), ds[st], dq[db]);
+    }
+  };
+
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dq[db][v] = 0.0f;
+    if (want_part) {
+      flo = fhi = plo = phi = fnear = 0.0f;
+      for (int x = lane; x < R; x += 64) mine[x] = 0.0f;
+    }
+    if (ntiles > 0) issue(0);
+    for (int t = 0; t < ntiles; ++t) {
+      wait_vmcnt<0>();
+      tile_barrier();
+      if (t + 1 < ntiles) issue(t + 1);
+      if (pass) {
+        tr_clean<D, DT>(smem[t & 1][0], nullptr, tid);
+        tr_clean<D, DT>(smem[t & 1][1], nullptr, tid);
+        __syncthreads();
+        if (t < t_end) tile(t, true);
+        __syncthreads();
+      } else if (t < t_mask) {
+        tile(t, false);
+      } else if (t < t_end) {
+        tile(t, true);
+      }
+    }
+    const bool bad = !(tr_nonfinite(dq) == 0.0f);
+    if (!__syncthreads_or(on && bad)) break;
+  }
+
+  const float f = __builtin_ldexpf(a.scale, -ex);
+  uint16_t* op = a.dq + (a.cu_q ? 0 : s.b * a.dqb) + (s.qr + ir) * a.dqs + s.h * a.dqh;
+#pragma unroll
+  for (int db = 0; db < G::NDB; ++db) tr_store<DT>(dq[db], f, op + 32 * db, hf, on);
+
+  if (want_part) {
+    // The row sums of ds are 0, but D holds the rounding of o to 16 bits and of its weights: sum_j ds = D' - D, exactly the error of
+    // D.  In a far bucket, which holds most of a long row's weight, it would not average out: it is taken from there.
+    const float delta = add_xor32_f32(fnear + flo + fhi);
+    flo -= delta * __builtin_ldexpf(plo, -ex);
+    fhi -= delta * __builtin_ldexpf(phi, -ex);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) flo += __shfl_xor(flo, o), fhi += __shfl_xor(fhi, o);
+    if (lane == 0) mine[0] += flo, mine[2 * a.reach] += fhi;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int x = tid; x < R; x += TR_THREADS)
+      by_distance[x] = (by_distance[x] + by_distance[R + x]) + (by_distance[2 * R + x] + by_distance[3 * R + x]);
+    __syncthreads();
+    float* part = a.bias_part + (s.h * a.parts + s.part) * map.buckets;
+    for (int b = wave; b < map.buckets; b += TR_THREADS / 64) {
+      int lo, hi;
+      map.range(b, lo, hi);
+      float y = 0.0f;
+      for (int x = lo + lane; x <= hi; x += 64) y += by_distance[a.reach + x];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) y += __shfl_xor(y, o);
+      if (lane == 0) part[b] = __builtin_ldexpf(y, -ex);
+    }
+  }
+}
+
+// ---- dk, dv --------------------------------------------------------------------------------------------------------------------
+
+template <int D, int DT, bool EX>
+__global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainArgs a) {
+  using G = TrGeo<D>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
+  __shared__ __attribute__((aligned(256))) float stat[2][2][TR_ROWS];
+  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+
+  TrSeq s;
+  if (!tr_tile<true>(a, blockIdx.x, s)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  const int group = a.H / a.Hkv;
+  const int off = s.k_len - s.q_len;
+  const int w0 = s.c0 + wave * 32, j = w0 + ln;   // the wave's first key, the lane's
+  const bool on = j < s.k_len;
+  const int jr = on ? j : s.k_len - 1;
+
+  v4i kf[G::NK], vf[G::NK];
+  {
+    const uint16_t* kp = a.k + (a.cu_q ? 0 : s.b * a.kb) + (s.kr + jr) * a.ks + s.h * a.kh + 8 * hf;
+    const uint16_t* vp = a.v + (a.cu_q ? 0 : s.b * a.vb) + (s.kr + jr) * a.vs + s.h * a.vh + 8 * hf;
+#pragma unroll
+    for (int x = 0; x < G::NK; ++x) {
+      kf[x] = *reinterpret_cast<const v4i*>(kp + 16 * x);
+      vf[x] = *reinterpret_cast<const v4i*>(vp + 16 * x);
+    }
+  }
+  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
+  const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
+
+  TrLoader<D> ld;
+  ld.init(wave, lane);
+  TrAddr<D> at;
+  at.init_rows(lane);
+  at.init_cols(lane);
+
+  const int t_all = (s.q_len + TR_ROWS - 1) / TR_ROWS;
+  int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
+  if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / TR_ROWS);
+  const int nt = t_all - t0;
+  const int steps = nt * group;
+  // tiles before t_first see no key of the wave, from t_full on every query sees every key of the wave
+  int t_first = 0, t_full = 0;
+  if (a.causal) {
+    t_first = max(0, w0 - off) / TR_ROWS;
+    t_full = (max(0, w0 + 31 - off) + TR_ROWS - 1) / TR_ROWS;
+  }
+  if (w0 >= s.k_len) t_first = t_all;
+  if (EX && a.bits) t_full = t_all;
+
+  int h = s.h * group, t = t0;                    // of the step that runs
+  int hn = h, tn = t0;                            // of the step that is loaded
+  auto issue = [&](int u) {
+    const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + hn * a.qh;
+    const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + hn * a.gh;
+    ld.issue(qp, a.qs, tn * TR_ROWS, s.q_len, smem[u & 1][0], wave);
+    ld.issue(gp, a.gs, tn * TR_ROWS, s.q_len, smem[u & 1][1], wave);
+    const int64_t r = tr_stat_row(a, s, hn) + tn * TR_ROWS + lane;
+    if (wave == 0) tr_copy4(a.nl + r, stat[u & 1][0]);
+    if (wave == 1) tr_copy4(a.nd + r, stat[u & 1][1]);
+    if (++tn == t_all) tn = t0, ++hn;
+  };
+
+  v16f dk[G::NDB], dv[G::NDB];
+  auto tile = [&](int u, bool masked) {
+    const uint8_t* qt = smem[u & 1][0];
+    const uint8_t* gt = smem[u & 1][1];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      v16f x = {}, dp;
+      float nl[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const v4f y = *reinterpret_cast<const v4f*>(&stat[u & 1][0][32 * qb + 8 * g + 4 * hf]);
+        const v4f z = *reinterpret_cast<const v4f*>(&stat[u & 1][1][32 * qb + 8 * g + 4 * hf]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nl[4 * g + e] = y[e], dp[4 * g + e] = z[e];
+      }
+#pragma unroll
+      for (int kk = 0; kk < G::NK; ++kk) {
+        x = tr_mfma<DT>(at.rows(qt, qb, kk), kf[kk], x);
+        dp = tr_mfma<DT>(at.rows(gt, qb, kk), vf[kk], dp);
+      }
+      const int q0 = t * TR_ROWS + 32 * qb;
+      if (EX) {
+        const int d0 = jr - off - q0 - 4 * hf;    // key - query of register 0; a row further is 1 less
+        const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
+        if (a.bias && !(whi <= -a.reach || wlo >= a.reach)) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int d = min(max(d0 - 8 * (v >> 2) - (v & 3), -a.reach), a.reach);
+            x[v] = __builtin_fmaf(x[v], a.c, bl[a.reach + d]);
+          }
+        } else {
+          const float far = a.bias ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(x[v], a.c, far);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float n = nl[v] + BWD_SHIFT<DT>;
+        x[v] = __builtin_amdgcn_exp2f(EX ? x[v] + n : __builtin_fmaf(x[v], a.c, n));
+      }
+      if (masked) {
+        const int room = a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          v4i w = {~0, ~0, ~0, ~0};
+          if (EX && a.bits && w0 < s.k_len) {
+            const uint32_t* p = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw;
+            if (a.mi) w = *reinterpret_cast<const v4i*>(p + q0 + 8 * g + 4 * hf);
+            else w = v4i{1, 1, 1, 1} * (int)*p;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = 4 * g + e;
+            if ((a.causal && 8 * g + e + room < 0) || !(((uint32_t)w[e] >> ln) & 1u)) x[v] = 0.0f, dp[v] = 0.0f;
+          }
+        }
+      }
+      v4i p[2], ds[2];
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        p[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
+        float d0 = x[v] * dp[v], d1 = x[v + 1] * dp[v + 1];
+        if (DT == DT_F16) d0 *= ds_mul, d1 *= ds_mul;
+        ds[v >> 3][(v & 7) >> 1] = tr_pack<DT>(d0, d1);
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int db = 0; db < G::NDB; ++db) {
+          dv[db] = tr_mfma<DT>(at.cols(gt, 2 * qb + st, db), p[st], dv[db]);
+          dk[db] = tr_mfma<DT>(at.cols(qt, 2 * qb + st, db), ds[st], dk[db]);
+        }
+    }
+  };
+
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dk[db][v] = 0.0f, dv[db][v] = 0.0f;
+    h = hn = s.h * group, t = tn = t0;
+    if (steps > 0) issue(0);
+    int bias_head = -1;
+    for (int u = 0; u < steps; ++u) {
+      wait_vmcnt<0>();
+      tile_barrier();
+      if (u + 1 < steps) issue(u + 1);
+      if (EX && a.bias && bias_head != h) {
+        bias_head = h;
+        for (int x = tid; x <= 2 * a.reach; x += TR_THREADS) bl[x] = a.bias[(int64_t)h * (2 * a.reach + 1) + x];
+        __syncthreads();
+      }
+      if (pass) {
+        tr_clean<D, DT>(smem[u & 1][0], nullptr, tid);
+        tr_clean<D, DT>(smem[u & 1][1], nullptr, tid);
+        __syncthreads();
+        if (t >= t_first) tile(u, true);
+        __syncthreads();
+      } else if (t >= t_full) {
+        if (t >= t_first) tile(u, false);
+      } else if (t >= t_first) {
+        tile(u, true);
+      }
+      if (++t == t_all) t = t0, ++h;
+    }
+    const bool bad = !(tr_nonfinite(dk) + tr_nonfinite(dv) == 0.0f);
+    if (!__syncthreads_or(on && bad)) break;
+  }
+
+  const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
+  uint16_t* kp = a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh;
+  uint16_t* vp = a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
+#pragma unroll
+  for (int db = 0; db < G::NDB; ++db) {
+    tr_store<DT>(dk[db], fk, kp + 32 * db, hf, on);
+    tr_store<DT>(dv[db], fv, vp + 32 * db, hf, on);
+  }
+}
+
+template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap& m, hipStream_t st) {
+  const int B = a.cu_q ? 1 : a.B;
+  const unsigned rows = (unsigned)((int64_t)B * a.H * a.q_tiles);
+  int norm_blocks = 0;
+  if (DT == DT_F16) {
+    train_norms_zero<<<1, 64, 0, st>>>(a.norms);
+    const int64_t need = ((int64_t)B * a.Hkv * a.Skv * (D == 96 ? 16 : D / 8) + TR_THREADS - 1) / TR_THREADS;
+    norm_blocks = (int)(need < 1024 ? need : 1024);
+  }
+  train_prep<D, DT><<<rows + norm_blocks, TR_THREADS, 0, st>>>(a, (int)rows, norm_blocks);
+  const unsigned keys = (unsigned)((int64_t)B * a.Hkv * a.k_tiles);
+  if (a.bits || a.bias) {
+    const unsigned lds = a.bias_part ? 4u * 4u * (2u * a.reach + 1u) : 0u;
+    if (a.dk) train_dkv<D, DT, true><<<keys, TR_THREADS, 0, st>>>(a);
+    if (a.dq) train_dq<D, DT, true><<<rows, TR_THREADS, lds, st>>>(a, m);
+  } else {
+    if (a.dk) train_dkv<D, DT, false><<<keys, TR_THREADS, 0, st>>>(a);
+    if (a.dq) train_dq<D, DT, false><<<rows, TR_THREADS, 0, st>>>(a, m);
+  }
+  return check_launch("train_bwd");
+}
+
+#define SAGE_BWD(D) template int train_bwd_launch<D, DT_BF16>(const TrainArgs&, const BiasMap&, hipStream_t); \
+                    template int train_bwd_launch<D, DT_F16>(const TrainArgs&, const BiasMap&, hipStream_t);
+SAGE_BWD(64) SAGE_BWD(96) SAGE_BWD(128) SAGE_BWD(256)
+
+}  // namespace sage

@@ -1,0 +1,203 @@
+// Forward pass of the attention for training: see sage_train.h for the form.
+#include "sage_train.h"
+
+namespace sage {
+
+// P is rounded to 16 bits for its product with V.  fp16: weights are taken times 2^6 against a running reference that trails the
+// maximum by at most 2^8, so they stay below 2^15 and keep full precision down to 2^-20 of the reference.
+template <int DT> constexpr float FWD_SHIFT = DT == DT_F16 ? 6.0f : 0.0f;
+constexpr float FWD_LAG = 8.0f;
+
+template <int D, int DT, bool EX>
+__global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainArgs a) {
+  using G = TrGeo<D>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
+  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  __shared__ int poison[TR_ROWS];
+
+  TrSeq s;
+  if (!tr_tile<false>(a, blockIdx.x, s)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  const int hk = s.h / (a.H / a.Hkv);
+  const int off = s.k_len - s.q_len;
+  const int w0 = s.c0 + wave * 32, i = w0 + ln;   // the wave's first query, the lane's
+  const bool on = i < s.q_len;
+  const int ir = on ? i : s.q_len - 1;
+
+  const uint16_t* kp = a.k + s.b * (a.cu_q ? 0 : a.kb) + s.kr * a.ks + hk * a.kh;
+  const uint16_t* vp = a.v + s.b * (a.cu_q ? 0 : a.vb) + s.kr * a.vs + hk * a.vh;
+
+  v4i qf[G::NK];
+  {
+    const uint16_t* p = a.q + s.b * (a.cu_q ? 0 : a.qb) + (s.qr + ir) * a.qs + s.h * a.qh + 8 * hf;
+#pragma unroll
+    for (int x = 0; x < G::NK; ++x) qf[x] = *reinterpret_cast<const v4i*>(p + 16 * x);
+  }
+  TrLoader<D> ld;
+  ld.init(wave, lane);
+  TrAddr<D> at;
+  at.init_rows(lane);
+  at.init_cols(lane);
+
+  int kv_end = s.k_len;
+  if (a.causal) kv_end = min(kv_end, min(s.c0 + TR_COLS, s.q_len) + off);
+  const int ntiles = kv_end > 0 ? (kv_end + TR_ROWS - 1) / TR_ROWS : 0;
+  const int lim = a.causal ? min(s.k_len - 1, ir + off) : s.k_len - 1;           // the lane's last visible key
+  // tiles before t_mask show every key to every query of the wave, from t_end on none
+  int t_mask = s.k_len / TR_ROWS, t_end = ntiles;
+  if (a.causal) {
+    t_mask = min(t_mask, max(0, w0 + off + 1) / TR_ROWS);
+    t_end = min(t_end, (max(0, min(w0 + 31, s.q_len - 1) + off + 1) + TR_ROWS - 1) / TR_ROWS);
+  }
+  if (w0 >= s.q_len) t_end = 0;
+  const uint32_t* bits = nullptr;
+  if (EX && a.bits) {
+    bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
+    t_mask = 0;
+  }
+  const bool biased = EX && a.bias;
+  if (biased)
+    for (int x = tid; x <= 2 * a.reach; x += TR_THREADS) bl[x] = a.bias[(int64_t)s.h * (2 * a.reach + 1) + x];
+
+  float m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
+  v16f o[G::NDB];
+  auto issue = [&](int t) {
+    ld.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave);
+    ld.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave);
+  };
+
+  auto tile = [&](int t, bool masked, bool slow) {
+    const uint8_t* kt = smem[t & 1][0];
+    const uint8_t* vt = smem[t & 1][1];
+    v16f x[2] = {};
+#pragma unroll
+    for (int kk = 0; kk < G::NK; ++kk) {
+      x[0] = tr_mfma<DT>(at.rows(kt, 0, kk), qf[kk], x[0]);
+      x[1] = tr_mfma<DT>(at.rows(kt, 1, kk), qf[kk], x[1]);
+    }
+    if (EX) {
+      // scores in the log2 domain, with the bias
+      const int d0 = t * TR_ROWS + 4 * hf - (ir + off);
+      const int wlo = t * TR_ROWS - (min(w0 + 31, s.q_len - 1) + off), whi = t * TR_ROWS + TR_ROWS - 1 - (w0 + off);
+      if (biased && !(whi <= -a.reach || wlo >= a.reach)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int d = min(max(d0 + 32 * kb + 8 * (v >> 2) + (v & 3), -a.reach), a.reach);
+            x[kb][v] = __builtin_fmaf(x[kb][v], a.c, bl[a.reach + d]);
+          }
+      } else {
+        const float far = biased ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[kb][v] = __builtin_fmaf(x[kb][v], a.c, far);
+      }
+    }
+    if (slow) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (poison[32 * kb + 8 * (v >> 2) + 4 * hf + (v & 3)]) x[kb][v] = NAN;
+    }
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int key0 = t * TR_ROWS + 32 * kb;
+        uint32_t w = ~0u;
+        if (EX && bits && key0 < s.k_len) w = bits[(int64_t)(key0 >> 5) * a.mw];
+        tr_hide_keys(x[kb], key0, lim, w, hf);
+      }
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) mx = fmaxf(mx, x[0][v]);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, x[1][v]);
+    mx = max_xor32_f32(mx);
+    if (!EX) mx *= a.c;
+    if (__ballot(mx > m + FWD_LAG) != 0) {
+      const float m_new = fmaxf(m, mx);
+      const float corr = m == m_new ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+      l *= corr;
+#pragma unroll
+      for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= corr;
+      m = m_new;
+      negm = m == -INFINITY ? FWD_SHIFT<DT> : FWD_SHIFT<DT> - m;
+    }
+    v4i p[4];
+    float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(EX ? x[kb][v] + negm : __builtin_fmaf(x[kb][v], a.c, negm));
+        const float e1 = __builtin_amdgcn_exp2f(EX ? x[kb][v + 1] + negm : __builtin_fmaf(x[kb][v + 1], a.c, negm));
+        ps[v & 2] += e0;
+        ps[(v & 2) + 1] += e1;
+        p[2 * kb + (v >> 3)][(v & 7) >> 1] = tr_pack<DT>(e0, e1);
+      }
+    l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int db = 0; db < G::NDB; ++db) o[db] = tr_mfma<DT>(at.cols(vt, st, db), p[st], o[db]);
+  };
+
+  for (int pass = 0; pass < 2; ++pass) {
+    m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[db][v] = 0.0f;
+    if (ntiles > 0) issue(0);
+    for (int t = 0; t < ntiles; ++t) {
+      wait_vmcnt<0>();
+      tile_barrier();
+      if (t + 1 < ntiles) issue(t + 1);
+      if (pass) {
+        if (tid < TR_ROWS) poison[tid] = 0;
+        __syncthreads();
+        tr_clean<D, DT>(smem[t & 1][0], poison, tid);
+        tr_clean<D, DT>(smem[t & 1][1], poison, tid);
+        __syncthreads();
+        if (t < t_end) tile(t, true, true);
+        __syncthreads();
+      } else if (t < t_mask) {
+        tile(t, false, false);
+      } else if (t < t_end) {
+        tile(t, true, false);
+      }
+    }
+    const bool bad = !(tr_nonfinite(o) == 0.0f);
+    if (!__syncthreads_or(on && bad)) break;
+  }
+
+  l = add_xor32_f32(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = a.out + s.b * (a.cu_q ? 0 : a.ob) + (s.qr + ir) * a.os + s.h * a.oh;
+#pragma unroll
+  for (int db = 0; db < G::NDB; ++db) tr_store<DT>(o[db], inv, op + 32 * db, hf, on);
+  if (on && hf == 0) {
+    const float lse = l == 0.0f ? -INFINITY : (m - FWD_SHIFT<DT> + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    a.lse[(a.cu_q ? (int64_t)s.h * a.Sq + s.qr : ((int64_t)s.b * a.H + s.h) * a.Sq) + i] = lse;
+  }
+}
+
+template <int D, int DT> int train_fwd_launch(const TrainArgs& a, hipStream_t st) {
+  const unsigned n = (unsigned)((int64_t)(a.cu_q ? 1 : a.B) * a.H * a.q_tiles);
+  if (a.bits || a.bias) train_fwd<D, DT, true><<<n, TR_THREADS, 0, st>>>(a);
+  else train_fwd<D, DT, false><<<n, TR_THREADS, 0, st>>>(a);
+  return check_launch("train_fwd");
+}
+
+#define SAGE_FWD(D) template int train_fwd_launch<D, DT_BF16>(const TrainArgs&, hipStream_t); \
+                    template int train_fwd_launch<D, DT_F16>(const TrainArgs&, hipStream_t);
+SAGE_FWD(64) SAGE_FWD(96) SAGE_FWD(128) SAGE_FWD(256)
+
+}  // namespace sage
