@@ -102,59 +102,66 @@ __device__ __forceinline__ void tr_copy4(const void* g, void* lds) {
                                    (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
 }
 
-// A workgroup's loads of 64-row tiles: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.
+// A workgroup's loads of 64-row tiles of one tensor: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.  Whole
+// tiles: the tile's address in scalar registers and a lane's 32-bit offset.
 template <int D> struct TrLoader {
   using G = TrGeo<D>;
-  int row[G::LOADS];      // of the tile
-  int elem[G::LOADS];     // channel
-  __device__ __forceinline__ void init(int wave, int lane) {
+  uint32_t off[G::LOADS];
+  bool fits;              // 64 rows' offsets pass 32 bits otherwise
+  __device__ __forceinline__ void init(int64_t stride, int wave, int lane) {
+    fits = stride >= 0 && stride < (1 << 24);
 #pragma unroll
     for (int j = 0; j < G::LOADS; ++j) {
-      const int L = (wave * G::LOADS + j) * 64 + lane;
-      row[j] = L / G::KCH;
-      elem[j] = tr_swz<D>(row[j], L % G::KCH) * 8;
+      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
+      off[j] = (uint32_t)((row * stride + tr_swz<D>(row, L % G::KCH) * 8) * 2);
     }
   }
   // rows row0 .. row0 + 63 of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
-  __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave) const {
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave, int lane) {
+    if (row0 + TR_ROWS <= len && fits) {
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(base + row0 * stride);
+      asm volatile("" : "+s"(p));
 #pragma unroll
-    for (int j = 0; j < G::LOADS; ++j) {
-      const int r = min(row0 + row[j], len - 1);
-      tr_copy16(base + r * stride + elem[j], lds + (wave * G::LOADS + j) * 1024);
+      for (int j = 0; j < G::LOADS; ++j) {
+        asm volatile("" : "+v"(off[j]));
+        tr_copy16(p + off[j], lds + (wave * G::LOADS + j) * 1024);
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < G::LOADS; ++j) {
+        const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
+        tr_copy16(base + min(row0 + row, len - 1) * stride + tr_swz<D>(row, L % G::KCH) * 8, lds + (wave * G::LOADS + j) * 1024);
+      }
     }
   }
 };
 
 // Byte offsets of a lane's operands in a tile.  Row operands: row l % 32 (a block of 32 rows adds 32 * ROWB), chunk 2 i + half.
 // Transposed operands: rows 16 s + 8 e + 4 half + (l % 16) / 4, channels 32 db + 16 ((l / 16) % 2) + 4 (l % 4) ..; s adds
-// 16 * ROWB.
+// 16 * ROWB.  The swizzle is an exclusive or, so the operands of i and of db follow from the first one's offset by one (head dim
+// 96, whose swizzle leaves the chunk's upper bits alone, by an addition where those are concerned).
 template <int D> struct TrAddr {
   using G = TrGeo<D>;
-  int row[G::NK], col[G::NDB][2];
-  __device__ __forceinline__ void init_rows(int lane) {
-    const int ln = lane & 31, hf = lane >> 5;
+  int row, col[2];
+  __device__ __forceinline__ void init(int lane) {
+    const int ln = lane & 31, hf = lane >> 5, r = (lane & 15) >> 2, c = lane & 3, g = (lane >> 4) & 1;
+    row = ln * G::ROWB + tr_swz<D>(ln, hf) * 16;
 #pragma unroll
-    for (int i = 0; i < G::NK; ++i) row[i] = ln * G::ROWB + tr_swz<D>(ln, 2 * i + hf) * 16;
-  }
-  __device__ __forceinline__ void init_cols(int lane) {
-    const int hf = lane >> 5, r = (lane & 15) >> 2, c = lane & 3, g = (lane >> 4) & 1;
-#pragma unroll
-    for (int db = 0; db < G::NDB; ++db)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int rw = 8 * e + 4 * hf + r;
-        col[db][e] = rw * G::ROWB + tr_swz<D>(rw, 4 * db + 2 * g + (c >> 1)) * 16 + (c & 1) * 8;
-      }
+    for (int e = 0; e < 2; ++e) {
+      const int rw = 8 * e + 4 * hf + r;
+      col[e] = rw * G::ROWB + tr_swz<D>(rw, 2 * g + (c >> 1)) * 16 + (c & 1) * 8;
+    }
   }
   __device__ __forceinline__ v4i rows(const uint8_t* lds, int blk, int i) const {
-    return *reinterpret_cast<const v4i*>(lds + row[i] + blk * 32 * G::ROWB);
+    const int at = D == 96 ? (row ^ ((i & 1) * 32)) + (i >> 1) * 64 : row ^ (32 * i);
+    return *reinterpret_cast<const v4i*>(lds + at + blk * 32 * G::ROWB);
   }
   __device__ __forceinline__ v4i cols(const uint8_t* lds, int s, int db) const {
     v4i r;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(lds + col[db][e] + s * 16 * G::ROWB));
+      const int at = D == 96 ? col[e] + 64 * db : col[e] ^ (64 * db);
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at + s * 16 * G::ROWB));
       const v2i y = __builtin_bit_cast(v2i, x);
       r[2 * e] = y[0];
       r[2 * e + 1] = y[1];

@@ -4,6 +4,8 @@
 // (dq), one owns keys and streams queries (dk, dv).  That is seven products for the five of the formulas, and it needs neither
 // atomics nor partial results in memory: every gradient is one sum in a fixed order, so equal inputs give equal bits.  A single
 // kernel would have to add dq over its workgroups: 4 bytes written and read for every 2 * 128 keys' products of a channel.
+#include <type_traits>
+
 #include "sage_train.h"
 
 namespace sage {
@@ -148,11 +150,11 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
   nl += (float)ex;
 
-  TrLoader<D> ld;
-  ld.init(wave, lane);
+  TrLoader<D> lk, lv;
+  lk.init(a.ks, wave, lane);
+  lv.init(a.vs, wave, lane);
   TrAddr<D> at;
-  at.init_rows(lane);
-  at.init_cols(lane);
+  at.init(lane);
 
   int kv_end = s.k_len;
   if (a.causal) kv_end = min(kv_end, min(s.c0 + TR_COLS, s.q_len) + off);
@@ -164,6 +166,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
     t_end = min(t_end, (max(0, min(w0 + 31, s.q_len - 1) + off + 1) + TR_ROWS - 1) / TR_ROWS);
   }
   if (w0 >= s.q_len) t_end = 0;
+  t_mask = min(t_mask, t_end);
   const uint32_t* bits = nullptr;
   if (EX && a.bits) {
     bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
@@ -179,10 +182,11 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   float flo = 0.0f, fhi = 0.0f, plo = 0.0f, phi = 0.0f, fnear = 0.0f;
 
   auto issue = [&](int t) {
-    ld.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave);
-    ld.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave);
+    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave, lane);
+    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave, lane);
   };
-  auto tile = [&](int t, bool masked) {
+  auto tile = [&](int t, auto masked_) {
+    constexpr bool masked = decltype(masked_)::value;
     const uint8_t* kt = smem[t & 1][0];
     const uint8_t* vt = smem[t & 1][1];
 #pragma unroll
@@ -275,24 +279,29 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
       for (int x = lane; x < R; x += 64) mine[x] = 0.0f;
     }
     if (ntiles > 0) issue(0);
-    for (int t = 0; t < ntiles; ++t) {
+    int t = 0;
+    auto next = [&]() {   // tile t has arrived, the one before is read: the one after goes there
       wait_vmcnt<0>();
       tile_barrier();
       if (t + 1 < ntiles) issue(t + 1);
+    };
+    for (; t < t_mask; ++t) {
+      next();
+      tile(t, std::false_type{});
+    }
+    for (; t < ntiles; ++t) {
+      next();
       if (pass) {
         tr_clean<D, DT>(smem[t & 1][0], nullptr, tid);
         tr_clean<D, DT>(smem[t & 1][1], nullptr, tid);
         __syncthreads();
-        if (t < t_end) tile(t, true);
-        __syncthreads();
-      } else if (t < t_mask) {
-        tile(t, false);
-      } else if (t < t_end) {
-        tile(t, true);
       }
+      if (t < t_end) tile(t, std::true_type{});
+      if (pass) __syncthreads();
     }
     const bool bad = !(tr_nonfinite(dq) == 0.0f);
     if (!__syncthreads_or(on && bad)) break;
+    t_mask = 0;   // every tile cleaned, hidden keys taken out
   }
 
   const float f = __builtin_ldexpf(a.scale, -ex);
@@ -330,7 +339,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
 // ---- dk, dv --------------------------------------------------------------------------------------------------------------------
 
 template <int D, int DT, bool EX>
-__global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainArgs a) {
+__global__ __launch_bounds__(TR_THREADS, D >= 128 ? 1 : 2) void train_dkv(TrainArgs a) {
   using G = TrGeo<D>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
   __shared__ __attribute__((aligned(256))) float stat[2][2][TR_ROWS];
@@ -359,11 +368,11 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainA
   const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
   const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
 
-  TrLoader<D> ld;
-  ld.init(wave, lane);
+  TrLoader<D> lq, lg;
+  lq.init(a.qs, wave, lane);
+  lg.init(a.gs, wave, lane);
   TrAddr<D> at;
-  at.init_rows(lane);
-  at.init_cols(lane);
+  at.init(lane);
 
   const int t_all = (s.q_len + TR_ROWS - 1) / TR_ROWS;
   int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
@@ -376,16 +385,17 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainA
     t_first = max(0, w0 - off) / TR_ROWS;
     t_full = (max(0, w0 + 31 - off) + TR_ROWS - 1) / TR_ROWS;
   }
-  if (w0 >= s.k_len) t_first = t_all;
+  if (w0 >= s.k_len) t_first = t_full = t_all;
   if (EX && a.bits) t_full = t_all;
+  t_full = min(max(t_full, t0), t_all);
 
   int h = s.h * group, t = t0;                    // of the step that runs
   int hn = h, tn = t0;                            // of the step that is loaded
   auto issue = [&](int u) {
     const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + hn * a.qh;
     const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + hn * a.gh;
-    ld.issue(qp, a.qs, tn * TR_ROWS, s.q_len, smem[u & 1][0], wave);
-    ld.issue(gp, a.gs, tn * TR_ROWS, s.q_len, smem[u & 1][1], wave);
+    lq.issue(qp, a.qs, tn * TR_ROWS, s.q_len, smem[u & 1][0], wave, lane);
+    lg.issue(gp, a.gs, tn * TR_ROWS, s.q_len, smem[u & 1][1], wave, lane);
     const int64_t r = tr_stat_row(a, s, hn) + tn * TR_ROWS + lane;
     if (wave == 0) tr_copy4(a.nl + r, stat[u & 1][0]);
     if (wave == 1) tr_copy4(a.nd + r, stat[u & 1][1]);
@@ -393,7 +403,8 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainA
   };
 
   v16f dk[G::NDB], dv[G::NDB];
-  auto tile = [&](int u, bool masked) {
+  auto tile = [&](int u, auto masked_) {
+    constexpr bool masked = decltype(masked_)::value;
     const uint8_t* qt = smem[u & 1][0];
     const uint8_t* gt = smem[u & 1][1];
 #pragma unroll
@@ -475,31 +486,38 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dkv(TrainA
       for (int v = 0; v < 16; ++v) dk[db][v] = 0.0f, dv[db][v] = 0.0f;
     h = hn = s.h * group, t = tn = t0;
     if (steps > 0) issue(0);
-    int bias_head = -1;
-    for (int u = 0; u < steps; ++u) {
+    int u = 0;
+    auto next = [&]() {   // step u has arrived, the one before is read: the one after goes there
       wait_vmcnt<0>();
       tile_barrier();
       if (u + 1 < steps) issue(u + 1);
-      if (EX && a.bias && bias_head != h) {
-        bias_head = h;
+    };
+    for (int g = 0; g < group; ++g, ++h) {
+      if (EX && a.bias) {
+        __syncthreads();
         for (int x = tid; x <= 2 * a.reach; x += TR_THREADS) bl[x] = a.bias[(int64_t)h * (2 * a.reach + 1) + x];
         __syncthreads();
       }
-      if (pass) {
-        tr_clean<D, DT>(smem[u & 1][0], nullptr, tid);
-        tr_clean<D, DT>(smem[u & 1][1], nullptr, tid);
-        __syncthreads();
-        if (t >= t_first) tile(u, true);
-        __syncthreads();
-      } else if (t >= t_full) {
-        if (t >= t_first) tile(u, false);
-      } else if (t >= t_first) {
-        tile(u, true);
+      // first the tiles that hide keys of the wave, then, in a loop of their own, those that do not
+      t = t0;
+      for (; t < t_full; ++t, ++u) {
+        next();
+        if (pass) {
+          tr_clean<D, DT>(smem[u & 1][0], nullptr, tid);
+          tr_clean<D, DT>(smem[u & 1][1], nullptr, tid);
+          __syncthreads();
+        }
+        if (t >= t_first) tile(u, std::true_type{});
+        if (pass) __syncthreads();
       }
-      if (++t == t_all) t = t0, ++h;
+      for (; t < t_all; ++t, ++u) {
+        next();
+        tile(u, std::false_type{});
+      }
     }
     const bool bad = !(tr_nonfinite(dk) + tr_nonfinite(dv) == 0.0f);
     if (!__syncthreads_or(on && bad)) break;
+    t_full = t_all;   // every tile cleaned, hidden keys taken out
   }
 
   const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;

@@ -1,4 +1,6 @@
 // Forward pass of the attention for training: see sage_train.h for the form.
+#include <type_traits>
+
 #include "sage_train.h"
 
 namespace sage {
@@ -34,11 +36,11 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
 #pragma unroll
     for (int x = 0; x < G::NK; ++x) qf[x] = *reinterpret_cast<const v4i*>(p + 16 * x);
   }
-  TrLoader<D> ld;
-  ld.init(wave, lane);
+  TrLoader<D> lk, lv;
+  lk.init(a.ks, wave, lane);
+  lv.init(a.vs, wave, lane);
   TrAddr<D> at;
-  at.init_rows(lane);
-  at.init_cols(lane);
+  at.init(lane);
 
   int kv_end = s.k_len;
   if (a.causal) kv_end = min(kv_end, min(s.c0 + TR_COLS, s.q_len) + off);
@@ -51,6 +53,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     t_end = min(t_end, (max(0, min(w0 + 31, s.q_len - 1) + off + 1) + TR_ROWS - 1) / TR_ROWS);
   }
   if (w0 >= s.q_len) t_end = 0;
+  t_mask = min(t_mask, t_end);
   const uint32_t* bits = nullptr;
   if (EX && a.bits) {
     bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
@@ -63,11 +66,12 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   float m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
   v16f o[G::NDB];
   auto issue = [&](int t) {
-    ld.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave);
-    ld.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave);
+    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave, lane);
+    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave, lane);
   };
 
-  auto tile = [&](int t, bool masked, bool slow) {
+  auto tile = [&](int t, auto masked_, bool slow) {
+    constexpr bool masked = decltype(masked_)::value;
     const uint8_t* kt = smem[t & 1][0];
     const uint8_t* vt = smem[t & 1][1];
     v16f x[2] = {};
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
           for (int v = 0; v < 16; ++v) x[kb][v] = __builtin_fmaf(x[kb][v], a.c, far);
       }
     }
-    if (slow) {
+    if (masked && slow) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -156,26 +160,32 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[db][v] = 0.0f;
     if (ntiles > 0) issue(0);
-    for (int t = 0; t < ntiles; ++t) {
+    int t = 0;
+    auto next = [&]() {   // tile t has arrived, the one before is read: the one after goes there
       wait_vmcnt<0>();
       tile_barrier();
       if (t + 1 < ntiles) issue(t + 1);
+    };
+    // the tiles without hidden keys for the wave, in a loop of their own
+    for (; t < t_mask; ++t) {
+      next();
+      tile(t, std::false_type{}, false);
+    }
+    for (; t < ntiles; ++t) {
+      next();
       if (pass) {
         if (tid < TR_ROWS) poison[tid] = 0;
         __syncthreads();
         tr_clean<D, DT>(smem[t & 1][0], poison, tid);
         tr_clean<D, DT>(smem[t & 1][1], poison, tid);
         __syncthreads();
-        if (t < t_end) tile(t, true, true);
-        __syncthreads();
-      } else if (t < t_mask) {
-        tile(t, false, false);
-      } else if (t < t_end) {
-        tile(t, true, false);
       }
+      if (t < t_end) tile(t, std::true_type{}, pass != 0);
+      if (pass) __syncthreads();
     }
     const bool bad = !(tr_nonfinite(o) == 0.0f);
     if (!__syncthreads_or(on && bad)) break;
+    t_mask = 0;   // every tile cleaned, hidden keys taken out
   }
 
   l = add_xor32_f32(l);
