@@ -16,6 +16,9 @@
 // channel i's four rows.  No score goes through LDS and nothing is transposed in memory.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "sage_bias.h"
 #include "sage_common.h"
 #include "sage_host.h"
@@ -45,7 +48,7 @@ struct TrainArgs {
   int causal;                      // bottom-right: query i of a sequence sees keys j <= i + (kv_len - q_len)
   float scale, c;                  // sm_scale, sm_scale * log2(e)
   float* lse;                      // fp32 [B, H, Sq] (packed [H, Sq]), natural log
-  // backward: -lse * log2(e) and -D of every row, -inf and 0 in the padding: rows of `pad` entries per (b, h) (packed: per
+  // backward: -lse / sm_scale and -D of every row, where the sums of the scores and of dout . v begin; -inf and 0 in the padding: rows of `pad` entries per (b, h) (packed: per
   // h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
   float *nl, *nd;
   int64_t pad;
@@ -63,10 +66,17 @@ struct TrainArgs {
   int64_t parts;
 };
 
-template <int D> struct TrGeo {
+// f(0), f(1), .. f(N - 1) with constants for arguments
+template <class F, int... I> __device__ __forceinline__ void tr_unrolled(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F> __device__ __forceinline__ void tr_unroll(F&& f) { tr_unrolled(f, std::make_integer_sequence<int, N>{}); }
+
+template <int D, int ROWS_ = TR_ROWS> struct TrGeo {
+  static constexpr int ROWS = ROWS_;                    // rows per tile
   static constexpr int ROWB = 2 * D;                    // bytes per LDS row
   static constexpr int KCH = D / 8;                     // 16-byte chunks per row
-  static constexpr int TILE = TR_ROWS * ROWB;           // bytes per tile
+  static constexpr int TILE = ROWS * ROWB;              // bytes per tile
   static constexpr int LOADS = TILE / 1024 / 4;         // 1 KiB direct loads per wave and tile
   static constexpr int NK = D / 16;                     // products over the channels per 32 x 32 block
   static constexpr int NDB = D / 32;                    // 32-channel blocks
@@ -93,38 +103,55 @@ template <int DT> __device__ __forceinline__ int tr_pack(float a, float b) {
   else return __builtin_bit_cast(int, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 
-__device__ __forceinline__ void tr_copy16(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// Direct loads from memory to LDS: lane l's 16 (4) bytes go to lds + 16 l (4 l).  As assembly, which has no result register: behind
+// the builtin the compiler, which cannot tell tiles apart, waits for every load in flight before each transposed LDS read (dk and dv
+// at 1 x 24 x 4608 x 128: 636 us with such waits).  The kernels wait for their tiles themselves, by vmcnt; a wait that the
+// compiler places for a load of its own counts these too, and so waits for more than it needs, never less.
+__device__ __forceinline__ uint32_t tr_lds(const void* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
 }
-__device__ __forceinline__ void tr_copy4(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+__device__ __forceinline__ void tr_copy16(const void* g, const void* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(tr_lds(lds)), "v"(g) : "memory", "m0");
+}
+__device__ __forceinline__ void tr_copy16(const void* base, uint32_t off, const void* lds) {   // base: the same in every lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(tr_lds(lds)), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void tr_copy4(const void* g, const void* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(tr_lds(lds)), "v"(g) : "memory", "m0");
 }
 
-// A workgroup's loads of 64-row tiles of one tensor: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.  Whole
-// tiles: the tile's address in scalar registers and a lane's 32-bit offset.
-template <int D> struct TrLoader {
-  using G = TrGeo<D>;
-  uint32_t off[G::LOADS];
-  bool fits;              // 64 rows' offsets pass 32 bits otherwise
+// A workgroup's loads of tiles of one tensor: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.  Whole
+// tiles: the address of the load's first row in scalar registers and a lane's 32-bit offset, which follows from load 0's: the
+// rows of a load are as many for each, and the swizzle of a sum of row numbers without carries is the sums' exclusive or.  (Head
+// dim 96, with 5 1/3 rows a load, keeps its three offsets.)
+template <int D, int ROWS = TR_ROWS> struct TrLoader {
+  using G = TrGeo<D, ROWS>;
+  static constexpr int N = D == 96 ? G::LOADS : 1;
+  uint32_t off[N], chunk;  // bytes: of load 0's row and, apart from it, of its chunk
+  bool fits;               // 64 rows' offsets pass 32 bits otherwise
   __device__ __forceinline__ void init(int64_t stride, int wave, int lane) {
     fits = stride >= 0 && stride < (1 << 24);
 #pragma unroll
-    for (int j = 0; j < G::LOADS; ++j) {
-      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
-      off[j] = (uint32_t)((row * stride + tr_swz<D>(row, L % G::KCH) * 8) * 2);
+    for (int j = 0; j < N; ++j) {
+      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH, c = tr_swz<D>(row, L % G::KCH);
+      off[j] = (uint32_t)((row * stride + (D == 96 ? c * 8 : 0)) * 2);
+      chunk = c * 16;
     }
   }
-  // rows row0 .. row0 + 63 of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
+  // rows row0 .. of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
   __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave, int lane) {
-    if (row0 + TR_ROWS <= len && fits) {
+    if (row0 + ROWS <= len && fits) {
       const uint8_t* p = reinterpret_cast<const uint8_t*>(base + row0 * stride);
       asm volatile("" : "+s"(p));
 #pragma unroll
       for (int j = 0; j < G::LOADS; ++j) {
-        asm volatile("" : "+v"(off[j]));
-        tr_copy16(p + off[j], lds + (wave * G::LOADS + j) * 1024);
+        if constexpr (D == 96) {
+          tr_copy16(p, off[j], lds + (wave * G::LOADS + j) * 1024);
+        } else {
+          constexpr int RPL = 64 / G::KCH;   // rows per load
+          uint32_t x = off[0] + (chunk ^ (uint32_t)(tr_swz<D>(RPL * j, 0) * 16));
+          tr_copy16(p + j * RPL * stride * 2, x, lds + (wave * G::LOADS + j) * 1024);
+        }
       }
     } else {
 #pragma unroll 1
@@ -152,16 +179,25 @@ template <int D> struct TrAddr {
       col[e] = rw * G::ROWB + tr_swz<D>(rw, 2 * g + (c >> 1)) * 16 + (c & 1) * 8;
     }
   }
-  __device__ __forceinline__ v4i rows(const uint8_t* lds, int blk, int i) const {
-    const int at = D == 96 ? (row ^ ((i & 1) * 32)) + (i >> 1) * 64 : row ^ (32 * i);
-    return *reinterpret_cast<const v4i*>(lds + at + blk * 32 * G::ROWB);
+  // the same in the tile at `lds` (a multiple of 1 KiB, above every bit that the swizzles touch)
+  __device__ __forceinline__ TrAddr in(const uint8_t* lds) const {
+    const int base = (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)lds;
+    TrAddr r;
+    r.row = row + base;
+    r.col[0] = col[0] + base;
+    r.col[1] = col[1] + base;
+    return r;
   }
-  __device__ __forceinline__ v4i cols(const uint8_t* lds, int s, int db) const {
+  __device__ __forceinline__ v4i rows(int blk, int i) const {
+    const int at = D == 96 ? (row ^ ((i & 1) * 32)) + (i >> 1) * 64 : row ^ (32 * i);
+    return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(uint32_t)(at + blk * 32 * G::ROWB);
+  }
+  __device__ __forceinline__ v4i cols(int s, int db) const {
     v4i r;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int at = D == 96 ? col[e] + 64 * db : col[e] ^ (64 * db);
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at + s * 16 * G::ROWB));
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(uint32_t)(at + s * 16 * G::ROWB));
       const v2i y = __builtin_bit_cast(v2i, x);
       r[2 * e] = y[0];
       r[2 * e + 1] = y[1];
@@ -169,6 +205,13 @@ template <int D> struct TrAddr {
     return r;
   }
 };
+
+// The operands that a wave keeps have arrived from here on (so that no wait for them lands in a loop, where it would be one for the
+// tiles on their way)
+template <int N> __device__ __forceinline__ void tr_arrived(v4i (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
 
 // Channels 32 db .. of column l % 32, held as acc registers (row 8 (v / 4) + 4 half + v % 4 = channel), times f, to 16 bits at p:
 // one exchange between the halves makes 16-byte stores.
@@ -270,10 +313,10 @@ template <int N> __device__ __forceinline__ float tr_nonfinite(const v16f (&a)[N
 // The infinities and NaN of a tile become 0; poison[r] is set where row r had one.  A hidden pair has weight 0, but 0 times an
 // infinity is NaN: results that come out non-finite are computed a second time from tiles cleaned like this, in which the rows
 // that see a poisoned one get NaN by their scores.  Two barriers are the caller's.
-template <int D, int DT> __device__ __forceinline__ void tr_clean(uint8_t* tile, int* poison, int tid) {
-  using G = TrGeo<D>;
+template <int D, int DT, int ROWS = TR_ROWS, int THREADS = TR_THREADS> __device__ __forceinline__ void tr_clean(uint8_t* tile, int* poison, int tid) {
+  using G = TrGeo<D, ROWS>;
   constexpr uint32_t E = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
-  for (int i = tid; i < G::TILE / 16; i += TR_THREADS) {
+  for (int i = tid; i < G::TILE / 16; i += THREADS) {
     v4i* p = reinterpret_cast<v4i*>(tile) + i;
     v4i w = *p;
     bool bad = false;

@@ -1,6 +1,4 @@
 // Forward pass of the attention for training: see sage_train.h for the form.
-#include <type_traits>
-
 #include "sage_train.h"
 
 namespace sage {
@@ -72,13 +70,12 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
 
   auto tile = [&](int t, auto masked_, bool slow) {
     constexpr bool masked = decltype(masked_)::value;
-    const uint8_t* kt = smem[t & 1][0];
-    const uint8_t* vt = smem[t & 1][1];
+    const TrAddr<D> kt = at.in(smem[t & 1][0]), vt = at.in(smem[t & 1][1]);
     v16f x[2] = {};
 #pragma unroll
     for (int kk = 0; kk < G::NK; ++kk) {
-      x[0] = tr_mfma<DT>(at.rows(kt, 0, kk), qf[kk], x[0]);
-      x[1] = tr_mfma<DT>(at.rows(kt, 1, kk), qf[kk], x[1]);
+      x[0] = tr_mfma<DT>(kt.rows(0, kk), qf[kk], x[0]);
+      x[1] = tr_mfma<DT>(kt.rows(1, kk), qf[kk], x[1]);
     }
     if (EX) {
       // scores in the log2 domain, with the bias
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int db = 0; db < G::NDB; ++db) o[db] = tr_mfma<DT>(at.cols(vt, st, db), p[st], o[db]);
+      for (int db = 0; db < G::NDB; ++db) o[db] = tr_mfma<DT>(vt.cols(st, db), p[st], o[db]);
   };
 
   for (int pass = 0; pass < 2; ++pass) {
