@@ -29,7 +29,7 @@ MANIFEST = PKG / "manifest.json"
 ARCH = "gfx950"
 SOURCES = ("sage_capi.hip", "sage_quant.hip", "sage_attn.hip", "sage_lse.hip", "sage_varlen.hip", "sage_mask.hip",
            "sage_rope.hip", "sage_cache.hip", "sage_cache_attn.hip", "sage_bias.hip", "sage_train.hip", "sage_train_fwd.hip",
-           "sage_train_bwd.hip")
+           "sage_train_bwd.hip", "sage_train_dkv.hip")
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -43,6 +43,8 @@ HIP_FLAGS = [
     # no packed-fp32 instructions anywhere in the device code
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+# of single sources: results of matrix products in ordinary registers where they are read again
+SOURCE_FLAGS = {"sage_train_dkv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def hipcc() -> str:
@@ -72,7 +74,8 @@ def build(verbose: bool = False) -> Path:
         outs = [str(Path(objects) / (s + ".o")) for s in SOURCES]
         compile_flags = [f for f in HIP_FLAGS if f != "-shared"]
         with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-            list(pool.map(lambda so: run([hipcc(), *compile_flags, f"-I{INCLUDE}", "-c", "-o", so[1], str(CSRC / so[0])]),
+            list(pool.map(lambda so: run([hipcc(), *compile_flags, *SOURCE_FLAGS.get(so[0], ()),
+                                          f"-I{INCLUDE}", "-c", "-o", so[1], str(CSRC / so[0])]),
                           zip(SOURCES, outs)))
         run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", str(tmp), *outs])
     os.replace(tmp, LIB)

@@ -121,45 +121,34 @@ __device__ __forceinline__ void tr_copy4(const void* g, const void* lds) {
 }
 
 // A workgroup's loads of tiles of one tensor: load j of wave w fills chunks (w * LOADS + j) * 64 + lane of the tile.  Whole
-// tiles: the address of the load's first row in scalar registers and a lane's 32-bit offset, which follows from load 0's: the
-// rows of a load are as many for each, and the swizzle of a sum of row numbers without carries is the sums' exclusive or.  (Head
-// dim 96, with 5 1/3 rows a load, keeps its three offsets.)
+// tiles: the tile's address in scalar registers and a lane's 32-bit offsets.
 template <int D, int ROWS = TR_ROWS> struct TrLoader {
   using G = TrGeo<D, ROWS>;
-  static constexpr int N = D == 96 ? G::LOADS : 1;
-  uint32_t off[N], chunk;  // bytes: of load 0's row and, apart from it, of its chunk
-  bool fits;               // 64 rows' offsets pass 32 bits otherwise
+  uint32_t off[G::LOADS];
+  bool fits;               // a tile's offsets pass 32 bits otherwise
   __device__ __forceinline__ void init(int64_t stride, int wave, int lane) {
     fits = stride >= 0 && stride < (1 << 24);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH, c = tr_swz<D>(row, L % G::KCH);
-      off[j] = (uint32_t)((row * stride + (D == 96 ? c * 8 : 0)) * 2);
-      chunk = c * 16;
+    for (int j = 0; j < G::LOADS; ++j) {
+      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
+      off[j] = (uint32_t)((row * stride + tr_swz<D>(row, L % G::KCH) * 8) * 2);
     }
   }
-  // rows row0 .. of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
-  __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave, int lane) {
-    if (row0 + ROWS <= len && fits) {
-      const uint8_t* p = reinterpret_cast<const uint8_t*>(base + row0 * stride);
-      asm volatile("" : "+s"(p));
+  __device__ __forceinline__ void whole(const void* tile, uint8_t* lds, int wave) const {
 #pragma unroll
-      for (int j = 0; j < G::LOADS; ++j) {
-        if constexpr (D == 96) {
-          tr_copy16(p, off[j], lds + (wave * G::LOADS + j) * 1024);
-        } else {
-          constexpr int RPL = 64 / G::KCH;   // rows per load
-          uint32_t x = off[0] + (chunk ^ (uint32_t)(tr_swz<D>(RPL * j, 0) * 16));
-          tr_copy16(p + j * RPL * stride * 2, x, lds + (wave * G::LOADS + j) * 1024);
-        }
-      }
-    } else {
+    for (int j = 0; j < G::LOADS; ++j) tr_copy16(tile, off[j], lds + (wave * G::LOADS + j) * 1024);
+  }
+  // rows row0 .. of a sequence of `len` (>= 1) rows; rows behind it repeat its last one
+  __device__ __forceinline__ void part(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave, int lane) const {
 #pragma unroll 1
-      for (int j = 0; j < G::LOADS; ++j) {
-        const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
-        tr_copy16(base + min(row0 + row, len - 1) * stride + tr_swz<D>(row, L % G::KCH) * 8, lds + (wave * G::LOADS + j) * 1024);
-      }
+    for (int j = 0; j < G::LOADS; ++j) {
+      const int L = (wave * G::LOADS + j) * 64 + lane, row = L / G::KCH;
+      tr_copy16(base + min(row0 + row, len - 1) * stride + tr_swz<D>(row, L % G::KCH) * 8, lds + (wave * G::LOADS + j) * 1024);
     }
+  }
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t stride, int row0, int len, uint8_t* lds, int wave, int lane) const {
+    if (row0 + ROWS <= len && fits) whole(base + row0 * stride, lds, wave);
+    else part(base, stride, row0, len, lds, wave, lane);
   }
 };
 
@@ -188,16 +177,17 @@ template <int D> struct TrAddr {
     r.col[1] = col[1] + base;
     return r;
   }
-  __device__ __forceinline__ v4i rows(int blk, int i) const {
+  // (more: bytes to another tile)
+  __device__ __forceinline__ v4i rows(int blk, int i, int more = 0) const {
     const int at = D == 96 ? (row ^ ((i & 1) * 32)) + (i >> 1) * 64 : row ^ (32 * i);
-    return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(uint32_t)(at + blk * 32 * G::ROWB);
+    return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(uint32_t)(at + blk * 32 * G::ROWB + more);
   }
-  __device__ __forceinline__ v4i cols(int s, int db) const {
+  __device__ __forceinline__ v4i cols(int s, int db, int more = 0) const {
     v4i r;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int at = D == 96 ? col[e] + 64 * db : col[e] ^ (64 * db);
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(uint32_t)(at + s * 16 * G::ROWB));
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(uint32_t)(at + s * 16 * G::ROWB + more));
       const v2i y = __builtin_bit_cast(v2i, x);
       r[2 * e] = y[0];
       r[2 * e + 1] = y[1];
@@ -334,7 +324,20 @@ template <int D, int DT, int ROWS = TR_ROWS, int THREADS = TR_THREADS> __device_
   }
 }
 
+// fp16 holds ds only in a window of 2^30.  |do_i . v_j - D_i| <= 2 max |do| max |v|, so ds times this power of two stays below
+// 2^15, and full precision reaches down to 2^-29 of the bound.  (bf16 has float32's exponents: 0.)
+__device__ __forceinline__ int tr_exponent(const uint32_t* norms) {
+  const float n = __uint_as_float(norms[0]) * __uint_as_float(norms[1]);   // the squared bound / 4
+  if (!(n > 0.0f && n < INFINITY)) return 0;
+  int e;
+  (void)frexpf(n, &e);                       // n < 2^e, so the bound is below 2^(e / 2 + 1)
+  return min(max(13 - ((e + 1) >> 1), -100), 100);
+}
+// P is at most 1 and is taken times 2^15 in fp16 where it is an operand
+template <int DT> constexpr float BWD_SHIFT = DT == DT_F16 ? 15.0f : 0.0f;
+
 template <int D, int DT> int train_fwd_launch(const TrainArgs& a, hipStream_t st);
 template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap& m, hipStream_t st);
+template <int D, int DT> int train_dkv_launch(const TrainArgs& a, hipStream_t st);
 
 }  // namespace sage

@@ -8,18 +8,6 @@
 
 namespace sage {
 
-// fp16 holds ds only in a window of 2^30.  |do_i . v_j - D_i| <= 2 max |do| max |v|, so ds times this power of two stays below
-// 2^15, and full precision reaches down to 2^-29 of the bound.  (bf16 has float32's exponents: 0.)
-__device__ __forceinline__ int tr_exponent(const uint32_t* norms) {
-  const float n = __uint_as_float(norms[0]) * __uint_as_float(norms[1]);   // the squared bound / 4
-  if (!(n > 0.0f && n < INFINITY)) return 0;
-  int e;
-  (void)frexpf(n, &e);                       // n < 2^e, so the bound is below 2^(e / 2 + 1)
-  return min(max(13 - ((e + 1) >> 1), -100), 100);
-}
-// P is at most 1 and is taken times 2^15 in fp16 where it is an operand
-template <int DT> constexpr float BWD_SHIFT = DT == DT_F16 ? 15.0f : 0.0f;
-
 // ---- preparation: -lse / sm_scale and -D of every row; the norms of fp16 inputs -----------------------------------------------
 
 template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_prep(TrainArgs a, int row_blocks, int norm_blocks) {
@@ -93,8 +81,16 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
     }
   }
   if (DT == DT_F16) {
+    // (a maximum does not depend on the order; few workgroups are the first to see a larger one)
+    __shared__ float tops[TR_THREADS / 64];
     top = wave_max_pos(top);
-    if ((tid & 63) == 0 && top > 0.0f) atomicMax(a.norms + ((int)blockIdx.x >= row_blocks ? 1 : 0), __float_as_uint(top));
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t* norm = a.norms + ((int)blockIdx.x >= row_blocks ? 1 : 0);
+      const uint32_t m = __float_as_uint(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+      if (m > __atomic_load_n(norm, __ATOMIC_RELAXED)) atomicMax(norm, m);
+    }
   }
 }
 
@@ -335,513 +331,6 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   }
 }
 
-// ---- dk, dv --------------------------------------------------------------------------------------------------------------------
-//
-// A wave's keys and values (D / 2 registers) and the sums of its dk and dv (2 D) leave room for one wave per SIMD, so a wave has to
-// keep the matrix unit busy by itself: a tile is a stream of products in an order of its own, the operands of product n + AHEAD read
-// from LDS when product n is issued, into the next tile too, and the weights of one block of 32 queries made beside the products
-// of the other.  (Two waves per SIMD with half of the registers each, four operands ahead: 625 us at 1 x 24 x 4608 x 128.)
-template <int D> struct DkvGeo {
-  static constexpr int ROWS = 64;                  // queries per tile
-  static constexpr int SLOTS = 3;                  // tiles in LDS: one at work, one arrived, one on its way
-  static constexpr int AHEAD = D == 64 ? 4 : 8;    // products between an operand's read and its use
-  static constexpr int OCC = D == 64 ? 2 : 1;      // waves per SIMD
-};
-
-template <int D, int DT, bool EX>
-__global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArgs a) {
-  using P = DkvGeo<D>;
-  using G = TrGeo<D, P::ROWS>;
-  constexpr int ROWS = P::ROWS;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[P::SLOTS][2][G::TILE];
-  __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
-  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
-
-  TrSeq s;
-  if (!tr_tile<true>(a, blockIdx.x, s)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ln = lane & 31, hf = lane >> 5;
-  const int group = a.H / a.Hkv;
-  const int off = s.k_len - s.q_len;
-  const int w0 = s.c0 + wave * 32, j = w0 + ln;   // the wave's first key, the lane's
-  const bool on = j < s.k_len;
-  const int jr = on ? j : s.k_len - 1;
-
-  TrAddr<D> at;
-  at.init(lane);
-  v4i kf[G::NK], vf[G::NK];
-  {
-    const uint16_t* kp = a.k + (a.cu_q ? 0 : s.b * a.kb) + (s.kr + jr) * a.ks + s.h * a.kh + 8 * hf;
-    const uint16_t* vp = a.v + (a.cu_q ? 0 : s.b * a.vb) + (s.kr + jr) * a.vs + s.h * a.vh + 8 * hf;
-#pragma unroll
-    for (int x = 0; x < G::NK; ++x) {
-      kf[x] = *reinterpret_cast<const v4i*>(kp + 16 * x);
-      vf[x] = *reinterpret_cast<const v4i*>(vp + 16 * x);
-    }
-  }
-  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
-  const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
-
-  const int t_all = (s.q_len + ROWS - 1) / ROWS;
-  int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
-  if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
-  const int nt = t_all - t0;
-  const int steps = nt * group;
-  int t_full = 0;                                 // from this tile on every query sees every key of the wave
-  if (a.causal) t_full = (max(0, w0 + 31 - off) + ROWS - 1) / ROWS;
-  if (EX && a.bits) t_full = t_all;
-  t_full = min(max(t_full, t0), t_all);
-
-  // Loads, from the last tile back to the diagonal: workgroups of one head that start together stream the same tiles together.
-  TrLoader<D, ROWS> lq, lg;
-  lq.init(a.qs, wave, lane);
-  lg.init(a.gs, wave, lane);
-  const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + s.h * group * a.qh;
-  const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * group * a.gh;
-  const float* sp = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group);
-  int tn = t_all - 1, un = 0, sn = 0;             // of the tile that is loaded next: its number, the step, the slot
-  auto issue = [&]() {
-    if (un < steps) {
-      lq.issue(qp, a.qs, tn * ROWS, s.q_len, smem[sn][0], wave, lane);
-      lg.issue(gp, a.gs, tn * ROWS, s.q_len, smem[sn][1], wave, lane);
-      if (wave < 2) tr_copy4(sp + tn * ROWS + lane, stat[sn][wave]);
-      if (--tn < t0) tn = t_all - 1, qp += a.qh, gp += a.gh, sp += a.pad;
-      ++un;
-      sn = sn + 1 == P::SLOTS ? 0 : sn + 1;
-    }
-  };
-
-  v16f dk[G::NDB], dv[G::NDB], x[2], dp[2];
-  v4i ring[P::AHEAD];
-  auto begin = [&](int slot, int qb) __attribute__((always_inline)) {   // the first products' sums begin at the rows' numbers
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const v4f y = *reinterpret_cast<const v4f*>(&stat[slot][0][32 * qb + 8 * g + 4 * hf]);
-      const v4f z = *reinterpret_cast<const v4f*>(&stat[slot][1][32 * qb + 8 * g + 4 * hf]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[qb][4 * g + e] = y[e], dp[qb][4 * g + e] = z[e];
-    }
-  };
-  constexpr int N = 2 * G::NK;                     // products per quarter of a tile
-  auto operand = [&](const TrAddr<D>& qt, const TrAddr<D>& gt, auto n_) __attribute__((always_inline)) {
-    constexpr int n = decltype(n_)::value, part = n / N, y = n % N;
-    if constexpr (part < 2) return (y & 1) ? gt.rows(part, y >> 1) : qt.rows(part, y >> 1);
-    else return (y & 1) ? qt.cols(2 * (part - 2) + y / (2 * G::NDB), y % (2 * G::NDB) >> 1)
-                        : gt.cols(2 * (part - 2) + y / (2 * G::NDB), y % (2 * G::NDB) >> 1);
-  };
-  // One tile: the products of block 0's scores and weights' gradients, those of block 1's while block 0's weights are made, block
-  // 0's parts of dv and dk while block 1's weights are made, block 1's parts.
-  auto tile = [&](int slot, int next, int t, int h, auto masked_) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(masked_)::value;
-    constexpr int AHEAD = P::AHEAD;
-    const TrAddr<D> qt = at.in(smem[slot][0]), gt = at.in(smem[slot][1]);
-    const TrAddr<D> qn = at.in(smem[next][0]), gn = at.in(smem[next][1]);
-    v4i p[2][2], ds[2][2];
-    // the weights of elements v0 .. v1 (in pairs) of a block
-    auto weights = [&](int qb, int v0, int v1) __attribute__((always_inline)) {
-      const int q0 = t * ROWS + 32 * qb;
-      const int d0 = jr - off - q0 - 4 * hf;      // key - query of register 0; a row further is 1 less
-      const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
-      const bool near = EX && a.bias && !(whi <= -a.reach || wlo >= a.reach);
-      const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
-#pragma unroll
-      for (int v = v0; v < v1; ++v) {
-        float y = x[qb][v];
-        if (EX) {
-          float more = far;
-          if (near) more = bl[a.reach + min(max(d0 - 8 * (v >> 2) - (v & 3), -a.reach), a.reach)] + BWD_SHIFT<DT>;
-          y = __builtin_fmaf(y, a.c, more);
-        } else {
-          y = DT == DT_F16 ? __builtin_fmaf(y, a.c, BWD_SHIFT<DT>) : y * a.c;
-        }
-        y = __builtin_amdgcn_exp2f(y);
-        if (masked) {
-          const int r = 8 * (v >> 2) + (v & 3), room = q0 + 4 * hf - (jr - off);   // row r sees the key where r + room >= 0
-          bool hidden = a.causal && r + room < 0;
-          if (EX && a.bits && w0 < s.k_len) {
-            const uint32_t* w = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw;
-            hidden |= !((w[a.mi ? q0 + r + 4 * hf : 0] >> ln) & 1u);
-          }
-          if (hidden) y = 0.0f, dp[qb][v] = 0.0f;
-        }
-        x[qb][v] = y;
-      }
-#pragma unroll
-      for (int v = v0; v < v1; v += 2) {
-        p[qb][v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[qb][v], x[qb][v + 1]);
-        float e0 = x[qb][v] * dp[qb][v], e1 = x[qb][v + 1] * dp[qb][v + 1];
-        if (DT == DT_F16) e0 *= ds_mul, e1 *= ds_mul;
-        ds[qb][v >> 3][(v & 7) >> 1] = tr_pack<DT>(e0, e1);
-      }
-    };
-    begin(slot, 1);
-    tr_unroll<4 * N>([&](auto n_) __attribute__((always_inline)) {
-      constexpr int n = decltype(n_)::value, part = n / N, y = n % N;
-      const v4i f = ring[n % AHEAD];
-      if constexpr (part < 2) {
-        if constexpr (y & 1) dp[part] = tr_mfma<DT>(f, vf[y >> 1], dp[part]);
-        else x[part] = tr_mfma<DT>(f, kf[y >> 1], x[part]);
-      } else {
-        constexpr int st = y / (2 * G::NDB), db = y % (2 * G::NDB) >> 1;
-        if constexpr (y & 1) dk[db] = tr_mfma<DT>(f, ds[part - 2][st], dk[db]);
-        else dv[db] = tr_mfma<DT>(f, p[part - 2][st], dv[db]);
-      }
-      if constexpr (n + AHEAD < 4 * N) ring[n % AHEAD] = operand(qt, gt, std::integral_constant<int, n + AHEAD>{});
-      else ring[n % AHEAD] = operand(qn, gn, std::integral_constant<int, n + AHEAD - 4 * N>{});
-      // 8 pairs over the quarter's products but the first
-      if constexpr (part == 1 || part == 2) {
-        constexpr int e0 = y < 1 ? 0 : (y - 1) * 8 / (N - 1) * 2, e1 = y * 8 / (N - 1) * 2;
-        if constexpr (e1 > e0) weights(part - 1, e0, e1);
-      }
-      if constexpr (n == 3 * N + N / 2) begin(next, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    });
-  };
-
-  for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-    for (int db = 0; db < G::NDB; ++db)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) dk[db][v] = 0.0f, dv[db][v] = 0.0f;
-    if (pass) qp -= group * a.qh, gp -= group * a.gh, sp -= group * a.pad;   // (the loads begin anew)
-    un = sn = 0;
-    int slot = 0, u = 0;
-    // The tile after u has arrived, the one before u is read and its place free
-    auto top = [&]() __attribute__((always_inline)) {
-      wait_vmcnt<0>();
-      tile_barrier();
-      issue();
-      if (pass) {   // a tile is cleaned when it has arrived, one step before anything of it is read
-        const int c = slot + 1 == P::SLOTS ? 0 : slot + 1;
-        if (u == 0) tr_clean<D, DT, ROWS>(smem[0][0], nullptr, tid), tr_clean<D, DT, ROWS>(smem[0][1], nullptr, tid);
-        if (u + 1 < steps) tr_clean<D, DT, ROWS>(smem[c][0], nullptr, tid), tr_clean<D, DT, ROWS>(smem[c][1], nullptr, tid);
-        __syncthreads();
-      }
-    };
-    issue();
-    issue();
-    tr_arrived(kf);
-    tr_arrived(vf);
-    if (steps > 0) {
-      top();
-      begin(0, 0);
-      const TrAddr<D> qt = at.in(smem[0][0]), gt = at.in(smem[0][1]);
-      tr_unroll<P::AHEAD>([&](auto n_) __attribute__((always_inline)) { ring[decltype(n_)::value] = operand(qt, gt, n_); });
-    }
-    int h = s.h * group;
-    for (int g = 0; g < group && nt > 0; ++g, ++h) {
-      if (EX && a.bias) {
-        __syncthreads();
-        for (int y = tid; y <= 2 * a.reach; y += TR_THREADS) bl[y] = a.bias[(int64_t)h * (2 * a.reach + 1) + y];
-        __syncthreads();
-      }
-      // first the tiles that hide no keys of the wave, then, in a loop of their own, those that do
-      int t = t_all - 1;
-      auto one = [&](auto masked_) __attribute__((always_inline)) {
-        const int next = slot + 1 == P::SLOTS ? 0 : slot + 1;
-        tile(slot, next, t, h, masked_);
-        slot = next, ++u;
-        if (u < steps) top();
-      };
-      const int full = pass ? t_all : t_full;      // (a second pass takes hidden keys out of every tile)
-      for (; t >= full; --t) one(std::false_type{});
-      for (; t >= t0; --t) one(std::true_type{});
-    }
-    const bool bad = !(tr_nonfinite(dk) + tr_nonfinite(dv) == 0.0f);
-    if (!__syncthreads_or(on && bad)) break;   // (a second time with every tile cleaned)
-    tn = t_all - 1;
-  }
-
-  const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
-  uint16_t* kp = a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh;
-  uint16_t* vp = a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
-#pragma unroll
-  for (int db = 0; db < G::NDB; ++db) {
-    tr_store<DT>(dk[db], fk, kp + 32 * db, hf, on);
-    tr_store<DT>(dv[db], fv, vp + 32 * db, hf, on);
-  }
-}
-
-// Two waves share each 32 keys: the first recomputes the scores, makes the weights and sums dv, the second recomputes the gradient
-// of the weights, multiplies it by the weights, which it gets in fp32 through LDS one tile later, and sums dk.  Each has half of the
-// accumulators and half of the operands, so both fit a SIMD's registers together with operands read far ahead, and one's exponentials
-// run beside the other's products.  (One wave with everything: 695 us at 1 x 24 x 4608 x 128 with one wave per SIMD, 636 with
-// two, whose registers left four operands ahead.)
-//
-// Step u: the first waves work on tile u of 32 queries, the second ones on tile u - 1, and both read the first operands of their next
-// tile ahead; tiles u + 2 and u + 3 are on their way.  One barrier a step.  (Head dim 256, for whose tiles there is less room: the
-// next tile's operands are read after the barrier, one tile on its way.)
-template <int D> struct DkvPairGeo {
-  static constexpr int ROWS = 32;                  // queries per tile
-  static constexpr int WAVES = 8;
-  static constexpr bool CROSS = D != 256;          // reads ahead into the next tile
-  static constexpr int SLOTS = CROSS ? 5 : 3;      // tiles in LDS
-  static constexpr int AHEAD = D == 128 ? 8 : 4;   // products between an operand's read and its use
-  static constexpr int PER_WAVE = D == 64 ? 1 : D == 256 ? 4 : 2;   // 1 KiB loads of a wave per step, of q or of dout
-  static constexpr int PER_TENSOR = D * ROWS * 2 / 1024;            // (96: 6, so that the last two waves repeat some)
-  static constexpr int OCC = D == 64 ? 4 : 2;      // waves per SIMD
-};
-
-template <int D, int DT, bool EX>
-__global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainArgs a) {
-  using P = DkvPairGeo<D>;
-  using G = TrGeo<D, P::ROWS>;
-  constexpr int ROWS = P::ROWS;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[P::SLOTS][2][G::TILE];
-  __shared__ __attribute__((aligned(16))) v4f pmem[2][4][4][64];   // the weights of a tile: slot, pair of waves, quarter, lane
-  __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
-  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
-
-  TrSeq s;
-  if (!tr_tile<true>(a, blockIdx.x, s)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ln = lane & 31, hf = lane >> 5;
-  const int pair = wave & 3, second = wave >> 2;
-  const int group = a.H / a.Hkv;
-  const int off = s.k_len - s.q_len;
-  const int w0 = s.c0 + pair * 32, j = w0 + ln;   // the pair's first key, the lane's
-  const bool on = j < s.k_len;
-  const int jr = on ? j : s.k_len - 1;
-
-  TrAddr<D> at;
-  at.init(lane);
-  v4i of[G::NK];                                  // keys or values
-  {
-    const uint16_t* p = second ? a.v + (a.cu_q ? 0 : s.b * a.vb) + (s.kr + jr) * a.vs + s.h * a.vh
-                               : a.k + (a.cu_q ? 0 : s.b * a.kb) + (s.kr + jr) * a.ks + s.h * a.kh;
-#pragma unroll
-    for (int x = 0; x < G::NK; ++x) of[x] = *reinterpret_cast<const v4i*>(p + 8 * hf + 16 * x);
-  }
-  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
-  const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
-
-  const int t_all = (s.q_len + ROWS - 1) / ROWS;
-  int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
-  if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
-  const int nt = t_all - t0;
-  const int steps = nt * group;
-
-  // Loads: a wave's are all of q or all of dout.  From the last tile back to the diagonal: workgroups of one head that start
-  // together stream the same tiles together.
-  const int l0 = wave * P::PER_WAVE % (2 * P::PER_TENSOR), side = l0 / P::PER_TENSOR;
-  const int64_t ls = side ? a.gs : a.qs, lh = side ? a.gh : a.qh;
-  const uint16_t* lsrc = (side ? a.dout + (a.cu_q ? 0 : s.b * a.gb) : a.q + (a.cu_q ? 0 : s.b * a.qb)) + s.qr * ls + s.h * group * lh;
-  const float* stat_src = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group);
-  const int row_l = (l0 - side * P::PER_TENSOR) * 64 + lane;   // the lane's chunk of the wave's first load
-  const bool fits = ls >= 0 && ls < (1 << 24);
-  uint32_t loff[D == 96 ? P::PER_WAVE : 1], lchunk = 0;
-#pragma unroll
-  for (int x = 0; x < (D == 96 ? P::PER_WAVE : 1); ++x) {
-    const int L = row_l + 64 * x, row = L / G::KCH, c = tr_swz<D>(row, L % G::KCH);
-    loff[x] = (uint32_t)((row * ls + (D == 96 ? c * 8 : 0)) * 2);
-    lchunk = c * 16;
-  }
-  int tn = t_all - 1, un = 0;                     // of the step that is loaded
-  auto issue = [&]() {
-    if (un < steps) {
-      const int slot = un % P::SLOTS;
-      uint8_t* dst = &smem[slot][side][0] + (l0 - side * P::PER_TENSOR) * 1024;
-      if ((tn + 1) * ROWS <= s.q_len && fits) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(lsrc + (int64_t)(tn * ROWS) * ls);
-        asm volatile("" : "+s"(p));
-#pragma unroll
-        for (int x = 0; x < P::PER_WAVE; ++x) {
-          constexpr int RPL = 64 / G::KCH;
-          uint32_t o = D == 96 ? loff[D == 96 ? x : 0] : loff[0] + (lchunk ^ (uint32_t)(tr_swz<D>(RPL * x, 0) * 16));
-          tr_copy16(p + (D == 96 ? 0 : x * RPL * ls * 2), o, dst + x * 1024);
-        }
-      } else {
-#pragma unroll 1
-        for (int x = 0; x < P::PER_WAVE; ++x) {
-          const int L = row_l + 64 * x, row = L / G::KCH;
-          tr_copy16(lsrc + min(tn * ROWS + row, s.q_len - 1) * ls + tr_swz<D>(row, L % G::KCH) * 8, dst + x * 1024);
-        }
-      }
-      if (wave < 2 && lane < ROWS) tr_copy4(stat_src + tn * ROWS + lane, stat[slot][wave]);
-    }
-    ++un;
-    if (--tn < t0) tn = t_all - 1, lsrc += lh, stat_src += a.pad;
-  };
-
-  v16f acc[G::NDB], x;
-  v4i ring[P::AHEAD], w[2];
-  constexpr int N = G::NK;                         // products of either kind per tile
-  TrAddr<D> rt, ct;                                // operands of the tile: by rows, transposed
-  auto fetch = [&](const TrAddr<D>& r, const TrAddr<D>& c, auto n_) __attribute__((always_inline)) {
-    constexpr int n = decltype(n_)::value, z = n - N;
-    if constexpr (n < N) ring[n % P::AHEAD] = r.rows(0, n);
-    else ring[n % P::AHEAD] = c.cols(z / G::NDB, z % G::NDB);
-  };
-  auto begin = [&](const float* st) __attribute__((always_inline)) {   // the sums of the first products begin at the rows' numbers
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const v4f y = *reinterpret_cast<const v4f*>(st + 8 * g + 4 * hf);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * g + e] = y[e];
-    }
-  };
-  // The products of the tile in rt, ct: first those over the channels into x, then `middle` makes of x (elements v0 .. v1) the
-  // operand w, then those over the tile's rows into acc.
-  auto stream = [&](int next, auto middle) __attribute__((always_inline)) {
-    const TrAddr<D> rn = at.in(smem[next][second]);
-    tr_unroll<2 * N>([&](auto n_) __attribute__((always_inline)) {
-      constexpr int n = decltype(n_)::value;
-      const v4i f = ring[n % P::AHEAD];
-      if constexpr (n < N) {
-        x = tr_mfma<DT>(f, of[n], x);
-      } else {
-        constexpr int z = n - N;
-        acc[z % G::NDB] = tr_mfma<DT>(f, w[z / G::NDB], acc[z % G::NDB]);
-      }
-      if constexpr (n + P::AHEAD < 2 * N) fetch(rt, ct, std::integral_constant<int, n + P::AHEAD>{});
-      else if constexpr (P::CROSS) ring[n % P::AHEAD] = rn.rows(0, n + P::AHEAD - 2 * N);
-      if constexpr (n == N - 1) middle(0, 8);
-      if constexpr (n >= N && n < N + N / 2) {
-        constexpr int e0 = (n - N) * 4 / (N / 2) * 2, e1 = (n - N + 1) * 4 / (N / 2) * 2;
-        if constexpr (e1 > e0) middle(8 + e0, 8 + e1);
-      }
-      if constexpr (P::CROSS && n == 2 * N - 1) begin(stat[next][second]);
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    rt = rn;
-  };
-  auto enter = [&](int slot) __attribute__((always_inline)) {   // without reads ahead: before a tile
-    rt = at.in(smem[slot][second]);
-    begin(stat[slot][second]);
-    tr_unroll<P::AHEAD>([&](auto n_) __attribute__((always_inline)) { fetch(rt, ct, n_); });
-  };
-
-  for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-    for (int db = 0; db < G::NDB; ++db)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[db][v] = 0.0f;
-    // (a second pass begins its loads anew)
-    if (pass) lsrc -= group * lh, stat_src -= group * a.pad;
-    un = 0, tn = t_all - 1;
-    int u = 0, slot = 0;
-    auto next_slot = [&](int x) { return x + 1 == P::SLOTS ? 0 : x + 1; };
-    // The loads of the tile after u (without reads ahead: of u) have arrived, what step u - 1 read may be overwritten
-    auto top = [&]() __attribute__((always_inline)) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (P::CROSS && u + 2 < steps && !pass) {
-        if (wave < 2) wait_vmcnt<P::PER_WAVE + 1>();
-        else wait_vmcnt<P::PER_WAVE>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      tile_barrier();
-      issue();
-      if (pass) {   // tiles are cleaned one step before anything of them is read
-        const int c = P::CROSS ? next_slot(slot) : slot;
-        auto clean = [&](int y) {
-          tr_clean<D, DT, ROWS, 512>(smem[y][0], nullptr, tid);
-          tr_clean<D, DT, ROWS, 512>(smem[y][1], nullptr, tid);
-        };
-        if (P::CROSS && u == 0 && steps > 0) clean(0);
-        if (P::CROSS ? u + 1 < steps : u < steps) clean(c);
-        __syncthreads();
-      }
-    };
-    if (steps > 0) {
-      issue();
-      if (P::CROSS) issue(), issue();
-    }
-    tr_arrived(of);
-    // a head's bias, when the first waves come to its first tile
-    auto bias = [&]() __attribute__((always_inline)) {
-      if (EX && a.bias && u < steps && u % nt == 0) {
-        __syncthreads();
-        const float* b = a.bias + (int64_t)(s.h * group + u / nt) * (2 * a.reach + 1);
-        for (int y = tid; y <= 2 * a.reach; y += 512) bl[y] = b[y];
-        __syncthreads();
-      }
-    };
-    bias();
-    top();
-    if (second == 0) {
-      int t = t_all - 1, h = s.h * group;
-      if (P::CROSS && steps > 0) enter(slot);
-      while (u < steps) {
-        if (!P::CROSS) enter(slot);
-        ct = at.in(smem[slot][1]);
-        const int q0 = t * ROWS, nx = next_slot(slot);
-        int room = a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
-        asm volatile("" : "+v"(room));                        // (16 comparisons' operands are not to be kept for all tiles)
-        const int d0 = jr - off - q0 - 4 * hf;                // key - query of register 0; a row further is 1 less
-        const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
-        const bool near = EX && a.bias && !(whi <= -a.reach || wlo >= a.reach);
-        const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
-        const bool masked = EX && a.bits && w0 < s.k_len;
-        const uint32_t* bits = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw + (a.mi ? q0 + 4 * hf : 0);
-        stream(nx, [&](int v0, int v1) __attribute__((always_inline)) {
-#pragma unroll
-          for (int v = v0; v < v1; ++v) {
-            const int r = 8 * (v >> 2) + (v & 3);
-            float y = x[v];
-            if (EX) {
-              float more = far;
-              if (near) more = bl[a.reach + min(max(d0 - r, -a.reach), a.reach)] + BWD_SHIFT<DT>;
-              y = __builtin_fmaf(y, a.c, more);
-            } else {
-              y = DT == DT_F16 ? __builtin_fmaf(y, a.c, BWD_SHIFT<DT>) : y * a.c;
-            }
-            y = __builtin_amdgcn_exp2f(y);
-            y = r + room < 0 ? 0.0f : y;
-            if (masked) y = (bits[a.mi ? r : 0] >> ln) & 1u ? y : 0.0f;
-            x[v] = y;
-          }
-#pragma unroll
-          for (int v = v0; v < v1; v += 2) w[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (v1 >= 4 * q + 4 && v0 < 4 * q + 4)
-              pmem[u & 1][pair][q][lane] = v4f{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-        });
-        if (--t < t0) t = t_all - 1, ++h;
-        slot = nx, ++u;
-        bias();
-        top();
-      }
-    } else if (steps > 0) {
-      slot = next_slot(slot), ++u;
-      bias();
-      top();
-      int mine = 0;                                            // the slot of tile u - 1
-      if (P::CROSS) enter(mine);
-      for (;;) {
-        if (!P::CROSS) enter(mine);
-        ct = at.in(smem[mine][0]);
-        v4f pw[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) pw[q] = pmem[(u - 1) & 1][pair][q][lane];
-        stream(slot, [&](int v0, int v1) __attribute__((always_inline)) {
-          // (0 where the weight is, whatever its key or query holds)
-#pragma unroll
-          for (int v = v0; v < v1; ++v) {
-            const float y = pw[v >> 2][v & 3];
-            x[v] = y == 0.0f ? 0.0f : x[v] * (DT == DT_F16 ? y * ds_mul : y);
-          }
-#pragma unroll
-          for (int v = v0; v < v1; v += 2) w[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
-        });
-        if (u == steps) break;
-        mine = slot, slot = next_slot(slot), ++u;
-        bias();
-        top();
-      }
-    }
-    const bool bad = !(tr_nonfinite(acc) == 0.0f);
-    if (!__syncthreads_or(on && bad)) break;   // (a second time with every tile cleaned)
-  }
-
-  const float f = second ? __builtin_ldexpf(a.scale, -ex) : DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
-  uint16_t* p = second ? a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh
-                       : a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
-#pragma unroll
-  for (int db = 0; db < G::NDB; ++db) tr_store<DT>(acc[db], f, p + 32 * db, hf, on);
-}
-
 template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap& m, hipStream_t st) {
   const int B = a.cu_q ? 1 : a.B;
   const unsigned rows = (unsigned)((int64_t)B * a.H * a.q_tiles);
@@ -852,20 +341,14 @@ template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap&
     norm_blocks = (int)(need < 1024 ? need : 1024);
   }
   train_prep<D, DT><<<rows + norm_blocks, TR_THREADS, 0, st>>>(a, (int)rows, norm_blocks);
-  const unsigned keys = (unsigned)((int64_t)B * a.Hkv * a.k_tiles);
+  if (a.dk)
+    if (int rc = train_dkv_launch<D, DT>(a, st)) return rc;
+  if (!a.dq) return check_launch("train_prep");
   if (a.bits || a.bias) {
     const unsigned lds = a.bias_part ? 4u * 4u * (2u * a.reach + 1u) : 0u;
-    if (a.dk) {
-      if constexpr (D == 256) train_dkv_pair<D, DT, true><<<keys, 512, 0, st>>>(a);
-      else train_dkv<D, DT, true><<<keys, TR_THREADS, 0, st>>>(a);
-    }
-    if (a.dq) train_dq<D, DT, true><<<rows, TR_THREADS, lds, st>>>(a, m);
+    train_dq<D, DT, true><<<rows, TR_THREADS, lds, st>>>(a, m);
   } else {
-    if (a.dk) {
-      if constexpr (D == 256) train_dkv_pair<D, DT, false><<<keys, 512, 0, st>>>(a);
-      else train_dkv<D, DT, false><<<keys, TR_THREADS, 0, st>>>(a);
-    }
-    if (a.dq) train_dq<D, DT, false><<<rows, TR_THREADS, 0, st>>>(a, m);
+    train_dq<D, DT, false><<<rows, TR_THREADS, 0, st>>>(a, m);
   }
   return check_launch("train_bwd");
 }

@@ -1,0 +1,586 @@
+// Backward pass of the attention for training, dk and dv: see sage_train.h for the form and sage_train_bwd.hip for the split.
+// (Compiled with the results of matrix products in ordinary registers where they are read again: else the compiler moves every
+// score to and from the accumulation registers.)
+#include "sage_train.h"
+
+namespace sage {
+
+// ---- dk, dv --------------------------------------------------------------------------------------------------------------------
+//
+// A wave's keys and values (D / 2 registers) and the sums of its dk and dv (2 D) leave room for one wave per SIMD, so a wave has to
+// keep the matrix unit busy by itself.  It walks blocks of 32 queries, two a tile, as one stream of products: those of block b + 1's
+// scores and weights' gradients in turn with block b - 1's parts of dv and dk, and beside them the weights of block b.  The operands
+// of product n + AHEAD are read from LDS when product n is issued, whatever tile they are of.  (Two waves per SIMD with half of the
+// registers each, four operands ahead: 625 us at 1 x 24 x 4608 x 128; the weights beside half of the products only: 606.)
+template <int D> struct DkvGeo {
+  static constexpr int ROWS = 64;                  // queries per tile
+  static constexpr int SLOTS = 4;                  // tiles in LDS: one still read, one at work, one arrived, one on its way
+  static constexpr int AHEAD = 4;                  // products between an operand's read and its use (a power of two)
+  static constexpr int OCC = D == 64 ? 2 : 1;      // waves per SIMD
+};
+
+template <int D, int DT, bool EX>
+__global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArgs a) {
+  using P = DkvGeo<D>;
+  using G = TrGeo<D, P::ROWS>;
+  constexpr int ROWS = P::ROWS, AHEAD = P::AHEAD;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[P::SLOTS][2][G::TILE];
+  __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
+  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+
+  TrSeq s;
+  if (!tr_tile<true>(a, blockIdx.x, s)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  const int group = a.H / a.Hkv;
+  const int off = s.k_len - s.q_len;
+  const int w0 = s.c0 + wave * 32, j = w0 + ln;   // the wave's first key, the lane's
+  const bool on = j < s.k_len;
+  const int jr = on ? j : s.k_len - 1;
+
+  TrAddr<D> at;
+  at.init(lane);
+  v4i kf[G::NK], vf[G::NK];
+  {
+    const uint16_t* kp = a.k + (a.cu_q ? 0 : s.b * a.kb) + (s.kr + jr) * a.ks + s.h * a.kh + 8 * hf;
+    const uint16_t* vp = a.v + (a.cu_q ? 0 : s.b * a.vb) + (s.kr + jr) * a.vs + s.h * a.vh + 8 * hf;
+#pragma unroll
+    for (int x = 0; x < G::NK; ++x) {
+      kf[x] = *reinterpret_cast<const v4i*>(kp + 16 * x);
+      vf[x] = *reinterpret_cast<const v4i*>(vp + 16 * x);
+    }
+  }
+  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
+  const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
+
+  const int t_all = (s.q_len + ROWS - 1) / ROWS;
+  int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
+  if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
+  const int nt = t_all - t0;
+  const int steps = nt * group;
+  int t_full = 0;                                 // from this tile on every query sees every key of the wave
+  if (a.causal) t_full = (max(0, w0 + 31 - off) + ROWS - 1) / ROWS;
+  if (EX && a.bits) t_full = t_all;
+  t_full = min(max(t_full, t0), t_all);
+
+  // Loads, from the last tile back to the diagonal: workgroups of one head that start together stream the same tiles together.
+  TrLoader<D, ROWS> lq, lg;
+  lq.init(a.qs, wave, lane);
+  lg.init(a.gs, wave, lane);
+  const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + s.h * group * a.qh;
+  const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * group * a.gh;
+  const float* sp = (wave & 1 ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group) + lane;
+  const uint16_t *qt = qp + (int64_t)(t_all - 1) * ROWS * a.qs, *gt = gp + (int64_t)(t_all - 1) * ROWS * a.gs;   // of the next tile
+  int tn = t_all - 1, un = 0;                     // its number and step
+  auto issue = [&]() __attribute__((always_inline)) {
+    if (un >= steps) return;
+    uint8_t* dst = smem[un & (P::SLOTS - 1)][0];
+    if ((tn + 1) * ROWS <= s.q_len && lq.fits && lg.fits) {
+      lq.whole(qt, dst, wave);
+      lg.whole(gt, dst + G::TILE, wave);
+    } else {
+      lq.part(qp, a.qs, tn * ROWS, s.q_len, dst, wave, lane);
+      lg.part(gp, a.gs, tn * ROWS, s.q_len, dst + G::TILE, wave, lane);
+    }
+    if (wave < 2) tr_copy4(sp + tn * ROWS, stat[un & (P::SLOTS - 1)][wave]);
+    qt -= ROWS * a.qs, gt -= ROWS * a.gs, ++un;
+    if (--tn < t0) {
+      tn = t_all - 1, qp += a.qh, gp += a.gh, sp += a.pad;
+      qt = qp + (int64_t)tn * ROWS * a.qs, gt = gp + (int64_t)tn * ROWS * a.gs;
+    }
+  };
+
+  constexpr int N = 2 * G::NK;                     // products of either kind per block
+  v16f dk[G::NDB], dv[G::NDB], x[2], dp[2];        // (x, dp, p, ds: of even and odd blocks)
+  v4i ring[AHEAD], p[2][2], ds[2][2];
+  TrAddr<D> prev, cur, next;                       // the tiles of steps u - 1, u, u + 1 (q's; dout's lie behind them)
+  auto slot_of = [&](int u) __attribute__((always_inline)) { return at.in(smem[u & (P::SLOTS - 1)][0]); };
+  auto begin = [&](int u, auto qb_) __attribute__((always_inline)) {   // the first products' sums begin at the rows' numbers
+    constexpr int qb = decltype(qb_)::value;
+    const float(&st)[2][ROWS] = stat[u & (P::SLOTS - 1)];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v4f y = *reinterpret_cast<const v4f*>(&st[0][32 * qb + 8 * g + 4 * hf]);
+      const v4f z = *reinterpret_cast<const v4f*>(&st[1][32 * qb + 8 * g + 4 * hf]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[qb][4 * g + e] = y[e], dp[qb][4 * g + e] = z[e];
+    }
+  };
+  // Product y of a block's first kind (over the channels) and of its second (over its 32 queries): operand and product
+  auto first_op = [&](const TrAddr<D>& tile, int qb, int y) __attribute__((always_inline)) {
+    return tile.rows(qb, y >> 1, y & 1 ? G::TILE : 0);
+  };
+  auto second_op = [&](const TrAddr<D>& tile, int qb, int y) __attribute__((always_inline)) {
+    return tile.cols(2 * qb + y / (2 * G::NDB), y % (2 * G::NDB) >> 1, y & 1 ? 0 : G::TILE);
+  };
+  auto first = [&](const v4i& f, auto qb_, auto y_) __attribute__((always_inline)) {
+    constexpr int qb = decltype(qb_)::value, y = decltype(y_)::value;
+    if constexpr (y & 1) dp[qb] = tr_mfma<DT>(f, vf[y >> 1], dp[qb]);
+    else x[qb] = tr_mfma<DT>(f, kf[y >> 1], x[qb]);
+  };
+  auto second = [&](const v4i& f, auto qb_, auto y_) __attribute__((always_inline)) {
+    constexpr int qb = decltype(qb_)::value, y = decltype(y_)::value, st = y / (2 * G::NDB), db = y % (2 * G::NDB) >> 1;
+    if constexpr (y & 1) dk[db] = tr_mfma<DT>(f, ds[qb][st], dk[db]);
+    else dv[db] = tr_mfma<DT>(f, p[qb][st], dv[db]);
+  };
+  // The products beside the weights of block `par` of tile u: first ones of the block after it, second ones of the block before it
+  // (both of the other parity), in turn.
+  auto operand = [&](auto par_, auto n_) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_)::value, n = decltype(n_)::value;
+    if constexpr (n & 1) return second_op(par ? cur : prev, 1 - par, n >> 1);
+    else return first_op(par ? next : cur, 1 - par, n >> 1);
+  };
+  auto half = [&](int u, int t, int h, auto par_, auto masked_) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_)::value;
+    constexpr bool masked = decltype(masked_)::value;
+    using Other = std::integral_constant<int, 1 - par>;
+    const int q0 = t * ROWS + 32 * par;
+    const int d0 = jr - off - q0 - 4 * hf;        // key - query of register 0; a row further is 1 less
+    const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
+    const bool near = EX && a.bias && !(whi <= -a.reach || wlo >= a.reach);
+    const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
+    int room = masked && a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
+    if (masked) asm volatile("" : "+v"(room));                      // (16 comparisons' operands are not to be kept for all tiles)
+    const bool hiding = masked && EX && a.bits && w0 < s.k_len;
+    const uint32_t* bits = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw + (a.mi ? q0 + 4 * hf : 0);
+    // Elements v, v + 1 in four slices of about as many instructions as there is time for beside a product; where a quarter of
+    // the block's numbers has been used up, those of the block after the next take its place.
+    float w0_ = 0.0f, w1_ = 0.0f, e0_ = 0.0f, e1_ = 0.0f;
+    const float(&st)[2][ROWS] = stat[(u + 1) & (P::SLOTS - 1)];
+    auto score = [&](int v) __attribute__((always_inline)) {
+      const int r = 8 * (v >> 2) + (v & 3);
+      if (EX) {
+        float more = far;
+        if (near) more = bl[a.reach + min(max(d0 - r, -a.reach), a.reach)] + BWD_SHIFT<DT>;
+        return __builtin_fmaf(x[par][v], a.c, more);
+      }
+      return DT == DT_F16 ? __builtin_fmaf(x[par][v], a.c, BWD_SHIFT<DT>) : x[par][v] * a.c;
+    };
+    auto shown = [&](int v, float& w) __attribute__((always_inline)) {
+      if (masked) {
+        const int r = 8 * (v >> 2) + (v & 3);
+        bool hidden = r + room < 0;
+        if (hiding) hidden |= !((bits[a.mi ? r : 0] >> ln) & 1u);
+        if (hidden) w = 0.0f, dp[par][v] = 0.0f;
+      }
+    };
+    auto slice = [&](auto m_) __attribute__((always_inline)) {
+      constexpr int m = decltype(m_)::value, v = m / 4 * 2;
+      if constexpr (m % 4 == 0) {
+        w0_ = score(v), w1_ = score(v + 1);
+        w0_ = __builtin_amdgcn_exp2f(w0_);
+      } else if constexpr (m % 4 == 1) {
+        w1_ = __builtin_amdgcn_exp2f(w1_);
+        shown(v, w0_);
+        e0_ = w0_ * dp[par][v];
+      } else if constexpr (m % 4 == 2) {
+        shown(v + 1, w1_);
+        e1_ = w1_ * dp[par][v + 1];
+        int pw = tr_pack<DT>(w0_, w1_);
+        asm volatile("" : "+v"(pw));              // (here, not where the next tile's products use it)
+        p[par][v >> 3][(v & 7) >> 1] = pw;
+      } else {
+        if (DT == DT_F16) e0_ *= ds_mul, e1_ *= ds_mul;
+        int dw = tr_pack<DT>(e0_, e1_);
+        asm volatile("" : "+v"(dw));
+        ds[par][v >> 3][(v & 7) >> 1] = dw;
+        if constexpr ((v & 3) == 2) {
+          constexpr int g = v >> 2;
+          const v4f y = *reinterpret_cast<const v4f*>(&st[0][32 * par + 8 * g + 4 * hf]);
+          const v4f z = *reinterpret_cast<const v4f*>(&st[1][32 * par + 8 * g + 4 * hf]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[par][4 * g + e] = y[e], dp[par][4 * g + e] = z[e];
+        }
+      }
+    };
+    tr_unroll<2 * N>([&](auto n_) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_)::value;
+      const v4i f = ring[n % AHEAD];
+      if constexpr (n & 1) second(f, Other{}, std::integral_constant<int, (n >> 1)>{});
+      else first(f, Other{}, std::integral_constant<int, (n >> 1)>{});
+      if constexpr (n + AHEAD < 2 * N) {
+        ring[n % AHEAD] = operand(par_, std::integral_constant<int, n + AHEAD>{});
+      } else {
+        // of the half after this one: (next, 0) and (cur, 0) of the same tile, or (cur, 1) and (prev, 1) of the tile after it
+        constexpr int m = n + AHEAD - 2 * N;
+        if constexpr (m & 1) ring[n % AHEAD] = second_op(cur, par, m >> 1);
+        else ring[n % AHEAD] = first_op(next, par, m >> 1);
+      }
+      // 32 slices over the products but the first and the last three
+      if constexpr (n >= 1 && n < 2 * N - 3) {
+        constexpr int m0 = (n - 1) * 32 / (2 * N - 4), m1 = n * 32 / (2 * N - 4);
+        tr_unroll<m1 - m0>([&](auto m_) __attribute__((always_inline)) { slice(std::integral_constant<int, m0 + decltype(m_)::value>{}); });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dk[db][v] = 0.0f, dv[db][v] = 0.0f;
+    p[1][0] = p[1][1] = ds[1][0] = ds[1][1] = v4i{0, 0, 0, 0};   // (before the first block there is none)
+    // The tile after u has arrived, the one two before u is read and its place free
+    auto top = [&](int u) __attribute__((always_inline)) {
+      wait_vmcnt<0>();
+      tile_barrier();
+      issue();
+      if (pass) {   // a tile is cleaned when it has arrived, one step before anything of it is read
+        for (int y = u ? 1 : 0; y < 2; ++y) {
+          if (u + y >= steps) break;
+          uint8_t* tile = smem[(u + y) & (P::SLOTS - 1)][0];
+          tr_clean<D, DT, ROWS>(tile, nullptr, tid);
+          tr_clean<D, DT, ROWS>(tile + G::TILE, nullptr, tid);
+        }
+        __syncthreads();
+      }
+    };
+    issue();
+    issue();
+    tr_arrived(kf);
+    tr_arrived(vf);
+    if (steps > 0) {
+      using Zero = std::integral_constant<int, 0>;
+      using One = std::integral_constant<int, 1>;
+      top(0);
+      prev = cur = slot_of(0), next = slot_of(1);
+      begin(0, Zero{});
+      begin(0, One{});
+      tr_unroll<N>([&](auto y_) __attribute__((always_inline)) { first(first_op(cur, 0, decltype(y_)::value), Zero{}, y_); });
+      tr_unroll<AHEAD>([&](auto n_) __attribute__((always_inline)) { ring[decltype(n_)::value] = operand(Zero{}, n_); });
+      int u = 0, h = s.h * group;
+      for (int g = 0; g < group; ++g, ++h) {
+        if (EX && a.bias) {
+          __syncthreads();
+          for (int y = tid; y <= 2 * a.reach; y += TR_THREADS) bl[y] = a.bias[(int64_t)h * (2 * a.reach + 1) + y];
+          __syncthreads();
+        }
+        // first the tiles that hide no keys of the wave, then, in a loop of their own, those that do
+        int t = t_all - 1;
+        auto one = [&](auto masked_) __attribute__((always_inline)) {
+          half(u, t, h, Zero{}, masked_);
+          half(u, t, h, One{}, masked_);
+          prev = cur, cur = next, next = slot_of(u + 2), ++u;
+          if (u < steps) top(u);
+        };
+        const int full = pass ? t_all : t_full;      // (a second pass takes hidden keys out of every tile)
+        for (; t >= full; --t) one(std::false_type{});
+        for (; t >= t0; --t) one(std::true_type{});
+      }
+      tr_unroll<N>([&](auto y_) __attribute__((always_inline)) { second(second_op(prev, 1, decltype(y_)::value), One{}, y_); });
+    }
+    const bool bad = !(tr_nonfinite(dk) + tr_nonfinite(dv) == 0.0f);
+    if (!__syncthreads_or(on && bad)) break;   // (a second time with every tile cleaned: the loads begin anew)
+    qp -= group * a.qh, gp -= group * a.gh, sp -= group * a.pad;
+    tn = t_all - 1, un = 0;
+    qt = qp + (int64_t)tn * ROWS * a.qs, gt = gp + (int64_t)tn * ROWS * a.gs;
+  }
+
+  const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
+  uint16_t* kp = a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh;
+  uint16_t* vp = a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
+#pragma unroll
+  for (int db = 0; db < G::NDB; ++db) {
+    tr_store<DT>(dk[db], fk, kp + 32 * db, hf, on);
+    tr_store<DT>(dv[db], fv, vp + 32 * db, hf, on);
+  }
+}
+
+// Two waves share each 32 keys: the first recomputes the scores, makes the weights and sums dv, the second recomputes the gradient
+// of the weights, multiplies it by the weights, which it gets in fp32 through LDS one tile later, and sums dk.  Each has half of the
+// accumulators and half of the operands, so both fit a SIMD's registers together with operands read far ahead, and one's exponentials
+// run beside the other's products.  (One wave with everything: 695 us at 1 x 24 x 4608 x 128 with one wave per SIMD, 636 with
+// two, whose registers left four operands ahead.)
+//
+// Step u: the first waves work on tile u of 32 queries, the second ones on tile u - 1, and both read the first operands of their next
+// tile ahead; tiles u + 2 and u + 3 are on their way.  One barrier a step.  (Head dim 256, for whose tiles there is less room: the
+// next tile's operands are read after the barrier, one tile on its way.)
+template <int D> struct DkvPairGeo {
+  static constexpr int ROWS = 32;                  // queries per tile
+  static constexpr int WAVES = 8;
+  static constexpr bool CROSS = D != 256;          // reads ahead into the next tile
+  static constexpr int SLOTS = CROSS ? 5 : 3;      // tiles in LDS
+  static constexpr int AHEAD = D == 128 ? 8 : 4;   // products between an operand's read and its use
+  static constexpr int PER_WAVE = D == 64 ? 1 : D == 256 ? 4 : 2;   // 1 KiB loads of a wave per step, of q or of dout
+  static constexpr int PER_TENSOR = D * ROWS * 2 / 1024;            // (96: 6, so that the last two waves repeat some)
+  static constexpr int OCC = D == 64 ? 4 : 2;      // waves per SIMD
+};
+
+template <int D, int DT, bool EX>
+__global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainArgs a) {
+  using P = DkvPairGeo<D>;
+  using G = TrGeo<D, P::ROWS>;
+  constexpr int ROWS = P::ROWS;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[P::SLOTS][2][G::TILE];
+  __shared__ __attribute__((aligned(16))) v4f pmem[2][4][4][64];   // the weights of a tile: slot, pair of waves, quarter, lane
+  __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
+  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+
+  TrSeq s;
+  if (!tr_tile<true>(a, blockIdx.x, s)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  const int pair = wave & 3, second = wave >> 2;
+  const int group = a.H / a.Hkv;
+  const int off = s.k_len - s.q_len;
+  const int w0 = s.c0 + pair * 32, j = w0 + ln;   // the pair's first key, the lane's
+  const bool on = j < s.k_len;
+  const int jr = on ? j : s.k_len - 1;
+
+  TrAddr<D> at;
+  at.init(lane);
+  v4i of[G::NK];                                  // keys or values
+  {
+    const uint16_t* p = second ? a.v + (a.cu_q ? 0 : s.b * a.vb) + (s.kr + jr) * a.vs + s.h * a.vh
+                               : a.k + (a.cu_q ? 0 : s.b * a.kb) + (s.kr + jr) * a.ks + s.h * a.kh;
+#pragma unroll
+    for (int x = 0; x < G::NK; ++x) of[x] = *reinterpret_cast<const v4i*>(p + 8 * hf + 16 * x);
+  }
+  const int ex = DT == DT_F16 ? tr_exponent(a.norms) : 0;
+  const float ds_mul = __builtin_ldexpf(1.0f, ex - (int)BWD_SHIFT<DT>);
+
+  const int t_all = (s.q_len + ROWS - 1) / ROWS;
+  int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
+  if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
+  const int nt = t_all - t0;
+  const int steps = nt * group;
+
+  // Loads: a wave's are all of q or all of dout.  From the last tile back to the diagonal: workgroups of one head that start
+  // together stream the same tiles together.
+  const int l0 = wave * P::PER_WAVE % (2 * P::PER_TENSOR), side = l0 / P::PER_TENSOR;
+  const int64_t ls = side ? a.gs : a.qs, lh = side ? a.gh : a.qh;
+  const uint16_t* lsrc = (side ? a.dout + (a.cu_q ? 0 : s.b * a.gb) : a.q + (a.cu_q ? 0 : s.b * a.qb)) + s.qr * ls + s.h * group * lh;
+  const float* stat_src = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group);
+  const int row_l = (l0 - side * P::PER_TENSOR) * 64 + lane;   // the lane's chunk of the wave's first load
+  const bool fits = ls >= 0 && ls < (1 << 24);
+  uint32_t loff[D == 96 ? P::PER_WAVE : 1], lchunk = 0;
+#pragma unroll
+  for (int x = 0; x < (D == 96 ? P::PER_WAVE : 1); ++x) {
+    const int L = row_l + 64 * x, row = L / G::KCH, c = tr_swz<D>(row, L % G::KCH);
+    loff[x] = (uint32_t)((row * ls + (D == 96 ? c * 8 : 0)) * 2);
+    lchunk = c * 16;
+  }
+  int tn = t_all - 1, un = 0;                     // of the step that is loaded
+  auto issue = [&]() {
+    if (un < steps) {
+      const int slot = un % P::SLOTS;
+      uint8_t* dst = &smem[slot][side][0] + (l0 - side * P::PER_TENSOR) * 1024;
+      if ((tn + 1) * ROWS <= s.q_len && fits) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(lsrc + (int64_t)(tn * ROWS) * ls);
+        asm volatile("" : "+s"(p));
+#pragma unroll
+        for (int x = 0; x < P::PER_WAVE; ++x) {
+          constexpr int RPL = 64 / G::KCH;
+          uint32_t o = D == 96 ? loff[D == 96 ? x : 0] : loff[0] + (lchunk ^ (uint32_t)(tr_swz<D>(RPL * x, 0) * 16));
+          tr_copy16(p + (D == 96 ? 0 : x * RPL * ls * 2), o, dst + x * 1024);
+        }
+      } else {
+#pragma unroll 1
+        for (int x = 0; x < P::PER_WAVE; ++x) {
+          const int L = row_l + 64 * x, row = L / G::KCH;
+          tr_copy16(lsrc + min(tn * ROWS + row, s.q_len - 1) * ls + tr_swz<D>(row, L % G::KCH) * 8, dst + x * 1024);
+        }
+      }
+      if (wave < 2 && lane < ROWS) tr_copy4(stat_src + tn * ROWS + lane, stat[slot][wave]);
+    }
+    ++un;
+    if (--tn < t0) tn = t_all - 1, lsrc += lh, stat_src += a.pad;
+  };
+
+  v16f acc[G::NDB], x;
+  v4i ring[P::AHEAD], w[2];
+  constexpr int N = G::NK;                         // products of either kind per tile
+  TrAddr<D> rt, ct;                                // operands of the tile: by rows, transposed
+  auto fetch = [&](const TrAddr<D>& r, const TrAddr<D>& c, auto n_) __attribute__((always_inline)) {
+    constexpr int n = decltype(n_)::value, z = n - N;
+    if constexpr (n < N) ring[n % P::AHEAD] = r.rows(0, n);
+    else ring[n % P::AHEAD] = c.cols(z / G::NDB, z % G::NDB);
+  };
+  auto begin = [&](const float* st) __attribute__((always_inline)) {   // the sums of the first products begin at the rows' numbers
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v4f y = *reinterpret_cast<const v4f*>(st + 8 * g + 4 * hf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * g + e] = y[e];
+    }
+  };
+  // The products of the tile in rt, ct: first those over the channels into x, then `middle` makes of x (elements v0 .. v1) the
+  // operand w, then those over the tile's rows into acc.
+  auto stream = [&](int next, auto middle) __attribute__((always_inline)) {
+    const TrAddr<D> rn = at.in(smem[next][second]);
+    tr_unroll<2 * N>([&](auto n_) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_)::value;
+      const v4i f = ring[n % P::AHEAD];
+      if constexpr (n < N) {
+        x = tr_mfma<DT>(f, of[n], x);
+      } else {
+        constexpr int z = n - N;
+        acc[z % G::NDB] = tr_mfma<DT>(f, w[z / G::NDB], acc[z % G::NDB]);
+      }
+      if constexpr (n + P::AHEAD < 2 * N) fetch(rt, ct, std::integral_constant<int, n + P::AHEAD>{});
+      else if constexpr (P::CROSS) ring[n % P::AHEAD] = rn.rows(0, n + P::AHEAD - 2 * N);
+      if constexpr (n == N - 1) middle(0, 8);
+      if constexpr (n >= N && n < N + N / 2) {
+        constexpr int e0 = (n - N) * 4 / (N / 2) * 2, e1 = (n - N + 1) * 4 / (N / 2) * 2;
+        if constexpr (e1 > e0) middle(8 + e0, 8 + e1);
+      }
+      if constexpr (P::CROSS && n == 2 * N - 1) begin(stat[next][second]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    rt = rn;
+  };
+  auto enter = [&](int slot) __attribute__((always_inline)) {   // without reads ahead: before a tile
+    rt = at.in(smem[slot][second]);
+    begin(stat[slot][second]);
+    tr_unroll<P::AHEAD>([&](auto n_) __attribute__((always_inline)) { fetch(rt, ct, n_); });
+  };
+
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[db][v] = 0.0f;
+    // (a second pass begins its loads anew)
+    if (pass) lsrc -= group * lh, stat_src -= group * a.pad;
+    un = 0, tn = t_all - 1;
+    int u = 0, slot = 0;
+    auto next_slot = [&](int x) { return x + 1 == P::SLOTS ? 0 : x + 1; };
+    // The loads of the tile after u (without reads ahead: of u) have arrived, what step u - 1 read may be overwritten
+    auto top = [&]() __attribute__((always_inline)) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (P::CROSS && u + 2 < steps && !pass) {
+        if (wave < 2) wait_vmcnt<P::PER_WAVE + 1>();
+        else wait_vmcnt<P::PER_WAVE>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      tile_barrier();
+      issue();
+      if (pass) {   // tiles are cleaned one step before anything of them is read
+        const int c = P::CROSS ? next_slot(slot) : slot;
+        auto clean = [&](int y) {
+          tr_clean<D, DT, ROWS, 512>(smem[y][0], nullptr, tid);
+          tr_clean<D, DT, ROWS, 512>(smem[y][1], nullptr, tid);
+        };
+        if (P::CROSS && u == 0 && steps > 0) clean(0);
+        if (P::CROSS ? u + 1 < steps : u < steps) clean(c);
+        __syncthreads();
+      }
+    };
+    if (steps > 0) {
+      issue();
+      if (P::CROSS) issue(), issue();
+    }
+    tr_arrived(of);
+    // a head's bias, when the first waves come to its first tile
+    auto bias = [&]() __attribute__((always_inline)) {
+      if (EX && a.bias && u < steps && u % nt == 0) {
+        __syncthreads();
+        const float* b = a.bias + (int64_t)(s.h * group + u / nt) * (2 * a.reach + 1);
+        for (int y = tid; y <= 2 * a.reach; y += 512) bl[y] = b[y];
+        __syncthreads();
+      }
+    };
+    bias();
+    top();
+    if (second == 0) {
+      int t = t_all - 1, h = s.h * group;
+      if (P::CROSS && steps > 0) enter(slot);
+      while (u < steps) {
+        if (!P::CROSS) enter(slot);
+        ct = at.in(smem[slot][1]);
+        const int q0 = t * ROWS, nx = next_slot(slot);
+        int room = a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
+        asm volatile("" : "+v"(room));                        // (16 comparisons' operands are not to be kept for all tiles)
+        const int d0 = jr - off - q0 - 4 * hf;                // key - query of register 0; a row further is 1 less
+        const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
+        const bool near = EX && a.bias && !(whi <= -a.reach || wlo >= a.reach);
+        const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
+        const bool masked = EX && a.bits && w0 < s.k_len;
+        const uint32_t* bits = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw + (a.mi ? q0 + 4 * hf : 0);
+        stream(nx, [&](int v0, int v1) __attribute__((always_inline)) {
+#pragma unroll
+          for (int v = v0; v < v1; ++v) {
+            const int r = 8 * (v >> 2) + (v & 3);
+            float y = x[v];
+            if (EX) {
+              float more = far;
+              if (near) more = bl[a.reach + min(max(d0 - r, -a.reach), a.reach)] + BWD_SHIFT<DT>;
+              y = __builtin_fmaf(y, a.c, more);
+            } else {
+              y = DT == DT_F16 ? __builtin_fmaf(y, a.c, BWD_SHIFT<DT>) : y * a.c;
+            }
+            y = __builtin_amdgcn_exp2f(y);
+            y = r + room < 0 ? 0.0f : y;
+            if (masked) y = (bits[a.mi ? r : 0] >> ln) & 1u ? y : 0.0f;
+            x[v] = y;
+          }
+#pragma unroll
+          for (int v = v0; v < v1; v += 2) w[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (v1 >= 4 * q + 4 && v0 < 4 * q + 4)
+              pmem[u & 1][pair][q][lane] = v4f{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        });
+        if (--t < t0) t = t_all - 1, ++h;
+        slot = nx, ++u;
+        bias();
+        top();
+      }
+    } else if (steps > 0) {
+      slot = next_slot(slot), ++u;
+      bias();
+      top();
+      int mine = 0;                                            // the slot of tile u - 1
+      if (P::CROSS) enter(mine);
+      for (;;) {
+        if (!P::CROSS) enter(mine);
+        ct = at.in(smem[mine][0]);
+        v4f pw[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pw[q] = pmem[(u - 1) & 1][pair][q][lane];
+        stream(slot, [&](int v0, int v1) __attribute__((always_inline)) {
+          // (0 where the weight is, whatever its key or query holds)
+#pragma unroll
+          for (int v = v0; v < v1; ++v) {
+            const float y = pw[v >> 2][v & 3];
+            x[v] = y == 0.0f ? 0.0f : x[v] * (DT == DT_F16 ? y * ds_mul : y);
+          }
+#pragma unroll
+          for (int v = v0; v < v1; v += 2) w[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
+        });
+        if (u == steps) break;
+        mine = slot, slot = next_slot(slot), ++u;
+        bias();
+        top();
+      }
+    }
+    const bool bad = !(tr_nonfinite(acc) == 0.0f);
+    if (!__syncthreads_or(on && bad)) break;   // (a second time with every tile cleaned)
+  }
+
+  const float f = second ? __builtin_ldexpf(a.scale, -ex) : DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
+  uint16_t* p = second ? a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh
+                       : a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
+#pragma unroll
+  for (int db = 0; db < G::NDB; ++db) tr_store<DT>(acc[db], f, p + 32 * db, hf, on);
+}
+
+template <int D, int DT> int train_dkv_launch(const TrainArgs& a, hipStream_t st) {
+  const unsigned n = (unsigned)((int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * a.k_tiles);
+  if constexpr (D == 256) {
+    if (a.bits || a.bias) train_dkv_pair<D, DT, true><<<n, 512, 0, st>>>(a);
+    else train_dkv_pair<D, DT, false><<<n, 512, 0, st>>>(a);
+  } else {
+    if (a.bits || a.bias) train_dkv<D, DT, true><<<n, TR_THREADS, 0, st>>>(a);
+    else train_dkv<D, DT, false><<<n, TR_THREADS, 0, st>>>(a);
+  }
+  return check_launch("train_dkv");
+}
+
+#define SAGE_DKV(D) template int train_dkv_launch<D, DT_BF16>(const TrainArgs&, hipStream_t); \
+                    template int train_dkv_launch<D, DT_F16>(const TrainArgs&, hipStream_t);
+SAGE_DKV(64) SAGE_DKV(96) SAGE_DKV(128) SAGE_DKV(256)
+
+}  // namespace sage
