@@ -329,7 +329,7 @@ int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype
  * [B, H, Sq, D], k, v, dk, dv [B, Hkv, Skv, D] by (b, s, h) strides, dtype bf16 or fp16; lse fp32 [B, H, Sq], natural log.
  * causal: query i sees the keys j <= i + Skv - Sq.  mask: one byte per element, nonzero = visible, (b, h, i, j) at mask +
  * b * msb + h * msh + i * msq + j * msk, or NULL.  buckets: 0, or of a relative position bias (above; query i at position
- * i + Skv - Sq) whose last bucket begins at a distance of at most 768.  A query that sees no key is written as 0 (lse -inf) and
+ * i + Skv - Sq) whose last bucket begins at a distance of at most 760.  A query that sees no key is written as 0 (lse -inf) and
  * has no gradient; what hidden keys and such queries hold does not matter; a query that sees an infinity or a NaN is NaN.
  *
  * Packed batches (cu_q, cu_k not NULL; int32 [B + 1], device memory): B sequences one behind the other, Sq and Skv the totals of

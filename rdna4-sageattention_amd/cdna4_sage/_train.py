@@ -36,24 +36,28 @@ def _bias(table, heads, bidirectional, max_distance, gpu):
     return n, bool(bidirectional), int(max_distance)
 
 
-def _check(q, k, v, layout, attn_mask, table, bidirectional, max_distance, packed):
-    """((B, H, Hkv, Sq, Skv, D, GPU index), bias); B is 0 where packed."""
-    if not packed and layout not in ("HND", "NHD"):
-        raise Unsupported(f"layout {layout!r}")
-    dims = 3 if packed else 4
-    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
-        raise Unsupported(f"{dims}D tensors required")
-    if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise Unsupported(f"dtype {q.dtype}/{k.dtype}/{v.dtype} (fp16 or bf16 required)")
-    if k.shape != v.shape or k.shape[-1] != q.shape[-1]:
-        raise Unsupported("k and v of one shape, and of q's head_dim, required")
+def _check(q, k, v, layout, packed):
+    """(B, H, Hkv, Sq, Skv, D, GPU index); B is 0 where packed."""
+    qs, ks = q.shape, k.shape
     if packed:
-        (Sq, H, D), (Skv, Hkv, _), B = q.shape, k.shape, 0
+        if len(qs) != 3 or len(ks) != 3 or v.dim() != 3:
+            raise Unsupported("3D tensors required")
+        (Sq, H, D), (Skv, Hkv, _), B = qs, ks, 0
     else:
-        (B, H, Sq, D) = q.shape if layout == "HND" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
-        (Bk, Hkv, Skv, _) = k.shape if layout == "HND" else (k.shape[0], k.shape[2], k.shape[1], k.shape[3])
+        if layout != "HND" and layout != "NHD":
+            raise Unsupported(f"layout {layout!r}")
+        if len(qs) != 4 or len(ks) != 4 or v.dim() != 4:
+            raise Unsupported("4D tensors required")
+        if layout == "HND":
+            (B, H, Sq, D), (Bk, Hkv, Skv, _) = qs, ks
+        else:
+            (B, Sq, H, D), (Bk, Skv, Hkv, _) = qs, ks
         if Bk != B:
             raise Unsupported("q and k must have the same batch")
+    if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise Unsupported(f"dtype {q.dtype}/{k.dtype}/{v.dtype} (fp16 or bf16 required)")
+    if ks != v.shape or ks[-1] != D:
+        raise Unsupported("k and v of one shape, and of q's head_dim, required")
     if D not in HEAD_DIMS:
         raise Unsupported(f"head_dim {D} (supported {HEAD_DIMS})")
     if H and (Hkv == 0 or H % Hkv):
@@ -63,20 +67,24 @@ def _check(q, k, v, layout, attn_mask, table, bidirectional, max_distance, packe
         raise Unsupported("tensors must be on one ROCm GPU")
     if gpu_arch(gpu) not in ARCHS:
         raise Unsupported("not a CDNA4 GPU")
-    if attn_mask is not None:
-        if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool:
-            raise Unsupported("attn_mask must be a boolean tensor (learned biases: bias_table)")
-        if attn_mask.get_device() != gpu:
-            raise Unsupported("attn_mask must be on the device of q")
-        if attn_mask.dim() > 4:
-            raise Unsupported(f"attn_mask with {attn_mask.dim()} dims")
-        try:
-            torch.broadcast_shapes(attn_mask.shape, (B, H, Sq, Skv))
-            attn_mask.expand(B, H, Sq, Skv)
-        except RuntimeError as e:
-            raise Unsupported(f"attn_mask of shape {tuple(attn_mask.shape)} does not broadcast to {(B, H, Sq, Skv)}") from e
-    bias = None if table is None else _bias(table, H, bidirectional, max_distance, gpu)
-    return (B, H, Hkv, Sq, Skv, D, gpu), bias
+    return B, H, Hkv, Sq, Skv, D, gpu
+
+
+def _mask(attn_mask, shape):
+    """The mask expanded to [B, H, Sq, Skv], with its (batch, head, row, key) strides, 0 where it is the same along an axis."""
+    B, H, _, Sq, Skv, _, gpu = shape
+    if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool:
+        raise Unsupported("attn_mask must be a boolean tensor (learned biases: bias_table)")
+    if attn_mask.get_device() != gpu:
+        raise Unsupported("attn_mask must be on the device of q")
+    if attn_mask.dim() > 4:
+        raise Unsupported(f"attn_mask with {attn_mask.dim()} dims")
+    try:
+        m = attn_mask.expand(B, H, Sq, Skv)
+    except RuntimeError as e:
+        raise Unsupported(f"attn_mask of shape {tuple(attn_mask.shape)} does not broadcast to {(B, H, Sq, Skv)}") from e
+    s = m.stride()
+    return m, (s[0] if B > 1 else 0, s[1] if H > 1 else 0, s[2] if Sq > 1 else 0, s[3])
 
 
 def _scale(sm_scale):
@@ -87,26 +95,6 @@ def _scale(sm_scale):
     if not 2.0 ** -126 <= sm <= 3.4028234663852886e38:
         raise Unsupported(f"sm_scale {sm_scale} (a normal number of float32)")
     return sm
-
-
-def _mask_axes(attn_mask):
-    """Which of batch, head and row the mask differs along."""
-    if attn_mask is None:
-        return None
-    s = (1,) * (4 - attn_mask.dim()) + tuple(attn_mask.shape)
-    return tuple(int(s[i] > 1) for i in range(3))
-
-
-def _mask_strides(attn_mask, shape):
-    m = attn_mask.expand(*shape)
-    axes = _mask_axes(attn_mask)
-    return m, tuple(m.stride(i) if axes[i] else 0 for i in range(3)) + (m.stride(3),)
-
-
-# (an axis that differs may still have stride 0, as in an expanded tensor; the kernels tell broadcast axes by a stride of 0,
-# so such a mask is one that does not differ along it)
-def _seen_axes(strides):
-    return tuple(int(x != 0) for x in strides[:3])
 
 
 # ---- launches -------------------------------------------------------------------------------------------------------------
@@ -123,54 +111,54 @@ def _table_args(table, bias):
     if bias is None:
         return None, 0, 0, 0, 0, 0, None
     n, two, far = bias
-    return table.data_ptr(), TABLE_DTYPES[table.dtype], table.stride(0), table.stride(1), n, int(two), _capi.bias_borders(n, two, far)
+    return table.data_ptr(), TABLE_DTYPES[table.dtype], *table.stride(), n, int(two), _capi.bias_borders(n, two, far)
 
 
-def _sizes(shape, bias, mask_axes, cu_q):
-    """(state bytes, workspace bytes, B); raises Unsupported for a bias too far for the kernels."""
+def _sizes(shape, bias, axes, cu_q):
+    """(state bytes, workspace bytes, batch); raises Unsupported for a bias that reaches too far for the kernels."""
     B, H, Hkv, Sq, Skv, D, _ = shape
     if cu_q is not None:
         B = cu_q.shape[0] - 1
     try:
-        return (*_capi.train_workspace(cu_q is not None, B, H, Hkv, Sq, Skv, D, mask_axes, bias), B)
+        return (*_capi.train_workspace(cu_q is not None, B, H, Hkv, Sq, Skv, D, axes, bias), B)
     except _capi.SageError as e:
         raise Unsupported(str(e)) from e
 
 
 def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance):
-    """(out, lse, state, what the kernels loaded of q, k and v)."""
+    """(out, lse, state, what the kernels loaded of q, k and v, the call's plan for the backward pass)."""
     packed = cu_q is not None
-    shape, bias = _check(q, k, v, layout, attn_mask, table, bidirectional, max_distance, packed)
+    shape = _check(q, k, v, layout, packed)
     B, H, Hkv, Sq, Skv, D, gpu = shape
-    out = out_like(q) if not packed else torch.empty((Sq, H, D), dtype=q.dtype, device=q.device)
+    bias = None if table is None else _bias(table, H, bidirectional, max_distance, gpu)
+    mask, ms, axes = None, (0, 0, 0, 0), None
+    if attn_mask is not None:
+        mask, ms = _mask(attn_mask, shape)
+        axes = (int(ms[0] != 0), int(ms[1] != 0), int(ms[2] != 0))
+    out = torch.empty((Sq, H, D), dtype=q.dtype, device=q.device) if packed else out_like(q)
     lse = torch.empty((H, Sq) if packed else (B, H, Sq), dtype=torch.float32, device=q.device)
     if q.numel() == 0 or k.numel() == 0:
         out.zero_()
         lse.fill_(float("-inf"))
-        return out, lse, torch.empty(0, dtype=torch.uint8, device=q.device), (q, k, v)
-    mask, ms = None, (0, 0, 0, 0)
-    if attn_mask is not None:
-        mask, ms = _mask_strides(attn_mask, (B, H, Sq, Skv))
-    state_bytes, _, nb = _sizes(shape, bias, None if mask is None else _seen_axes(ms), cu_q)
+        return out, lse, torch.empty(0, dtype=torch.uint8, device=q.device), (q, k, v), (shape, bias, axes, 0, 0, 0)
+    state_bytes, ws_bytes, nb = _sizes(shape, bias, axes, cu_q)
     state = torch.empty(state_bytes, dtype=torch.uint8, device=q.device)
     q, sq = _strides(q, layout, packed)
     k, sk = _strides(k, layout, packed)
     v, sv = _strides(v, layout, packed)
     so = _strides(out, layout, packed)[1]
     _capi.call_on(gpu, "sage_train_fwd", q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, out.data_ptr(), *so,
-                  lse.data_ptr(), nb, H, Hkv, Sq, Skv, D, DTYPES[q.dtype], int(causal), sm_scale,
+                  lse.data_ptr(), nb, H, Hkv, Sq, Skv, D, DTYPES[q.dtype], causal, sm_scale,
                   None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
                   None if mask is None else mask.data_ptr(), *ms, *_table_args(table, bias),
                   state.data_ptr() if state_bytes else None, state_bytes)
-    return out, lse, state, (q, k, v)
+    return out, lse, state, (q, k, v), (shape, bias, axes, state_bytes, ws_bytes, nb)
 
 
-def backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance,
-                    mask_axes, need):
-    """(dq, dk, dv, dtable); need: of q, of k or v, of the table."""
+def backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, causal, plan, need):
+    """(dq, dk, dv, dtable); need: of q, of k or v, of the table.  table: any of the shape and type."""
     packed = cu_q is not None
-    shape, bias = _check(q, k, v, layout, None, table, bidirectional, max_distance, packed)
-    B, H, Hkv, Sq, Skv, D, gpu = shape
+    (B, H, Hkv, Sq, Skv, D, gpu), bias, axes, state_bytes, ws_bytes, nb = plan
     want_q, want_kv, want_table = need
     want_q = want_q or want_table   # (the table's gradient comes from the kernel of dq)
     like = (lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)) if packed else out_like
@@ -182,27 +170,35 @@ def backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, s
             if t is not None:
                 t.zero_()
         return dq, dk, dv, dtable
-    state_bytes, ws_bytes, nb = _sizes(shape, bias, mask_axes, cu_q)
-    ws = torch.empty(max(ws_bytes, _ALIGN), dtype=torch.uint8, device=q.device)
-    keep = []
-    args = []
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    args, keep = [], []
     for t in (dout, q, k, v, out):
         t, s = _strides(t, layout, packed)
         keep.append(t)
-        args += [t.data_ptr(), *s]
+        args += (t.data_ptr(), *s)
     args.append(lse.data_ptr())
     for t in (dq, dk, dv):
-        args += [None, 0, 0, 0] if t is None else [t.data_ptr(), *_strides(t, layout, packed)[1]]
-    ta = _table_args(table, bias)
-    if want_table:
-        ta = (dtable.data_ptr(), ta[1], dtable.stride(0), dtable.stride(1), *ta[4:])
+        args += (None, 0, 0, 0) if t is None else (t.data_ptr(), *_strides(t, layout, packed)[1])
+    if bias is None:
+        ta = (None, 0, 0, 0, 0, 0, None)
+    elif want_table:
+        ta = _table_args(dtable, bias)
     else:
-        ta = (None, *ta[1:])
-    _capi.call_on(gpu, "sage_train_bwd", *args, nb, H, Hkv, Sq, Skv, D, DTYPES[q.dtype], int(causal), sm_scale,
+        ta = (None, _capi.DTYPE_F32, 0, 0, *bias[:2], _capi.bias_borders(*bias))
+    _capi.call_on(gpu, "sage_train_bwd", *args, nb, H, Hkv, Sq, Skv, D, DTYPES[q.dtype], causal, sm_scale,
                   None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
-                  int(mask_axes is not None), *(mask_axes or (0, 0, 0)), *ta, state.data_ptr() if state_bytes else None,
-                  state_bytes, ws.data_ptr(), ws.numel())
+                  axes is not None, *(axes or (0, 0, 0)), *ta, state.data_ptr() if state_bytes else None,
+                  state_bytes, ws.data_ptr(), ws_bytes)
     return dq, dk, dv, dtable
+
+
+def backward_plan(q, k, v, layout, table, cu_q, bidirectional, max_distance, axes):
+    """forward_launch's plan, from the same tensors."""
+    shape = _check(q, k, v, layout, cu_q is not None)
+    bias = None if table is None else _bias(table, shape[1], bidirectional, max_distance, shape[6])
+    if q.numel() == 0 or k.numel() == 0:
+        return shape, bias, axes, 0, 0, 0
+    return (shape, bias, axes, *_sizes(shape, bias, axes, cu_q))
 
 
 class _Train(torch.autograd.Function):
@@ -210,10 +206,9 @@ class _Train(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, attn_mask, cu_q, cu_k, *how):
-        out, lse, state, used = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how)
+        out, lse, state, used, ctx.plan = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how)
         ctx.save_for_backward(*used, out, lse, state, table, cu_q, cu_k)
-        ctx.how = how
-        ctx.axes = None if attn_mask is None else _axes_of(attn_mask, q, k, how[0])
+        ctx.how = how[:3]
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -223,16 +218,9 @@ class _Train(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return (None,) * 12
-        q, k, v, out, lse, state, table, cu_q, cu_k = ctx.saved_tensors
         nq, nk, nv, nt = ctx.needs_input_grad[:4]
-        dq, dk, dv, dt = backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, *ctx.how, ctx.axes,
-                                         (nq, nk or nv, nt))
-        return (dq if nq else None, dk if nk else None, dv if nv else None, dt) + (None,) * 8
-
-
-def _axes_of(attn_mask, q, k, layout):
-    s = 2 if layout == "HND" else 1
-    return _seen_axes(_mask_strides(attn_mask, (q.shape[0], q.shape[3 - s], q.shape[s], k.shape[s]))[1])
+        dq, dk, dv, dt = backward_launch(dout, *ctx.saved_tensors, *ctx.how, ctx.plan, (nq, nk or nv, nt))
+        return dq if nq else None, dk if nk else None, dv if nv else None, dt, *(None,) * 8
 
 
 def _attention(q, k, v, table, attn_mask, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance, return_lse):
@@ -260,7 +248,7 @@ def attention_train(q, k, v, tensor_layout="HND", sm_scale=None, is_causal=False
     is_causal: query i sees the keys up to i + kv_len - q_len (bottom-right), any lengths.  attn_mask: boolean (True =
     attend), broadcastable to [B, H, q_len, kv_len].  bias_table: learned values [buckets, H] (fp32, bf16 or fp16), added by the
     relative position as relative_bias does, without a [H, q_len, kv_len] tensor; its last bucket has to begin at a distance of
-    at most 768.  A query that sees no key gives 0 (lse -inf) and has no gradient, whatever it holds, and so do keys that no
+    at most 760.  A query that sees no key gives 0 (lse -inf) and has no gradient, whatever it holds, and so do keys that no
     query sees; a query that sees an infinity or a NaN gives NaN.  Equal inputs give equal bits, gradients too.
 
     Gradients are of first order, in reverse mode; under torch.compile too.  Before a backward pass is captured into a graph,

@@ -167,9 +167,13 @@ def _fake_cache_attention_lse(q, k8, v8, k_scale, v_scale, block_table, lengths,
 # ---- attention for training and the relative position bias (no counterparts in the reference) --------------------------------
 
 def _mask_axes(attn_mask, q, k, layout):
-    from . import _train
-
-    return [] if attn_mask is None else list(_train._axes_of(attn_mask, q, k, layout))
+    """Whether the mask differs along batch, heads and rows; empty without one."""
+    if attn_mask is None:
+        return []
+    a = 2 if layout == "HND" else 1
+    shape = (q.shape[0], q.shape[3 - a], q.shape[a], k.shape[a])
+    s = attn_mask.expand(shape).stride()
+    return [int(n > 1 and x != 0) for n, x in zip(shape[:3], s)]
 
 
 @torch.library.custom_op("cdna4_sage::attention_train", mutates_args=())
@@ -213,9 +217,9 @@ def attention_train_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     """(dq, dk, dv, dtable), the last one empty without a table; mask_axes: whether the mask had a batch, head and row axis."""
     from . import _train
 
+    plan = _train.backward_plan(q, k, v, layout, table, cu_q, bidirectional, max_distance, tuple(mask_axes) or None)
     dq, dk, dv, dt = _train.backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, is_causal,
-                                            bidirectional, max_distance, tuple(mask_axes) or None,
-                                            (True, True, table is not None))
+                                            plan, (True, True, table is not None))
     return dq, dk, dv, q.new_empty(0) if dt is None else dt
 
 

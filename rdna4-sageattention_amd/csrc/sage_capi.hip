@@ -160,7 +160,7 @@ const char* sage_manifest_json(void) {
          "\"layout\": \"[pages, kv_heads, page_size, head_dim]\", \"page_size\": \"power of two, 16 to 1024\", "
          "\"attn\": {\"threads\": 256, \"keys_per_wave\": 32, \"rows\": [16, 32, 48], \"mfma\": \"v_mfma_f32_16x16x32_f16\"}}, "
          "\"train\": {\"columns\": 128, \"rows\": 64, \"threads\": 256, \"mfma\": \"v_mfma_f32_32x32x16_{bf16,f16}\", "
-         "\"masks\": [\"bool\"], \"bias_reach\": 768, \"bias_buckets\": 256}}";
+         "\"masks\": [\"bool\"], \"bias_reach\": 760, \"bias_buckets\": 256}}";
 }
 
 int sage_forward_workspace(int B, int H, int Hkv, int Sq, int Skv, int D, int causal, int64_t* workspace_bytes) {

@@ -59,6 +59,10 @@ struct TrainArgs {
   // boolean masks as bits: word w of row i holds keys 32 w ..; word w of row i at bits + b*mb + h*mh + w*mw + i*mi
   const uint32_t* bits;
   int64_t mb, mh, mw, mi;
+  // which blocks of 64 rows x 64 keys of it show anything: for each row block a bit for every key block, at any + b*ab + h*ah +
+  // block*aw (64-bit words), and for each key block a bit for every row block, at any_t + ..
+  const uint64_t *any, *any_t;
+  int64_t ab, ah, aw, tb, th, tw;
   // bias by distance: [H, 2 reach + 1] fp32 times log2(e); entry reach + d for key - query = d, clamped to +-reach
   const float* bias;
   int reach;
@@ -221,6 +225,56 @@ template <int DT> __device__ __forceinline__ void tr_store(const v16f& acc, floa
   }
 }
 
+// Blocks of a mask, by the words of two neighbouring blocks that a workgroup's columns are in (m0 NULL: no mask).
+struct TrBlocks {
+  const uint64_t *m0 = nullptr, *m1 = nullptr;
+  __device__ __forceinline__ uint64_t word(int i) const { return m0[i] | m1[i]; }
+  // the first block behind t that shows anything, `end` where none before it does
+  __device__ __forceinline__ int next(int t, int end) const {
+    if (++t >= end || !m0) return min(t, end);
+    for (;;) {
+      const uint64_t w = word(t >> 6) >> (t & 63);
+      if (w) return min(t + __builtin_ctzll(w), end);
+      t = (t | 63) + 1;
+      if (t >= end) return end;
+    }
+  }
+  // The same backwards for tiles of 64 >> S rows: the last one before t, t0 - 1 where there is none
+  template <int S> __device__ __forceinline__ int prev(int t, int t0) const {
+    if (--t < t0 || !m0) return max(t, t0 - 1);
+    for (;;) {
+      const int b = t >> S;
+      const uint64_t w = word(b >> 6) << (63 - (b & 63));
+      if (w) {
+        const int skip = __builtin_clzll(w);
+        if (skip) t = ((b - skip) << S) + (1 << S) - 1;
+        return max(t, t0 - 1);
+      }
+      t = ((b & ~63) << S) - 1;
+      if (t < t0) return t0 - 1;
+    }
+  }
+  // how many tiles t0 .. t1 - 1 of 64 >> S rows show anything
+  template <int S> __device__ __forceinline__ int count(int t0, int t1) const {
+    if (t1 <= t0) return 0;
+    if (!m0) return t1 - t0;
+    const int b0 = t0 >> S, b1 = (t1 - 1) >> S;
+    int n = 0;
+    for (int i = b0 >> 6; i <= b1 >> 6; ++i) {
+      uint64_t w = word(i);
+      if (i == b0 >> 6) w &= ~0ull << (b0 & 63);
+      if (i == b1 >> 6) w &= ~0ull >> (63 - (b1 & 63));
+      n += __builtin_popcountll(w);
+    }
+    n <<= S;
+    if (S) {   // halves of blocks that lie outside
+      if (t0 & 1) n -= (int)(word(b0 >> 6) >> (b0 & 63) & 1);
+      if (t1 & 1) n -= (int)(word(b1 >> 6) >> (b1 & 63) & 1);
+    }
+    return n;
+  }
+};
+
 // What a workgroup works on: a 128-column tile of one head of one sequence.
 struct TrSeq {
   int b, h;                // batch entry (packed: sequence) and head
@@ -269,13 +323,81 @@ template <bool KEYS> __device__ __forceinline__ bool tr_tile(const TrainArgs& a,
   return true;
 }
 
+// The blocks that a column tile's queries see / a column tile's keys are seen by
+__device__ __forceinline__ TrBlocks tr_key_blocks(const TrainArgs& a, const TrSeq& s) {
+  TrBlocks r;
+  if (!a.bits) return r;
+  r.m0 = r.m1 = a.any + s.b * a.ab + s.h * a.ah + (a.mi ? s.c0 / 64 * a.aw : 0);
+  if (a.mi && s.c0 + 64 < s.q_len) r.m1 += a.aw;
+  return r;
+}
+__device__ __forceinline__ TrBlocks tr_row_blocks(const TrainArgs& a, const TrSeq& s, int h, bool& none) {
+  TrBlocks r;
+  none = false;
+  if (!a.bits) return r;
+  r.m0 = r.m1 = a.any_t + s.b * a.tb + h * a.th + s.c0 / 64 * a.tw;
+  if (s.c0 + 64 < s.k_len) r.m1 += a.tw;
+  if (!a.mi) {   // the same for every row
+    none = r.word(0) == 0;
+    r.m0 = r.m1 = nullptr;
+  }
+  return r;
+}
+
+// The tiles of a head's queries that see a key tile: from the last one before `end` to first
+struct TrRows {
+  TrBlocks m;
+  int first;
+};
+__device__ __forceinline__ TrRows tr_rows(const TrainArgs& a, const TrSeq& s, int h, int first, int end) {
+  bool none;
+  TrRows r;
+  r.m = tr_row_blocks(a, s, h, none);
+  r.first = none ? end : first;
+  return r;
+}
+// How many tiles a workgroup of keys walks, over the heads that share them
+template <int S> __device__ __forceinline__ int tr_steps(const TrainArgs& a, const TrSeq& s, int group, int first, int end) {
+  if (!a.bits) return (end - first) * group;
+  int n = 0;
+  for (int g = 0; g < group; ++g) {
+    const TrRows r = tr_rows(a, s, s.h * group + g, first, end);
+    n += r.m.template count<S>(r.first, end);
+  }
+  return n;
+}
+// A walk over them: tile t of head g
+template <int S, bool MASKS> struct TrWalk {
+  int g, t;
+  TrRows rows;
+  __device__ __forceinline__ void head(const TrainArgs& a, const TrSeq& s, int group, int first, int end) {
+    if constexpr (MASKS) rows = tr_rows(a, s, s.h * group + g, first, end);
+    else rows.first = first;
+    t = MASKS ? rows.m.template prev<S>(end, rows.first) : end - 1;
+  }
+  // to the next tile; the number of heads that were passed (the last one's end: t stays below its first)
+  __device__ __forceinline__ int advance(const TrainArgs& a, const TrSeq& s, int group, int first, int end) {
+    t = MASKS ? rows.m.template prev<S>(t, rows.first) : t - 1;
+    int passed = 0;
+    while (t < rows.first && g + 1 < group) ++g, ++passed, head(a, s, group, first, end);
+    return passed;
+  }
+  __device__ __forceinline__ int start(const TrainArgs& a, const TrSeq& s, int group, int first, int end) {
+    g = 0;
+    head(a, s, group, first, end);
+    int passed = 0;
+    while (t < rows.first && g + 1 < group) ++g, ++passed, head(a, s, group, first, end);
+    return passed;
+  }
+};
+
 __device__ __forceinline__ int64_t tr_stat_row(const TrainArgs& a, const TrSeq& s, int h) {
   return a.cu_q ? h * a.pad + s.lr : ((int64_t)s.b * a.H + h) * a.pad;
 }
 
 // Largest distance of a bias inside the kernels: it and four waves' sums by distance have to fit the LDS that tiles of 256
 // channels leave.
-constexpr int TR_REACH = 768;
+constexpr int TR_REACH = 760;
 
 // Hidden pairs and the bias of one 32 x 32 block of scores whose columns are queries: register v of lane l is key
 // key0 + 8 (v / 4) + 4 (l / 32) + v % 4.  Values at the keys of `bits` (the word of the lane's query and these 32 keys) that are 0,

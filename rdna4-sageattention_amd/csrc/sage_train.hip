@@ -63,11 +63,22 @@ __global__ __launch_bounds__(TR_THREADS) void train_gaps(TrainGaps a, const int*
   }
 }
 
-// A boolean mask as bits, word-major: word w (keys 32 w ..) of 64 consecutive rows side by side.  A wave reads 64 keys of 64
-// rows, a byte per lane; the ballot of a row is its two words, lane r keeps row r's.
+// Four bytes' truth as four bits: each byte's bits folded onto its lowest, and those gathered by a product
+__device__ __forceinline__ uint32_t truth4(uint32_t w) {
+  w |= w >> 4;
+  w |= w >> 2;
+  w |= w >> 1;
+  return ((w & 0x01010101u) * 0x01020408u) >> 24 & 15u;
+}
+typedef uint32_t v4u_a1 __attribute__((ext_vector_type(4), aligned(1)));
+
+// A boolean mask as bits, word-major: word w (keys 32 w ..) of 64 consecutive rows side by side.  A wave makes the words of 64
+// keys of 64 rows: lane r reads row r's 64 bytes, or, at the last keys and where keys are not contiguous, the wave reads a byte per
+// lane of row after row and lane r keeps row r's ballot.  (1250 x 1250 x 6: 25 us with the latter alone.)
 __global__ __launch_bounds__(TR_THREADS) void train_mask_bits(const uint8_t* __restrict__ mask, int64_t msb, int64_t msh, int64_t msq,
                                                               int64_t msk, int heads, int rows, int row_pad, int keys, int chunks,
-                                                              int blocks, int64_t units, uint32_t* __restrict__ bits) {
+                                                              int blocks, int64_t units, uint32_t* __restrict__ bits,
+                                                              uint8_t* __restrict__ shows) {
   const int lane = threadIdx.x & 63;
   const int64_t u = (int64_t)blockIdx.x * (TR_THREADS / 64) + (threadIdx.x >> 6);
   if (u >= units) return;
@@ -80,28 +91,61 @@ __global__ __launch_bounds__(TR_THREADS) void train_mask_bits(const uint8_t* __r
   const bool in = key < keys;
   const int r0 = rb * 64, n = min(64, rows - r0);
   uint32_t lo = 0, hi = 0;
-  p += (int64_t)(in ? key : 0) * msk;
-  auto one = [&](int r) {
-    const uint64_t w = __ballot(in && p[(r0 + r) * msq] != 0);
-    if (lane == r) lo = (uint32_t)w, hi = (uint32_t)(w >> 32);
-  };
-  if (n == 64) {
-#pragma unroll 16
-    for (int r = 0; r < 64; ++r) one(r);
+  if (msk == 1 && c * 64 + 64 <= keys) {
+    if (lane < n) {
+      const v4u_a1* q = (const v4u_a1*)(p + (r0 + lane) * msq + c * 64);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const v4u_a1 w = q[x];
+        const uint32_t b = truth4(w[0]) | truth4(w[1]) << 4 | truth4(w[2]) << 8 | truth4(w[3]) << 12;
+        if (x < 2) lo |= b << (16 * x);
+        else hi |= b << (16 * x - 32);
+      }
+    }
   } else {
-    for (int r = 0; r < n; ++r) one(r);
+    p += (int64_t)(in ? key : 0) * msk;
+    auto one = [&](int r) {
+      const uint64_t w = __ballot(in && p[(r0 + r) * msq] != 0);
+      if (lane == r) lo = (uint32_t)w, hi = (uint32_t)(w >> 32);
+    };
+    if (n == 64) {
+#pragma unroll 16
+      for (int r = 0; r < 64; ++r) one(r);
+    } else {
+      for (int r = 0; r < n; ++r) one(r);
+    }
   }
   if (r0 + lane < row_pad) {
     uint32_t* o = bits + (bh * chunks * 2 + 2 * c) * row_pad + r0 + lane;
     o[0] = lo;
     o[row_pad] = hi;
   }
+  const bool any = __ballot(lo | hi) != 0;
+  if (lane == 0) shows[u] = any;   // [batch x head][block of 64 rows][block of 64 keys]
+}
+
+// What blocks show, as bits both ways: a wave for 64 key blocks of a row block, or for 64 row blocks of a key block
+__global__ __launch_bounds__(TR_THREADS) void train_mask_any(const uint8_t* __restrict__ shows, int blocks, int chunks, int aw, int tw,
+                                                             int64_t units, int64_t units_t, uint64_t* __restrict__ any,
+                                                             uint64_t* __restrict__ any_t) {
+  const int lane = threadIdx.x & 63;
+  int64_t u = (int64_t)blockIdx.x * (TR_THREADS / 64) + (threadIdx.x >> 6);
+  if (u < units) {
+    const int w = (int)(u % aw), c = 64 * w + lane;
+    const uint64_t m = __ballot(c < chunks && shows[u / aw * chunks + c] != 0);
+    if (lane == 0) any[u] = m;
+  } else if ((u -= units) < units_t) {
+    const int w = (int)(u % tw), b = 64 * w + lane, c = (int)(u / tw % chunks);
+    const int64_t bh = u / tw / chunks;
+    const uint64_t m = __ballot(b < blocks && shows[(bh * blocks + b) * chunks + c] != 0);
+    if (lane == 0) any_t[u] = m;
+  }
 }
 
 // Where everything lies in the state that the forward pass leaves to the backward pass, and in its workspace.
 struct TrainLayout {
-  int q_tiles, k_tiles, mask_b, mask_h, row_pad, words;
-  int64_t q_tab, k_tab, bits, vec, state;      // byte offsets; bounds at 0
+  int q_tiles, k_tiles, mask_b, mask_h, row_pad, words, blocks, chunks, aw, tw;
+  int64_t q_tab, k_tab, bits, shows, any, any_t, vec, state;      // byte offsets; bounds at 0
   int64_t pad, nl, nd, norms, parts, part, work;
 };
 static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool mask, bool mb, bool mh, bool mq, int reach,
@@ -122,7 +166,12 @@ static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool
   }
   if (mask) {
     l.mask_b = mb ? B : 1, l.mask_h = mh ? H : 1, l.row_pad = mq ? (Sq + 63) / 64 * 64 : 1, l.words = (Skv + 63) / 64 * 2;
-    l.bits = take(at, (int64_t)l.mask_b * l.mask_h * l.row_pad * l.words * 4);
+    l.blocks = mq ? (Sq + 63) / 64 : 1, l.chunks = l.words / 2, l.aw = (l.chunks + 63) / 64, l.tw = (l.blocks + 63) / 64;
+    const int64_t bh = (int64_t)l.mask_b * l.mask_h;
+    l.bits = take(at, bh * l.row_pad * l.words * 4);
+    l.shows = take(at, bh * l.blocks * l.chunks);
+    l.any = take(at, bh * l.blocks * l.aw * 8);
+    l.any_t = take(at, bh * l.chunks * l.tw * 8);
   }
   if (reach) l.vec = take(at, (int64_t)H * (2 * reach + 1) * 4);
   l.state = at;
@@ -196,6 +245,10 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
     const int64_t per = (int64_t)l.row_pad * l.words;
     a.bits = (const uint32_t*)(base + l.bits);
     a.mb = msb ? per * l.mask_h : 0, a.mh = msh ? per : 0, a.mw = l.row_pad, a.mi = msq ? 1 : 0;
+    const int64_t na = (int64_t)l.blocks * l.aw, nt = (int64_t)l.chunks * l.tw;
+    a.any = (const uint64_t*)(base + l.any), a.any_t = (const uint64_t*)(base + l.any_t);
+    a.ab = msb ? na * l.mask_h : 0, a.ah = msh ? na : 0, a.aw = l.aw;
+    a.tb = msb ? nt * l.mask_h : 0, a.th = msh ? nt : 0, a.tw = l.tw;
   }
   if (buckets) a.bias = (const float*)(base + l.vec), a.reach = reach;
   return SAGE_OK;
@@ -255,11 +308,15 @@ extern "C" int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t q
     train_gaps<<<dim3(Sq < 1024 ? Sq : 1024, 1), TR_THREADS, 0, st>>>(g, (const int*)state);
   }
   if (mask) {
-    const int rows = msq ? Sq : 1, blocks = (rows + 63) / 64, chunks = l.words / 2;
-    const int64_t units = (int64_t)l.mask_b * l.mask_h * blocks * chunks;
+    const int64_t bh = (int64_t)l.mask_b * l.mask_h, units = bh * l.blocks * l.chunks;
     SAGE_REQUIRE(units <= 0x7FFFFFFF, "sage_train_fwd: mask too large");
-    train_mask_bits<<<(unsigned)((units + 3) / 4), TR_THREADS, 0, st>>>((const uint8_t*)mask, msb, msh, msq, msk, l.mask_h, rows,
-                                                                        l.row_pad, Skv, chunks, blocks, units, (uint32_t*)a.bits);
+    uint8_t* shows = (uint8_t*)state + l.shows;
+    train_mask_bits<<<(unsigned)((units + 3) / 4), TR_THREADS, 0, st>>>((const uint8_t*)mask, msb, msh, msq, msk, l.mask_h,
+                                                                        msq ? Sq : 1, l.row_pad, Skv, l.chunks, l.blocks, units,
+                                                                        (uint32_t*)a.bits, shows);
+    const int64_t n = bh * l.blocks * l.aw, nt = bh * l.chunks * l.tw;
+    train_mask_any<<<(unsigned)((n + nt + 3) / 4), TR_THREADS, 0, st>>>(shows, l.blocks, l.chunks, l.aw, l.tw, n, nt, (uint64_t*)a.any,
+                                                                        (uint64_t*)a.any_t);
   }
   if (buckets)
     if (int rc = bias_expand_launch(table, table_dtype, tb, th, H, m, TR_LOG2E, (float*)a.bias, st)) return rc;

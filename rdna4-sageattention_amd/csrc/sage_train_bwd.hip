@@ -105,6 +105,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   using G = TrGeo<D>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
   __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  __shared__ __attribute__((aligned(256))) uint32_t wl[2][4][EX ? 64 : 1];   // a mask's words of the tiles, for each wave's queries
   extern __shared__ float by_distance[];   // EX with bias_part: 4 waves x (2 reach + 1)
 
   TrSeq s;
@@ -165,7 +166,8 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   t_mask = min(t_mask, t_end);
   const uint32_t* bits = nullptr;
   if (EX && a.bits) {
-    bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
+    // lane l brings word l / 32 of the tile's two for row l % 32
+    bits = a.bits + s.b * a.mb + s.h * a.mh + hf * a.mw + (a.mi ? min((int64_t)i, a.mw - 1) : 0);
     t_mask = 0;
   }
   float* mine = by_distance + wave * R;
@@ -177,13 +179,15 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   // and of ds over the others
   float flo = 0.0f, fhi = 0.0f, plo = 0.0f, phi = 0.0f, fnear = 0.0f;
 
-  auto issue = [&](int t) {
-    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave, lane);
-    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave, lane);
+  const TrBlocks blocks = EX ? tr_key_blocks(a, s) : TrBlocks();
+  auto issue = [&](int t, int slot) {
+    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[slot][0], wave, lane);
+    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[slot][1], wave, lane);
+    if (EX && bits) tr_copy4(bits + (int64_t)(2 * t) * a.mw, wl[slot][wave]);
   };
-  auto tile = [&](int t, auto masked_) {
+  auto tile = [&](int t, int slot, auto masked_) {
     constexpr bool masked = decltype(masked_)::value;
-    const TrAddr<D> kt = at.in(smem[t & 1][0]), vt = at.in(smem[t & 1][1]);
+    const TrAddr<D> kt = at.in(smem[slot][0]), vt = at.in(smem[slot][1]);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       v16f x = {}, dp;
@@ -215,7 +219,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
       for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(EX ? x[v] + nl : __builtin_fmaf(x[v], a.c, nl));
       if (masked) {
         uint32_t w = ~0u;
-        if (EX && bits && key0 < s.k_len) w = bits[(int64_t)(key0 >> 5) * a.mw];
+        if (EX && bits) w = wl[slot][wave][32 * kb + ln];
         const int room = lim - key0 - 4 * hf;
         w >>= 4 * hf;
 #pragma unroll
@@ -273,25 +277,26 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
       flo = fhi = plo = phi = fnear = 0.0f;
       for (int x = lane; x < R; x += 64) mine[x] = 0.0f;
     }
-    if (ntiles > 0) issue(0);
-    int t = 0;
+    int t = EX ? blocks.next(-1, ntiles) : 0, slot = 0, tn = 0;
+    if (t < ntiles) issue(t, 0);
     auto next = [&]() {   // tile t has arrived, the one before is read: the one after goes there
       wait_vmcnt<0>();
       tile_barrier();
-      if (t + 1 < ntiles) issue(t + 1);
+      tn = EX ? blocks.next(t, ntiles) : t + 1;
+      if (tn < ntiles) issue(tn, slot ^ 1);
     };
-    for (; t < t_mask; ++t) {
+    for (; t < t_mask; t = tn, slot ^= 1) {
       next();
-      tile(t, std::false_type{});
+      tile(t, slot, std::false_type{});
     }
-    for (; t < ntiles; ++t) {
+    for (; t < ntiles; t = tn, slot ^= 1) {
       next();
       if (pass) {
-        tr_clean<D, DT>(smem[t & 1][0], nullptr, tid);
-        tr_clean<D, DT>(smem[t & 1][1], nullptr, tid);
+        tr_clean<D, DT>(smem[slot][0], nullptr, tid);
+        tr_clean<D, DT>(smem[slot][1], nullptr, tid);
         __syncthreads();
       }
-      if (t < t_end) tile(t, std::true_type{});
+      if (t < t_end) tile(t, slot, std::true_type{});
       if (pass) __syncthreads();
     }
     const bool bad = !(tr_nonfinite(dq) == 0.0f);

@@ -27,6 +27,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   __shared__ __attribute__((aligned(1024))) uint8_t smem[P::SLOTS][2][G::TILE];
   __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
   __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  __shared__ __attribute__((aligned(256))) uint32_t wl[P::SLOTS][4][EX ? ROWS : 1];   // a mask's words of the tiles, for each wave's keys
 
   TrSeq s;
   if (!tr_tile<true>(a, blockIdx.x, s)) return;
@@ -56,8 +57,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   const int t_all = (s.q_len + ROWS - 1) / ROWS;
   int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
   if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
-  const int nt = t_all - t0;
-  const int steps = nt * group;
+  const int steps = EX ? tr_steps<0>(a, s, group, t0, t_all) : (t_all - t0) * group;
   int t_full = 0;                                 // from this tile on every query sees every key of the wave
   if (a.causal) t_full = (max(0, w0 + 31 - off) + ROWS - 1) / ROWS;
   if (EX && a.bits) t_full = t_all;
@@ -70,24 +70,25 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + s.h * group * a.qh;
   const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * group * a.gh;
   const float* sp = (wave & 1 ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group) + lane;
-  const uint16_t *qt = qp + (int64_t)(t_all - 1) * ROWS * a.qs, *gt = gp + (int64_t)(t_all - 1) * ROWS * a.gs;   // of the next tile
-  int tn = t_all - 1, un = 0;                     // its number and step
+  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h * group * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
+  TrWalk<0, EX> ld;                               // the tile that is loaded next
+  int un = 0;
+  auto shift = [&](int heads) { qp += heads * a.qh, gp += heads * a.gh, sp += heads * a.pad, mp += heads * a.mh; };
   auto issue = [&]() __attribute__((always_inline)) {
     if (un >= steps) return;
-    uint8_t* dst = smem[un & (P::SLOTS - 1)][0];
-    if ((tn + 1) * ROWS <= s.q_len && lq.fits && lg.fits) {
-      lq.whole(qt, dst, wave);
-      lg.whole(gt, dst + G::TILE, wave);
+    const int slot = un & (P::SLOTS - 1), row = ld.t * ROWS;
+    uint8_t* dst = smem[slot][0];
+    if (row + ROWS <= s.q_len && lq.fits && lg.fits) {
+      lq.whole(qp + row * a.qs, dst, wave);
+      lg.whole(gp + row * a.gs, dst + G::TILE, wave);
     } else {
-      lq.part(qp, a.qs, tn * ROWS, s.q_len, dst, wave, lane);
-      lg.part(gp, a.gs, tn * ROWS, s.q_len, dst + G::TILE, wave, lane);
+      lq.part(qp, a.qs, row, s.q_len, dst, wave, lane);
+      lg.part(gp, a.gs, row, s.q_len, dst + G::TILE, wave, lane);
     }
-    if (wave < 2) tr_copy4(sp + tn * ROWS, stat[un & (P::SLOTS - 1)][wave]);
-    qt -= ROWS * a.qs, gt -= ROWS * a.gs, ++un;
-    if (--tn < t0) {
-      tn = t_all - 1, qp += a.qh, gp += a.gh, sp += a.pad;
-      qt = qp + (int64_t)tn * ROWS * a.qs, gt = gp + (int64_t)tn * ROWS * a.gs;
-    }
+    if (wave < 2) tr_copy4(sp + row, stat[slot][wave]);
+    if (EX && a.bits) tr_copy4(mp + (a.mi ? row + lane : 0), wl[slot][wave]);
+    ++un;
+    shift(ld.advance(a, s, group, t0, t_all));
   };
 
   constexpr int N = 2 * G::NK;                     // products of either kind per block
@@ -141,8 +142,9 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
     const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
     int room = masked && a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
     if (masked) asm volatile("" : "+v"(room));                      // (16 comparisons' operands are not to be kept for all tiles)
-    const bool hiding = masked && EX && a.bits && w0 < s.k_len;
-    const uint32_t* bits = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw + (a.mi ? q0 + 4 * hf : 0);
+    const bool hiding = masked && EX && a.bits;
+    const uint32_t* bits = &wl[u & (P::SLOTS - 1)][wave][EX ? 32 * par + 4 * hf : 0];
+    v4i seen;                                                       // the words of four rows
     // Elements v, v + 1 in four slices of about as many instructions as there is time for beside a product; where a quarter of
     // the block's numbers has been used up, those of the block after the next take its place.
     float w0_ = 0.0f, w1_ = 0.0f, e0_ = 0.0f, e1_ = 0.0f;
@@ -160,13 +162,14 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
       if (masked) {
         const int r = 8 * (v >> 2) + (v & 3);
         bool hidden = r + room < 0;
-        if (hiding) hidden |= !((bits[a.mi ? r : 0] >> ln) & 1u);
+        if (hiding) hidden |= !(((uint32_t)seen[v & 3] >> ln) & 1u);
         if (hidden) w = 0.0f, dp[par][v] = 0.0f;
       }
     };
     auto slice = [&](auto m_) __attribute__((always_inline)) {
       constexpr int m = decltype(m_)::value, v = m / 4 * 2;
       if constexpr (m % 4 == 0) {
+        if (hiding && (v & 3) == 0) seen = *reinterpret_cast<const v4i*>(bits + 8 * (v >> 2));
         w0_ = score(v), w1_ = score(v + 1);
         w0_ = __builtin_amdgcn_exp2f(w0_);
       } else if constexpr (m % 4 == 1) {
@@ -236,6 +239,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
         __syncthreads();
       }
     };
+    shift(ld.start(a, s, group, t0, t_all));
     issue();
     issue();
     tr_arrived(kf);
@@ -249,32 +253,35 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
       begin(0, One{});
       tr_unroll<N>([&](auto y_) __attribute__((always_inline)) { first(first_op(cur, 0, decltype(y_)::value), Zero{}, y_); });
       tr_unroll<AHEAD>([&](auto n_) __attribute__((always_inline)) { ring[decltype(n_)::value] = operand(Zero{}, n_); });
-      int u = 0, h = s.h * group;
-      for (int g = 0; g < group; ++g, ++h) {
+      TrWalk<0, EX> at_work;
+      at_work.start(a, s, group, t0, t_all);
+      int u = 0;
+      while (u < steps) {
+        const int h = s.h * group + at_work.g;
         if (EX && a.bias) {
           __syncthreads();
           for (int y = tid; y <= 2 * a.reach; y += TR_THREADS) bl[y] = a.bias[(int64_t)h * (2 * a.reach + 1) + y];
           __syncthreads();
         }
-        // first the tiles that hide no keys of the wave, then, in a loop of their own, those that do
-        int t = t_all - 1;
+        // a head: first the tiles that hide no keys of the wave, then, in a loop of their own, those that do
+        bool same = true;
         auto one = [&](auto masked_) __attribute__((always_inline)) {
-          half(u, t, h, Zero{}, masked_);
-          half(u, t, h, One{}, masked_);
+          half(u, at_work.t, h, Zero{}, masked_);
+          half(u, at_work.t, h, One{}, masked_);
           prev = cur, cur = next, next = slot_of(u + 2), ++u;
+          same = at_work.advance(a, s, group, t0, t_all) == 0 && u < steps;
           if (u < steps) top(u);
         };
         const int full = pass ? t_all : t_full;      // (a second pass takes hidden keys out of every tile)
-        for (; t >= full; --t) one(std::false_type{});
-        for (; t >= t0; --t) one(std::true_type{});
+        while (same && at_work.t >= full) one(std::false_type{});
+        while (same) one(std::true_type{});
       }
       tr_unroll<N>([&](auto y_) __attribute__((always_inline)) { second(second_op(prev, 1, decltype(y_)::value), One{}, y_); });
     }
     const bool bad = !(tr_nonfinite(dk) + tr_nonfinite(dv) == 0.0f);
     if (!__syncthreads_or(on && bad)) break;   // (a second time with every tile cleaned: the loads begin anew)
-    qp -= group * a.qh, gp -= group * a.gh, sp -= group * a.pad;
-    tn = t_all - 1, un = 0;
-    qt = qp + (int64_t)tn * ROWS * a.qs, gt = gp + (int64_t)tn * ROWS * a.gs;
+    shift(-ld.g);
+    un = 0;
   }
 
   const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
@@ -287,28 +294,22 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   }
 }
 
-// Two waves share each 32 keys: the first recomputes the scores, makes the weights and sums dv, the second recomputes the gradient
-// of the weights, multiplies it by the weights, which it gets in fp32 through LDS one tile later, and sums dk.  Each has half of the
-// accumulators and half of the operands, so both fit a SIMD's registers together with operands read far ahead, and one's exponentials
-// run beside the other's products.  (One wave with everything: 695 us at 1 x 24 x 4608 x 128 with one wave per SIMD, 636 with
-// two, whose registers left four operands ahead.)
-//
-// Step u: the first waves work on tile u of 32 queries, the second ones on tile u - 1, and both read the first operands of their next
-// tile ahead; tiles u + 2 and u + 3 are on their way.  One barrier a step.  (Head dim 256, for whose tiles there is less room: the
-// next tile's operands are read after the barrier, one tile on its way.)
+// Head dim 256, where one wave's operands and sums pass its 512 registers: two waves share each 32 keys.  The first recomputes the
+// scores, makes the weights and sums dv; the second recomputes the gradient of the weights, multiplies it by the weights, which it
+// gets in fp32 through LDS one tile later, and sums dk.  Each has half of the operands and sums, so two waves fit a SIMD, and one's
+// exponentials run beside the other's products.  Step u: the first waves work on tile u of 32 queries, the second ones on tile
+// u - 1, tile u + 1 is on its way.  (2 x 12 x 2180 x 256: 648 us in one wave, whose registers spill, 385 like this; at head dim 128 one wave
+// is faster, 702 and 567 us at 1 x 24 x 4608.)
 template <int D> struct DkvPairGeo {
   static constexpr int ROWS = 32;                  // queries per tile
-  static constexpr int WAVES = 8;
-  static constexpr bool CROSS = D != 256;          // reads ahead into the next tile
-  static constexpr int SLOTS = CROSS ? 5 : 3;      // tiles in LDS
-  static constexpr int AHEAD = D == 128 ? 8 : 4;   // products between an operand's read and its use
-  static constexpr int PER_WAVE = D == 64 ? 1 : D == 256 ? 4 : 2;   // 1 KiB loads of a wave per step, of q or of dout
-  static constexpr int PER_TENSOR = D * ROWS * 2 / 1024;            // (96: 6, so that the last two waves repeat some)
-  static constexpr int OCC = D == 64 ? 4 : 2;      // waves per SIMD
+  static constexpr int SLOTS = 3;                  // tiles in LDS
+  static constexpr int AHEAD = 4;                  // products between an operand's read and its use
+  static constexpr int PER_WAVE = D * ROWS * 4 / 1024 / 8;    // 1 KiB loads of a wave per step, of q or of dout
+  static constexpr int PER_TENSOR = D * ROWS * 2 / 1024;
 };
 
 template <int D, int DT, bool EX>
-__global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainArgs a) {
+__global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
   using P = DkvPairGeo<D>;
   using G = TrGeo<D, P::ROWS>;
   constexpr int ROWS = P::ROWS;
@@ -316,6 +317,7 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
   __shared__ __attribute__((aligned(16))) v4f pmem[2][4][4][64];   // the weights of a tile: slot, pair of waves, quarter, lane
   __shared__ __attribute__((aligned(256))) float stat[P::SLOTS][2][ROWS];
   __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  __shared__ __attribute__((aligned(256))) uint32_t wl[P::SLOTS][4][EX ? ROWS : 1];   // a mask's words of the tiles, for each pair's keys
 
   TrSeq s;
   if (!tr_tile<true>(a, blockIdx.x, s)) return;
@@ -343,38 +345,34 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
   const int t_all = (s.q_len + ROWS - 1) / ROWS;
   int t0 = 0;                                     // the first tile that sees one of the workgroup's keys
   if (a.causal) t0 = min(t_all, max(0, s.c0 - off) / ROWS);
-  const int nt = t_all - t0;
-  const int steps = nt * group;
+  const int steps = EX ? tr_steps<1>(a, s, group, t0, t_all) : (t_all - t0) * group;
 
   // Loads: a wave's are all of q or all of dout.  From the last tile back to the diagonal: workgroups of one head that start
   // together stream the same tiles together.
-  const int l0 = wave * P::PER_WAVE % (2 * P::PER_TENSOR), side = l0 / P::PER_TENSOR;
+  const int l0 = wave * P::PER_WAVE, side = l0 / P::PER_TENSOR;
   const int64_t ls = side ? a.gs : a.qs, lh = side ? a.gh : a.qh;
   const uint16_t* lsrc = (side ? a.dout + (a.cu_q ? 0 : s.b * a.gb) : a.q + (a.cu_q ? 0 : s.b * a.qb)) + s.qr * ls + s.h * group * lh;
   const float* stat_src = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group);
   const int row_l = (l0 - side * P::PER_TENSOR) * 64 + lane;   // the lane's chunk of the wave's first load
   const bool fits = ls >= 0 && ls < (1 << 24);
-  uint32_t loff[D == 96 ? P::PER_WAVE : 1], lchunk = 0;
+  uint32_t loff[P::PER_WAVE];
 #pragma unroll
-  for (int x = 0; x < (D == 96 ? P::PER_WAVE : 1); ++x) {
-    const int L = row_l + 64 * x, row = L / G::KCH, c = tr_swz<D>(row, L % G::KCH);
-    loff[x] = (uint32_t)((row * ls + (D == 96 ? c * 8 : 0)) * 2);
-    lchunk = c * 16;
+  for (int x = 0; x < P::PER_WAVE; ++x) {
+    const int L = row_l + 64 * x, row = L / G::KCH;
+    loff[x] = (uint32_t)((row * ls + tr_swz<D>(row, L % G::KCH) * 8) * 2);
   }
-  int tn = t_all - 1, un = 0;                     // of the step that is loaded
+  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h * group * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
+  TrWalk<1, EX> ld;                               // the tile that is loaded next
+  int un = 0;
+  auto shift = [&](int heads) { lsrc += heads * lh, stat_src += heads * a.pad, mp += heads * a.mh; };
   auto issue = [&]() {
     if (un < steps) {
-      const int slot = un % P::SLOTS;
+      const int slot = un % P::SLOTS, tn = ld.t;
       uint8_t* dst = &smem[slot][side][0] + (l0 - side * P::PER_TENSOR) * 1024;
       if ((tn + 1) * ROWS <= s.q_len && fits) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(lsrc + (int64_t)(tn * ROWS) * ls);
-        asm volatile("" : "+s"(p));
+        const uint16_t* p = lsrc + (int64_t)(tn * ROWS) * ls;
 #pragma unroll
-        for (int x = 0; x < P::PER_WAVE; ++x) {
-          constexpr int RPL = 64 / G::KCH;
-          uint32_t o = D == 96 ? loff[D == 96 ? x : 0] : loff[0] + (lchunk ^ (uint32_t)(tr_swz<D>(RPL * x, 0) * 16));
-          tr_copy16(p + (D == 96 ? 0 : x * RPL * ls * 2), o, dst + x * 1024);
-        }
+        for (int x = 0; x < P::PER_WAVE; ++x) tr_copy16(p, loff[x], dst + x * 1024);
       } else {
 #pragma unroll 1
         for (int x = 0; x < P::PER_WAVE; ++x) {
@@ -383,9 +381,10 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
         }
       }
       if (wave < 2 && lane < ROWS) tr_copy4(stat_src + tn * ROWS + lane, stat[slot][wave]);
+      if (EX && a.bits && !second && lane < ROWS) tr_copy4(mp + (a.mi ? tn * ROWS + lane : 0), wl[slot][pair]);
+      shift(ld.advance(a, s, group, t0, t_all));
     }
     ++un;
-    if (--tn < t0) tn = t_all - 1, lsrc += lh, stat_src += a.pad;
   };
 
   v16f acc[G::NDB], x;
@@ -407,8 +406,7 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
   };
   // The products of the tile in rt, ct: first those over the channels into x, then `middle` makes of x (elements v0 .. v1) the
   // operand w, then those over the tile's rows into acc.
-  auto stream = [&](int next, auto middle) __attribute__((always_inline)) {
-    const TrAddr<D> rn = at.in(smem[next][second]);
+  auto stream = [&](auto middle) __attribute__((always_inline)) {
     tr_unroll<2 * N>([&](auto n_) __attribute__((always_inline)) {
       constexpr int n = decltype(n_)::value;
       const v4i f = ring[n % P::AHEAD];
@@ -419,18 +417,15 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
         acc[z % G::NDB] = tr_mfma<DT>(f, w[z / G::NDB], acc[z % G::NDB]);
       }
       if constexpr (n + P::AHEAD < 2 * N) fetch(rt, ct, std::integral_constant<int, n + P::AHEAD>{});
-      else if constexpr (P::CROSS) ring[n % P::AHEAD] = rn.rows(0, n + P::AHEAD - 2 * N);
       if constexpr (n == N - 1) middle(0, 8);
       if constexpr (n >= N && n < N + N / 2) {
         constexpr int e0 = (n - N) * 4 / (N / 2) * 2, e1 = (n - N + 1) * 4 / (N / 2) * 2;
         if constexpr (e1 > e0) middle(8 + e0, 8 + e1);
       }
-      if constexpr (P::CROSS && n == 2 * N - 1) begin(stat[next][second]);
       __builtin_amdgcn_sched_barrier(0);
     });
-    rt = rn;
   };
-  auto enter = [&](int slot) __attribute__((always_inline)) {   // without reads ahead: before a tile
+  auto enter = [&](int slot) __attribute__((always_inline)) {   // before a tile
     rt = at.in(smem[slot][second]);
     begin(stat[slot][second]);
     tr_unroll<P::AHEAD>([&](auto n_) __attribute__((always_inline)) { fetch(rt, ct, n_); });
@@ -442,64 +437,56 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[db][v] = 0.0f;
     // (a second pass begins its loads anew)
-    if (pass) lsrc -= group * lh, stat_src -= group * a.pad;
-    un = 0, tn = t_all - 1;
+    if (pass) shift(-ld.g);
+    shift(ld.start(a, s, group, t0, t_all));
+    un = 0;
     int u = 0, slot = 0;
     auto next_slot = [&](int x) { return x + 1 == P::SLOTS ? 0 : x + 1; };
-    // The loads of the tile after u (without reads ahead: of u) have arrived, what step u - 1 read may be overwritten
+    // Tile u has arrived, what step u - 1 read last may be overwritten
     auto top = [&]() __attribute__((always_inline)) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (P::CROSS && u + 2 < steps && !pass) {
-        if (wave < 2) wait_vmcnt<P::PER_WAVE + 1>();
-        else wait_vmcnt<P::PER_WAVE>();
-      } else {
-        wait_vmcnt<0>();
-      }
+      wait_vmcnt<0>();
       tile_barrier();
       issue();
-      if (pass) {   // tiles are cleaned one step before anything of them is read
-        const int c = P::CROSS ? next_slot(slot) : slot;
-        auto clean = [&](int y) {
-          tr_clean<D, DT, ROWS, 512>(smem[y][0], nullptr, tid);
-          tr_clean<D, DT, ROWS, 512>(smem[y][1], nullptr, tid);
-        };
-        if (P::CROSS && u == 0 && steps > 0) clean(0);
-        if (P::CROSS ? u + 1 < steps : u < steps) clean(c);
+      if (pass) {   // a tile is cleaned when it has arrived
+        if (u < steps) {
+          tr_clean<D, DT, ROWS, 512>(smem[slot][0], nullptr, tid);
+          tr_clean<D, DT, ROWS, 512>(smem[slot][1], nullptr, tid);
+        }
         __syncthreads();
       }
     };
-    if (steps > 0) {
-      issue();
-      if (P::CROSS) issue(), issue();
-    }
+    issue();
     tr_arrived(of);
+    TrWalk<1, EX> at_work;                         // tile u
+    at_work.start(a, s, group, t0, t_all);
+    bool entered = true;                           // tile u is the first of its head
     // a head's bias, when the first waves come to its first tile
     auto bias = [&]() __attribute__((always_inline)) {
-      if (EX && a.bias && u < steps && u % nt == 0) {
+      if (EX && a.bias && u < steps && entered) {
         __syncthreads();
-        const float* b = a.bias + (int64_t)(s.h * group + u / nt) * (2 * a.reach + 1);
+        const float* b = a.bias + (int64_t)(s.h * group + at_work.g) * (2 * a.reach + 1);
         for (int y = tid; y <= 2 * a.reach; y += 512) bl[y] = b[y];
         __syncthreads();
       }
     };
+    auto step = [&]() __attribute__((always_inline)) { entered = at_work.advance(a, s, group, t0, t_all) != 0, ++u; };
     bias();
     top();
     if (second == 0) {
-      int t = t_all - 1, h = s.h * group;
-      if (P::CROSS && steps > 0) enter(slot);
       while (u < steps) {
-        if (!P::CROSS) enter(slot);
+        enter(slot);
         ct = at.in(smem[slot][1]);
-        const int q0 = t * ROWS, nx = next_slot(slot);
+        const int q0 = at_work.t * ROWS, nx = next_slot(slot);
         int room = a.causal ? q0 + 4 * hf - (jr - off) : 0;   // row r sees the key where r + room >= 0
         asm volatile("" : "+v"(room));                        // (16 comparisons' operands are not to be kept for all tiles)
         const int d0 = jr - off - q0 - 4 * hf;                // key - query of register 0; a row further is 1 less
         const int whi = w0 + 31 - off - q0, wlo = w0 - off - q0 - 31;
         const bool near = EX && a.bias && !(whi <= -a.reach || wlo >= a.reach);
         const float far = (EX && a.bias && !near ? bl[whi <= -a.reach ? 0 : 2 * a.reach] : 0.0f) + BWD_SHIFT<DT>;
-        const bool masked = EX && a.bits && w0 < s.k_len;
-        const uint32_t* bits = a.bits + s.b * a.mb + h * a.mh + (int64_t)(w0 >> 5) * a.mw + (a.mi ? q0 + 4 * hf : 0);
-        stream(nx, [&](int v0, int v1) __attribute__((always_inline)) {
+        const bool masked = EX && a.bits;
+        const uint32_t* bits = &wl[slot][pair][EX ? 4 * hf : 0];
+        stream([&](int v0, int v1) __attribute__((always_inline)) {
 #pragma unroll
           for (int v = v0; v < v1; ++v) {
             const int r = 8 * (v >> 2) + (v & 3);
@@ -513,7 +500,7 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
             }
             y = __builtin_amdgcn_exp2f(y);
             y = r + room < 0 ? 0.0f : y;
-            if (masked) y = (bits[a.mi ? r : 0] >> ln) & 1u ? y : 0.0f;
+            if (masked) y = (bits[r] >> ln) & 1u ? y : 0.0f;
             x[v] = y;
           }
 #pragma unroll
@@ -523,24 +510,24 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
             if (v1 >= 4 * q + 4 && v0 < 4 * q + 4)
               pmem[u & 1][pair][q][lane] = v4f{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
         });
-        if (--t < t0) t = t_all - 1, ++h;
-        slot = nx, ++u;
+        slot = nx;
+        step();
         bias();
         top();
       }
     } else if (steps > 0) {
-      slot = next_slot(slot), ++u;
+      slot = next_slot(slot);
+      step();
       bias();
       top();
       int mine = 0;                                            // the slot of tile u - 1
-      if (P::CROSS) enter(mine);
       for (;;) {
-        if (!P::CROSS) enter(mine);
+        enter(mine);
         ct = at.in(smem[mine][0]);
         v4f pw[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) pw[q] = pmem[(u - 1) & 1][pair][q][lane];
-        stream(slot, [&](int v0, int v1) __attribute__((always_inline)) {
+        stream([&](int v0, int v1) __attribute__((always_inline)) {
           // (0 where the weight is, whatever its key or query holds)
 #pragma unroll
           for (int v = v0; v < v1; ++v) {
@@ -551,7 +538,8 @@ __global__ __launch_bounds__(512, DkvPairGeo<D>::OCC) void train_dkv_pair(TrainA
           for (int v = v0; v < v1; v += 2) w[v >> 3][(v & 7) >> 1] = tr_pack<DT>(x[v], x[v + 1]);
         });
         if (u == steps) break;
-        mine = slot, slot = next_slot(slot), ++u;
+        mine = slot, slot = next_slot(slot);
+        step();
         bias();
         top();
       }

@@ -13,6 +13,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   using G = TrGeo<D>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
   __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
+  __shared__ __attribute__((aligned(256))) uint32_t wl[2][4][EX ? 64 : 1];   // a mask's words of the tiles, for each wave's queries
   __shared__ int poison[TR_ROWS];
 
   TrSeq s;
@@ -54,7 +55,8 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   t_mask = min(t_mask, t_end);
   const uint32_t* bits = nullptr;
   if (EX && a.bits) {
-    bits = a.bits + s.b * a.mb + s.h * a.mh + (int64_t)ir * a.mi;
+    // lane l brings word l / 32 of the tile's two for row l % 32
+    bits = a.bits + s.b * a.mb + s.h * a.mh + hf * a.mw + (a.mi ? min((int64_t)i, a.mw - 1) : 0);
     t_mask = 0;
   }
   const bool biased = EX && a.bias;
@@ -63,14 +65,16 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
 
   float m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
   v16f o[G::NDB];
-  auto issue = [&](int t) {
-    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[t & 1][0], wave, lane);
-    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[t & 1][1], wave, lane);
+  const TrBlocks blocks = EX ? tr_key_blocks(a, s) : TrBlocks();
+  auto issue = [&](int t, int slot) {
+    lk.issue(kp, a.ks, t * TR_ROWS, s.k_len, smem[slot][0], wave, lane);
+    lv.issue(vp, a.vs, t * TR_ROWS, s.k_len, smem[slot][1], wave, lane);
+    if (EX && bits) tr_copy4(bits + (int64_t)(2 * t) * a.mw, wl[slot][wave]);
   };
 
-  auto tile = [&](int t, auto masked_, bool slow) {
+  auto tile = [&](int t, int slot, auto masked_, bool slow) {
     constexpr bool masked = decltype(masked_)::value;
-    const TrAddr<D> kt = at.in(smem[t & 1][0]), vt = at.in(smem[t & 1][1]);
+    const TrAddr<D> kt = at.in(smem[slot][0]), vt = at.in(smem[slot][1]);
     v16f x[2] = {};
 #pragma unroll
     for (int kk = 0; kk < G::NK; ++kk) {
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
       for (int kb = 0; kb < 2; ++kb) {
         const int key0 = t * TR_ROWS + 32 * kb;
         uint32_t w = ~0u;
-        if (EX && bits && key0 < s.k_len) w = bits[(int64_t)(key0 >> 5) * a.mw];
+        if (EX && bits) w = wl[slot][wave][32 * kb + ln];
         tr_hide_keys(x[kb], key0, lim, w, hf);
       }
     }
@@ -156,28 +160,29 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     for (int db = 0; db < G::NDB; ++db)
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[db][v] = 0.0f;
-    if (ntiles > 0) issue(0);
-    int t = 0;
+    int t = EX ? blocks.next(-1, ntiles) : 0, slot = 0, tn = 0;
+    if (t < ntiles) issue(t, 0);
     auto next = [&]() {   // tile t has arrived, the one before is read: the one after goes there
       wait_vmcnt<0>();
       tile_barrier();
-      if (t + 1 < ntiles) issue(t + 1);
+      tn = EX ? blocks.next(t, ntiles) : t + 1;
+      if (tn < ntiles) issue(tn, slot ^ 1);
     };
     // the tiles without hidden keys for the wave, in a loop of their own
-    for (; t < t_mask; ++t) {
+    for (; t < t_mask; t = tn, slot ^= 1) {
       next();
-      tile(t, std::false_type{}, false);
+      tile(t, slot, std::false_type{}, false);
     }
-    for (; t < ntiles; ++t) {
+    for (; t < ntiles; t = tn, slot ^= 1) {
       next();
       if (pass) {
         if (tid < TR_ROWS) poison[tid] = 0;
         __syncthreads();
-        tr_clean<D, DT>(smem[t & 1][0], poison, tid);
-        tr_clean<D, DT>(smem[t & 1][1], poison, tid);
+        tr_clean<D, DT>(smem[slot][0], poison, tid);
+        tr_clean<D, DT>(smem[slot][1], poison, tid);
         __syncthreads();
       }
-      if (t < t_end) tile(t, std::true_type{}, pass != 0);
+      if (t < t_end) tile(t, slot, std::true_type{}, pass != 0);
       if (pass) __syncthreads();
     }
     const bool bad = !(tr_nonfinite(o) == 0.0f);
