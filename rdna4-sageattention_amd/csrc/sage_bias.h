@@ -18,7 +18,8 @@ struct BiasMap {
   int side, near, two_sided, buckets;
   int borders[BIAS_BUCKETS / 2];                  // side - near of them; borders[0] = near
   __host__ __device__ int reach() const { return borders[side - near - 1]; }   // from here on the bucket is the same
-  __device__ __forceinline__ int bucket(int64_t d) const {
+  // (at: the borders, or a copy of them where lanes that look for different ones are served faster)
+  __device__ __forceinline__ int bucket(int64_t d, const int* at) const {
     const int64_t far = two_sided ? (d < 0 ? -d : d) : (d < 0 ? -d : 0);
     const int n = (int)(far < reach() ? far : reach());
     int b = n;
@@ -26,7 +27,7 @@ struct BiasMap {
       int lo = 0, hi = side - near - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (borders[mid] <= n) lo = mid;
+        if (at[mid] <= n) lo = mid;
         else hi = mid - 1;
       }
       b = near + lo;
@@ -49,6 +50,39 @@ __device__ __forceinline__ float bias_value(const void* table, int dtype, int64_
   if (dtype == SAGE_DTYPE_F32) return ((const float*)table)[at];
   const uint32_t u = ((const uint16_t*)table)[at];
   return dtype == SAGE_DTYPE_BF16 ? bf16_lo(u) : f16_lo(u);
+}
+
+// part[b] = f times the sum over bucket b's distances of sums (LDS, n entries; entry x is of distance d0 + x), for a workgroup of
+// THREADS: each wave takes every so manieth 64 buckets, its lanes their ranges, and then sums the buckets that have any one by one.
+template <int THREADS>
+__device__ __forceinline__ void bias_sum_buckets(const BiasMap& m, const float* sums, int64_t d0, int n, float* part, int exponent) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < m.buckets; b0 += 64) {
+    const int b = b0 + lane;
+    int x0 = 0, x1 = 0;
+    if (b < m.buckets) {
+      int lo, hi;
+      m.range(b, lo, hi);
+      if (lo <= hi) {
+        const int64_t y0 = lo <= -m.reach() ? 0 : lo - d0, y1 = hi >= m.reach() ? n : hi + 1 - d0;
+        x0 = (int)max(min(y0, (int64_t)n), (int64_t)0);
+        x1 = (int)max(min(y1, (int64_t)n), (int64_t)0);
+      }
+    }
+    uint64_t some = __ballot(x0 < x1);
+    // (the buckets in turn to the waves)
+    for (int i = 0; some; ++i, some &= some - 1) {
+      if (i % (THREADS / 64) != (int)(threadIdx.x >> 6)) continue;
+      const int l = __builtin_ctzll(some);
+      const int first = __builtin_amdgcn_readlane(x0, l), end = __builtin_amdgcn_readlane(x1, l);
+      float s = 0.0f;
+      for (int x = first + lane; x < end; x += 64) s += sums[x];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+      if (lane == 0) part[b0 + l] = __builtin_ldexpf(s, exponent);
+    }
+    if (threadIdx.x < 64 && b < m.buckets && x0 >= x1) part[b] = 0.0f;
+  }
 }
 
 // vec [H, 2 reach + 1]: the bias by distance, times `mul`

@@ -13,7 +13,7 @@ __global__ __launch_bounds__(BIAS_THREADS) void bias_expand(const void* __restri
   const int64_t x = (int64_t)blockIdx.x * BIAS_THREADS + threadIdx.x;
   if (x >= (int64_t)H * R) return;
   const int h = (int)(x / R), d = (int)(x % R) - m.reach();
-  vec[x] = bias_value(table, dtype, m.bucket(d) * tb + h * th) * mul;
+  vec[x] = bias_value(table, dtype, m.bucket(d, m.borders) * tb + h * th) * mul;
 }
 
 int bias_expand_launch(const void* table, int table_dtype, int64_t tb, int64_t th, int H, const BiasMap& m, float mul, float* vec,
@@ -27,7 +27,8 @@ int bias_expand_launch(const void* table, int table_dtype, int64_t tb, int64_t t
 //
 // A row's values follow from key - query alone: a workgroup looks the buckets of its rows' and columns' distances up once and
 // keeps their values in LDS, in the output's type, as `16 / size` copies, each shifted by one value, so that any run of 16
-// bytes is one aligned LDS read, ready to be stored.  Bound by the stores.
+// bytes is one aligned LDS read, ready to be stored.  Bound by the stores: 24 x 4352 x 4352 in 16
+// bits at 4.9 TB/s (non-temporal ones: 4.0), odd rows of 16 x 2047 x 2511 at 4.7.
 
 struct BiasOut {
   const void* table;
@@ -39,10 +40,9 @@ struct BiasOut {
   const void* offset_at;   // where it is in device memory instead, int64 or int32
   int offset64;
   int rows;                // per workgroup
-  int segs;                // column segments
-  int tpr;                 // threads per row (a power of two)
+  int segs, seg;           // column segments, columns of each
 };
-constexpr int BIAS_SEG = 2048;   // columns per workgroup
+constexpr int BIAS_SEG = 2048;   // columns per workgroup, at most
 constexpr int BIAS_ROWS = 64;    // rows per workgroup, at most
 
 template <int DT> struct BiasElem { using T = uint16_t; };
@@ -57,49 +57,62 @@ template <int DT> __global__ __launch_bounds__(BIAS_THREADS) void bias_write(Bia
   constexpr int N = 16 / sizeof(T);                      // values per store, and copies
   constexpr int W = BIAS_SEG + BIAS_ROWS + 4 * N;        // values per copy (a multiple of N)
   __shared__ __attribute__((aligned(16))) T tab[N][W];
+  __shared__ int borders[BIAS_BUCKETS / 2];
+  __shared__ T learned[BIAS_BUCKETS];
   const int seg = blockIdx.x % a.segs, h = blockIdx.y;
   const int i0 = blockIdx.x / a.segs * a.rows, i1 = min(i0 + a.rows, a.q_len);
-  const int c0 = seg * BIAS_SEG, c1 = min(c0 + BIAS_SEG, a.kv_len);
+  const int c0 = seg * a.seg, c1 = min(c0 + a.seg, a.kv_len);
   int64_t off = a.offset;
   if (a.offset_at) off = a.offset64 ? *(const int64_t*)a.offset_at : (int64_t)*(const int*)a.offset_at;
+  for (int x = threadIdx.x; x < m.buckets; x += BIAS_THREADS) {
+    learned[x] = bias_bits<DT>(bias_value(a.table, a.table_dtype, x * a.tb + h * a.th));
+    if (x < m.side - m.near) borders[x] = m.borders[x];
+  }
+  __syncthreads();
   // value x of the table is that of (row, column) with column - row = x + c0 - N - (i1 - 1)
   const int used = (c1 - c0) + (i1 - i0) + 2 * N;
   for (int x = threadIdx.x; x < used + N; x += BIAS_THREADS) {
     const int64_t d = (int64_t)x + c0 - N - (i1 - 1) - off;
-    const T y = bias_bits<DT>(bias_value(a.table, a.table_dtype, m.bucket(d) * a.tb + h * a.th));
+    const T y = learned[m.bucket(d, borders)];
 #pragma unroll
     for (int c = 0; c < N; ++c)
       if (x >= c) tab[c][x - c] = y;
   }
   __syncthreads();
-  const int t = threadIdx.x & (a.tpr - 1), step = BIAS_THREADS / a.tpr;
-  for (int i = i0 + (int)threadIdx.x / a.tpr; i < i1; i += step) {
+  // the threads side by side over the rows' chunks, a row's at 16-byte boundaries: up to two more than fit it
+  const int chunks = (c1 - c0) / N + 2;
+  int i = i0 + (int)threadIdx.x / chunks, k = (int)threadIdx.x % chunks;
+  const int di = BIAS_THREADS / chunks, dk = BIAS_THREADS % chunks;
+  while (i < i1) {
     T* row = (T*)a.out + ((int64_t)h * a.q_len + i) * a.kv_len;
-    const int skew = (int)(((uintptr_t)(row + c0) & 15u) / sizeof(T));    // chunks begin at 16-byte boundaries
-    for (int k = t;; k += a.tpr) {
-      const int j = c0 - skew + k * N;
-      if (j >= c1) break;
+    const int skew = (int)(((uintptr_t)(row + c0) & 15u) / sizeof(T));
+    const int j = c0 - skew + k * N;
+    if (j < c1) {
       const int x = j - i - c0 + N + (i1 - 1), c = x & (N - 1);
-      const v4i w = *reinterpret_cast<const v4i*>(&tab[c][x - c]);
       if (j >= c0 && j + N <= c1) {
-        *reinterpret_cast<v4i*>(row + j) = w;
+        *reinterpret_cast<v4i*>(row + j) = *reinterpret_cast<const v4i*>(&tab[c][x - c]);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
           if (j + e >= c0 && j + e < c1) row[j + e] = tab[0][x + e];
       }
     }
+    i += di, k += dk;
+    if (k >= chunks) k -= chunks, ++i;
   }
 }
 
 // ---- the table's gradient -----------------------------------------------------------------------------------------------------------
 //
-// Every diagonal (key - query) is in one bucket.  A thread owns `16 / size` neighbouring diagonals and walks down a chunk of
-// rows: its loads move one value to the right from row to row, 16 bytes at any alignment, and neighbouring threads' loads lie
-// side by side.  The workgroup's diagonals are then summed by bucket in LDS, a wave for each bucket, and written as one part;
-// the parts are summed in a second launch.  No atomics: one order.  Bound by the loads.
+// Every diagonal (key - query) is in one bucket.  A thread walks down a chunk of rows N = 16 / size at a time, N columns further
+// right each time: its N x N squares all lie on the same 2 N - 1 diagonals, whose sums it keeps, and its loads are 16 bytes, aligned
+// where rows are.  (A thread with N diagonals of its own, one column further right every row: 107 us where this takes 60, at
+// 16 x 2047 x 2511, whose odd rows cost unaligned loads.)  Neighbours share N - 1 diagonals, which are added in LDS; there the workgroup's diagonals are summed by bucket
+// and written as one part; the parts are summed in a second launch.  No atomics: one order.  Bound by the
+// loads.
 
-constexpr int BIAS_CHUNK = 128;   // rows per workgroup
+constexpr int BIAS_CHUNK = 64;        // rows per workgroup
+constexpr int BIAS_GRAD_THREADS = 256;
 
 struct BiasIn {
   const void* d;
@@ -112,77 +125,73 @@ struct BiasIn {
   float* part;             // [H][chunks * segs][buckets]
 };
 
-template <int DT> __global__ __launch_bounds__(BIAS_THREADS) void bias_grad(BiasIn a, BiasMap m) {
+// rows of a chunk and columns as the squares cover them: the first diagonal of chunk rows i0 .. i1 - 1, and how many
+__host__ __device__ inline int64_t bias_first(int i1, int n) { return -(int64_t)((i1 - 1 + n - 1) / n * n); }
+
+template <int DT> __global__ __launch_bounds__(BIAS_GRAD_THREADS) void bias_grad(BiasIn a, BiasMap m) {
   using T = typename BiasElem<DT>::T;
   constexpr int N = 16 / sizeof(T);
-  constexpr int SEG = BIAS_THREADS * N;
-  __shared__ float sums[SEG];
+  constexpr int SEG = BIAS_GRAD_THREADS * N;
+  __shared__ float sums[SEG + N - 1];
   const int seg = blockIdx.x % a.segs, chunk = blockIdx.x / a.segs, h = blockIdx.y;
   const int i0 = chunk * BIAS_CHUNK, i1 = min(i0 + BIAS_CHUNK, a.q_len);
-  const int64_t g0 = (int64_t)seg * SEG - (i1 - 1);      // key - query index of the workgroup's first diagonal
+  const int64_t g0 = bias_first(i1, N) + (int64_t)seg * SEG;   // key - query index of the first thread's middle diagonal
   const int64_t g = g0 + (int64_t)threadIdx.x * N;
-  float acc[N];
+  float acc[2 * N - 1];
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+  for (int e = 0; e < 2 * N - 1; ++e) acc[e] = 0.0f;
   const T* base = (const T*)a.d + h * a.sh;
-  // rows in which all N keys exist: 0 <= i + g and i + g + N <= kv_len
-  const int64_t f0 = max((int64_t)i0, -g), f1 = min((int64_t)i1, (int64_t)a.kv_len - N - g + 1);
-  auto edge = [&](int64_t i) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int64_t j = i + g + e;
-      if (j >= 0 && j < a.kv_len) {
-        if constexpr (DT == SAGE_DTYPE_F32) acc[e] += ((const float*)base)[i * a.sq + j];
-        else acc[e] += elem_lo<DT>(base[i * a.sq + j]);
-      }
-    }
-  };
   typedef uint32_t v4u_a4 __attribute__((ext_vector_type(4), aligned(4)));
-  auto whole = [&](int64_t i) {
-    if constexpr (DT == SAGE_DTYPE_F32) {
-      const v4u_a4 w = *(const v4u_a4*)(base + i * a.sq + i + g);
+  // (i0 and g are multiples of N, so columns are)
+#pragma unroll 1
+  for (int i = i0; i < i1; i += N) {
+    const int64_t j = i + g;
+    if (j + N <= 0 || j >= a.kv_len) continue;
+    const T* p = base + i * a.sq + j;
+    if (j >= 0 && j + N <= a.kv_len && i + N <= i1) {
+      v4i w[N];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += __uint_as_float(w[e]);
-    } else {
-      const v4i w = load16_2aligned(base + i * a.sq + i + g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[2 * e] += elem_lo<DT>((uint32_t)w[e]);
-        acc[2 * e + 1] += elem_hi<DT>((uint32_t)w[e]);
+      for (int r = 0; r < N; ++r) {
+        if constexpr (DT == SAGE_DTYPE_F32) w[r] = __builtin_bit_cast(v4i, *(const v4u_a4*)(p + r * a.sq));
+        else w[r] = load16_2aligned(p + r * a.sq);
       }
-    }
-  };
-  // before the whole rows only those can touch the tensor whose last key does, after them those whose first does
-  if (f1 > f0) {
-    for (int64_t i = max((int64_t)i0, f0 - N); i < f0; ++i) edge(i);
-#pragma unroll 8
-    for (int64_t i = f0; i < f1; ++i) whole(i);
-    for (int64_t i = f1; i < min((int64_t)i1, f1 + N); ++i) edge(i);
-  } else {
-    for (int64_t i = max((int64_t)i0, -g - N + 1); i < min((int64_t)i1, (int64_t)a.kv_len - g); ++i) edge(i);
-  }
 #pragma unroll
-  for (int e = 0; e < N; ++e) sums[threadIdx.x * N + e] = acc[e];
+      for (int r = 0; r < N; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (DT == SAGE_DTYPE_F32) {
+            acc[e - r + N - 1] += __int_as_float(w[r][e]);
+          } else {
+            acc[2 * e - r + N - 1] += elem_lo<DT>((uint32_t)w[r][e]);
+            acc[2 * e + 1 - r + N - 1] += elem_hi<DT>((uint32_t)w[r][e]);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i + r < i1 && j + e >= 0 && j + e < a.kv_len) {
+            if constexpr (DT == SAGE_DTYPE_F32) acc[e - r + N - 1] += ((const float*)p)[r * a.sq + e];
+            else acc[e - r + N - 1] += elem_lo<DT>(p[r * a.sq + e]);
+          }
+    }
+  }
+  // sums[x]: of diagonal g0 - (N - 1) + x
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int e = 0; e < N - 1; ++e) sums[e] = 0.0f;
+#pragma unroll
+  for (int e = N - 1; e < 2 * N - 1; ++e) sums[threadIdx.x * N + e] = acc[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e) sums[threadIdx.x * N + e] += acc[e];
   __syncthreads();
 
   int64_t off = a.offset;
   if (a.offset_at) off = a.offset64 ? *(const int64_t*)a.offset_at : (int64_t)*(const int*)a.offset_at;
   float* part = a.part + ((int64_t)h * (a.chunks * a.segs) + blockIdx.x) * m.buckets;
-  const int lane = threadIdx.x & 63;
-  for (int b = threadIdx.x >> 6; b < m.buckets; b += BIAS_THREADS / 64) {
-    int lo, hi;
-    m.range(b, lo, hi);
-    // as diagonals of the workgroup: d = g0 + x - off
-    int64_t x0 = lo <= -m.reach() ? 0 : lo - g0 + off, x1 = hi >= m.reach() ? SEG : hi + 1 - g0 + off;
-    if (lo > hi) x1 = x0;
-    x0 = max(x0, (int64_t)0);
-    x1 = min(x1, (int64_t)SEG);
-    float s = 0.0f;
-    for (int64_t x = x0 + lane; x < x1; x += 64) s += sums[x];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-    if (lane == 0) part[b] = s;
-  }
+  bias_sum_buckets<BIAS_GRAD_THREADS>(m, sums, g0 - (N - 1) - off, SEG + N - 1, part, 0);
 }
 
 // One workgroup per head and 64 buckets: four waves each sum a quarter of the parts in fp64.
@@ -318,9 +327,8 @@ extern "C" int sage_relative_bias(const void* table, int table_dtype, int64_t tb
   a.table = table, a.table_dtype = table_dtype, a.tb = tb, a.th = th, a.out = out, a.q_len = q_len, a.kv_len = kv_len;
   a.offset = offset, a.offset_at = offset_at, a.offset64 = offset64;
   a.segs = (kv_len + BIAS_SEG - 1) / BIAS_SEG;
+  a.seg = ((kv_len + a.segs - 1) / a.segs + 127) / 128 * 128;   // (equal ones: 2511 columns as 2048 and 463 take 72 us for 16 x 2047 rows)
   a.rows = q_len < BIAS_ROWS ? q_len : BIAS_ROWS;
-  const int per = dtype == SAGE_DTYPE_F32 ? 4 : 8, most = (kv_len < BIAS_SEG ? kv_len : BIAS_SEG) / per + 2;
-  for (a.tpr = 1; a.tpr < most && a.tpr < BIAS_THREADS; a.tpr *= 2) {}
   const int64_t blocks = (int64_t)((q_len + a.rows - 1) / a.rows) * a.segs;
   SAGE_REQUIRE(blocks <= 0x7FFFFFFF, "sage_relative_bias: too large");
   const dim3 grid((unsigned)blocks, H);
@@ -331,14 +339,22 @@ extern "C" int sage_relative_bias(const void* table, int table_dtype, int64_t tb
   return check_launch("bias_write");
 }
 
+namespace sage {
+// workgroups side by side for a chunk's diagonals (the first chunk's are the most)
+static int bias_segs(int q_len, int kv_len, int dtype) {
+  const int n = dtype == SAGE_DTYPE_F32 ? 4 : 8, seg = BIAS_GRAD_THREADS * n;
+  const int64_t width = -bias_first(q_len < BIAS_CHUNK ? q_len : BIAS_CHUNK, n) + kv_len;
+  return (int)((width + seg - 1) / seg);
+}
+}  // namespace sage
+
 extern "C" int sage_relative_bias_grad_workspace(int H, int buckets, int q_len, int kv_len, int dtype, int64_t* workspace_bytes) {
   using namespace sage;
   clear_error();
   SAGE_REQUIRE(workspace_bytes, "sage_relative_bias_grad_workspace: workspace_bytes is NULL");
   SAGE_REQUIRE(H > 0 && buckets > 0 && q_len > 0 && kv_len > 0, "sage_relative_bias_grad_workspace: sizes must be positive");
-  const int64_t seg = BIAS_THREADS * (dtype == SAGE_DTYPE_F32 ? 4 : 8), rows = q_len < BIAS_CHUNK ? q_len : BIAS_CHUNK;
-  const int64_t segs = (kv_len + rows - 1 + seg - 1) / seg, chunks = ((int64_t)q_len + BIAS_CHUNK - 1) / BIAS_CHUNK;
-  *workspace_bytes = 4 * segs * chunks * H * buckets;
+  const int64_t chunks = ((int64_t)q_len + BIAS_CHUNK - 1) / BIAS_CHUNK;
+  *workspace_bytes = 4 * (int64_t)bias_segs(q_len, kv_len, dtype) * chunks * H * buckets;
   return SAGE_OK;
 }
 
@@ -361,16 +377,15 @@ extern "C" int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq
   BiasIn a = {};
   a.d = dbias, a.sh = sh, a.sq = sq, a.q_len = q_len, a.kv_len = kv_len;
   a.offset = offset, a.offset_at = offset_at, a.offset64 = offset64;
-  const int seg = BIAS_THREADS * (dtype == SAGE_DTYPE_F32 ? 4 : 8), rows = q_len < BIAS_CHUNK ? q_len : BIAS_CHUNK;
-  a.segs = (int)(((int64_t)kv_len + rows - 1 + seg - 1) / seg);
+  a.segs = bias_segs(q_len, kv_len, dtype);
   a.chunks = (q_len + BIAS_CHUNK - 1) / BIAS_CHUNK;
   a.part = (float*)workspace;
   SAGE_REQUIRE((int64_t)a.segs * a.chunks <= 0x7FFFFFFF, "sage_relative_bias_grad: too large");
   const dim3 grid(a.segs * a.chunks, H);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == SAGE_DTYPE_BF16) bias_grad<SAGE_DTYPE_BF16><<<grid, BIAS_THREADS, 0, st>>>(a, m);
-  else if (dtype == SAGE_DTYPE_F16) bias_grad<SAGE_DTYPE_F16><<<grid, BIAS_THREADS, 0, st>>>(a, m);
-  else bias_grad<SAGE_DTYPE_F32><<<grid, BIAS_THREADS, 0, st>>>(a, m);
+  if (dtype == SAGE_DTYPE_BF16) bias_grad<SAGE_DTYPE_BF16><<<grid, BIAS_GRAD_THREADS, 0, st>>>(a, m);
+  else if (dtype == SAGE_DTYPE_F16) bias_grad<SAGE_DTYPE_F16><<<grid, BIAS_GRAD_THREADS, 0, st>>>(a, m);
+  else bias_grad<SAGE_DTYPE_F32><<<grid, BIAS_GRAD_THREADS, 0, st>>>(a, m);
   if (int rc = check_launch("bias_grad")) return rc;
   return bias_reduce_launch(a.part, (int64_t)a.segs * a.chunks, H, m, dtable, table_dtype, tb, th, st);
 }

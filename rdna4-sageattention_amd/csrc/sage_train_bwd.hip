@@ -324,15 +324,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
       by_distance[x] = (by_distance[x] + by_distance[R + x]) + (by_distance[2 * R + x] + by_distance[3 * R + x]);
     __syncthreads();
     float* part = a.bias_part + (s.h * a.parts + s.part) * map.buckets;
-    for (int b = wave; b < map.buckets; b += TR_THREADS / 64) {
-      int lo, hi;
-      map.range(b, lo, hi);
-      float y = 0.0f;
-      for (int x = lo + lane; x <= hi; x += 64) y += by_distance[a.reach + x];
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) y += __shfl_xor(y, o);
-      if (lane == 0) part[b] = __builtin_ldexpf(y, -ex);
-    }
+    bias_sum_buckets<TR_THREADS>(map, by_distance, -a.reach, R, part, -ex);
   }
 }
 
