@@ -125,7 +125,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     mx = max_xor32_f32(mx);
     if (!EX) mx *= a.c;
     if (__ballot(mx > m + FWD_LAG) != 0) {
-      const float m_new = fmaxf(m, mx);
+      const float m_new = mx > m + FWD_LAG ? mx : m;   // (each row by itself: its bits follow from what it sees alone)
       const float corr = m == m_new ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
       l *= corr;
 #pragma unroll
