@@ -337,18 +337,18 @@ int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype
  * covers, and all rows where offsets fall or pass the totals, are written as 0 (their lse stays as it is).
  *
  * sage_train_workspace: the bytes of the state, which the forward pass writes and the backward pass reads, and of the backward
- * pass' workspace; both 256-byte aligned.  sage_train_bwd: dq NULL (then dtable too) or dk and dv NULL leave those out; dtable
+ * pass' workspace; both 256-byte aligned.  keep: 0 where no backward pass comes (its part of the state, as large as out, falls away).  sage_train_bwd: dq NULL (then dtable too) or dk and dv NULL leave those out; dtable
  * NULL leaves the table's gradient out.  Equal inputs give equal bits.
  */
 int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, int Skv, int D, int has_mask, int64_t msb, int64_t msh,
-                         int64_t msq, int buckets, int two_sided, const int* borders, int64_t* state_bytes,
+                         int64_t msq, int buckets, int two_sided, const int* borders, int keep, int64_t* state_bytes,
                          int64_t* workspace_bytes);
 int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* k, int64_t ksb, int64_t kss, int64_t ksh,
                    const void* v, int64_t vsb, int64_t vss, int64_t vsh, void* out, int64_t osb, int64_t oss, int64_t osh,
                    float* lse, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype, int causal, float sm_scale,
                    const int* cu_q, const int* cu_k, const void* mask, int64_t msb, int64_t msh, int64_t msq, int64_t msk,
                    const void* table, int table_dtype, int64_t tb, int64_t th, int buckets, int two_sided, const int* borders,
-                   void* state, int64_t state_bytes, void* stream);
+                   int keep, void* state, int64_t state_bytes, void* stream);
 int sage_train_bwd(const void* dout, int64_t gsb, int64_t gss, int64_t gsh, const void* q, int64_t qsb, int64_t qss, int64_t qsh,
                    const void* k, int64_t ksb, int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss, int64_t vsh,
                    const void* out, int64_t osb, int64_t oss, int64_t osh, const float* lse, void* dq, int64_t dqb, int64_t dqs,

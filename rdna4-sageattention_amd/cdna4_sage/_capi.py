@@ -68,9 +68,9 @@ SIGNATURES = {
     "sage_relative_bias": ([_P, _I, _L, _L, _I, _I, _I, _P, _I, _I, _L, _P, _I, _P, _I, _P], _I),
     "sage_relative_bias_grad_workspace": ([_I, _I, _I, _I, _I, _P], _I),
     "sage_relative_bias_grad": ([_P, _L, _L, _I, _I, _I, _I, _P, _I, _I, _L, _P, _I, _P, _I, _L, _L, _P, _L, _P], _I),
-    "sage_train_workspace": ([_I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _L, _I, _I, _P, _P, _P], _I),
+    "sage_train_workspace": ([_I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _L, _I, _I, _P, _I, _P, _P], _I),
     "sage_train_fwd": ([_P, _L, _L, _L] * 4 + [_P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _L, _L, _L,
-                                               _P, _I, _L, _L, _I, _I, _P, _P, _L, _P], _I),
+                                               _P, _I, _L, _L, _I, _I, _P, _I, _P, _L, _P], _I),
     "sage_train_bwd": ([_P, _L, _L, _L] * 5 + [_P] + [_P, _L, _L, _L] * 3 +
                        [_I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _L, _L, _L, _P, _I, _L, _L, _I, _I, _P, _P, _L, _P, _L,
                         _P], _I),
@@ -189,13 +189,13 @@ def bias_borders(buckets: int, two_sided: bool, max_distance: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def train_workspace(packed: bool, B: int, H: int, Hkv: int, Sq: int, Skv: int, D: int, mask, bias):
+def train_workspace(packed: bool, B: int, H: int, Hkv: int, Sq: int, Skv: int, D: int, mask, bias, keep: bool):
     """(state bytes, workspace bytes) of sage_train_fwd / sage_train_bwd; mask: None or whether it has a batch, head and
-    row axis; bias: None or (buckets, two_sided, max_distance).  Host arithmetic only."""
+    row axis; bias: None or (buckets, two_sided, max_distance); keep: a backward pass comes.  Host arithmetic only."""
     state, ws = ctypes.c_int64(), ctypes.c_int64()
     m = (0, 0, 0, 0) if mask is None else (1, *mask)
     b = (0, 0, None) if bias is None else (bias[0], int(bias[1]), bias_borders(*bias))
-    call("sage_train_workspace", int(packed), B, H, Hkv, Sq, Skv, D, *m, *b, ctypes.byref(state), ctypes.byref(ws))
+    call("sage_train_workspace", int(packed), B, H, Hkv, Sq, Skv, D, *m, *b, int(keep), ctypes.byref(state), ctypes.byref(ws))
     return state.value, ws.value
 
 

@@ -114,19 +114,19 @@ def _table_args(table, bias):
     return table.data_ptr(), TABLE_DTYPES[table.dtype], *table.stride(), n, int(two), _capi.bias_borders(n, two, far)
 
 
-def _sizes(shape, bias, axes, cu_q):
+def _sizes(shape, bias, axes, cu_q, keep):
     """(state bytes, workspace bytes, batch); raises Unsupported for a bias that reaches too far for the kernels."""
     B, H, Hkv, Sq, Skv, D, _ = shape
     if cu_q is not None:
         B = cu_q.shape[0] - 1
     try:
-        return (*_capi.train_workspace(cu_q is not None, B, H, Hkv, Sq, Skv, D, axes, bias), B)
+        return (*_capi.train_workspace(cu_q is not None, B, H, Hkv, Sq, Skv, D, axes, bias, keep), B)
     except _capi.SageError as e:
         raise Unsupported(str(e)) from e
 
 
-def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance):
-    """(out, lse, state, what the kernels loaded of q, k and v, the call's plan for the backward pass)."""
+def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance, keep):
+    """(out, lse, state, what the kernels loaded of q, k and v, the call's plan for the backward pass); keep: one comes."""
     packed = cu_q is not None
     shape = _check(q, k, v, layout, packed)
     B, H, Hkv, Sq, Skv, D, gpu = shape
@@ -141,7 +141,7 @@ def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, caus
         out.zero_()
         lse.fill_(float("-inf"))
         return out, lse, torch.empty(0, dtype=torch.uint8, device=q.device), (q, k, v), (shape, bias, axes, 0, 0, 0)
-    state_bytes, ws_bytes, nb = _sizes(shape, bias, axes, cu_q)
+    state_bytes, ws_bytes, nb = _sizes(shape, bias, axes, cu_q, keep)
     state = torch.empty(state_bytes, dtype=torch.uint8, device=q.device)
     q, sq = _strides(q, layout, packed)
     k, sk = _strides(k, layout, packed)
@@ -150,7 +150,7 @@ def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, caus
     _capi.call_on(gpu, "sage_train_fwd", q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, out.data_ptr(), *so,
                   lse.data_ptr(), nb, H, Hkv, Sq, Skv, D, DTYPES[q.dtype], causal, sm_scale,
                   None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
-                  None if mask is None else mask.data_ptr(), *ms, *_table_args(table, bias),
+                  None if mask is None else mask.data_ptr(), *ms, *_table_args(table, bias), keep,
                   state.data_ptr() if state_bytes else None, state_bytes)
     return out, lse, state, (q, k, v), (shape, bias, axes, state_bytes, ws_bytes, nb)
 
@@ -198,7 +198,7 @@ def backward_plan(q, k, v, layout, table, cu_q, bidirectional, max_distance, axe
     bias = None if table is None else _bias(table, shape[1], bidirectional, max_distance, shape[6])
     if q.numel() == 0 or k.numel() == 0:
         return shape, bias, axes, 0, 0, 0
-    return (shape, bias, axes, *_sizes(shape, bias, axes, cu_q))
+    return (shape, bias, axes, *_sizes(shape, bias, axes, cu_q, True))
 
 
 class _Train(torch.autograd.Function):
@@ -206,7 +206,7 @@ class _Train(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, attn_mask, cu_q, cu_k, *how):
-        out, lse, state, used, ctx.plan = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how)
+        out, lse, state, used, ctx.plan = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how, True)
         ctx.save_for_backward(*used, out, lse, state, table, cu_q, cu_k)
         ctx.how = how[:3]
         ctx.mark_non_differentiable(lse)
@@ -226,14 +226,15 @@ class _Train(torch.autograd.Function):
 def _attention(q, k, v, table, attn_mask, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance, return_lse):
     ts = [t for t in (q, k, v, table) if t is not None]
     how = (layout, _scale(sm_scale), bool(causal), bool(bidirectional), int(max_distance))
+    recording = torch.is_grad_enabled() and any(t.requires_grad for t in ts)
     if _plain_eager(*ts, grad=True):
-        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        if recording:
             out, lse = _Train.apply(q, k, v, table, attn_mask, cu_q, cu_k, *how)
         else:
-            out, lse = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how)[:2]
+            out, lse = forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, *how, False)[:2]
     else:
         refuse_tangents("attention_train", *ts)
-        out, lse, _ = ops.attention_train(q, k, v, attn_mask, table, cu_q, cu_k, *how)
+        out, lse, _ = ops.attention_train(q, k, v, attn_mask, table, cu_q, cu_k, *how, recording)
     return (out, lse) if return_lse else out
 
 

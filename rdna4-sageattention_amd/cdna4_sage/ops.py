@@ -179,17 +179,18 @@ def _mask_axes(attn_mask, q, k, layout):
 @torch.library.custom_op("cdna4_sage::attention_train", mutates_args=())
 def attention_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn_mask: Optional[torch.Tensor],
                     table: Optional[torch.Tensor], cu_q: Optional[torch.Tensor], cu_k: Optional[torch.Tensor], layout: str,
-                    sm_scale: float, is_causal: bool, bidirectional: bool,
-                    max_distance: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Attention on 16-bit inputs: (out, lse, the state that the backward pass reads); packed sequences where cu_q is given."""
+                    sm_scale: float, is_causal: bool, bidirectional: bool, max_distance: int,
+                    keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Attention on 16-bit inputs: (out, lse, the state that the backward pass reads, where `keep` says that one comes); packed
+    sequences where cu_q is given."""
     from . import _train
 
     return _train.forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, is_causal, bidirectional,
-                                 max_distance)[:3]
+                                 max_distance, keep)[:3]
 
 
 @attention_train.register_fake
-def _fake_attention_train(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, is_causal, bidirectional, max_distance):
+def _fake_attention_train(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, is_causal, bidirectional, max_distance, keep):
     from . import _capi, _rope
 
     packed = cu_q is not None
@@ -204,7 +205,7 @@ def _fake_attention_train(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scal
     if q.numel() != 0 and k.numel() != 0:
         state = _capi.train_workspace(packed, int(B), int(H), int(Hkv), int(Sq), int(Skv), int(D),
                                       tuple(_mask_axes(attn_mask, q, k, layout)) or None,
-                                      None if table is None else (int(table.shape[0]), bidirectional, max_distance))[0]
+                                      None if table is None else (int(table.shape[0]), bidirectional, max_distance), keep)[0]
     return out, lse, q.new_empty((state,), dtype=torch.uint8)
 
 
@@ -233,7 +234,9 @@ def _fake_attention_train_backward(dout, q, k, v, out, lse, state, table, cu_q, 
 
 
 def _train_setup(ctx, inputs, output):
-    q, k, v, attn_mask, table, cu_q, cu_k, *ctx.how = inputs
+    q, k, v, attn_mask, table, cu_q, cu_k, *ctx.how, keep = inputs
+    if not keep:
+        raise RuntimeError("cdna4_sage::attention_train: keep=True is needed for a backward pass")
     ctx.axes = _mask_axes(attn_mask, q, k, ctx.how[0])
     ctx.save_for_backward(q, k, v, *output, table, cu_q, cu_k)
     ctx.mark_non_differentiable(output[1], output[2])
@@ -241,7 +244,7 @@ def _train_setup(ctx, inputs, output):
 
 def _train_backward(ctx, dout, *_):
     dq, dk, dv, dt = attention_train_backward(dout, *ctx.saved_tensors, *ctx.how, ctx.axes)
-    return (dq, dk, dv, None, dt if ctx.saved_tensors[6] is not None else None) + (None,) * 7
+    return (dq, dk, dv, None, dt if ctx.saved_tensors[6] is not None else None) + (None,) * 8
 
 
 attention_train.register_autograd(_train_backward, setup_context=_train_setup)

@@ -48,6 +48,9 @@ struct TrainArgs {
   int causal;                      // bottom-right: query i of a sequence sees keys j <= i + (kv_len - q_len)
   float scale, c;                  // sm_scale, sm_scale * log2(e)
   float* lse;                      // fp32 [B, H, Sq] (packed [H, Sq]), natural log
+  // what the rounding of out to 16 bits took away, in 16 bits, [B, H, Sq, D] (packed [H, Sq, D]); NULL where no backward pass comes.
+  // D_i is the sum of do_i . o_i, whose terms' roundings would be the largest part of ds' error in rows of few keys.
+  uint16_t* lo;
   // backward: -lse / sm_scale and -D of every row, where the sums of the scores and of dout . v begin; -inf and 0 in the padding: rows of `pad` entries per (b, h) (packed: per
   // h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
   float *nl, *nd;

@@ -145,11 +145,11 @@ __global__ __launch_bounds__(TR_THREADS) void train_mask_any(const uint8_t* __re
 // Where everything lies in the state that the forward pass leaves to the backward pass, and in its workspace.
 struct TrainLayout {
   int q_tiles, k_tiles, mask_b, mask_h, row_pad, words, blocks, chunks, aw, tw;
-  int64_t q_tab, k_tab, bits, shows, any, any_t, vec, state;      // byte offsets; bounds at 0
+  int64_t q_tab, k_tab, bits, shows, any, any_t, vec, lo, state;      // byte offsets; bounds at 0
   int64_t pad, nl, nd, norms, parts, part, work;
 };
 static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool mask, bool mb, bool mh, bool mq, int reach,
-                                int buckets) {
+                                int buckets, int keep) {   // keep: D where a backward pass comes, else 0
   TrainLayout l = {};
   auto take = [](int64_t& at, int64_t n) {
     const int64_t r = at;
@@ -174,6 +174,7 @@ static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool
     l.any_t = take(at, bh * l.chunks * l.tw * 8);
   }
   if (reach) l.vec = take(at, (int64_t)H * (2 * reach + 1) * 4);
+  if (keep) l.lo = take(at, (int64_t)(packed ? 1 : B) * H * Sq * keep * 2);
   l.state = at;
   at = 0;
   l.pad = packed ? (int64_t)Sq / 64 * 64 + 64 * ((int64_t)B + 1) : ((int64_t)Sq + 63) / 64 * 64;
@@ -220,7 +221,7 @@ static int train_dispatch(bool bwd, const TrainArgs& a, const BiasMap& m, int D,
 // What both passes check and fill in alike
 static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& m, int B, int H, int Hkv, int Sq, int Skv, int D,
                         int dtype, int causal, float sm_scale, const int* cu_q, const int* cu_k, bool mask, int64_t msb,
-                        int64_t msh, int64_t msq, int buckets, int two_sided, const int* borders, int table_dtype, void* state,
+                        int64_t msh, int64_t msq, int buckets, int two_sided, const int* borders, int table_dtype, int keep, void* state,
                         int64_t state_bytes) {
   if (int rc = train_sizes(who, B, H, Hkv, Sq, Skv, D, dtype)) return rc;
   SAGE_REQUIRE((cu_q != nullptr) == (cu_k != nullptr), "%s: cu_q and cu_k go together", who);
@@ -233,13 +234,14 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
     if (reach > TR_REACH)
       return fail(SAGE_ERR_UNSUPPORTED, "%s: the last bucket begins at distance %d (at most %d)", who, reach, TR_REACH);
   }
-  l = train_layout(cu_q != nullptr, B, H, Sq, Skv, mask, msb != 0, msh != 0, msq != 0, reach, buckets);
+  l = train_layout(cu_q != nullptr, B, H, Sq, Skv, mask, msb != 0, msh != 0, msq != 0, reach, buckets, keep ? D : 0);
   SAGE_REQUIRE(l.state == 0 || (state && ((uintptr_t)state & 255u) == 0 && state_bytes >= l.state),
                "%s: a state of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)l.state, (long long)state_bytes);
   a.B = B, a.H = H, a.Hkv = Hkv, a.Sq = Sq, a.Skv = Skv, a.q_tiles = l.q_tiles, a.k_tiles = l.k_tiles, a.causal = causal != 0;
   a.scale = sm_scale > 0.0f ? sm_scale : 1.0f / __builtin_sqrtf((float)D);
   a.c = (float)((double)a.scale * 1.4426950408889634);
   char* base = (char*)state;
+  if (keep) a.lo = (uint16_t*)(base + l.lo);
   if (cu_q) a.cu_q = cu_q, a.cu_k = cu_k, a.q_tab = (const int2*)(base + l.q_tab), a.k_tab = (const int2*)(base + l.k_tab);
   if (mask) {
     const int64_t per = (int64_t)l.row_pad * l.words;
@@ -257,8 +259,8 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
 }  // namespace sage
 
 extern "C" int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, int Skv, int D, int has_mask, int64_t msb,
-                                    int64_t msh, int64_t msq, int buckets, int two_sided, const int* borders, int64_t* state_bytes,
-                                    int64_t* workspace_bytes) {
+                                    int64_t msh, int64_t msq, int buckets, int two_sided, const int* borders, int keep,
+                                    int64_t* state_bytes, int64_t* workspace_bytes) {
   using namespace sage;
   clear_error();
   SAGE_REQUIRE(state_bytes && workspace_bytes, "sage_train_workspace: a result is NULL");
@@ -271,7 +273,7 @@ extern "C" int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, i
     if (reach > TR_REACH)
       return fail(SAGE_ERR_UNSUPPORTED, "sage_train_workspace: the last bucket begins at distance %d (at most %d)", reach, TR_REACH);
   }
-  const TrainLayout l = train_layout(packed != 0, B, H, Sq, Skv, has_mask != 0, msb != 0, msh != 0, msq != 0, reach, buckets);
+  const TrainLayout l = train_layout(packed != 0, B, H, Sq, Skv, has_mask != 0, msb != 0, msh != 0, msq != 0, reach, buckets, keep ? D : 0);
   *state_bytes = l.state;
   *workspace_bytes = l.work;
   return SAGE_OK;
@@ -282,14 +284,14 @@ extern "C" int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t q
                               int64_t oss, int64_t osh, float* lse, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype,
                               int causal, float sm_scale, const int* cu_q, const int* cu_k, const void* mask, int64_t msb,
                               int64_t msh, int64_t msq, int64_t msk, const void* table, int table_dtype, int64_t tb, int64_t th,
-                              int buckets, int two_sided, const int* borders, void* state, int64_t state_bytes, void* stream) {
+                              int buckets, int two_sided, const int* borders, int keep, void* state, int64_t state_bytes, void* stream) {
   using namespace sage;
   clear_error();
   TrainArgs a = {};
   TrainLayout l;
   BiasMap m = {};
   if (int rc = train_common("sage_train_fwd", a, l, m, B, H, Hkv, Sq, Skv, D, dtype, causal, sm_scale, cu_q, cu_k, mask != nullptr,
-                            msb, msh, msq, buckets, two_sided, borders, table_dtype, state, state_bytes))
+                            msb, msh, msq, buckets, two_sided, borders, table_dtype, keep, state, state_bytes))
     return rc;
   const TrainTensor ts[] = {{q, qsb, qss, qsh, "q"}, {k, ksb, kss, ksh, "k"}, {v, vsb, vss, vsh, "v"}, {out, osb, oss, osh, "out"}};
   if (int rc = train_tensors("sage_train_fwd", ts, 4)) return rc;
@@ -338,7 +340,7 @@ extern "C" int sage_train_bwd(const void* dout, int64_t gsb, int64_t gss, int64_
   TrainLayout l;
   BiasMap m = {};
   if (int rc = train_common("sage_train_bwd", a, l, m, B, H, Hkv, Sq, Skv, D, dtype, causal, sm_scale, cu_q, cu_k, has_mask != 0,
-                            msb, msh, msq, buckets, two_sided, borders, table_dtype, (void*)state, state_bytes))
+                            msb, msh, msq, buckets, two_sided, borders, table_dtype, 1, (void*)state, state_bytes))
     return rc;
   const TrainTensor ts[] = {{q, qsb, qss, qsh, "q"},    {k, ksb, kss, ksh, "k"},       {v, vsb, vss, vsh, "v"},
                             {out, osb, oss, osh, "out"}, {dout, gsb, gss, gsh, "dout"}, {dq, dqb, dqs, dqh, "dq"},

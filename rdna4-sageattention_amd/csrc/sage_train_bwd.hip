@@ -53,14 +53,16 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
     const int end = min(s.c0 + TR_COLS, (s.q_len + 63) / 64 * 64);
     const uint16_t* op = a.o + (a.cu_q ? 0 : s.b * a.ob) + s.qr * a.os + s.h * a.oh + l * 8;
     const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * a.gh + l * 8;
+    const uint16_t* lp = a.lo + lse_at * D + l * 8;
     for (int i = s.c0 + r; i < end; i += ROWS) {
       float d = 0.0f, g2 = 0.0f;
       if (i < s.q_len && has) {
         const v4i x = *reinterpret_cast<const v4i*>(op + i * a.os), g = *reinterpret_cast<const v4i*>(gp + i * a.gs);
+        const v4i y = *reinterpret_cast<const v4i*>(lp + (int64_t)i * D);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float g0 = elem_lo<DT>(g[e]), g1 = elem_hi<DT>(g[e]);
-          d = __builtin_fmaf(elem_lo<DT>(x[e]), g0, __builtin_fmaf(elem_hi<DT>(x[e]), g1, d));
+          d = __builtin_fmaf(elem_lo<DT>(x[e]) + elem_lo<DT>(y[e]), g0, __builtin_fmaf(elem_hi<DT>(x[e]) + elem_hi<DT>(y[e]), g1, d));
           if (DT == DT_F16) g2 = __builtin_fmaf(g0, g0, __builtin_fmaf(g1, g1, g2));
         }
       }
@@ -310,8 +312,8 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   for (int db = 0; db < G::NDB; ++db) tr_store<DT>(dq[db], f, op + 32 * db, hf, on);
 
   if (want_part) {
-    // The row sums of ds are 0, but D holds the rounding of o to 16 bits and of its weights: sum_j ds = D' - D, exactly the error of
-    // D.  In a far bucket, which holds most of a long row's weight, it would not average out: it is taken from there.
+    // The row sums of ds are 0, but D holds the rounding of o's weights to 16 bits: sum_j ds = D' - D, exactly the error of D.  In a
+    // far bucket, which holds most of a long row's weight, it would not average out: it is taken from there.
     const float delta = add_xor32_f32(fnear + flo + fhi);
     flo -= delta * __builtin_ldexpf(plo, -ex);
     fhi -= delta * __builtin_ldexpf(phi, -ex);

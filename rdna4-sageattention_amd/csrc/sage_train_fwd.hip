@@ -195,6 +195,20 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   uint16_t* op = a.out + s.b * (a.cu_q ? 0 : a.ob) + (s.qr + ir) * a.os + s.h * a.oh;
 #pragma unroll
   for (int db = 0; db < G::NDB; ++db) tr_store<DT>(o[db], inv, op + 32 * db, hf, on);
+  if (a.lo) {
+    // the same channels' remainders: as many as there are, in 16 bits again
+    uint16_t* lp = a.lo + ((a.cu_q ? (int64_t)s.h * a.Sq + s.qr : ((int64_t)s.b * a.H + s.h) * a.Sq) + ir) * D;
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db) {
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        const int w = tr_pack<DT>(o[db][v] * inv, o[db][v + 1] * inv);
+        o[db][v] = __builtin_fmaf(o[db][v], inv, -elem_lo<DT>((uint32_t)w));
+        o[db][v + 1] = __builtin_fmaf(o[db][v + 1], inv, -elem_hi<DT>((uint32_t)w));
+      }
+      tr_store<DT>(o[db], 1.0f, lp + 32 * db, hf, on);
+    }
+  }
   if (on && hf == 0) {
     const float lse = l == 0.0f ? -INFINITY : (m - FWD_SHIFT<DT> + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     a.lse[(a.cu_q ? (int64_t)s.h * a.Sq + s.qr : ((int64_t)s.b * a.H + s.h) * a.Sq) + i] = lse;

@@ -210,7 +210,7 @@ def test_traced(dev, layout):
     ops = torch.ops.cdna4_sage
     t = [x.clone().requires_grad_() for x in (q, k, v, table)]
     # (the full comparison of outputs would also compare what lies between the parts of the state, which nothing writes)
-    torch.library.opcheck(ops.attention_train.default, (*t[:3], mask, t[3], None, None, layout, 0.0, False, True, 128),
+    torch.library.opcheck(ops.attention_train.default, (*t[:3], mask, t[3], None, None, layout, 0.0, False, True, 128, True),
                           test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
     torch.library.opcheck(ops.relative_bias.default, (t[3], 5, 9, True, 128, torch.float32, 4, None))
 

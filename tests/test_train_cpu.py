@@ -89,15 +89,14 @@ def _ints(*x):
 T = lambda n: {f"{n}": P, f"{n}b": 8 * 64 * 2, f"{n}s": 64 * 2, f"{n}h": 64}  # noqa: E731
 SIZES = dict(B=1, H=2, Hkv=2, Sq=8, Skv=8, D=64, dtype=0, causal=0, sm=0.0, cu_q=None, cu_k=None)
 FWD = dict(**T("q"), **T("k"), **T("v"), **T("o"), lse=P, **SIZES, mask=None, msb=0, msh=0, msq=0, msk=0, table=None, tdtype=0, tb=0,
-           th=0, buckets=0, two=0, borders=None, state=None, state_bytes=0, stream=None)
+           th=0, buckets=0, two=0, borders=None, keep=0, state=None, state_bytes=0, stream=None)
 BWD = dict(**T("g"), **T("q"), **T("k"), **T("v"), **T("o"), lse=P, **T("dq"), **T("dk"), **T("dv"), **SIZES, has_mask=0, msb=0, msh=0,
-           msq=0, dtable=None, tdtype=0, tb=0, th=0, buckets=0, two=0, borders=None, state=None, state_bytes=0, ws=P, ws_bytes=1 << 20,
-           stream=None)
+           msq=0, dtable=None, tdtype=0, tb=0, th=0, buckets=0, two=0, borders=None, state=P, state_bytes=1 << 20, ws=P, ws_bytes=1 << 20, stream=None)
 COMMON = [
     (dict(q=None), 1, "q is NULL"), (dict(k=P + 8), 1, "k must be"), (dict(vs=7), 1, "v must be"), (dict(lse=None), 1, "lse"),
     (dict(H=3), 1, "multiple"), (dict(D=80), 2, "head_dim 80"), (dict(dtype=2), 2, "dtype"), (dict(Sq=0), 1, "positive"),
     (dict(sm=-1.0), 1, "sm_scale"), (dict(sm=float("nan")), 1, "sm_scale"), (dict(sm=float("inf")), 1, "sm_scale"),
-    (dict(cu_q=P), 1, "go together"), (dict(cu_q=P, cu_k=P), 1, "state"),
+    (dict(cu_q=P), 1, "go together"), (dict(cu_q=P, cu_k=P, state=None), 1, "state"),
     (dict(buckets=32, borders=None), 1, "borders"), (dict(buckets=1, borders=_ints(1)), 1, "buckets"),
     (dict(buckets=4, two=1, borders=_ints(5)), 1, "borders"),
     (dict(buckets=4, borders=_ints(2, 1)), 1, "must not fall"),
@@ -107,7 +106,7 @@ COMMON = [
 
 @built
 @pytest.mark.parametrize("change,code,message", COMMON + [
-    (dict(o=None), 1, "out is NULL"), (dict(mask=P), 1, "state"), (dict(mask=P, cu_q=P, cu_k=P), 1, "no mask"),
+    (dict(o=None), 1, "out is NULL"), (dict(mask=P), 1, "state"), (dict(keep=1), 1, "state"), (dict(mask=P, cu_q=P, cu_k=P), 1, "no mask"),
     (dict(buckets=4, borders=_ints(2, 5), state=P, state_bytes=1 << 20), 1, "table is NULL"),
     (dict(mask=P, state=P + 16, state_bytes=1 << 20), 1, "256-byte"),
 ])
@@ -119,7 +118,7 @@ def test_forward_entry_refuses(change, code, message):
 @pytest.mark.parametrize("change,code,message", COMMON + [
     (dict(g=None), 1, "dout is NULL"), (dict(dqs=4), 1, "dq must be"), (dict(dk=None), 1, "go together"), (dict(ws=None), 1, "workspace"),
     (dict(ws_bytes=100), 1, "workspace"), (dict(dq=None, dk=None, dv=None), 1, "no gradient"), (dict(dq=None, dtable=P), 1, "dtable"),
-    (dict(has_mask=1), 1, "state"),
+    (dict(state=None), 1, "state"), (dict(state=P + 16), 1, "256-byte"),
 ])
 def test_backward_entry_refuses(change, code, message):
     assert _capi.lib().sage_train_bwd(*{**BWD, **change}.values()) == code and message in _err(), _err()
@@ -144,12 +143,12 @@ def test_bias_entries_refuse():
 def test_workspaces():
     """Sizes follow from the shapes alone: none without masks, bias or packing; a mask costs its bits and little more."""
     ws = _capi.train_workspace
-    state, work = ws(False, 2, 8, 8, 1000, 1000, 64, None, None)
-    assert state == 0 and work >= 2 * 4 * 2 * 8 * 1024
-    assert ws(False, 2, 8, 8, 1000, 1000, 64, (0, 0, 0), None)[0] <= 2048
-    full = ws(False, 2, 8, 8, 1000, 1000, 64, (1, 1, 1), None)[0]
+    state, work = ws(False, 2, 8, 8, 1000, 1000, 64, None, None, False)
+    assert state == 0 and ws(False, 2, 8, 8, 1000, 1000, 64, None, None, True)[0] == 2 * 8 * 1000 * 64 * 2 and work >= 2 * 4 * 2 * 8 * 1024
+    assert ws(False, 2, 8, 8, 1000, 1000, 64, (0, 0, 0), None, False)[0] <= 2048
+    full = ws(False, 2, 8, 8, 1000, 1000, 64, (1, 1, 1), None, False)[0]
     assert 2 * 8 * 1024 * 1024 // 8 <= full <= 1.1 * 2 * 8 * 1024 * 1024 // 8
-    assert ws(True, 5, 8, 8, 1000, 900, 64, None, None)[0] > 0
-    assert ws(False, 2, 8, 8, 1000, 1000, 64, None, (32, True, 128))[0] >= 8 * 183 * 4
+    assert ws(True, 5, 8, 8, 1000, 900, 64, None, None, False)[0] > 0
+    assert ws(False, 2, 8, 8, 1000, 1000, 64, None, (32, True, 128), False)[0] >= 8 * 183 * 4
     with pytest.raises(_capi.SageError, match="distance"):
-        ws(False, 2, 8, 8, 1000, 1000, 64, None, (32, True, 2000))
+        ws(False, 2, 8, 8, 1000, 1000, 64, None, (32, True, 2000), False)

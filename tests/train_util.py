@@ -100,7 +100,9 @@ class Exact:
         self.dk = back(ds.transpose(2, 3) @ q) * scale
         self.dv = back(p.transpose(2, 3) @ do)
         off_dp = F32 * (D + 8) * (do.abs() @ v.abs().transpose(2, 3) + (do * self.out).abs().sum(-1, keepdim=True))
-        off_d = (do.abs() * self.room_out).sum(dim=-1, keepdim=True)     # of delta, by the rounding of out and of its weights
+        # of delta, by the rounding of out's weights; out itself is known to 2 u^2 (fp16: to half of its smallest step)
+        kept = self.room_out - u * self.out.abs() + 2 * u * u * self.out.abs()
+        off_d = (do.abs() * kept).sum(dim=-1, keepdim=True)
         self.sums = 3 * ep * ds.abs() + p * off_dp                      # of ds in float32, delta's error apart
         domax = float(do.abs().max())
         small = 2.0 ** -34 * domax * vmax if self.dtype == torch.float16 else 0.0   # fp16's smallest steps of scaled ds
