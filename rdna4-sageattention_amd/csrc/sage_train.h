@@ -58,6 +58,7 @@ struct TrainArgs {
   uint32_t* norms;                 // fp16: the largest squared norms of dout's and v's rows, as bits
   // packed batches: offsets and the (sequence, tile) of each tile id, sequence -1 for none
   const int *cu_q, *cu_k;
+  const int* bounds;               // the rows of q, [0] .. [1] - 1, and of k, [2] .. [3] - 1, that the sequences cover
   const int2 *q_tab, *k_tab;
   // boolean masks as bits: word w of row i holds keys 32 w ..; word w of row i at bits + b*mb + h*mh + w*mw + i*mi
   const uint32_t* bits;
@@ -71,6 +72,9 @@ struct TrainArgs {
   int reach;
   float* bias_part;                // backward: [H][parts][buckets] sums of ds, a part for every tile of queries
   int64_t parts;
+  // dk, dv: the query heads of a kv head in `split` workgroups, whose fp32 sums [split][2][B, Skv (packed: Skv)][Hkv][D] are added up
+  int split;
+  float* kv_part;
 };
 
 // f(0), f(1), .. f(N - 1) with constants for arguments
@@ -228,6 +232,13 @@ template <int DT> __device__ __forceinline__ void tr_store(const v16f& acc, floa
   }
 }
 
+// The same in 32 bits
+__device__ __forceinline__ void tr_store_f32(const v16f& acc, float f, float* p, int hf, bool on) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (on) *reinterpret_cast<v4f*>(p + 8 * g + 4 * hf) = v4f{acc[4 * g] * f, acc[4 * g + 1] * f, acc[4 * g + 2] * f, acc[4 * g + 3] * f};
+}
+
 // Blocks of a mask, by the words of two neighbouring blocks that a workgroup's columns are in (m0 NULL: no mask).
 struct TrBlocks {
   const uint64_t *m0 = nullptr, *m1 = nullptr;
@@ -286,17 +297,20 @@ struct TrSeq {
   int64_t qr, kr;          // first row of the sequence in q and k (packed), 0 otherwise
   int64_t lr;              // its row 0 in nl / nd
   int part;                // the tile's number among all of a head
+  int h0, hn, z;           // keys: the query heads that the workgroup takes, and which of the `split` workgroups it is
 };
 
 // The tile of workgroup `id`; false where there is none.  keys: column tiles of keys (heads are kv heads).  Heads of one batch
-// entry that share the streamed side follow each other on one XCD; causal launches take long tiles first.
+// entry that share the streamed side follow each other on one XCD; causal launches take long tiles first, over all pairs (in turn over
+// the XCDs where the pairs do not divide over them: dq at 3 x 10 x 1777 x 2049 x 96 53 us, 56 with each XCD's pairs to itself).
 template <bool KEYS> __device__ __forceinline__ bool tr_tile(const TrainArgs& a, int id, TrSeq& s) {
-  const int heads = KEYS ? a.Hkv : a.H, tiles = KEYS ? a.k_tiles : a.q_tiles;
+  const int heads = KEYS ? a.Hkv * a.split : a.H, tiles = KEYS ? a.k_tiles : a.q_tiles;
   const int pairs = a.cu_q ? heads : a.B * heads;
   int bh, t;
-  if (a.causal) {
-    causal_tile(id, pairs, tiles, bh, t);
-    if (KEYS) t = tiles - 1 - t;   // (the first keys are seen by the most queries)
+  if (a.causal || (KEYS && a.cu_q)) {
+    if (pairs % 8) bh = id % pairs, t = tiles - 1 - id / pairs;
+    else causal_tile(id, pairs, tiles, bh, t);
+    if (KEYS) t = tiles - 1 - t;   // (the first keys are seen by the most queries; packed: train_order's order)
   } else {
     const int lg = xcd_remap(id, pairs * tiles);
     bh = lg / tiles;
@@ -304,6 +318,12 @@ template <bool KEYS> __device__ __forceinline__ bool tr_tile(const TrainArgs& a,
   }
   s.part = a.cu_q ? t : bh / heads * tiles + t;
   s.h = a.cu_q ? bh : bh % heads;
+  if (KEYS) {
+    s.z = s.h % a.split;
+    s.h /= a.split;
+    s.hn = a.H / a.Hkv / a.split;
+    s.h0 = (s.h * a.split + s.z) * s.hn;
+  }
   if (a.cu_q) {
     const int2 e = (KEYS ? a.k_tab : a.q_tab)[t];
     if (e.x < 0) return false;
@@ -364,7 +384,7 @@ template <int S> __device__ __forceinline__ int tr_steps(const TrainArgs& a, con
   if (!a.bits) return (end - first) * group;
   int n = 0;
   for (int g = 0; g < group; ++g) {
-    const TrRows r = tr_rows(a, s, s.h * group + g, first, end);
+    const TrRows r = tr_rows(a, s, s.h0 + g, first, end);
     n += r.m.template count<S>(r.first, end);
   }
   return n;
@@ -374,7 +394,7 @@ template <int S, bool MASKS> struct TrWalk {
   int g, t;
   TrRows rows;
   __device__ __forceinline__ void head(const TrainArgs& a, const TrSeq& s, int group, int first, int end) {
-    if constexpr (MASKS) rows = tr_rows(a, s, s.h * group + g, first, end);
+    if constexpr (MASKS) rows = tr_rows(a, s, s.h0 + g, first, end);
     else rows.first = first;
     t = MASKS ? rows.m.template prev<S>(end, rows.first) : end - 1;
   }
@@ -393,6 +413,12 @@ template <int S, bool MASKS> struct TrWalk {
     return passed;
   }
 };
+
+// Row `r` of the workgroup's sums for dk (which 0) or dv (1) among those that are added up
+template <int D> __device__ __forceinline__ float* tr_kv_part(const TrainArgs& a, const TrSeq& s, int which, int r) {
+  const int64_t rows = (int64_t)(a.cu_q ? 1 : a.B) * a.Skv, row = a.cu_q ? s.kr + r : (int64_t)s.b * a.Skv + r;
+  return a.kv_part + (((2 * s.z + which) * rows + row) * a.Hkv + s.h) * D;
+}
 
 __device__ __forceinline__ int64_t tr_stat_row(const TrainArgs& a, const TrSeq& s, int h) {
   return a.cu_q ? h * a.pad + s.lr : ((int64_t)s.b * a.H + h) * a.pad;

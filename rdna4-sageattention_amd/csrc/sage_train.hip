@@ -45,6 +45,62 @@ __global__ __launch_bounds__(TR_THREADS) void train_plan(const int* cu_q, const 
   for (int i = at_k + tid; i < k_tiles; i += TR_THREADS) k_tab[i] = make_int2(-1, 0);
 }
 
+// The tiles of keys from the one that the most queries see to the one that the fewest do, those of about the same number in their
+// order: so the units end at about the same time, with short tiles.  One workgroup, a counting sort by 256 lengths.  (14 sequences of 77 to 3001, causal, 32 heads on 8 x 128: dk and dv in 942 us, 1045 without;
+// q's tiles, four times as many workgroups on twice as many places, are no faster sorted.)
+__global__ __launch_bounds__(TR_THREADS) void train_order(const int* cu_q, const int* cu_k, int causal, const int2* from, int2* to,
+                                                          int tiles) {
+  const int tid = threadIdx.x;
+  __shared__ __attribute__((aligned(16))) uint8_t bin[TR_THREADS];
+  __shared__ int scan[TR_THREADS], most;   // of every length: how many tiles there are, then where the next one goes
+  auto length = [&](int i) -> int {        // queries; -1 where there is no tile
+    const int2 e = i < tiles ? from[i] : make_int2(-1, 0);
+    if (e.x < 0) return -1;
+    const int c0 = e.y * TR_COLS, nq = cu_q[e.x + 1] - cu_q[e.x], nk = cu_k[e.x + 1] - cu_k[e.x];
+    return causal ? nq - min(nq, max(0, c0 - (nk - nq))) : nq;
+  };
+  if (tid == 0) most = 1;
+  scan[tid] = 0;
+  __syncthreads();
+  const int own = length(tid);
+  int mine = own;
+  for (int i = tid + TR_THREADS; i < tiles; i += TR_THREADS) mine = max(mine, length(i));
+  atomicMax(&most, mine);
+  __syncthreads();
+  const int top = most;
+  auto bin_of = [&](int i) {               // (the longest first, none at the end)
+    const int n = i == tid ? own : length(i);
+    return n < 0 ? 255 : 254 - (int)((int64_t)n * 254 / top);
+  };
+  for (int i = tid; i < tiles; i += TR_THREADS) atomicAdd(&scan[bin_of(i)], 1);
+  __syncthreads();
+  const int many = scan[tid];
+  for (int o = 1; o < TR_THREADS; o <<= 1) {
+    const int x = tid >= o ? scan[tid - o] : 0;
+    __syncthreads();
+    scan[tid] += x;
+    __syncthreads();
+  }
+  const int first = scan[tid] - many;
+  __syncthreads();
+  scan[tid] = first;
+  for (int i0 = 0; i0 < tiles; i0 += TR_THREADS) {
+    const int i = i0 + tid, b = bin_of(i);
+    bin[tid] = (uint8_t)b;
+    __syncthreads();
+    int rank = 0;                          // among the 256 tiles
+    for (int x = 0; x < TR_THREADS; x += 16) {
+      const v4i w = *reinterpret_cast<const v4i*>(bin + x);
+#pragma unroll
+      for (int y = 0; y < 16; ++y) rank += ((uint32_t)w[y >> 2] >> (8 * (y & 3)) & 255u) == (uint32_t)b && x + y < tid;
+    }
+    if (i < tiles) to[scan[b] + rank] = from[i];
+    __syncthreads();
+    if (i < tiles) atomicAdd(&scan[b], 1);
+    __syncthreads();
+  }
+}
+
 // Packed batches: zeros in the rows that no sequence covers, of up to three tensors [rows, heads, D].
 struct TrainGaps {
   uint16_t* p[3];
@@ -146,10 +202,25 @@ __global__ __launch_bounds__(TR_THREADS) void train_mask_any(const uint8_t* __re
 struct TrainLayout {
   int q_tiles, k_tiles, mask_b, mask_h, row_pad, words, blocks, chunks, aw, tw;
   int64_t q_tab, k_tab, bits, shows, any, any_t, vec, lo, state;      // byte offsets; bounds at 0
-  int64_t pad, nl, nd, norms, parts, part, work;
+  int64_t pad, nl, nd, norms, parts, part, kv_part, k_order, work;
 };
-static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool mask, bool mb, bool mh, bool mq, int reach,
-                                int buckets, int keep) {   // keep: D where a backward pass comes, else 0
+
+// In how many workgroups the query heads of a kv head go for dk and dv, where there are tiles of keys for half of the places at most.
+// Tiles that see different numbers of queries, under causal or a mask or packed, are twice as many as places then, so that the long
+// ones do not last alone.  The sums that are added up afterwards are 8 D bytes a key and workgroup.  (6 x 16 heads on 4 x 1250 x 64,
+// masked, 240 tiles for 512 places: 145 us whole, 89 + 8 in two, 77 + 12 in four.  3 x 10 heads on 5 x 1777 x 2049 x 96, causal, 255
+// tiles for 256 places: 85 us whole, 75 + 10 in two.)
+static int train_split(bool packed, bool uneven, int B, int H, int Hkv, int k_tiles, int D) {
+  const int64_t places = D == 64 ? 512 : 256, n = (int64_t)(packed ? 1 : B) * Hkv * k_tiles;   // (256 units, DkvGeo::OCC workgroups each)
+  const int group = H / Hkv;
+  int s = 1;
+  for (int x = 2; x <= group && 2 * n <= places && n * x <= (uneven ? 2 : 1) * places; ++x)
+    if (group % x == 0) s = x;
+  return s;
+}
+
+static TrainLayout train_layout(bool packed, int B, int H, int Hkv, int Sq, int Skv, int D, bool mask, bool mb, bool mh, bool mq,
+                                int reach, int buckets, bool keep) {   // keep: a backward pass comes
   TrainLayout l = {};
   auto take = [](int64_t& at, int64_t n) {
     const int64_t r = at;
@@ -174,7 +245,7 @@ static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool
     l.any_t = take(at, bh * l.chunks * l.tw * 8);
   }
   if (reach) l.vec = take(at, (int64_t)H * (2 * reach + 1) * 4);
-  if (keep) l.lo = take(at, (int64_t)(packed ? 1 : B) * H * Sq * keep * 2);
+  if (keep) l.lo = take(at, (int64_t)(packed ? 1 : B) * H * Sq * D * 2);
   l.state = at;
   at = 0;
   l.pad = packed ? (int64_t)Sq / 64 * 64 + 64 * ((int64_t)B + 1) : ((int64_t)Sq + 63) / 64 * 64;
@@ -184,6 +255,9 @@ static TrainLayout train_layout(bool packed, int B, int H, int Sq, int Skv, bool
   l.norms = take(at, 8);
   l.parts = (int64_t)l.q_tiles * (packed ? 1 : B);
   l.part = take(at, reach ? l.parts * H * buckets * 4 : 0);
+  const int split = train_split(packed, true, B, H, Hkv, l.k_tiles, D);
+  l.kv_part = take(at, split > 1 ? (int64_t)split * 2 * (packed ? 1 : B) * Skv * Hkv * D * 4 : 0);
+  l.k_order = take(at, packed ? (int64_t)l.k_tiles * 8 : 0);
   l.work = at;
   return l;
 }
@@ -234,7 +308,7 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
     if (reach > TR_REACH)
       return fail(SAGE_ERR_UNSUPPORTED, "%s: the last bucket begins at distance %d (at most %d)", who, reach, TR_REACH);
   }
-  l = train_layout(cu_q != nullptr, B, H, Sq, Skv, mask, msb != 0, msh != 0, msq != 0, reach, buckets, keep ? D : 0);
+  l = train_layout(cu_q != nullptr, B, H, Hkv, Sq, Skv, D, mask, msb != 0, msh != 0, msq != 0, reach, buckets, keep != 0);
   SAGE_REQUIRE(l.state == 0 || (state && ((uintptr_t)state & 255u) == 0 && state_bytes >= l.state),
                "%s: a state of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)l.state, (long long)state_bytes);
   a.B = B, a.H = H, a.Hkv = Hkv, a.Sq = Sq, a.Skv = Skv, a.q_tiles = l.q_tiles, a.k_tiles = l.k_tiles, a.causal = causal != 0;
@@ -242,7 +316,7 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
   a.c = (float)((double)a.scale * 1.4426950408889634);
   char* base = (char*)state;
   if (keep) a.lo = (uint16_t*)(base + l.lo);
-  if (cu_q) a.cu_q = cu_q, a.cu_k = cu_k, a.q_tab = (const int2*)(base + l.q_tab), a.k_tab = (const int2*)(base + l.k_tab);
+  if (cu_q) a.cu_q = cu_q, a.cu_k = cu_k, a.q_tab = (const int2*)(base + l.q_tab), a.k_tab = (const int2*)(base + l.k_tab), a.bounds = (const int*)base;
   if (mask) {
     const int64_t per = (int64_t)l.row_pad * l.words;
     a.bits = (const uint32_t*)(base + l.bits);
@@ -273,7 +347,8 @@ extern "C" int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, i
     if (reach > TR_REACH)
       return fail(SAGE_ERR_UNSUPPORTED, "sage_train_workspace: the last bucket begins at distance %d (at most %d)", reach, TR_REACH);
   }
-  const TrainLayout l = train_layout(packed != 0, B, H, Sq, Skv, has_mask != 0, msb != 0, msh != 0, msq != 0, reach, buckets, keep ? D : 0);
+  const TrainLayout l = train_layout(packed != 0, B, H, Hkv, Sq, Skv, D, has_mask != 0, msb != 0, msh != 0, msq != 0, reach, buckets,
+                                     keep != 0);
   *state_bytes = l.state;
   *workspace_bytes = l.work;
   return SAGE_OK;
@@ -366,6 +441,7 @@ extern "C" int sage_train_bwd(const void* dout, int64_t gsb, int64_t gss, int64_
   a.lse = (float*)lse;
   char* w = (char*)workspace;
   a.nl = (float*)(w + l.nl), a.nd = (float*)(w + l.nd), a.pad = l.pad, a.norms = (uint32_t*)(w + l.norms);
+  a.split = train_split(cu_q != nullptr, causal || has_mask || cu_q, B, H, Hkv, l.k_tiles, D), a.kv_part = (float*)(w + l.kv_part);
   if (buckets && dtable) a.bias_part = (float*)(w + l.part), a.parts = l.parts;
   hipStream_t st = (hipStream_t)stream;
   if (cu_q) {
@@ -376,6 +452,10 @@ extern "C" int sage_train_bwd(const void* dout, int64_t gsb, int64_t gss, int64_
     g.p[2] = a.dv, g.s[2] = dvs, g.h[2] = dvh, g.heads[2] = Hkv, g.rows[2] = Skv, g.side[2] = 1;
     const int rows = Sq > Skv ? Sq : Skv;
     train_gaps<<<dim3(rows < 1024 ? rows : 1024, 3), TR_THREADS, 0, st>>>(g, (const int*)state);
+    if (dk) {
+      train_order<<<1, TR_THREADS, 0, st>>>(cu_q, cu_k, a.causal, a.k_tab, (int2*)(w + l.k_order), l.k_tiles);
+      a.k_tab = (const int2*)(w + l.k_order);
+    }
   }
   if (int rc = train_dispatch(true, a, m, D, dtype, st)) return rc;
   if (a.bias_part) return bias_reduce_launch(a.bias_part, l.parts, H, m, dtable, table_dtype, tb, th, st);

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   if (!tr_tile<true>(a, blockIdx.x, s)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  const int group = a.H / a.Hkv;
+  const int group = s.hn;
   const int off = s.k_len - s.q_len;
   const int w0 = s.c0 + wave * 32, j = w0 + ln;   // the wave's first key, the lane's
   const bool on = j < s.k_len;
@@ -67,10 +67,10 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   TrLoader<D, ROWS> lq, lg;
   lq.init(a.qs, wave, lane);
   lg.init(a.gs, wave, lane);
-  const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + s.h * group * a.qh;
-  const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * group * a.gh;
-  const float* sp = (wave & 1 ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group) + lane;
-  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h * group * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
+  const uint16_t* qp = a.q + (a.cu_q ? 0 : s.b * a.qb) + s.qr * a.qs + s.h0 * a.qh;
+  const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h0 * a.gh;
+  const float* sp = (wave & 1 ? a.nd : a.nl) + tr_stat_row(a, s, s.h0) + lane;
+  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h0 * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
   TrWalk<0, EX> ld;                               // the tile that is loaded next
   int un = 0;
   auto shift = [&](int heads) { qp += heads * a.qh, gp += heads * a.gh, sp += heads * a.pad, mp += heads * a.mh; };
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
       at_work.start(a, s, group, t0, t_all);
       int u = 0;
       while (u < steps) {
-        const int h = s.h * group + at_work.g;
+        const int h = s.h0 + at_work.g;
         if (EX && a.bias) {
           __syncthreads();
           for (int y = tid; y <= 2 * a.reach; y += TR_THREADS) bl[y] = a.bias[(int64_t)h * (2 * a.reach + 1) + y];
@@ -285,6 +285,15 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
   }
 
   const float fk = __builtin_ldexpf(a.scale, -ex), fv = DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
+  if (a.split > 1) {
+    float *kp = tr_kv_part<D>(a, s, 0, jr), *vp = tr_kv_part<D>(a, s, 1, jr);
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db) {
+      tr_store_f32(dk[db], fk, kp + 32 * db, hf, on);
+      tr_store_f32(dv[db], fv, vp + 32 * db, hf, on);
+    }
+    return;
+  }
   uint16_t* kp = a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh;
   uint16_t* vp = a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
 #pragma unroll
@@ -324,7 +333,7 @@ __global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   const int pair = wave & 3, second = wave >> 2;
-  const int group = a.H / a.Hkv;
+  const int group = s.hn;
   const int off = s.k_len - s.q_len;
   const int w0 = s.c0 + pair * 32, j = w0 + ln;   // the pair's first key, the lane's
   const bool on = j < s.k_len;
@@ -351,8 +360,8 @@ __global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
   // together stream the same tiles together.
   const int l0 = wave * P::PER_WAVE, side = l0 / P::PER_TENSOR;
   const int64_t ls = side ? a.gs : a.qs, lh = side ? a.gh : a.qh;
-  const uint16_t* lsrc = (side ? a.dout + (a.cu_q ? 0 : s.b * a.gb) : a.q + (a.cu_q ? 0 : s.b * a.qb)) + s.qr * ls + s.h * group * lh;
-  const float* stat_src = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h * group);
+  const uint16_t* lsrc = (side ? a.dout + (a.cu_q ? 0 : s.b * a.gb) : a.q + (a.cu_q ? 0 : s.b * a.qb)) + s.qr * ls + s.h0 * lh;
+  const float* stat_src = (wave ? a.nd : a.nl) + tr_stat_row(a, s, s.h0);
   const int row_l = (l0 - side * P::PER_TENSOR) * 64 + lane;   // the lane's chunk of the wave's first load
   const bool fits = ls >= 0 && ls < (1 << 24);
   uint32_t loff[P::PER_WAVE];
@@ -361,7 +370,7 @@ __global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
     const int L = row_l + 64 * x, row = L / G::KCH;
     loff[x] = (uint32_t)((row * ls + tr_swz<D>(row, L % G::KCH) * 8) * 2);
   }
-  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h * group * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
+  const uint32_t* mp = EX && a.bits ? a.bits + s.b * a.mb + s.h0 * a.mh + (int64_t)(min(w0, s.k_len - 1) >> 5) * a.mw : nullptr;
   TrWalk<1, EX> ld;                               // the tile that is loaded next
   int un = 0;
   auto shift = [&](int heads) { lsrc += heads * lh, stat_src += heads * a.pad, mp += heads * a.mh; };
@@ -465,7 +474,7 @@ __global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
     auto bias = [&]() __attribute__((always_inline)) {
       if (EX && a.bias && u < steps && entered) {
         __syncthreads();
-        const float* b = a.bias + (int64_t)(s.h * group + at_work.g) * (2 * a.reach + 1);
+        const float* b = a.bias + (int64_t)(s.h0 + at_work.g) * (2 * a.reach + 1);
         for (int y = tid; y <= 2 * a.reach; y += 512) bl[y] = b[y];
         __syncthreads();
       }
@@ -549,20 +558,53 @@ __global__ __launch_bounds__(512, 2) void train_dkv_pair(TrainArgs a) {
   }
 
   const float f = second ? __builtin_ldexpf(a.scale, -ex) : DT == DT_F16 ? 1.0f / 32768.0f : 1.0f;
+  if (a.split > 1) {
+    float* p = tr_kv_part<D>(a, s, 1 - second, jr);
+#pragma unroll
+    for (int db = 0; db < G::NDB; ++db) tr_store_f32(acc[db], f, p + 32 * db, hf, on);
+    return;
+  }
   uint16_t* p = second ? a.dk + (a.cu_q ? 0 : s.b * a.dkb) + (s.kr + jr) * a.dks + s.h * a.dkh
                        : a.dv + (a.cu_q ? 0 : s.b * a.dvb) + (s.kr + jr) * a.dvs + s.h * a.dvh;
 #pragma unroll
   for (int db = 0; db < G::NDB; ++db) tr_store<DT>(acc[db], f, p + 32 * db, hf, on);
 }
 
+// dk and dv where several workgroups share a kv head's query heads: their sums in the order of the heads, one thread per 8 channels
+template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_kv_join(TrainArgs a) {
+  const int64_t rows = (int64_t)(a.cu_q ? 1 : a.B) * a.Skv, n = rows * a.Hkv * (D / 8);
+  const int which = blockIdx.y;
+  for (int64_t x = (int64_t)blockIdx.x * TR_THREADS + threadIdx.x; x < n; x += (int64_t)gridDim.x * TR_THREADS) {
+    const int64_t rh = x / (D / 8), row = rh / a.Hkv;
+    const int ch = (int)(x % (D / 8)) * 8, h = (int)(rh % a.Hkv);
+    if (a.cu_q && (row < a.bounds[2] || row >= a.bounds[3])) continue;   // (zeros already)
+    const float* p = a.kv_part + (which * rows * a.Hkv + rh) * D + ch;
+    v4f lo = *reinterpret_cast<const v4f*>(p), hi = *reinterpret_cast<const v4f*>(p + 4);
+    for (int z = 1; z < a.split; ++z) {
+      p += 2 * rows * a.Hkv * D;
+      const v4f y = *reinterpret_cast<const v4f*>(p), w = *reinterpret_cast<const v4f*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lo[e] += y[e], hi[e] += w[e];
+    }
+    const int64_t b = a.cu_q ? 0 : row / a.Skv, r = a.cu_q ? row : row % a.Skv;
+    uint16_t* o = which ? a.dv + b * a.dvb + r * a.dvs + h * a.dvh : a.dk + b * a.dkb + r * a.dks + h * a.dkh;
+    *reinterpret_cast<v4i*>(o + ch) = v4i{tr_pack<DT>(lo[0], lo[1]), tr_pack<DT>(lo[2], lo[3]), tr_pack<DT>(hi[0], hi[1]),
+                                          tr_pack<DT>(hi[2], hi[3])};
+  }
+}
+
 template <int D, int DT> int train_dkv_launch(const TrainArgs& a, hipStream_t st) {
-  const unsigned n = (unsigned)((int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * a.k_tiles);
+  const unsigned n = (unsigned)((int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * a.split * a.k_tiles);
   if constexpr (D == 256) {
     if (a.bits || a.bias) train_dkv_pair<D, DT, true><<<n, 512, 0, st>>>(a);
     else train_dkv_pair<D, DT, false><<<n, 512, 0, st>>>(a);
   } else {
     if (a.bits || a.bias) train_dkv<D, DT, true><<<n, TR_THREADS, 0, st>>>(a);
     else train_dkv<D, DT, false><<<n, TR_THREADS, 0, st>>>(a);
+  }
+  if (a.split > 1) {
+    const int64_t need = ((int64_t)(a.cu_q ? 1 : a.B) * a.Skv * a.Hkv * (D / 8) + TR_THREADS - 1) / TR_THREADS;
+    train_kv_join<D, DT><<<dim3((unsigned)(need < 65536 ? need : 65536), 2), TR_THREADS, 0, st>>>(a);
   }
   return check_launch("train_dkv");
 }
