@@ -106,14 +106,16 @@ template <int D, int DT, bool EX>
 __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainArgs a, BiasMap map) {
   using G = TrGeo<D>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2][G::TILE];
-  __shared__ float bl[EX ? 2 * TR_REACH + 1 : 1];
   __shared__ __attribute__((aligned(256))) uint32_t wl[2][4][EX ? 64 : 1];   // a mask's words of the tiles, for each wave's queries
-  extern __shared__ float by_distance[];   // EX with bias_part: 4 waves x (2 reach + 1)
+  // With bias_part: 16 x 32 sums of each wave, unless D is 256, and 4 waves' sums by distance, 2 reach + 1 each; then the bias.  (As
+  // much as the reach needs: up to 128, two workgroups of 128 channels fit a unit.)
+  extern __shared__ __attribute__((aligned(16))) float diag[];
 
   TrSeq s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool biased = EX && a.bias, want_part = EX && a.bias_part;
   const int R = 2 * a.reach + 1;
+  float *by_distance = diag + (D < 256 ? 4 * 16 * 32 : 0), *bl = want_part ? by_distance + 4 * R : diag;
   if (!tr_tile<false>(a, blockIdx.x, s)) {
     if (want_part)   // (only packed batches have unused tiles)
       for (int x = tid; x < map.buckets; x += TR_THREADS) a.bias_part[(s.h * a.parts + s.part) * map.buckets + x] = 0.0f;
@@ -177,9 +179,9 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
     for (int x = tid; x < R; x += TR_THREADS) bl[x] = a.bias[(int64_t)s.h * R + x];
 
   v16f dq[G::NDB];
-  // the bias' gradient: the lane's sums of ds and p over the keys at distance -reach and farther behind, reach and farther ahead,
-  // and of ds over the others
-  float flo = 0.0f, fhi = 0.0f, plo = 0.0f, phi = 0.0f, fnear = 0.0f;
+  // the bias' gradient: the lane's sums of ds (of any rows of the wave's) and p (of its own row) over the keys at distance -reach and
+  // farther behind, reach and farther ahead, and its row's sum of ds over all keys
+  float flo = 0.0f, fhi = 0.0f, plo = 0.0f, phi = 0.0f, frow = 0.0f;
 
   const TrBlocks blocks = EX ? tr_key_blocks(a, s) : TrBlocks();
   auto issue = [&](int t, int slot) {
@@ -231,18 +233,59 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
         }
       }
       if (want_part) {
-        // d[v]: of ds; every lane of a half wave has a distance of its own, so one half at a time adds without conflicts and in
-        // one order
         float all = 0.0f, ps = 0.0f;
-        if (near) {
+        if (near && D < 256) {
+          // Sums along the block's diagonals: 16 queries at a time go through LDS, from where lane c of a half wave takes key
+          // (q + c) % 32 of query q, of 8 queries each: distance c where that is q + c, c - 32 where it began anew.
+          float* y = diag + wave * 16 * 32;
+          float s0 = 0.0f, s1 = 0.0f;
+          int c = ln + 8 * hf;
+          asm volatile("" : "+v"(c));            // (16 addresses are not to be kept for all tiles)
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if ((ln >> 4) == part) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<v4f*>(y + (ln & 15) * 32 + (((2 * g + hf) ^ (ln & 7)) << 2)) =
+                    v4f{x[4 * g] * dp[4 * g], x[4 * g + 1] * dp[4 * g + 1], x[4 * g + 2] * dp[4 * g + 2], x[4 * g + 3] * dp[4 * g + 3]};
+            }
+            asm volatile("" ::: "memory");       // (a wave's LDS accesses stay in order)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int r = c + 16 * part + k;
+              const float z = y[8 * 32 * hf + 32 * k + ((r & 31) ^ (k << 2))];
+              s0 += r < 32 ? z : 0.0f;
+              s1 += r < 32 ? 0.0f : z;
+            }
+            asm volatile("" ::: "memory");       // (a wave's LDS accesses stay in order)
+          }
+          s0 = add_xor32_f32(s0), s1 = add_xor32_f32(s1);
+          const float z = hf ? s1 : s0;
+          const int d = key0 - (w0 + off) + ln - 32 * hf;
+          if (d <= -a.reach) flo += z;
+          else if (d >= a.reach) fhi += z;
+          else mine[a.reach + d] += z;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) frow = __builtin_fmaf(x[v], dp[v], frow);
+          if (wlo <= -a.reach || whi >= a.reach) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int e = d0 + 8 * (v >> 2) + (v & 3);
+              plo += e <= -a.reach ? x[v] : 0.0f;
+              phi += e >= a.reach ? x[v] : 0.0f;
+            }
+          }
+        } else if (near) {
+          // Every lane of a half wave has a distance of its own, so one half at a time adds without conflicts and in one order.
+          // (256 channels leave no LDS for a block.)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
             const int d = d0 + 8 * (v >> 2) + (v & 3);
             const float y = x[v] * dp[v];
+            frow += y;
             if (d <= -a.reach) flo += y, plo += x[v];
             else if (d >= a.reach) fhi += y, phi += x[v];
             else {
-              fnear += y;
               __attribute__((address_space(3))) float* slot = (__attribute__((address_space(3))) float*)(mine + a.reach + d);
               if (hf == 0) {
                 __builtin_amdgcn_ds_faddf(slot, y, 0, 0, false);
@@ -256,6 +299,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
         } else {
 #pragma unroll
           for (int v = 0; v < 16; ++v) all += x[v] * dp[v], ps += x[v];
+          frow += all;
           if (whi <= -a.reach) flo += all, plo += ps;
           else fhi += all, phi += ps;
         }
@@ -276,7 +320,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
 #pragma unroll
       for (int v = 0; v < 16; ++v) dq[db][v] = 0.0f;
     if (want_part) {
-      flo = fhi = plo = phi = fnear = 0.0f;
+      flo = fhi = plo = phi = frow = 0.0f;
       for (int x = lane; x < R; x += 64) mine[x] = 0.0f;
     }
     int t = EX ? blocks.next(-1, ntiles) : 0, slot = 0, tn = 0;
@@ -314,7 +358,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
   if (want_part) {
     // The row sums of ds are 0, but D holds the rounding of o's weights to 16 bits: sum_j ds = D' - D, exactly the error of D.  In a
     // far bucket, which holds most of a long row's weight, it would not average out: it is taken from there.
-    const float delta = add_xor32_f32(fnear + flo + fhi);
+    const float delta = add_xor32_f32(frow);
     flo -= delta * __builtin_ldexpf(plo, -ex);
     fhi -= delta * __builtin_ldexpf(phi, -ex);
 #pragma unroll
@@ -344,7 +388,7 @@ template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap&
     if (int rc = train_dkv_launch<D, DT>(a, st)) return rc;
   if (!a.dq) return check_launch("train_prep");
   if (a.bits || a.bias) {
-    const unsigned lds = a.bias_part ? 4u * 4u * (2u * a.reach + 1u) : 0u;
+    const unsigned R = 2u * a.reach + 1u, lds = a.bias ? 4u * (R + (a.bias_part ? (D < 256 ? 4u * 16u * 32u : 0u) + 4u * R : 0u)) : 0u;
     train_dq<D, DT, true><<<rows, TR_THREADS, lds, st>>>(a, m);
   } else {
     train_dq<D, DT, false><<<rows, TR_THREADS, 0, st>>>(a, m);
