@@ -337,8 +337,9 @@ int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype
  * covers, and all rows where offsets fall or pass the totals, are written as 0 (their lse stays as it is).
  *
  * sage_train_workspace: the bytes of the state, which the forward pass writes and the backward pass reads, and of the backward
- * pass' workspace; both 256-byte aligned.  keep: 0 where no backward pass comes (its part of the state, as large as out, falls away).  sage_train_bwd: dq NULL (then dtable too) or dk and dv NULL leave those out; dtable
- * NULL leaves the table's gradient out.  Equal inputs give equal bits.
+ * pass' workspace; both 256-byte aligned.  keep: 0 where no backward pass comes (its part of the state, as large as out, falls
+ * away), the same in both calls.  sage_train_bwd, behind a forward pass with keep: dq NULL (then dtable too) or dk and dv NULL leave
+ * those out; dtable NULL leaves the table's gradient out.  Equal inputs give equal bits.
  */
 int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, int Skv, int D, int has_mask, int64_t msb, int64_t msh,
                          int64_t msq, int buckets, int two_sided, const int* borders, int keep, int64_t* state_bytes,

@@ -27,8 +27,8 @@ int bias_expand_launch(const void* table, int table_dtype, int64_t tb, int64_t t
 //
 // A row's values follow from key - query alone: a workgroup looks the buckets of its rows' and columns' distances up once and
 // keeps their values in LDS, in the output's type, as `16 / size` copies, each shifted by one value, so that any run of 16
-// bytes is one aligned LDS read, ready to be stored.  Bound by the stores: 24 x 4352 x 4352 in 16
-// bits at 4.9 TB/s (non-temporal ones: 4.0), odd rows of 16 x 2047 x 2511 at 4.7.
+// bytes is one aligned LDS read, ready to be stored.  Bound by the stores: 24 x 4352 x 4352 in 16 bits at 5.1 TB/s (non-temporal
+// ones: 4.0), odd rows of 16 x 2047 x 2511 at 4.7.
 
 struct BiasOut {
   const void* table;
@@ -106,10 +106,10 @@ template <int DT> __global__ __launch_bounds__(BIAS_THREADS) void bias_write(Bia
 //
 // Every diagonal (key - query) is in one bucket.  A thread walks down a chunk of rows N = 16 / size at a time, N columns further
 // right each time: its N x N squares all lie on the same 2 N - 1 diagonals, whose sums it keeps, and its loads are 16 bytes, aligned
-// where rows are.  (A thread with N diagonals of its own, one column further right every row: 107 us where this takes 60, at
-// 16 x 2047 x 2511, whose odd rows cost unaligned loads.)  Neighbours share N - 1 diagonals, which are added in LDS; there the workgroup's diagonals are summed by bucket
-// and written as one part; the parts are summed in a second launch.  No atomics: one order.  Bound by the
-// loads.
+// where rows are.  Neighbours share N - 1 diagonals, which are added in LDS; there the workgroup's diagonals are summed by bucket and
+// written as one part; the parts are summed in a second launch.  No atomics: one order.  Bound by the loads and what turns them into
+// fp32: 60 to 71 us from card to card for 16 x 2047 x 2511 fp16, whose odd rows cost unaligned loads (2.3 to 2.7 TB/s; 107 with a
+// thread per N diagonals, one column further right every row).
 
 constexpr int BIAS_CHUNK = 64;        // rows per workgroup
 constexpr int BIAS_GRAD_THREADS = 256;

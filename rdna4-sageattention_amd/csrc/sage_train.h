@@ -51,8 +51,8 @@ struct TrainArgs {
   // what the rounding of out to 16 bits took away, in 16 bits, [B, H, Sq, D] (packed [H, Sq, D]); NULL where no backward pass comes.
   // D_i is the sum of do_i . o_i, whose terms' roundings would be the largest part of ds' error in rows of few keys.
   uint16_t* lo;
-  // backward: -lse / sm_scale and -D of every row, where the sums of the scores and of dout . v begin; -inf and 0 in the padding: rows of `pad` entries per (b, h) (packed: per
-  // h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
+  // backward: -lse / sm_scale and -D of every row, where the sums of the scores and of dout . v begin; -inf and 0 in the padding: rows
+  // of `pad` entries per (b, h) (packed: per h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
   float *nl, *nd;
   int64_t pad;
   uint32_t* norms;                 // fp16: the largest squared norms of dout's and v's rows, as bits

@@ -11,7 +11,9 @@ namespace sage {
 // keep the matrix unit busy by itself.  It walks blocks of 32 queries, two a tile, as one stream of products: those of block b + 1's
 // scores and weights' gradients in turn with block b - 1's parts of dv and dk, and beside them the weights of block b.  The operands
 // of product n + AHEAD are read from LDS when product n is issued, whatever tile they are of.  (Two waves per SIMD with half of the
-// registers each, four operands ahead: 625 us at 1 x 24 x 4608 x 128; the weights beside half of the products only: 606.)
+// registers each, four operands ahead: 625 us at 1 x 24 x 4608 x 128; the weights beside half of the products only: 606; this
+// 543, 0.96 PFLOP/s, the matrix unit busy for 51%, and 2000 at 2 x 32 on 8 x 8192 x 128 causal, 1.10 PFLOP/s.)  What bounds it is
+// issue: one wave has to issue 64 products and some 400 other instructions a tile.
 template <int D> struct DkvGeo {
   static constexpr int ROWS = 64;                  // queries per tile
   static constexpr int SLOTS = 4;                  // tiles in LDS: one still read, one at work, one arrived, one on its way
@@ -307,8 +309,8 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
 // scores, makes the weights and sums dv; the second recomputes the gradient of the weights, multiplies it by the weights, which it
 // gets in fp32 through LDS one tile later, and sums dk.  Each has half of the operands and sums, so two waves fit a SIMD, and one's
 // exponentials run beside the other's products.  Step u: the first waves work on tile u of 32 queries, the second ones on tile
-// u - 1, tile u + 1 is on its way.  (2 x 12 x 2180 x 256: 648 us in one wave, whose registers spill, 385 like this; at head dim 128 one wave
-// is faster, 702 and 567 us at 1 x 24 x 4608.)
+// u - 1, tile u + 1 is on its way.  (2 x 12 x 2180 x 256: 648 us in one wave, whose registers spill, 400 like this; at head dim
+// 128 one wave is faster, 702 and 567 us at 1 x 24 x 4608 when they were compared.)
 template <int D> struct DkvPairGeo {
   static constexpr int ROWS = 32;                  // queries per tile
   static constexpr int SLOTS = 3;                  // tiles in LDS
