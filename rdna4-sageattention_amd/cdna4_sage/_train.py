@@ -97,6 +97,15 @@ def _scale(sm_scale):
     return sm
 
 
+def _check_offsets(cu_q, cu_k, gpu):
+    """(For callers of the op: attention_train_varlen makes them so.)"""
+    for c in (cu_q, cu_k):
+        if c is None or c.dtype != torch.int32 or c.dim() != 1 or c.get_device() != gpu or not c.is_contiguous():
+            raise Unsupported("cu_q and cu_k: contiguous int32 offsets on the GPU of q")
+    if cu_q.shape != cu_k.shape or cu_q.numel() < 2:
+        raise Unsupported("cu_q and cu_k must be of one length batch + 1 >= 2")
+
+
 # ---- launches -------------------------------------------------------------------------------------------------------------
 
 def _strides(t, layout, packed):
@@ -130,6 +139,10 @@ def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, caus
     packed = cu_q is not None
     shape = _check(q, k, v, layout, packed)
     B, H, Hkv, Sq, Skv, D, gpu = shape
+    if packed or cu_k is not None:
+        if attn_mask is not None:
+            raise Unsupported("packed sequences take no attn_mask")
+        _check_offsets(cu_q, cu_k, gpu)
     bias = None if table is None else _bias(table, H, bidirectional, max_distance, gpu)
     mask, ms, axes = None, (0, 0, 0, 0), None
     if attn_mask is not None:
@@ -192,13 +205,27 @@ def backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, s
     return dq, dk, dv, dtable
 
 
-def backward_plan(q, k, v, layout, table, cu_q, bidirectional, max_distance, axes):
-    """forward_launch's plan, from the same tensors."""
-    shape = _check(q, k, v, layout, cu_q is not None)
+def backward_plan(dout, q, k, v, out, lse, state, layout, table, cu_q, cu_k, bidirectional, max_distance, axes):
+    """forward_launch's plan, from the same tensors, which are checked (they may come from a caller of the op)."""
+    packed = cu_q is not None
+    shape = _check(q, k, v, layout, packed)
+    if packed or cu_k is not None:
+        _check_offsets(cu_q, cu_k, shape[6])
+    for t in (dout, out):
+        if t.shape != q.shape or t.dtype != q.dtype or t.get_device() != shape[6]:
+            raise Unsupported("dout and out must be like q")
+    rows = (shape[1], shape[3]) if packed else (shape[0], shape[1], shape[3])
+    if lse.shape != rows or lse.dtype != torch.float32 or lse.get_device() != shape[6] or not lse.is_contiguous():
+        raise Unsupported(f"lse must be fp32 {rows}, contiguous, on the GPU of q")
+    if axes is not None and len(axes) != 3:
+        raise Unsupported("mask_axes: none, or one for each of batch, heads and rows")
     bias = None if table is None else _bias(table, shape[1], bidirectional, max_distance, shape[6])
     if q.numel() == 0 or k.numel() == 0:
         return shape, bias, axes, 0, 0, 0
-    return (shape, bias, axes, *_sizes(shape, bias, axes, cu_q, True))
+    sizes = _sizes(shape, bias, axes, cu_q, True)
+    if state.dtype != torch.uint8 or state.numel() < sizes[0] or state.get_device() != shape[6] or not state.is_contiguous():
+        raise Unsupported(f"state: the {sizes[0]} bytes of attention_train with keep")
+    return (shape, bias, axes, *sizes)
 
 
 class _Train(torch.autograd.Function):
@@ -259,6 +286,15 @@ def attention_train(q, k, v, tensor_layout="HND", sm_scale=None, is_causal=False
                       max_distance, return_lse)
 
 
+def _offsets(cu, device):
+    """Token offsets as the kernels read them; int64 ones that int32 cannot hold stay too large or too small."""
+    if cu.dtype == torch.int64:
+        cu = cu.clamp(-1, 2**31 - 1)
+    elif cu.dtype != torch.int32:
+        raise Unsupported(f"cu_seqlens of {cu.dtype} (int32 or int64)")
+    return cu.to(device=device, dtype=torch.int32).contiguous()
+
+
 def attention_train_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=None, max_seqlen_k=None, sm_scale=None,
                            is_causal=False, bias_table=None, bidirectional=True, max_distance=128, return_lse=False):
     """attention_train of packed sequences: q [total_q, H, D], k / v [total_k, Hkv, D], cu_seqlens_q / cu_seqlens_k
@@ -268,7 +304,7 @@ def attention_train_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=Non
     outside the sequences."""
     if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape != cu_seqlens_k.shape or cu_seqlens_q.numel() < 2:
         raise Unsupported("cu_seqlens_q / cu_seqlens_k must be 1-D of one length batch + 1 >= 2")
-    cu_q, cu_k = (c.to(device=q.device, dtype=torch.int32).contiguous() for c in (cu_seqlens_q, cu_seqlens_k))
+    cu_q, cu_k = (_offsets(c, q.device) for c in (cu_seqlens_q, cu_seqlens_k))
     return _attention(q, k, v, bias_table, None, cu_q, cu_k, "NHD", sm_scale, is_causal, bidirectional, max_distance, return_lse)
 
 

@@ -218,7 +218,8 @@ def attention_train_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     """(dq, dk, dv, dtable), the last one empty without a table; mask_axes: whether the mask had a batch, head and row axis."""
     from . import _train
 
-    plan = _train.backward_plan(q, k, v, layout, table, cu_q, bidirectional, max_distance, tuple(mask_axes) or None)
+    plan = _train.backward_plan(dout, q, k, v, out, lse, state, layout, table, cu_q, cu_k, bidirectional, max_distance,
+                                tuple(mask_axes) or None)
     dq, dk, dv, dt = _train.backward_launch(dout, q, k, v, out, lse, state, table, cu_q, cu_k, layout, sm_scale, is_causal,
                                             plan, (True, True, table is not None))
     return dq, dk, dv, q.new_empty(0) if dt is None else dt

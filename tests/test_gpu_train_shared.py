@@ -87,3 +87,38 @@ def test_captured_packed_steps_of_shared_heads(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), r
         assert torch.isfinite(noise)
+
+
+def test_offsets_that_pass_32_bits(dev):
+    T, H, D = 40, 2, 64
+    ts = [torch.randn(T, H, D, generator=torch.Generator().manual_seed(i)).to(BF).to(dev).requires_grad_() for i in range(3)]
+    cu = torch.tensor([0, 15, 40], device=dev)
+    want = cdna4_sage.attention_train_varlen(*ts, cu, cu.to(torch.int32))
+    assert bool((want != 0).any())
+    for bad in (torch.tensor([0, 15, 40 + (1 << 32)]), torch.tensor([0, 15 - (1 << 32), 40])):
+        out = cdna4_sage.attention_train_varlen(*ts, bad.to(dev), cu)
+        grads = torch.autograd.grad(out, ts, torch.ones_like(out))
+        assert all(bool((t == 0).all()) for t in (out, *grads))
+    for other in (torch.float32, torch.int16, torch.bool):
+        with pytest.raises(cdna4_sage.Unsupported):
+            cdna4_sage.attention_train_varlen(*ts, cu.to(other), cu)
+
+
+def test_the_ops_check_what_callers_bring(dev):
+    op = torch.ops.cdna4_sage
+    q, k, v, do = (torch.randn(1, 2, 70, 64, generator=torch.Generator().manual_seed(i)).to(BF).to(dev) for i in range(4))
+    how = ("HND", 0.0, False, True, 128)
+    out, lse, state = op.attention_train(q, k, v, None, None, None, None, *how, True)
+    good = [do, q, k, v, out, lse, state, None, None, None, *how, []]
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(cdna4_sage.attention_train(*leaves), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(op.attention_train_backward(*good)[:3], want))
+    for place, bad in ((0, do[:, :1]), (0, do.float()), (0, do.cpu()), (4, out[:, :, :69]), (5, lse[:, :, :69]), (5, lse.double()),
+                       (5, lse.cpu()), (6, state[:16]), (6, state.cpu()), (15, [1]), (15, [1, 1, 1])):
+        with pytest.raises(cdna4_sage.Unsupported):
+            op.attention_train_backward(*good[:place], bad, *good[place + 1:])
+    rows = [t[0].transpose(0, 1) for t in (q, k, v)]
+    cu = torch.tensor([0, 30, 70], dtype=torch.int32, device=dev)
+    for a, b in ((cu.long(), cu), (cu, None), (None, cu), (cu.cpu(), cu), (cu, cu[:2]), (cu[:1], cu[:1])):
+        with pytest.raises(cdna4_sage.Unsupported):
+            op.attention_train(*(rows if a is not None else (q, k, v)), None, None, a, b, *how, False)
