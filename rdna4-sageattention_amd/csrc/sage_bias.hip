@@ -107,9 +107,9 @@ template <int DT> __global__ __launch_bounds__(BIAS_THREADS) void bias_write(Bia
 // Every diagonal (key - query) is in one bucket.  A thread walks down a chunk of rows N = 16 / size at a time, N columns further
 // right each time: its N x N squares all lie on the same 2 N - 1 diagonals, whose sums it keeps, and its loads are 16 bytes, aligned
 // where rows are.  Neighbours share N - 1 diagonals, which are added in LDS; there the workgroup's diagonals are summed by bucket and
-// written as one part; the parts are summed in a second launch.  No atomics: one order.  Bound by the loads and what turns them into
-// fp32: 60 to 71 us from card to card for 16 x 2047 x 2511 fp16, whose odd rows cost unaligned loads (2.3 to 2.7 TB/s; 107 with a
-// thread per N diagonals, one column further right every row).
+// written as one part; the parts are summed in a second launch.  No atomics: one order.  Bound by the loads, of
+// which odd rows' are unaligned: 59 us for 16 x 2047 x 2511 fp16 (2.8 TB/s), 33 for 16 x 2048 x 2048 out of the last-level cache.  (With
+// each place at the tensor's edges tested and loaded by itself 10 us more; with the next square's loads on their way 5 to 15 more.)
 
 constexpr int BIAS_CHUNK = 64;        // rows per workgroup
 constexpr int BIAS_GRAD_THREADS = 256;
@@ -142,19 +142,19 @@ template <int DT> __global__ __launch_bounds__(BIAS_GRAD_THREADS) void bias_grad
   for (int e = 0; e < 2 * N - 1; ++e) acc[e] = 0.0f;
   const T* base = (const T*)a.d + h * a.sh;
   typedef uint32_t v4u_a4 __attribute__((ext_vector_type(4), aligned(4)));
-  // (i0 and g are multiples of N, so columns are)
-#pragma unroll 1
-  for (int i = i0; i < i1; i += N) {
-    const int64_t j = i + g;
-    if (j + N <= 0 || j >= a.kv_len) continue;
-    const T* p = base + i * a.sq + j;
-    if (j >= 0 && j + N <= a.kv_len && i + N <= i1) {
-      v4i w[N];
+  // (i0 and g are multiples of N, so columns are.)
+  auto inside = [&](int i) { return i + N <= i1 && i + g >= 0 && i + g + N <= a.kv_len; };
+  auto bring = [&](int i, v4i(&w)[N]) {
+    const T* p = base + i * a.sq + (i + g);
 #pragma unroll
-      for (int r = 0; r < N; ++r) {
-        if constexpr (DT == SAGE_DTYPE_F32) w[r] = __builtin_bit_cast(v4i, *(const v4u_a4*)(p + r * a.sq));
-        else w[r] = load16_2aligned(p + r * a.sq);
-      }
+    for (int r = 0; r < N; ++r) {
+      if constexpr (DT == SAGE_DTYPE_F32) w[r] = __builtin_bit_cast(v4i, *(const v4u_a4*)(p + r * a.sq));
+      else w[r] = load16_2aligned(p + r * a.sq);
+    }
+  };
+  auto add = [&](int i, const v4i(&w)[N]) {
+    const int64_t j = i + g;
+    if (inside(i)) {
 #pragma unroll
       for (int r = 0; r < N; ++r)
 #pragma unroll
@@ -166,16 +166,32 @@ template <int DT> __global__ __launch_bounds__(BIAS_GRAD_THREADS) void bias_grad
             acc[2 * e + 1 - r + N - 1] += elem_hi<DT>((uint32_t)w[r][e]);
           }
         }
-    } else {
+    } else if (j + N > 0 && j < a.kv_len && i < i1) {
+      // rows or columns that end inside the square (none begins inside): columns from the last one that there is, so that no load
+      // waits for another
+      const int c = (int)j;
 #pragma unroll
       for (int r = 0; r < N; ++r)
+        if (i + r < i1) {
+          const T* row = base + (i + r) * a.sq;
+          T x[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (i + r < i1 && j + e >= 0 && j + e < a.kv_len) {
-            if constexpr (DT == SAGE_DTYPE_F32) acc[e - r + N - 1] += ((const float*)p)[r * a.sq + e];
-            else acc[e - r + N - 1] += elem_lo<DT>(p[r * a.sq + e]);
+          for (int e = 0; e < N; ++e) x[e] = row[min(c + e, a.kv_len - 1)];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            float y;
+            if constexpr (DT == SAGE_DTYPE_F32) y = __uint_as_float(x[e]);
+            else y = elem_lo<DT>(x[e]);
+            acc[e - r + N - 1] += c + e < a.kv_len ? y : 0.0f;
           }
+        }
     }
+  };
+  v4i w[N];
+#pragma unroll 1
+  for (int i = i0; i < i1; i += N) {
+    if (inside(i)) bring(i, w);
+    add(i, w);
   }
   // sums[x]: of diagonal g0 - (N - 1) + x
   if (threadIdx.x == 0)
