@@ -107,7 +107,7 @@ __global__ void train_norms_zero(uint32_t* norms) {
 //
 // A wave per 32 queries, 12 D / 32 products per 32 keys and two workgroups per unit: 356 us at 1 x 24 x 4608 x 128 bf16 (1.10 PFLOP/s;
 // the matrix unit busy for 62%), 1360 at 2 x 32 x 8192 x 128 causal (1.21).  With a table's gradient a block near the diagonal
-// costs 48 LDS accesses more: 54 us at 4 x 16 x 1024 x 64, reach 128, where an atomic per pair took 99.
+// costs 28 LDS accesses more: 55 us at 4 x 16 x 1024 x 64, reach 128, where an atomic per pair took 99.
 
 template <int D, int DT, bool EX>
 __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainArgs a, BiasMap map) {
