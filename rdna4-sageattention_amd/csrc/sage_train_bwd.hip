@@ -182,8 +182,10 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_dq(TrainAr
     t_mask = 0;
   }
   float* mine = by_distance + wave * R;
-  if (biased)
+  if (biased) {
     for (int x = tid; x < R; x += TR_THREADS) bl[x] = a.bias[(int64_t)s.h * R + x];
+    __syncthreads();   // (the tiles' barriers wait for no stores to LDS)
+  }
 
   v16f dq[G::NDB];
   // the bias' gradient: the lane's sums of ds (of any rows of the wave's) and p (of its own row) over the keys at distance -reach and

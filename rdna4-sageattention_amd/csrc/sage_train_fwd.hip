@@ -68,8 +68,10 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     t_mask = 0;
   }
   const bool biased = EX && a.bias;
-  if (biased)
+  if (biased) {
     for (int x = tid; x <= 2 * a.reach; x += TR_THREADS) bl[x] = a.bias[(int64_t)s.h * (2 * a.reach + 1) + x];
+    __syncthreads();   // (the tiles' barriers wait for no stores to LDS)
+  }
 
   float m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
   v16f o[G::NDB];
