@@ -451,6 +451,17 @@ template <int N> __device__ __forceinline__ float tr_nonfinite(const v16f (&a)[N
   return t;
 }
 
+// Whether any of a lane's 16-bit operands is an infinity or a NaN
+template <int DT, int N> __device__ __forceinline__ bool tr_nonfinite_operand(const v4i (&f)[N]) {
+  constexpr uint32_t E = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad |= ((uint32_t)f[i][e] & E) == E || ((uint32_t)f[i][e] & (E << 16)) == (E << 16);
+  return bad;
+}
+
 // The infinities and NaN of a tile become 0; poison[r] is set where row r had one.  A hidden pair has weight 0, but 0 times an
 // infinity is NaN: results that come out non-finite are computed a second time from tiles cleaned like this, in which the rows
 // that see a poisoned one get NaN by their scores.  Two barriers are the caller's.

@@ -74,6 +74,11 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   }
 
   float m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
+  // A score of -inf has weight 0 as a hidden one does, and leaves the sums finite.  The smallest score before bias and mask tells that
+  // there may be one (as the largest of the bits, one instruction for two scores: floats' minimum takes three), and the second pass
+  // whose it is: an infinite query's or key's, whose rows are NaN, or an overflow.
+  uint32_t low = 0;
+  bool qbad = false, sees = lim >= 0;   // the lane's query is non-finite, it sees a key: for the second pass
   v16f o[G::NDB];
   const TrBlocks blocks = EX ? tr_key_blocks(a, s) : TrBlocks();
   auto issue = [&](int t, int slot) {
@@ -90,6 +95,19 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     for (int kk = 0; kk < G::NK; ++kk) {
       x[0] = tr_mfma<DT>(kt.rows(0, kk), qf[kk], x[0]);
       x[1] = tr_mfma<DT>(kt.rows(1, kk), qf[kk], x[1]);
+    }
+    if (masked && slow) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (qbad || poison[32 * kb + 8 * (v >> 2) + 4 * hf + (v & 3)]) x[kb][v] = NAN;
+    }
+    if (EX || masked) {   // (elsewhere beside the exponentials: at 256 channels the scores would be moved about, 915 for 870 us a step)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) low = max(low, __float_as_uint(x[kb][v]));
     }
     if (EX) {
       // scores in the log2 domain, with the bias
@@ -111,19 +129,15 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
           for (int v = 0; v < 16; ++v) x[kb][v] = __builtin_fmaf(x[kb][v], a.c, far);
       }
     }
-    if (masked && slow) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (poison[32 * kb + 8 * (v >> 2) + 4 * hf + (v & 3)]) x[kb][v] = NAN;
-    }
     if (masked) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const int key0 = t * TR_ROWS + 32 * kb;
         uint32_t w = ~0u;
-        if (EX && bits) w = wl[slot][wave][32 * kb + ln];
+        if (EX && bits) {
+          w = wl[slot][wave][32 * kb + ln];
+          sees |= key0 <= lim && (w << max(0, 31 - (lim - key0))) != 0;
+        }
         tr_hide_keys(x[kb], key0, lim, w, hf);
       }
     }
@@ -151,6 +165,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int v = 0; v < 16; v += 2) {
+        if (!EX && !masked) low = max(max(low, __float_as_uint(x[kb][v])), __float_as_uint(x[kb][v + 1]));
         const float e0 = __builtin_amdgcn_exp2f(EX ? x[kb][v] + negm : __builtin_fmaf(x[kb][v], a.c, negm));
         const float e1 = __builtin_amdgcn_exp2f(EX ? x[kb][v + 1] + negm : __builtin_fmaf(x[kb][v + 1], a.c, negm));
         ps[v & 2] += e0;
@@ -165,7 +180,8 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   };
 
   for (int pass = 0; pass < 2; ++pass) {
-    m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f;
+    m = -INFINITY, negm = FWD_SHIFT<DT>, l = 0.0f, low = 0;
+    if (EX && bits) sees = false;
 #pragma unroll
     for (int db = 0; db < G::NDB; ++db)
 #pragma unroll
@@ -195,12 +211,16 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
       if (t < t_end) tile(t, slot, std::true_type{}, pass != 0);
       if (pass) __syncthreads();
     }
-    const bool bad = !(tr_nonfinite(o) == 0.0f);
+    const bool bad = !(tr_nonfinite(o) == 0.0f) || !(__uint_as_float(low) * a.c > -INFINITY);
     if (!__syncthreads_or(on && bad)) break;
     t_mask = 0;   // every tile cleaned, hidden keys taken out
+    qbad = tr_nonfinite_operand<DT>(qf);
+    qbad |= __shfl_xor((int)qbad, 32) != 0;
   }
 
   l = add_xor32_f32(l);
+  low = max(low, (uint32_t)__shfl_xor((int)low, 32));
+  if (l == 0.0f && sees && !(__uint_as_float(low) * a.c > -INFINITY)) l = NAN;   // (nothing but overflows: no row that sees nothing)
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* op = a.out + s.b * (a.cu_q ? 0 : a.ob) + (s.qr + ir) * a.os + s.h * a.oh;
 #pragma unroll
