@@ -55,7 +55,7 @@ struct TrainArgs {
   // of `pad` entries per (b, h) (packed: per h, sequence s at floor(cu_q[s] / 64) * 64 + 64 s)
   float *nl, *nd;
   int64_t pad;
-  uint32_t* norms;                 // fp16: the largest squared norms of dout's and v's rows, as bits
+  uint32_t* norms;                 // fp16: the largest squared norms of dout's and v's rows that take part, as bits
   // packed batches: offsets and the (sequence, tile) of each tile id, sequence -1 for none
   const int *cu_q, *cu_k;
   const int* bounds;               // the rows of q, [0] .. [1] - 1, and of k, [2] .. [3] - 1, that the sequences cover
@@ -67,6 +67,8 @@ struct TrainArgs {
   // block*aw (64-bit words), and for each key block a bit for every row block, at any_t + ..
   const uint64_t *any, *any_t;
   int64_t ab, ah, aw, tb, th, tw;
+  // fp16 with a backward pass: the keys of each key block that a row of 64 row blocks sees, at keys_seen + b*tb + h*th + block*tw + ..
+  const uint64_t* keys_seen;
   // bias by distance: [H, 2 reach + 1] fp32 times log2(e); entry reach + d for key - query = d, clamped to +-reach
   const float* bias;
   int reach;

@@ -120,6 +120,12 @@ __global__ __launch_bounds__(TR_THREADS) void train_gaps(TrainGaps a, const int*
   }
 }
 
+__device__ __forceinline__ uint64_t wave_or(uint64_t w) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) w |= (uint64_t)__shfl_xor((unsigned long long)w, o);
+  return w;
+}
+
 // Four bytes' truth as four bits: each byte's bits folded onto its lowest, and those gathered by a product
 __device__ __forceinline__ uint32_t truth4(uint32_t w) {
   w |= w >> 4;
@@ -131,11 +137,12 @@ typedef uint32_t v4u_a1 __attribute__((ext_vector_type(4), aligned(1)));
 
 // A boolean mask as bits, word-major: word w (keys 32 w ..) of 64 consecutive rows side by side.  A wave makes the words of 64
 // keys of 64 rows: lane r reads row r's 64 bytes, or, at the last keys and where keys are not contiguous, the wave reads a byte per
-// lane of row after row and lane r keeps row r's ballot.  (1250 x 1250 x 6: 25 us with the latter alone.)
+// lane of row after row and lane r keeps row r's ballot.  (1250 x 1250 x 6: 25 us with the latter alone.)  seen (or NULL): a block's
+// keys that one of its rows sees, of which row i, under a causal mask, those up to i + first (without: first is the last key).
 __global__ __launch_bounds__(TR_THREADS) void train_mask_bits(const uint8_t* __restrict__ mask, int64_t msb, int64_t msh, int64_t msq,
                                                               int64_t msk, int heads, int rows, int row_pad, int keys, int chunks,
                                                               int blocks, int64_t units, uint32_t* __restrict__ bits,
-                                                              uint8_t* __restrict__ shows) {
+                                                              uint8_t* __restrict__ shows, uint64_t* __restrict__ seen, int first) {
   const int lane = threadIdx.x & 63;
   const int64_t u = (int64_t)blockIdx.x * (TR_THREADS / 64) + (threadIdx.x >> 6);
   if (u >= units) return;
@@ -179,12 +186,20 @@ __global__ __launch_bounds__(TR_THREADS) void train_mask_bits(const uint8_t* __r
   }
   const bool any = __ballot(lo | hi) != 0;
   if (lane == 0) shows[u] = any;   // [batch x head][block of 64 rows][block of 64 keys]
+  if (seen) {
+    const int64_t last = (int64_t)r0 + lane + first - c * 64;   // of the 64 keys
+    uint64_t w = last < 0 ? 0 : ((uint64_t)hi << 32 | lo) & (last < 63 ? (2ull << last) - 1 : ~0ull);
+    w = wave_or(w);
+    if (lane == 0) seen[u] = w;
+  }
 }
 
-// What blocks show, as bits both ways: a wave for 64 key blocks of a row block, or for 64 row blocks of a key block
+// What blocks show, as bits both ways: a wave for 64 key blocks of a row block, or for 64 row blocks of a key block, which also
+// joins what those see of its keys
 __global__ __launch_bounds__(TR_THREADS) void train_mask_any(const uint8_t* __restrict__ shows, int blocks, int chunks, int aw, int tw,
                                                              int64_t units, int64_t units_t, uint64_t* __restrict__ any,
-                                                             uint64_t* __restrict__ any_t) {
+                                                             uint64_t* __restrict__ any_t, const uint64_t* __restrict__ seen,
+                                                             uint64_t* __restrict__ keys_seen) {
   const int lane = threadIdx.x & 63;
   int64_t u = (int64_t)blockIdx.x * (TR_THREADS / 64) + (threadIdx.x >> 6);
   if (u < units) {
@@ -196,13 +211,17 @@ __global__ __launch_bounds__(TR_THREADS) void train_mask_any(const uint8_t* __re
     const int64_t bh = u / tw / chunks;
     const uint64_t m = __ballot(b < blocks && shows[(bh * blocks + b) * chunks + c] != 0);
     if (lane == 0) any_t[u] = m;
+    if (seen) {
+      const uint64_t k = wave_or(b < blocks ? seen[(bh * blocks + b) * chunks + c] : 0);
+      if (lane == 0) keys_seen[u] = k;
+    }
   }
 }
 
 // Where everything lies in the state that the forward pass leaves to the backward pass, and in its workspace.
 struct TrainLayout {
   int q_tiles, k_tiles, mask_b, mask_h, row_pad, words, blocks, chunks, aw, tw;
-  int64_t q_tab, k_tab, bits, shows, any, any_t, vec, lo, state;      // byte offsets; bounds at 0
+  int64_t q_tab, k_tab, bits, shows, any, any_t, seen, keys_seen, vec, lo, state;      // byte offsets; bounds at 0
   int64_t pad, nl, nd, norms, parts, part, kv_part, k_order, work;
 };
 
@@ -244,6 +263,8 @@ static TrainLayout train_layout(bool packed, int B, int H, int Hkv, int Sq, int 
     l.shows = take(at, bh * l.blocks * l.chunks);
     l.any = take(at, bh * l.blocks * l.aw * 8);
     l.any_t = take(at, bh * l.chunks * l.tw * 8);
+    l.seen = take(at, keep ? bh * l.blocks * l.chunks * 8 : 0);       // (bf16 leaves them as they are)
+    l.keys_seen = take(at, keep ? bh * l.chunks * l.tw * 8 : 0);
   }
   if (reach) l.vec = take(at, (int64_t)H * (2 * reach + 1) * 4);
   if (keep) l.lo = take(at, (int64_t)(packed ? 1 : B) * H * Sq * D * 2);
@@ -324,6 +345,7 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
     a.mb = msb ? per * l.mask_h : 0, a.mh = msh ? per : 0, a.mw = l.row_pad, a.mi = msq ? 1 : 0;
     const int64_t na = (int64_t)l.blocks * l.aw, nt = (int64_t)l.chunks * l.tw;
     a.any = (const uint64_t*)(base + l.any), a.any_t = (const uint64_t*)(base + l.any_t);
+    if (keep && dtype == SAGE_DTYPE_F16) a.keys_seen = (const uint64_t*)(base + l.keys_seen);
     a.ab = msb ? na * l.mask_h : 0, a.ah = msh ? na : 0, a.aw = l.aw;
     a.tb = msb ? nt * l.mask_h : 0, a.th = msh ? nt : 0, a.tw = l.tw;
   }
@@ -389,12 +411,13 @@ extern "C" int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t q
     const int64_t bh = (int64_t)l.mask_b * l.mask_h, units = bh * l.blocks * l.chunks;
     SAGE_REQUIRE(units <= 0x7FFFFFFF, "sage_train_fwd: mask too large");
     uint8_t* shows = (uint8_t*)state + l.shows;
+    uint64_t* seen = a.keys_seen ? (uint64_t*)((char*)state + l.seen) : nullptr;
     train_mask_bits<<<(unsigned)((units + 3) / 4), TR_THREADS, 0, st>>>((const uint8_t*)mask, msb, msh, msq, msk, l.mask_h,
                                                                         msq ? Sq : 1, l.row_pad, Skv, l.chunks, l.blocks, units,
-                                                                        (uint32_t*)a.bits, shows);
+                                                                        (uint32_t*)a.bits, shows, seen, causal && msq ? Skv - Sq : Skv - 1);
     const int64_t n = bh * l.blocks * l.aw, nt = bh * l.chunks * l.tw;
     train_mask_any<<<(unsigned)((n + nt + 3) / 4), TR_THREADS, 0, st>>>(shows, l.blocks, l.chunks, l.aw, l.tw, n, nt, (uint64_t*)a.any,
-                                                                        (uint64_t*)a.any_t);
+                                                                        (uint64_t*)a.any_t, seen, (uint64_t*)a.keys_seen);
   }
   if (buckets)
     if (int rc = bias_expand_launch(table, table_dtype, tb, th, H, m, TR_LOG2E, (float*)a.bias, st)) return rc;

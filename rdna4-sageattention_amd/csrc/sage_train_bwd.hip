@@ -24,12 +24,26 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
     for (int o = 1; o < LPR; o <<= 1) x += __shfl_xor(x, o);
     return x;
   };
-  if ((int)blockIdx.x >= row_blocks) {            // fp16: the rows of v
-    const int64_t n = (int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * a.Skv;
+  if ((int)blockIdx.x >= row_blocks) {            // fp16: the rows of v that a query sees (what others hold is not to matter)
+    const int64_t len = a.cu_q ? (int64_t)a.k_tiles * TR_COLS : a.Skv, n = (int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * len;
     for (int64_t x = (int64_t)(blockIdx.x - row_blocks) * ROWS + r; x < n; x += (int64_t)norm_blocks * ROWS) {
-      const int64_t h = x % a.Hkv, t = x / a.Hkv, j = t % a.Skv, b = t / a.Skv;
+      const int64_t h = x % a.Hkv, t = x / a.Hkv, b = t / len;
+      int64_t j = t % len;
+      bool seen = true;
+      if (a.cu_q) {                               // (the last query of a sequence sees all of its keys)
+        const int2 e = a.k_tab[j / TR_COLS];
+        const int k0 = e.x < 0 ? 0 : a.cu_k[e.x], i = e.y * TR_COLS + (int)(j % TR_COLS);
+        seen = e.x >= 0 && k0 + i < a.cu_k[e.x + 1] && a.cu_q[e.x] < a.cu_q[e.x + 1];
+        j = k0 + i;
+      } else if (a.keys_seen) {
+        uint64_t w = 0;
+        const int heads = a.th ? a.H / a.Hkv : 1;
+        for (int g = 0; g < heads; ++g)
+          for (int y = 0; y < a.tw; ++y) w |= a.keys_seen[b * a.tb + (h * heads + g) * a.th + (j >> 6) * a.tw + y];
+        seen = w >> (j & 63) & 1;
+      }
       float s = 0.0f;
-      if (has) {
+      if (has && seen) {
         const v4i w = *reinterpret_cast<const v4i*>(a.v + b * a.vb + j * a.vs + h * a.vh + l * 8);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -70,13 +84,13 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
         }
       }
       d = row_sum(d);
+      const float lse = i < s.q_len ? a.lse[lse_at + i] : -INFINITY;
       if (DT == DT_F16) {
         g2 = row_sum(g2);
-        if (g2 < INFINITY) top = fmaxf(top, g2);
+        if (g2 < INFINITY && lse != -INFINITY) top = fmaxf(top, g2);
       }
       if (l == 0) {
         // a row that sees nothing: p = 0; one with an infinity or a NaN in it: p = NaN wherever it sees a key
-        const float lse = i < s.q_len ? a.lse[lse_at + i] : -INFINITY;
         float nl = -(lse / a.scale), nd = -d;
         if (lse == -INFINITY) nl = -INFINITY, nd = 0.0f;
         else if (!(fabsf(lse) < INFINITY) || !(fabsf(d) < INFINITY)) nl = NAN;
@@ -389,7 +403,8 @@ template <int D, int DT> int train_bwd_launch(const TrainArgs& a, const BiasMap&
   int norm_blocks = 0;
   if (DT == DT_F16) {
     train_norms_zero<<<1, 64, 0, st>>>(a.norms);
-    const int64_t need = ((int64_t)B * a.Hkv * a.Skv * (D == 96 ? 16 : D / 8) + TR_THREADS - 1) / TR_THREADS;
+    const int64_t len = a.cu_q ? (int64_t)a.k_tiles * TR_COLS : a.Skv;
+    const int64_t need = (B * a.Hkv * len * (D == 96 ? 16 : D / 8) + TR_THREADS - 1) / TR_THREADS;
     norm_blocks = (int)(need < 1024 ? need : 1024);
   }
   train_prep<D, DT><<<rows + norm_blocks, TR_THREADS, 0, st>>>(a, (int)rows, norm_blocks);
