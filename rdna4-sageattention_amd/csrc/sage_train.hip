@@ -284,14 +284,23 @@ static TrainLayout train_layout(bool packed, int B, int H, int Hkv, int Sq, int 
   return l;
 }
 
-static int train_sizes(const char* who, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype) {
+// A launch holds fewer than 2^32 threads, so fewer than 2^24 workgroups of 256 (dk and dv at 256 channels: 2^23 of 512), one for each
+// tile and head; the preparation adds 1024.  A tensor's rows and heads then fit 31 bits.
+static int train_sizes(const char* who, bool packed, int B, int H, int Hkv, int Sq, int Skv, int D, int dtype) {
   SAGE_REQUIRE(B > 0 && H > 0 && Hkv > 0 && Sq > 0 && Skv > 0, "%s: sizes must be positive", who);
   SAGE_REQUIRE(H % Hkv == 0, "%s: %d heads are no multiple of %d kv heads", who, H, Hkv);
   if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_F16) return fail(SAGE_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (!head_dim_ok(D)) return fail(SAGE_ERR_UNSUPPORTED, "%s: head_dim %d (supported 64, 96, 128, 256)", who, D);
   SAGE_REQUIRE(Sq <= 0x3FFFFFFF && Skv <= 0x3FFFFFFF && H <= 65535 && B <= 0xFFFFFF, "%s: too large", who);
-  const int64_t tiles = ((int64_t)(Sq > Skv ? Sq : Skv) / TR_COLS + 1 + B) * B * H;
-  SAGE_REQUIRE(tiles <= 0x3FFFFFFF, "%s: too large", who);
+  const int64_t rows = Sq > Skv ? Sq : Skv;
+  const int64_t tiles = packed ? (rows / TR_COLS + B) * H : (rows + TR_COLS - 1) / TR_COLS * B * H;
+  SAGE_REQUIRE(tiles < (D == 256 ? 1 << 23 : (1 << 24) - 1024), "%s: %lld tiles of 128 rows are too many", who, (long long)tiles);
+  return SAGE_OK;
+}
+
+// (a wave for each block of 64 rows x 64 keys of a mask, and one or two for its bits)
+static int train_mask_size(const char* who, const TrainLayout& l) {
+  SAGE_REQUIRE((int64_t)l.mask_b * l.mask_h * l.blocks * l.chunks < 1 << 25, "%s: mask too large", who);
   return SAGE_OK;
 }
 
@@ -319,7 +328,7 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
                         int dtype, int causal, float sm_scale, const int* cu_q, const int* cu_k, bool mask, int64_t msb,
                         int64_t msh, int64_t msq, int buckets, int two_sided, const int* borders, int table_dtype, int keep, void* state,
                         int64_t state_bytes) {
-  if (int rc = train_sizes(who, B, H, Hkv, Sq, Skv, D, dtype)) return rc;
+  if (int rc = train_sizes(who, cu_q != nullptr, B, H, Hkv, Sq, Skv, D, dtype)) return rc;
   SAGE_REQUIRE((cu_q != nullptr) == (cu_k != nullptr), "%s: cu_q and cu_k go together", who);
   SAGE_REQUIRE(!(cu_q && mask), "%s: packed batches take no mask", who);
   SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale %g", who, (double)sm_scale);
@@ -331,6 +340,7 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
       return fail(SAGE_ERR_UNSUPPORTED, "%s: the last bucket begins at distance %d (at most %d)", who, reach, TR_REACH);
   }
   l = train_layout(cu_q != nullptr, B, H, Hkv, Sq, Skv, D, mask, msb != 0, msh != 0, msq != 0, reach, buckets, keep != 0);
+  if (int rc = train_mask_size(who, l)) return rc;
   SAGE_REQUIRE(l.state == 0 || (state && ((uintptr_t)state & 255u) == 0 && state_bytes >= l.state),
                "%s: a state of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)l.state, (long long)state_bytes);
   a.B = B, a.H = H, a.Hkv = Hkv, a.Sq = Sq, a.Skv = Skv, a.q_tiles = l.q_tiles, a.k_tiles = l.k_tiles, a.causal = causal != 0;
@@ -361,7 +371,7 @@ extern "C" int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, i
   using namespace sage;
   clear_error();
   SAGE_REQUIRE(state_bytes && workspace_bytes, "sage_train_workspace: a result is NULL");
-  if (int rc = train_sizes("sage_train_workspace", B, H, Hkv, Sq, Skv, D, SAGE_DTYPE_BF16)) return rc;
+  if (int rc = train_sizes("sage_train_workspace", packed != 0, B, H, Hkv, Sq, Skv, D, SAGE_DTYPE_BF16)) return rc;
   int reach = 0;
   if (buckets) {
     BiasMap m;
@@ -372,6 +382,7 @@ extern "C" int sage_train_workspace(int packed, int B, int H, int Hkv, int Sq, i
   }
   const TrainLayout l = train_layout(packed != 0, B, H, Hkv, Sq, Skv, D, has_mask != 0, msb != 0, msh != 0, msq != 0, reach, buckets,
                                      keep != 0);
+  if (int rc = train_mask_size("sage_train_workspace", l)) return rc;
   *state_bytes = l.state;
   *workspace_bytes = l.work;
   return SAGE_OK;
@@ -409,7 +420,6 @@ extern "C" int sage_train_fwd(const void* q, int64_t qsb, int64_t qss, int64_t q
   }
   if (mask) {
     const int64_t bh = (int64_t)l.mask_b * l.mask_h, units = bh * l.blocks * l.chunks;
-    SAGE_REQUIRE(units <= 0x7FFFFFFF, "sage_train_fwd: mask too large");
     uint8_t* shows = (uint8_t*)state + l.shows;
     uint64_t* seen = a.keys_seen ? (uint64_t*)((char*)state + l.seen) : nullptr;
     train_mask_bits<<<(unsigned)((units + 3) / 4), TR_THREADS, 0, st>>>((const uint8_t*)mask, msb, msh, msq, msk, l.mask_h,

@@ -25,9 +25,10 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
     return x;
   };
   if ((int)blockIdx.x >= row_blocks) {            // fp16: the rows of v that a query sees (what others hold is not to matter)
-    const int64_t len = a.cu_q ? (int64_t)a.k_tiles * TR_COLS : a.Skv, n = (int64_t)(a.cu_q ? 1 : a.B) * a.Hkv * len;
-    for (int64_t x = (int64_t)(blockIdx.x - row_blocks) * ROWS + r; x < n; x += (int64_t)norm_blocks * ROWS) {
-      const int64_t h = x % a.Hkv, t = x / a.Hkv, b = t / len;
+    const uint32_t len = a.cu_q ? a.k_tiles * TR_COLS : a.Skv, n = (a.cu_q ? 1 : a.B) * a.Hkv * len;
+    for (uint32_t x = (blockIdx.x - row_blocks) * ROWS + r; x < n; x += norm_blocks * ROWS) {
+      const uint32_t t = x / a.Hkv;
+      const int64_t h = x % a.Hkv, b = t / len;
       int64_t j = t % len;
       bool seen = true;
       if (a.cu_q) {                               // (the last query of a sequence sees all of its keys)
