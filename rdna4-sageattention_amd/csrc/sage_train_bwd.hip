@@ -73,6 +73,7 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
     const uint16_t* gp = a.dout + (a.cu_q ? 0 : s.b * a.gb) + s.qr * a.gs + s.h * a.gh + l * 8;
     const uint16_t* lp = a.lo + lse_at * D + l * 8;
     for (int i = s.c0 + r; i < end; i += ROWS) {
+      const float lse = i < s.q_len ? a.lse[lse_at + i] : -INFINITY;
       float d = 0.0f, g2 = 0.0f;
       if (i < s.q_len && has) {
         const v4i x = *reinterpret_cast<const v4i*>(op + i * a.os), g = *reinterpret_cast<const v4i*>(gp + i * a.gs);
@@ -85,7 +86,6 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
         }
       }
       d = row_sum(d);
-      const float lse = i < s.q_len ? a.lse[lse_at + i] : -INFINITY;
       if (DT == DT_F16) {
         g2 = row_sum(g2);
         if (g2 < INFINITY && lse != -INFINITY) top = fmaxf(top, g2);
