@@ -325,7 +325,8 @@ int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype
 
 /*
  * Attention on 16-bit inputs with its backward pass (no counterpart in the reference, whose attention has no derivative):
- * softmax(sm_scale q k^T + bias) v, sm_scale 0 for 1 / sqrt(D), scores, statistics and sums in fp32.  q, out, dout, dq
+ * softmax(sm_scale q k^T + bias) v, sm_scale 0 for 1 / sqrt(D), at most 2^127 and, with a backward pass, at least 2^-100; scores,
+ * statistics and sums in fp32.  q, out, dout, dq
  * [B, H, Sq, D], k, v, dk, dv [B, Hkv, Skv, D] by (b, s, h) strides, dtype bf16 or fp16; lse fp32 [B, H, Sq], natural log.
  * causal: query i sees the keys j <= i + Skv - Sq.  mask: one byte per element, nonzero = visible, (b, h, i, j) at mask +
  * b * msb + h * msh + i * msq + j * msk, or NULL.  buckets: 0, or of a relative position bias (above; query i at position

@@ -15,6 +15,7 @@ from ._rope import out_like
 
 TABLE_DTYPES = {**DTYPES, torch.float32: _capi.DTYPE_F32}
 BIAS_BUCKETS = 256
+LEAST_SCALE = 2.0 ** -100   # with a backward pass
 
 
 # ---- checks ---------------------------------------------------------------------------------------------------------------
@@ -92,8 +93,8 @@ def _scale(sm_scale):
     if sm_scale is None or not sm_scale > 0:
         return 0.0
     sm = float(sm_scale)
-    if not 2.0 ** -126 <= sm <= 3.4028234663852886e38:
-        raise Unsupported(f"sm_scale {sm_scale} (a normal number of float32)")
+    if not 2.0 ** -126 <= sm <= 2.0 ** 127:
+        raise Unsupported(f"sm_scale {sm_scale} (2^-126 to 2^127)")
     return sm
 
 
@@ -137,6 +138,8 @@ def _sizes(shape, bias, axes, cu_q, keep):
 def forward_launch(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scale, causal, bidirectional, max_distance, keep):
     """(out, lse, state, what the kernels loaded of q, k and v, the call's plan for the backward pass); keep: one comes."""
     packed = cu_q is not None
+    if keep and 0.0 < sm_scale < LEAST_SCALE:
+        raise Unsupported(f"sm_scale {sm_scale} (where inputs require gradients at least 2^-100)")
     shape = _check(q, k, v, layout, packed)
     B, H, Hkv, Sq, Skv, D, gpu = shape
     if packed or cu_k is not None:
@@ -270,7 +273,8 @@ def attention_train(q, k, v, tensor_layout="HND", sm_scale=None, is_causal=False
     """Attention on 16-bit inputs, differentiable in q, k, v and bias_table: softmax(q k^T * sm_scale + bias) v with scores,
     statistics and sums in float32, the weights (and in the backward pass the scores' gradients) rounded to the inputs' type
     where they enter a product.  q: [B, H, q_len, D] for "HND", [B, q_len, H, D] for "NHD", k / v alike with kv heads of
-    which H is a multiple; bf16 or fp16, head dims 64, 96, 128, 256.  Returns out like q, or (out, lse) with the rows'
+    which H is a multiple; bf16 or fp16, head dims 64, 96, 128, 256.  sm_scale: None for D ** -0.5, at most 2^127 and at least
+    2^-100 (2^-126 where nothing requires a gradient).  Returns out like q, or (out, lse) with the rows'
     logsumexp, fp32 [B, H, q_len], which has no gradient.
 
     is_causal: query i sees the keys up to i + kv_len - q_len (bottom-right), any lengths.  attn_mask: boolean (True =

@@ -36,6 +36,8 @@ constexpr int TR_COLS = 128;     // columns per workgroup, 4 waves x 32
 constexpr int TR_ROWS = 64;      // rows per streamed tile
 constexpr int TR_THREADS = 256;
 constexpr float TR_LOG2E = 1.4426950408889634f;
+// Smallest sm_scale with a backward pass, which takes -lse / sm_scale as a score: below 2^128 for every |lse| below 2^28.
+constexpr float TR_LEAST_SCALE = 0x1p-100f;
 
 // Arguments of the three kernels and the preparation.  Strides in elements: b (batch), s (token), h (head).
 struct TrainArgs {

@@ -331,7 +331,9 @@ static int train_common(const char* who, TrainArgs& a, TrainLayout& l, BiasMap& 
   if (int rc = train_sizes(who, cu_q != nullptr, B, H, Hkv, Sq, Skv, D, dtype)) return rc;
   SAGE_REQUIRE((cu_q != nullptr) == (cu_k != nullptr), "%s: cu_q and cu_k go together", who);
   SAGE_REQUIRE(!(cu_q && mask), "%s: packed batches take no mask", who);
-  SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 3.402823466e38f, "%s: sm_scale %g", who, (double)sm_scale);
+  SAGE_REQUIRE(sm_scale >= 0.0f && sm_scale <= 0x1p127f, "%s: sm_scale %g", who, (double)sm_scale);   // (log2(e) times it is finite)
+  if (keep && sm_scale > 0.0f && sm_scale < TR_LEAST_SCALE)
+    return fail(SAGE_ERR_UNSUPPORTED, "%s: sm_scale %g (with a backward pass at least 2^-100)", who, (double)sm_scale);
   int reach = 0;
   if (buckets) {
     if (int rc = bias_map(who, H, buckets, two_sided, borders, table_dtype, &m)) return rc;

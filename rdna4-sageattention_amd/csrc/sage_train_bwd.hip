@@ -94,7 +94,7 @@ template <int D, int DT> __global__ __launch_bounds__(TR_THREADS) void train_pre
         // a row that sees nothing: p = 0; one with an infinity or a NaN in it: p = NaN wherever it sees a key
         float nl = -(lse / a.scale), nd = -d;
         if (lse == -INFINITY) nl = -INFINITY, nd = 0.0f;
-        else if (!(fabsf(lse) < INFINITY) || !(fabsf(d) < INFINITY)) nl = NAN;
+        else if (!(fabsf(nl) < INFINITY) || !(fabsf(d) < INFINITY)) nl = NAN;
         a.nl[at + i] = nl;
         a.nd[at + i] = nd;
       }
