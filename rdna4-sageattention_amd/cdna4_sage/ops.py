@@ -244,8 +244,9 @@ def _train_setup(ctx, inputs, output):
 
 
 def _train_backward(ctx, dout, *_):
-    dq, dk, dv, dt = attention_train_backward(dout, *ctx.saved_tensors, *ctx.how, ctx.axes)
-    return (dq, dk, dv, None, dt if ctx.saved_tensors[6] is not None else None) + (None,) * 8
+    saved = ctx.saved_tensors   # (once: a checkpoint's unpacking may not be asked for twice)
+    dq, dk, dv, dt = attention_train_backward(dout, *saved, *ctx.how, ctx.axes)
+    return (dq, dk, dv, None, dt if saved[6] is not None else None) + (None,) * 8
 
 
 attention_train.register_autograd(_train_backward, setup_context=_train_setup)
