@@ -176,6 +176,29 @@ def _mask_axes(attn_mask, q, k, layout):
     return [int(n > 1 and x != 0) for n, x in zip(shape[:3], s)]
 
 
+def _state_bytes(packed, B, H, Sq, Skv, D, axes, reach, keep):
+    """The bytes of the state, as sage_train_workspace has them, of sizes that may be symbols."""
+    def up(*n):
+        return sum((x + 255) // 256 * 256 for x in n)
+
+    n = 0
+    if packed:      # bounds, tiles of queries and of keys
+        n += up(16, 8 * (Sq // 128 + B), 8 * (Skv // 128 + B))
+    if axes:        # a mask's bits, what its blocks show, that both ways, the keys seen (twice)
+        bh = (B if axes[0] else 1) * (H if axes[1] else 1)
+        rows, blocks = ((Sq + 63) // 64 * 64, (Sq + 63) // 64) if axes[2] else (1, 1)
+        chunks = (Skv + 63) // 64
+        wide, high = (chunks + 63) // 64, (blocks + 63) // 64
+        n += up(bh * rows * chunks * 8, bh * blocks * chunks, bh * blocks * wide * 8, bh * chunks * high * 8)
+        if keep:
+            n += up(bh * blocks * chunks * 8, bh * chunks * high * 8)
+    if reach:       # the bias by distance
+        n += up(4 * H * (2 * reach + 1))
+    if keep:        # what the rounding of out took away
+        n += up(2 * (1 if packed else B) * H * Sq * D)
+    return n
+
+
 @torch.library.custom_op("cdna4_sage::attention_train", mutates_args=())
 def attention_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn_mask: Optional[torch.Tensor],
                     table: Optional[torch.Tensor], cu_q: Optional[torch.Tensor], cu_k: Optional[torch.Tensor], layout: str,
@@ -195,17 +218,16 @@ def _fake_attention_train(q, k, v, attn_mask, table, cu_q, cu_k, layout, sm_scal
 
     packed = cu_q is not None
     if packed:
-        out, (Sq, H, D), (Skv, Hkv, _), B = q.new_empty(q.shape), q.shape, k.shape, cu_q.shape[0] - 1
+        out, (Sq, H, D), Skv, B = q.new_empty(q.shape), q.shape, k.shape[0], cu_q.shape[0] - 1
         lse = q.new_empty((H, Sq), dtype=torch.float32)
     else:
         out, (B, H, Sq, D) = _rope.out_like(q), q.shape if layout == "HND" else [q.shape[i] for i in (0, 2, 1, 3)]
-        Hkv, Skv = (k.shape[1], k.shape[2]) if layout == "HND" else (k.shape[2], k.shape[1])
+        Skv = k.shape[2 if layout == "HND" else 1]
         lse = q.new_empty((B, H, Sq), dtype=torch.float32)
     state = 0
     if q.numel() != 0 and k.numel() != 0:
-        state = _capi.train_workspace(packed, int(B), int(H), int(Hkv), int(Sq), int(Skv), int(D),
-                                      tuple(_mask_axes(attn_mask, q, k, layout)) or None,
-                                      None if table is None else (int(table.shape[0]), bidirectional, max_distance), keep)[0]
+        reach = 0 if table is None else _capi.bias_borders(int(table.shape[0]), bidirectional, max_distance)[-1]
+        state = _state_bytes(packed, B, H, Sq, Skv, D, _mask_axes(attn_mask, q, k, layout), reach, keep)
     return out, lse, q.new_empty((state,), dtype=torch.uint8)
 
 
