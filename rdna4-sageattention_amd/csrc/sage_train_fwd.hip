@@ -78,7 +78,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
   // there may be one (as the largest of the bits, one instruction for two scores: floats' minimum takes three), and the second pass
   // whose it is: an infinite query's or key's, whose rows are NaN, or an overflow.
   uint32_t low = 0;
-  bool qbad = false, sees = lim >= 0;   // the lane's query is non-finite, it sees a key: for the second pass
+  bool qbad = false, sees = lim >= 0;   // the lane's query is non-finite (known in the second pass); it sees a key
   v16f o[G::NDB];
   const TrBlocks blocks = EX ? tr_key_blocks(a, s) : TrBlocks();
   auto issue = [&](int t, int slot) {
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(TR_THREADS, D == 256 ? 1 : 2) void train_fwd(TrainA
       if (t < t_end) tile(t, slot, std::true_type{}, pass != 0);
       if (pass) __syncthreads();
     }
-    const bool bad = !(tr_nonfinite(o) == 0.0f) || !(__uint_as_float(low) * a.c > -INFINITY);
+    const bool bad = !(tr_nonfinite(o) == 0.0f) || (sees && !(__uint_as_float(low) * a.c > -INFINITY));
     if (!__syncthreads_or(on && bad)) break;
     t_mask = 0;   // every tile cleaned, hidden keys taken out
     qbad = tr_nonfinite_operand<DT>(qf);
