@@ -133,7 +133,7 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
     if constexpr (n & 1) return second_op(par ? cur : prev, 1 - par, n >> 1);
     else return first_op(par ? next : cur, 1 - par, n >> 1);
   };
-  auto half = [&](int u, int t, int h, auto par_, auto masked_) __attribute__((always_inline)) {
+  auto half = [&](int u, int t, auto par_, auto masked_) __attribute__((always_inline)) {
     constexpr int par = decltype(par_)::value;
     constexpr bool masked = decltype(masked_)::value;
     using Other = std::integral_constant<int, 1 - par>;
@@ -268,8 +268,8 @@ __global__ __launch_bounds__(TR_THREADS, DkvGeo<D>::OCC) void train_dkv(TrainArg
         // a head: first the tiles that hide no keys of the wave, then, in a loop of their own, those that do
         bool same = true;
         auto one = [&](auto masked_) __attribute__((always_inline)) {
-          half(u, at_work.t, h, Zero{}, masked_);
-          half(u, at_work.t, h, One{}, masked_);
+          half(u, at_work.t, Zero{}, masked_);
+          half(u, at_work.t, One{}, masked_);
           prev = cur, cur = next, next = slot_of(u + 2), ++u;
           same = at_work.advance(a, s, group, t0, t_all) == 0 && u < steps;
           if (u < steps) top(u);
