@@ -114,3 +114,74 @@ def test_packed_gaps(dev, D, causal):
         for got, exact, room in zip((want[0][r], want[2][0][r], want[2][1][c], want[2][2][c]), (e.out, e.dq, e.dk, e.dv),
                                     (e.room_out, e.room_dq + 1e-6, e.room_dk + 1e-6, e.room_dv)):
             assert bool(((got.transpose(0, 1)[None].double().cpu() - exact).abs() <= room).all())
+
+
+def test_a_captured_step_whose_mask_changes(dev):
+    """The keys that a mask shows are found anew at every replay."""
+    B, H, Hkv, S, D = 2, 4, 2, 190, 64
+
+    def draw(seed):
+        q, k, v, do = _draw(B, H, Hkv, S, S, D, HF, seed=seed)
+        shown = torch.arange(S) < torch.tensor([20 + 30 * (seed % 5), S - 40 * (seed % 3)])[:, None]
+        v[~shown[:, None].expand(B, Hkv, S)] = LARGE
+        return [t.to(dev) for t in (q, k, v, do, shown[:, None, None])]
+
+    def step(q, k, v, do, mask):
+        out = cdna4_sage.attention_train(q, k, v, attn_mask=mask, is_causal=True)
+        return (out, *torch.autograd.grad(out, (q, k, v), do))
+
+    held = [t.requires_grad_(i < 3) for i, t in enumerate(draw(50))]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for seed in (51, 52, 53, 54):
+        new = draw(seed)
+        want = step(*(t.clone().requires_grad_(i < 3) for i, t in enumerate(new)))
+        clean = [t.clone() for t in new]
+        clean[2][clean[2] == LARGE] = 0.0
+        plain = step(*(t.requires_grad_(i < 3) for i, t in enumerate(clean)))
+        noise = torch.randn(1 << 20, device=dev).sum()
+        with torch.no_grad():
+            for a, b in zip(held, new):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, plain))
+        assert torch.isfinite(noise)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_the_largest_bf16_numbers_under_masks(dev, D):
+    """Products with them pass float32: an infinity times a weight of 0 is none of what is seen."""
+    B, H, Hkv, Sq, Skv = 3, 4, 2, 150, 260
+    q, k, v, do = _draw(B, H, Hkv, Sq, Skv, D, torch.bfloat16, seed=47)
+    for name, mask, causal in _forms(B, H, Hkv, Sq, Skv):
+        vis = mask.expand(B, H, Sq, Skv)
+        if causal:
+            vis = vis & torch.ones(Sq, Skv, dtype=torch.bool).tril(Skv - Sq)
+        keys, rows = ~vis.unflatten(1, (Hkv, H // Hkv)).any(2).any(2), ~vis.any(3)
+        kw = dict(attn_mask=mask.to(dev), is_causal=causal)
+        want = _run(dev, q, k, v, do, **kw)
+        ts = [t.clone() for t in (q, k, v, do)]
+        for t, gone in zip(ts, (rows, keys, keys, rows)):
+            t[gone] = 3e38
+            t[..., 2] = torch.where(gone, -3e38, t[..., 2])
+        _same(want, _run(dev, *ts, **kw))
+
+
+@pytest.mark.parametrize("D,dtype,large", [(64, HF, LARGE), (128, torch.bfloat16, 3e38), (256, HF, LARGE), (256, torch.bfloat16, 3e38)])
+def test_queries_before_the_first_key(dev, D, dtype, large):
+    """Causal, more queries than keys: without a mask, and with a bias inside."""
+    q, k, v, do = _draw(2, 4, 2, 300, 170, D, dtype, seed=48)
+    for bias in (None, torch.randn(16, 4, generator=torch.Generator().manual_seed(49)).to(dtype)):
+        kw = dict(is_causal=True, table=bias)
+        want = _run(dev, q, k, v, do, **kw)
+        ts = [q.clone(), k, v, do.clone()]
+        ts[0][:, :, :130], ts[3][:, :, :130] = large, -large
+        _same(want, _run(dev, *ts, **kw))
