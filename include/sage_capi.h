@@ -325,13 +325,13 @@ int sage_relative_bias_grad(const void* dbias, int64_t sh, int64_t sq, int dtype
 
 /*
  * Attention on 16-bit inputs with its backward pass (no counterpart in the reference, whose attention has no derivative):
- * softmax(sm_scale q k^T + bias) v, sm_scale 0 for 1 / sqrt(D), at most 2^127 and, with a backward pass, at least 2^-100; scores,
- * statistics and sums in fp32.  q, out, dout, dq
- * [B, H, Sq, D], k, v, dk, dv [B, Hkv, Skv, D] by (b, s, h) strides, dtype bf16 or fp16; lse fp32 [B, H, Sq], natural log.
- * causal: query i sees the keys j <= i + Skv - Sq.  mask: one byte per element, nonzero = visible, (b, h, i, j) at mask +
- * b * msb + h * msh + i * msq + j * msk, or NULL.  buckets: 0, or of a relative position bias (above; query i at position
- * i + Skv - Sq) whose last bucket begins at a distance of at most 760.  A query that sees no key is written as 0 (lse -inf) and
- * has no gradient; what hidden keys and such queries hold does not matter; a query that sees an infinity or a NaN is NaN.
+ * softmax(sm_scale q k^T + bias) v, sm_scale 0 for 1 / sqrt(D), at most 2^127 and, with a backward pass, at least 2^-100;
+ * scores, statistics and sums in fp32.  q, out, dout, dq [B, H, Sq, D], k, v, dk, dv [B, Hkv, Skv, D] by (b, s, h)
+ * strides, dtype bf16 or fp16; lse fp32 [B, H, Sq], natural log. causal: query i sees the keys j <= i + Skv - Sq.  mask:
+ * one byte per element, nonzero = visible, (b, h, i, j) at mask + b * msb + h * msh + i * msq + j * msk, or NULL.
+ * buckets: 0, or of a relative position bias (above; query i at position i + Skv - Sq) whose last bucket begins at a
+ * distance of at most 760; values of -inf hide their pairs.  A query that sees no key is written as 0 (lse -inf) and has
+ * no gradient; what hidden keys and such queries hold does not matter; a query that sees an infinity or a NaN is NaN.
  *
  * Packed batches (cu_q, cu_k not NULL; int32 [B + 1], device memory): B sequences one behind the other, Sq and Skv the totals of
  * rows, lse [H, Sq], batch strides unused, no mask; each sequence with its own diagonal and positions.  Rows that no sequence

@@ -280,7 +280,7 @@ def attention_train(q, k, v, tensor_layout="HND", sm_scale=None, is_causal=False
     is_causal: query i sees the keys up to i + kv_len - q_len (bottom-right), any lengths.  attn_mask: boolean (True =
     attend), broadcastable to [B, H, q_len, kv_len].  bias_table: learned values [buckets, H] (fp32, bf16 or fp16), added by the
     relative position as relative_bias does, without a [H, q_len, kv_len] tensor; its last bucket has to begin at a distance of
-    at most 760.  A query that sees no key gives 0 (lse -inf) and has no gradient, whatever it holds, and so do keys that no
+    at most 760 (values of -inf hide their pairs).  A query that sees no key gives 0 (lse -inf) and has no gradient, whatever it holds, and so do keys that no
     query sees; a query that sees an infinity or a NaN gives NaN.  Equal inputs give equal bits, gradients too.
 
     Gradients are of first order, in reverse mode; under torch.compile too.  Before a backward pass is captured into a graph,

@@ -2,11 +2,12 @@
 //
 // A wave per 32 queries, four in a workgroup, streams its keys once with a running reference and sum per row (online softmax); the
 // weights go from the score registers straight into the second product.  Two workgroups per unit, so that one wave's exponentials
-// run beside the other's products: 276 us at 1 x 24 x 4608 x 128 bf16 (0.94 PFLOP/s; the matrix unit busy for 50% of it, 17% of
-// the places empty while the last of 864 workgroups run) and 1040 at 2 x 32 x 8192 x 128 causal (1.06 PFLOP/s).  What bounds it is
-// the issue of both: 32 products and some 150 vector instructions a tile of 64 keys and wave.  One stream of products, scores a tile
-// ahead of the weights' products and the exponentials in slices beside them: 286 and 1100 us, 186 for 197 at 256 channels,
-// 41 for 35 with a bias at 64; higher wave priority around the products: within 1%, 228 for 196 us at 256 channels.
+// run beside the other's products: 283 us at 1 x 24 x 4608 x 128 bf16 (0.92 PFLOP/s; the matrix unit busy for 50% of it, 17% of
+// the places empty while the last of 864 workgroups run) and 1050 at 2 x 32 x 8192 x 128 causal (1.05 PFLOP/s).  What bounds it is
+// the issue of both: 32 products and some 165 vector instructions a tile of 64 keys and wave, 16 of which look for scores of -inf
+// (276, 1040, at 256 channels 196 for 202 and with a bias at 64 35 for 39 us without).  One stream of products, scores a tile
+// ahead of the weights' products and the exponentials in slices beside them: 286 for 278 and 1100 us then, 186 for 197 at 256
+// channels, 41 for 35 with a bias at 64; higher wave priority around the products: within 1%, 228 for 196 us at 256 channels.
 #include "sage_train.h"
 
 namespace sage {
